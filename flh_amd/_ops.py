@@ -754,6 +754,174 @@ def decode_attention_rope(q, k_new, v_new, cos, sin, positions, k_cache, v_cache
     return result
 
 
+def _check_cache_pair(q, k_cache, v_cache, batch, d):
+    for t_ in (q, k_cache, v_cache):
+        _check(t_.is_cuda and t_.dtype == torch.float16 and t_.is_contiguous() and t_.device == q.device,
+               "tensors must be contiguous float16 CUDA tensors on one device")
+    _check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.size(0) == batch and k_cache.size(3) == d,
+           "caches must be [B, Hkv, max_len, d]")
+
+
+def _check_lengths(lengths, batch, device):
+    _check(lengths.is_cuda and lengths.dtype == torch.int64 and lengths.is_contiguous() and tuple(lengths.shape) == (batch,)
+           and lengths.device == device, "lengths must be a contiguous int64 CUDA tensor [B]")
+
+
+def _attention_workspace(name, q, workspace, *sizes):
+    need = int(getattr(_lib.load(), name + "_workspace_bytes")(*sizes))
+    if workspace is None:
+        return _default_attention_workspace(q, need)
+    _check(workspace.is_cuda and workspace.dtype == torch.uint8 and workspace.is_contiguous()
+           and workspace.device == q.device and workspace.numel() >= need, f"workspace: {need} bytes of uint8 needed")
+    return workspace
+
+
+def tree_attention(q, k_new, v_new, cos, sin, lengths, mask, k_cache, v_cache, scale=None, workspace=None):
+    """Attention of a tree of T <= 256 drafted tokens (nodes) per sequence over a cache whose sequences have lengths of their
+    own, with the rotary embedding and the cache write inside: q [B, T, Hq, d], k_new / v_new [B, T, Hkv, d] fp16 as projected
+    (not rotated, left as they are), cos / sin [B, T, d] fp16 the rotary rows of the nodes' positions, lengths [B] int64 the
+    slots taken, mask bool [T, T] or [B, T, T]: whether node i sees node j; k_cache / v_cache [B, Hkv, max_len, d], node i's key
+    and value go to slot lengths[b] + i -> [B, T, Hq * d] fp16.  A node sees the lengths[b] slots in front of the tree and what
+    its mask names (nothing at all: zeros).  A sequence whose length is negative or above max_len - T takes no part: zeros, its
+    cache untouched.  d in {64, 128}.  `workspace` as in decode_attention."""
+    _check(q.dim() == 4 and k_new.dim() == 4, "q [B, T, Hq, d] and k_new, v_new [B, T, Hkv, d] expected")
+    B, T, Hq, d = q.shape
+    Hkv = k_new.size(2)
+    _check_cache_pair(q, k_cache, v_cache, B, d)
+    for t_ in (k_new, v_new, cos, sin):
+        _check(t_.is_cuda and t_.dtype == torch.float16 and t_.is_contiguous() and t_.device == q.device,
+               "tensors must be contiguous float16 CUDA tensors on one device")
+    _check(k_new.shape == (B, T, Hkv, d) and v_new.shape == k_new.shape and k_cache.size(1) == Hkv,
+           "q [B, T, Hq, d] and k_new, v_new [B, T, Hkv, d] expected")
+    _check(cos.shape == (B, T, d) and sin.shape == (B, T, d), "cos / sin must be [B, T, d]")
+    _check_lengths(lengths, B, q.device)
+    _check(mask.is_cuda and mask.dtype == torch.bool and mask.is_contiguous() and mask.device == q.device
+           and tuple(mask.shape) in ((T, T), (B, T, T)), "mask must be a contiguous bool CUDA tensor [T, T] or [B, T, T]")
+    _check(d in (64, 128), "head_dim must be 64 or 128")
+    _check(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, "Hq must be a multiple of Hkv")
+    _check(T <= 256, "at most 256 nodes")
+    out = torch.empty((B, T, Hq * d), dtype=torch.float16, device=q.device)
+    if B == 0 or T == 0:
+        return out
+    workspace = _attention_workspace("flh_tree_attention", q, workspace, B, T, Hq, Hkv, d)
+    _run("flh_tree_attention_f16", q.device, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+         lengths.data_ptr(), mask.data_ptr(), int(mask.dim() == 3), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), B, T, Hq,
+         Hkv, d, k_cache.size(2), float(scale if scale is not None else d ** -0.5), workspace.data_ptr(), workspace.numel(),
+         _stream(q))
+    return out
+
+
+def decode_attention_weights(q, k_cache, v_cache, lengths, weights, scale=None, workspace=None):
+    """One new token per sequence against the first lengths[b] slots of the caches (int64 [B] on the device), adding every
+    slot's probabilities, summed over the queries of its key / value head, to `weights` (float32 [B, Hkv, max_len], in place):
+    q [B, Hq, d] fp16 (rotated), k_cache / v_cache [B, Hkv, max_len, d] -> [B, Hq, d] fp16; Hq a multiple of Hkv, d in {64, 128}.
+    A length of zero, a negative one or one above max_len: zeros, no weights.  `workspace` as in decode_attention."""
+    _check(q.dim() == 3, "q [B, Hq, d] expected")
+    B, Hq, d = q.shape
+    _check_cache_pair(q, k_cache, v_cache, B, d)
+    Hkv, max_len = k_cache.size(1), k_cache.size(2)
+    _check_lengths(lengths, B, q.device)
+    _check_weights(weights, (B, Hkv, max_len), q.device)
+    _check(d in (64, 128), "head_dim must be 64 or 128")
+    _check(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, "Hq must be a multiple of Hkv")
+    _check(max_len > 0, "the caches have no slots")
+    out = torch.empty_like(q)
+    if B == 0:
+        return out
+    workspace = _attention_workspace("flh_decode_attention_weights", q, workspace, B, Hq, Hkv, d, max_len)
+    _run("flh_decode_attention_weights_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
+         out.data_ptr(), weights.data_ptr(), B, Hq, Hkv, d, max_len, float(scale if scale is not None else d ** -0.5),
+         workspace.data_ptr(), workspace.numel(), _stream(q))
+    return out
+
+
+def prefill_attention_weights(q, k_cache, v_cache, past, weights, scale=None, workspace=None):
+    """prefill_attention (the same output) that adds every slot's probabilities, summed over the queries of its key / value head
+    that see it, to `weights` (float32 [B, Hkv, max_len], in place).  `workspace` as in decode_attention."""
+    _check(q.dim() == 4, "q [B, T, Hq, d] and caches [B, Hkv, max_len, d] expected")
+    B, T, Hq, d = q.shape
+    _check_cache_pair(q, k_cache, v_cache, B, d)
+    Hkv, max_len = k_cache.size(1), k_cache.size(2)
+    _check_weights(weights, (B, Hkv, max_len), q.device)
+    _check(d == 128, "head_dim must be 128")
+    _check(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, "Hq must be a multiple of Hkv")
+    past = int(past)
+    _check(past >= 0 and past + T <= max_len, "past + T must fit the cache")
+    out = torch.empty((B, T, Hq * d), dtype=torch.float16, device=q.device)
+    if B == 0 or T == 0:
+        return out
+    workspace = _attention_workspace("flh_prefill_attention_weights", q, workspace, B, T, Hq)
+    _run("flh_prefill_attention_weights_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+         weights.data_ptr(), B, T, Hq, Hkv, d, past, max_len, float(scale if scale is not None else d ** -0.5),
+         workspace.data_ptr(), workspace.numel(), _stream(q))
+    return out
+
+
+def _check_weights(weights, shape, device):
+    _check(weights.is_cuda and weights.dtype == torch.float32 and weights.is_contiguous() and tuple(weights.shape) == shape
+           and weights.device == device, f"weights must be a contiguous float32 CUDA tensor {list(shape)}")
+
+
+def _cache_lists(k_caches, v_caches, device):
+    """The layers' caches as lists, and their common shape."""
+    ks, vs = ([c] if isinstance(c, torch.Tensor) else list(c) for c in (k_caches, v_caches))
+    _check(len(ks) > 0 and len(ks) == len(vs), "one key and one value cache per layer")
+    shape = ks[0].shape
+    _check(len(shape) == 4 and shape[1] > 0 and shape[2] > 0, "caches must be [B, Hkv, max_len, d]")
+    for t_ in ks + vs:
+        _check(t_.is_cuda and t_.dtype == torch.float16 and t_.is_contiguous() and t_.device == device and t_.shape == shape,
+               "caches must be contiguous float16 CUDA tensors of one shape on one device")
+    _check(shape[3] > 0 and shape[3] % 8 == 0 and shape[3] <= 512, "head_dim must be a multiple of 8, at most 512")
+    pointers = [(ctypes.c_void_p * len(ts))(*[t_.data_ptr() for t_ in ts]) for ts in (ks, vs)]
+    return pointers, len(ks), tuple(shape)
+
+
+def tree_commit_(tokens, parents, chosen, lengths, k_caches, v_caches):
+    """The end of a step over drafted tokens: tokens [B, T] int64 the drafted ones, parents [T] or [B, T] int64 each node's parent
+    (a lower index; node 0 is the root), chosen [B, T] int64 the token that the model picks behind each node, lengths [B] int64.
+    From node 0 on, the lowest child whose token is chosen[node] is accepted, until there is none.  In every layer's caches (a
+    tensor or a list of them, [B, Hkv, max_len, d]) the rows of the accepted nodes move from the slots lengths + path to lengths,
+    lengths + 1, ...  -> (path [B, T] int64, -1 behind the last; accepted [B]; next token [B]; new lengths [B]).  A sequence
+    whose length is negative or above max_len - T: nothing accepted or moved, next token -1, its length as it was."""
+    _check(tokens.dim() == 2, "tokens [B, T] expected")
+    B, T = tokens.shape
+    for t_ in (tokens, parents, chosen):
+        _check(t_.is_cuda and t_.dtype == torch.int64 and t_.is_contiguous() and t_.device == tokens.device,
+               "tokens, parents and chosen must be contiguous int64 CUDA tensors on one device")
+    _check(tuple(parents.shape) in ((T,), (B, T)) and chosen.shape == tokens.shape, "parents [T] or [B, T], chosen [B, T] expected")
+    _check(1 <= T <= 256, "1 to 256 nodes")
+    _check_lengths(lengths, B, tokens.device)
+    pointers, layers, shape = _cache_lists(k_caches, v_caches, tokens.device)
+    _check(shape[0] == B, "caches must be [B, Hkv, max_len, d]")
+    path = torch.empty_like(tokens)
+    accepted, following, new_lengths = (torch.empty_like(lengths) for _ in range(3))
+    if B:
+        _run("flh_tree_commit", tokens.device, tokens.data_ptr(), parents.data_ptr(), int(parents.dim() == 2), chosen.data_ptr(),
+             lengths.data_ptr(), path.data_ptr(), accepted.data_ptr(), following.data_ptr(), new_lengths.data_ptr(), layers, *pointers, B,
+             T, shape[1], shape[3], shape[2], _stream(tokens))
+    return path, accepted, following, new_lengths
+
+
+def evict_kv_cache_(k_caches, v_caches, weights, lengths, budget, recent):
+    """Cut every sequence of more than `budget` slots to that many: the last `recent` stay and of the others those with the
+    largest weights (equal ones: the lowest slot; NaN counts as largest), for every layer and key / value head by itself.  k_caches
+    / v_caches: a tensor or a list of them, [B, Hkv, max_len, d], compacted in place in the slots' order (rows behind the budget
+    stay as they were); weights float32 [layers, B, Hkv, max_len]; lengths [B] int64.  -> (kept [layers, B, Hkv, budget] int64,
+    -1 behind the last slot of a shorter sequence; the kept slots' weights, zeros behind, shaped as `weights`; the new lengths)."""
+    pointers, layers, shape = _cache_lists(k_caches, v_caches, weights.device)
+    B, Hkv, max_len, d = shape
+    _check_weights(weights, (layers, B, Hkv, max_len), weights.device)
+    _check_lengths(lengths, B, weights.device)
+    budget, recent = int(budget), int(recent)
+    _check(1 <= budget <= max_len and 0 <= recent <= budget, "the budget must be in 1 .. max_len, recent at most that")
+    kept = torch.empty((layers, B, Hkv, budget), dtype=torch.int64, device=weights.device)
+    new_weights, new_lengths = torch.empty_like(weights), torch.empty_like(lengths)
+    if B:
+        _run("flh_evict_kv_cache", weights.device, layers, *pointers, weights.data_ptr(), lengths.data_ptr(), kept.data_ptr(),
+             new_weights.data_ptr(), new_lengths.data_ptr(), B, Hkv, d, max_len, budget, recent, _stream(weights))
+    return kept, new_weights, new_lengths
+
+
 def _check_rows(x, width):
     _check(x.is_cuda, "Input tensor must be on CUDA")
     _check(x.dtype == torch.float16, "Input tensor must be float16 (half)")

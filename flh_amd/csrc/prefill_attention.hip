@@ -67,11 +67,14 @@ __device__ __forceinline__ void load_four_rows_to_lds(const v4i& d, unsigned vof
                "buffer_load_dwordx4 %1, %2, 0 offen offset:3072 lds" ::"s"(lds_base), "v"(voff), "s"(d) : "memory", "m0");
 }
 
+// STATS: every query's log2 of the sum of its exponentials is stored as well, [B, Hq, T] (a probability is exp2(scale_log2 * s - it)).
+template <bool STATS>
 __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(const __half* __restrict__ q,
                                                                    const __half* __restrict__ k_cache,
                                                                    const __half* __restrict__ v_cache,
                                                                    __half* __restrict__ out, int T, int Hq, int Hkv,
-                                                                   int past, int max_len, float scale_log2) {
+                                                                   int past, int max_len, float scale_log2,
+                                                                   float* __restrict__ stats) {
   extern __shared__ __align__(1024) uint8_t lds[];     // K[2], V[2] tiles; the output staging tile afterwards
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -268,6 +271,8 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(const __half*
   // ---- normalise, transpose through LDS, store whole rows
   const float l_all = l_run + lane_xor_f<32>(l_run);
   const float inv = 1.0f / l_all;
+  if constexpr (STATS)
+    if (h == 0 && q_first + n < T) stats[((size_t)b * Hq + head) * T + q_first + n] = m_run + __builtin_amdgcn_logf(l_all);
   __syncthreads();                                     // every wave is done with the tiles
   uint8_t* stage = lds + wave * (32 * kOutPitch);
 #pragma unroll
@@ -293,13 +298,9 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(const __half*
 
 }  // namespace
 
-}  // namespace flh
-
-using namespace flh;
-
-extern "C" int flh_prefill_attention_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, flh_half* out,
-                                         uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t past,
-                                         uint32_t max_len, float scale, void* stream) {
+// `stats` (may be null): see the kernel
+int prefill_attention(const __half* q, const __half* k_cache, const __half* v_cache, __half* out, float* stats, uint32_t B, uint32_t T,
+                      uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t past, uint32_t max_len, float scale, hipStream_t stream) {
   if (!q || !k_cache || !v_cache || !out) return fail(FLH_EINVAL, "prefill_attention: null pointer");
   if (misaligned16(q, k_cache, v_cache, out)) return fail(FLH_EINVAL, "prefill_attention: tensors must be 16-byte aligned");
   if (head_dim != kHeadDim) return fail(FLH_EINVAL, "prefill_attention: head_dim (%u) must be 128", head_dim);
@@ -312,11 +313,24 @@ extern "C" int flh_prefill_attention_f16(const flh_half* q, const flh_half* k_ca
   if (!(scale > 0.f)) return fail(FLH_EINVAL, "prefill_attention: the scale must be positive");
   const size_t smem = 4 * (size_t)kTileBytes;          // 64 KiB: two workgroups per compute unit
   static_assert(4 * 32 * kOutPitch <= 4 * kTileBytes, "the output staging tiles reuse the K / V buffers");
-  static LdsGrant grant;
-  if (int rc = reserve_lds((const void*)prefill_attention_kernel, smem, grant, "prefill_attention")) return rc;
   const unsigned blocks = (T + kQueriesPerBlock - 1) / kQueriesPerBlock;
-  hipLaunchKernelGGL(prefill_attention_kernel, dim3(blocks * Hq * B), dim3(256), smem, (hipStream_t)stream, (const __half*)q,
-                     (const __half*)k_cache, (const __half*)v_cache, (__half*)out, (int)T, (int)Hq, (int)Hkv, (int)past,
-                     (int)max_len, scale * 1.4426950408889634f);
-  return check_launch("prefill_attention");
+  auto go = [&](auto kern, LdsGrant& grant) {
+    if (int rc = reserve_lds((const void*)kern, smem, grant, "prefill_attention")) return rc;
+    hipLaunchKernelGGL(kern, dim3(blocks * Hq * B), dim3(256), smem, stream, q, k_cache, v_cache, out, (int)T, (int)Hq, (int)Hkv, (int)past,
+                       (int)max_len, scale * 1.4426950408889634f, stats);
+    return check_launch("prefill_attention");
+  };
+  static LdsGrant plain, with_stats;
+  return stats ? go(prefill_attention_kernel<true>, with_stats) : go(prefill_attention_kernel<false>, plain);
+}
+
+}  // namespace flh
+
+using namespace flh;
+
+extern "C" int flh_prefill_attention_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, flh_half* out,
+                                         uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t past,
+                                         uint32_t max_len, float scale, void* stream) {
+  return prefill_attention((const __half*)q, (const __half*)k_cache, (const __half*)v_cache, (__half*)out, nullptr, B, T, Hq, Hkv, head_dim,
+                           past, max_len, scale, (hipStream_t)stream);
 }

@@ -443,6 +443,65 @@ int flh_decode_attention_f16_static(const flh_half* q, const flh_half* k_cache, 
                                     uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t kv_len,
                                     uint32_t max_len, float scale, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Caches whose sequences have lengths of their own.  `lengths` [B] int64 ON THE DEVICE holds how many slots of each sequence are
+ * taken: one recorded launch serves every length.  No counterpart in the reference (its caches grow by one common length).
+ *
+ * Attention of a tree of T <= 256 drafted tokens (nodes) per sequence, the verification step of speculative decoding: node i of
+ * sequence b takes slot lengths[b] + i, and sees the lengths[b] slots in front of the tree and the nodes j with
+ * mask[b][i][j] != 0.  The rotary embedding and the cache write are inside:
+ *   q [B, T, Hq, d], k_new / v_new [B, T, Hkv, d] fp16 as projected, not rotated (left as they are);  cos, sin [B, T, d] the rotary rows
+ *   of the nodes' positions;  mask uint8 [T, T] (mask_per_sequence 0) or [B, T, T];  k_cache, v_cache [B, Hkv, max_len, d];
+ *   out [B, T, Hq * d] fp16.  Hq a multiple of Hkv, d 64 or 128.
+ * The rotation x cos + rotate_half(x) sin is computed in float32 and rounded once; softmax statistics and sums in float32,
+ * probabilities rounded to fp16 for the second product.  A node that sees nothing gets zeros.  A sequence whose length is negative
+ * or above max_len - T takes no part: zeros as output, its cache untouched.  What a query does not see may hold anything, except
+ * that the values v_new of the tree itself must be finite.
+ * workspace: 16-byte aligned, flh_tree_attention_workspace_bytes(...) bytes, contents irrelevant; launches that share one must not
+ * overlap. */
+size_t flh_tree_attention_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim);
+int flh_tree_attention_f16(const flh_half* q, const flh_half* k_new, const flh_half* v_new, const flh_half* cos, const flh_half* sin,
+                           const int64_t* lengths, const uint8_t* mask, int mask_per_sequence, flh_half* k_cache, flh_half* v_cache,
+                           flh_half* out, uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len,
+                           float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The end of that step.  tokens [B, T] int64 the drafted tokens, parents int64 [T] or [B, T] (parents_per_sequence) each node's parent
+ * (a lower index; node 0 is the root, the last token that was certain), chosen [B, T] int64 the token that the model picks behind
+ * each node.  From node 0 on, the lowest child whose token is chosen[node] is accepted, until there is none:
+ *   path [B, T] int64 the accepted nodes in order, -1 behind them;  accepted [B] their number;  next [B] chosen[last node];
+ *   new_lengths [B] = lengths + accepted (memory of its own),
+ * and in every layer's caches [B, Hkv, max_len, head_dim] the rows of slots lengths + path[i] move to lengths + i; all other rows stay.  A
+ * sequence whose length is negative or above max_len - T: nothing accepted or moved, next -1, its length as it was. */
+int flh_tree_commit(const int64_t* tokens, const int64_t* parents, int parents_per_sequence, const int64_t* chosen,
+                    const int64_t* lengths, int64_t* path, int64_t* accepted, int64_t* next, int64_t* new_lengths, int layers,
+                    flh_half* const* k_caches, flh_half* const* v_caches, uint32_t B, uint32_t T, uint32_t Hkv, uint32_t head_dim,
+                    uint32_t max_len, void* stream);
+
+/* Attention that also adds up how much each cache slot is looked at:
+ *   weights[b, g, j] += sum of the probabilities of slot j over the queries of key / value head g,  float32 [B, Hkv, max_len].
+ * decode: one query per sequence, q, out [B, Hq, d], over the slots 0 .. lengths[b] - 1 (the new token's key and value among them; a
+ * length of zero, a negative one or one above max_len: zeros, no weights); d 64 or 128.  prefill: flh_prefill_attention_f16 (d = 128, the
+ * same output bits), each query over the slots it sees.  Sums are taken in a fixed order: the same call gives the same bits. */
+size_t flh_decode_attention_weights_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len);
+int flh_decode_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, const int64_t* lengths,
+                                     flh_half* out, float* weights, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
+                                     uint32_t max_len, float scale, void* workspace, size_t workspace_bytes, void* stream);
+size_t flh_prefill_attention_weights_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq);
+int flh_prefill_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, flh_half* out, float* weights,
+                                      uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t past,
+                                      uint32_t max_len, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction: of every sequence with more than `budget` slots, the last `recent` slots stay and of the others the budget - recent with
+ * the largest weights (equal ones: the lowest slot; NaN counts as largest), for every layer and key / value head by itself.  The rows
+ * that stay move to the slots 0 .. budget - 1 in their order; rows behind are left as they were.
+ *   weights [layers, B, Hkv, max_len] float32 (as the calls above add them up);  kept [layers, B, Hkv, budget] int64 the slots that stay
+ *   (-1 behind the last of a shorter sequence);  new_weights [layers, B, Hkv, max_len] their weights, zeros behind;
+ *   new_lengths [B] = min(lengths, budget) (a length that is negative or above max_len stays, nothing kept).
+ * new_weights and new_lengths need memory of their own. */
+int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_half* const* v_caches, const float* weights, const int64_t* lengths,
+                       int64_t* kept, float* new_weights, int64_t* new_lengths, uint32_t B, uint32_t Hkv, uint32_t head_dim,
+                       uint32_t max_len, uint32_t budget, uint32_t recent, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
