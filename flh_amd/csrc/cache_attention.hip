@@ -7,8 +7,6 @@
 //
 //   out[r] = sum_j p[r, j] V[j],  p[r, j] = exp(s[r, j] - m[r]) / l[r],  s = scale q[r] . K[j],  m = max_j s,  l = sum_j exp(s - m)
 //   weights[j] += sum_r p[r, j]
-//
-// A wave per query: 64 keys at a time, a lane scores one of them, then holds two channels of the output.
 #include "lane_ops.h"
 
 namespace flh {
@@ -19,115 +17,465 @@ int prefill_attention(const __half* q, const __half* k_cache, const __half* v_ca
 
 namespace {
 
-// The drafted keys (rotated in float32, rounded once) and values into their slots: one lane per pair of channels d / 2 apart.
-__global__ __launch_bounds__(256) void tree_write_kernel(const __half* __restrict__ k, const __half* __restrict__ v,
-                                                         const __half* __restrict__ cos, const __half* __restrict__ sin,
-                                                         const long long* __restrict__ lengths, __half* __restrict__ k_cache,
-                                                         __half* __restrict__ v_cache, uint32_t B, uint32_t T, uint32_t Hkv, uint32_t d,
-                                                         uint32_t max_len) {
-  const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  const uint32_t half = d / 2, c = (uint32_t)(at % half);
-  const uint64_t item = at / half;                     // (b, t, head)
-  if (item >= (uint64_t)B * T * Hkv) return;
-  const uint32_t head = (uint32_t)(item % Hkv), token = (uint32_t)(item / Hkv), b = token / T, t = token % T;
-  const long long n = lengths[b];
-  if (n < 0 || n + T > max_len) return;
-  const _Float16 *kn = (const _Float16*)k + item * d, *vn = (const _Float16*)v + item * d;
-  const _Float16 *cf = (const _Float16*)cos + (size_t)token * d, *sf = (const _Float16*)sin + (size_t)token * d;
-  const size_t to = (((size_t)b * Hkv + head) * max_len + (size_t)n + t) * d;
-  const float x0 = kn[c], x1 = kn[c + half];
-  ((_Float16*)k_cache)[to + c] = (_Float16)round_here(x0 * (float)cf[c] - x1 * (float)sf[c]);
-  ((_Float16*)k_cache)[to + c + half] = (_Float16)round_here(x1 * (float)cf[c + half] + x0 * (float)sf[c + half]);
-  ((_Float16*)v_cache)[to + c] = vn[c];
-  ((_Float16*)v_cache)[to + c + half] = vn[c + half];
-}
+constexpr uint32_t kMaxNodes = 256;
+constexpr float kLowest = -1e30f;                      // running maximum of a query that has seen nothing yet: finite, so that
+                                                       // differences from it are no NaN; scores stay far above it
 
-// what a query sees: the slots below `before`, and of the T behind them those that its row of the mask (if there is one) names
-struct Seen {
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+// What the kernels of one call share
+struct Call {
+  const __half *q, *k_new, *v_new, *cos, *sin;         // k_new .. sin, mask: trees only
+  const long long* lengths;
   const uint8_t* mask;
-  uint32_t before, T;
-  __device__ bool operator()(uint32_t j) const { return j < before || (mask && j - before < T && mask[j - before]); }
+  __half *k_cache, *v_cache, *out;
+  float *partials, *scores, *weights;                  // scores, weights: attention weights only
+  uint32_t mask_stride, B, T, Hq, Hkv, rep, rows, row_blocks, max_len, score_pitch, groups, least;
+  float scale_log2;
 };
 
-template <int D>
-__device__ __forceinline__ float score(const float* q, const __half* key, float scale) {
-  float s = 0.f;
-#pragma unroll
-  for (int c = 0; c < D; c += 8) {
-    const h8 x = *(const h8*)(key + c);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = __builtin_fmaf(q[c + e], (float)x[e], s);
-  }
-  return s * scale;
+// The work of a call is one list of tiles of KT keys: for every sequence, every key / value head and every block of 32 WR query rows, the
+// tiles of the cache and then those of the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more
+// than the rounding of c, however the lengths differ, and nothing of it has to be known on the host.
+struct Plan {
+  uint32_t c, total;                                   // tiles of a workgroup, of all
+};
+
+template <int KT, bool TREE>
+__device__ __forceinline__ uint32_t tiles_of(const Call& a, uint32_t b) {
+  if (b >= a.B) return 0;
+  const long long n = a.lengths[b];
+  if (TREE) return n < 0 || n + a.T > a.max_len ? 0 : ((uint32_t)n + KT - 1) / KT + (a.T + KT - 1) / KT;
+  return n <= 0 || n > a.max_len ? 0 : ((uint32_t)n + KT - 1) / KT;
 }
 
-// One wave per query (b, t, h).  With cos / sin the query is rotated first.  stats (may be null): [B, Hq, T] log2 of
-// the sum of exponentials.
+__device__ __forceinline__ uint32_t scan_up(uint32_t v) {   // inclusive sums over the wave's lanes
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t x = __shfl_up(v, d);
+    v += lane >= d ? x : 0;
+  }
+  return v;
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+template <int KT, bool TREE>
+__device__ __forceinline__ Plan plan_of(const Call& a) {
+  const int lane = threadIdx.x & 63;
+  uint32_t tiles = 0;
+  for (uint32_t b0 = 0; b0 < a.B; b0 += 64) tiles += (uint32_t)__shfl(scan_up(tiles_of<KT, TREE>(a, b0 + lane)), 63);
+  const uint32_t total = uniform(tiles) * (a.Hkv * a.row_blocks);
+  return {max(a.least, (total + a.groups - 1) / a.groups), total};
+}
+
+// tiles (over all heads and row blocks) in front of sequence `of`, or of the sequence that holds tile `of` (of_tile) and that sequence
+struct Place {
+  uint32_t b, before, tiles;
+};
+template <int KT, bool TREE>
+__device__ __forceinline__ Place place_of(const Call& a, uint32_t of, bool of_tile) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t per = a.Hkv * a.row_blocks;
+  uint32_t before = 0;
+  for (uint32_t b0 = 0;; b0 += 64) {
+    const uint32_t mine = tiles_of<KT, TREE>(a, b0 + lane) * per, up = scan_up(mine);
+    const unsigned long long hit = __ballot(of_tile ? before + up > of : b0 + lane == of);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      return {uniform(b0 + l), uniform(before + (uint32_t)__shfl(up - mine, l)), uniform((uint32_t)__shfl(mine, l) / per)};
+    }
+    before += (uint32_t)__shfl(up, 63);
+    if (b0 + 64 >= a.B) return {a.B, before, 0};       // (not reached: the tile is in the list, the sequence below B)
+  }
+}
+
+// floats of one piece of partial results: 32 WR rows of D sums, their maxima and sums
+template <int D, int WR>
+constexpr uint32_t kPiece = 32 * WR * (D + 2);
+
+// 1 KiB: lane i's 16 bytes at voff go to lds_base + 16 i
+__device__ __forceinline__ void load_rows_to_lds(const v4i& d, unsigned voff, unsigned lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_base), "v"(voff), "s"(d) : "memory", "m0");
+}
+
+// Rows of D channels in LDS, 16-byte chunks XOR-swizzled by the row: K so that the 16 rows of a fragment read fall into different
+// bank groups, V so that the four rows of a transpose load (64 bytes of each) do.
 template <int D>
-__global__ __launch_bounds__(64) void query_attention_kernel(const __half* __restrict__ q, const __half* __restrict__ cos,
-                                                             const __half* __restrict__ sin, const __half* __restrict__ k_cache,
-                                                             const __half* __restrict__ v_cache, const long long* __restrict__ lengths,
-                                                             const uint8_t* __restrict__ mask, uint32_t mask_stride, __half* __restrict__ out,
-                                                             float* __restrict__ stats, uint32_t T, uint32_t Hq, uint32_t Hkv,
-                                                             uint32_t max_len, float scale) {
-  __shared__ float qs[D], ps[64];
-  const int lane = threadIdx.x;
-  const uint32_t item = blockIdx.x, h = item % Hq, token = item / Hq, b = token / T, t = token % T;
-  const _Float16* row = (const _Float16*)q + (size_t)item * D;
-  for (int c = lane; c < D; c += 64) {
-    float x = row[c];
-    if (cos) {
-      const float other = row[c ^ (D / 2)];
-      const float cf = ((const _Float16*)cos)[(size_t)token * D + c], sf = ((const _Float16*)sin)[(size_t)token * D + c];
-      x = c < D / 2 ? x * cf - other * sf : x * cf + other * sf;
-    }
-    qs[c] = x;
+struct Tile {
+  static constexpr int PITCH = D * 2, CHUNKS = D / 8;
+  static __device__ __forceinline__ int k_swizzle(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+  static __device__ __forceinline__ int v_swizzle(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+  static __device__ __forceinline__ int k_at(int r, int c) { return r * PITCH + ((c ^ k_swizzle(r)) << 4); }
+  static __device__ __forceinline__ int v_at(int r, int c) { return r * PITCH + ((c ^ v_swizzle(r)) << 4); }
+};
+
+// (x0, x1): eight channels and their partners half a head further; the rotary embedding in float32, rounded once
+__device__ __forceinline__ void rotate8(h8& x0, h8& x1, const __half* cos, const __half* sin, int c, int half) {
+  const h8 c0 = *(const h8*)(cos + c), c1 = *(const h8*)(cos + c + half), s0 = *(const h8*)(sin + c), s1 = *(const h8*)(sin + c + half);
+  const h8 a = x0, b = x1;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x0[e] = (_Float16)round_here((float)a[e] * (float)c0[e] - (float)b[e] * (float)s0[e]);
+    x1[e] = (_Float16)round_here((float)b[e] * (float)c1[e] + (float)a[e] * (float)s1[e]);
   }
-  __syncthreads();
-  // the length: of the cache in front of a tree, or all of it
-  uint32_t n = 0, end = 0;
-  if (const long long all = lengths[b]; all >= 0 && all + (mask ? T : 0) <= max_len) n = (uint32_t)all, end = n + (mask ? T : 0);
-  const Seen seen{mask ? mask + (size_t)b * mask_stride + (size_t)t * T : nullptr, n, mask && end ? T : 0};
-  const size_t base = ((size_t)b * Hkv + h / (Hq / Hkv)) * max_len * D;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (uint32_t j0 = 0; j0 < end; j0 += 64) {
-    const uint32_t j = j0 + lane;
-    const float s = j < end && seen(j) ? score<D>(qs, k_cache + base + (size_t)j * D, scale) : -INFINITY;
-    const float m_new = fmaxf(m, wave_max(s));
-    const float safe = m_new == -INFINITY ? 0.f : m_new;
-    const float p = __expf(s - safe), keep = __expf(m - safe);
-    l = l * keep + wave_sum(p);
-    o0 *= keep, o1 *= keep;
-    m = m_new;
-    ps[lane] = p;
-    __syncthreads();
-    for (uint32_t i = 0; i < 64 && j0 + i < end; ++i) {
-      const float w = ps[i];
-      if (w == 0.f) continue;                          // (what a query does not see adds nothing, whatever it holds)
-      const _Float16* v = (const _Float16*)v_cache + base + (size_t)(j0 + i) * D;
-      o0 = __builtin_fmaf(w, (float)v[lane], o0);
-      if constexpr (D == 128) o1 = __builtin_fmaf(w, (float)v[lane + 64], o1);
-    }
-    __syncthreads();
+}
+
+// The four waves of a workgroup are WR groups of 32 query rows (the queries of a key / value head: row t rep + i is head i of token t) times
+// WK = 4 / WR groups of the tile's keys.  Both products run transposed, so that a lane owns one query:
+//   S^T[key, query] = K Q^T (A: rows of K from LDS, B: the queries in registers),  O^T[d, query] += V^T P^T (A: transpose loads of V, B: P
+//   as it sits in the scores' accumulators),  v_mfma_f32_32x32x16_f16, softmax in base 2 with float32 statistics per lane, probabilities
+//   rounded to fp16 for the second product.
+// K and V of the cache come by direct-to-LDS loads, the next tile during the present one.  The tree's own tiles are staged by hand:
+// the keys have to be rotated, and go to the cache as well.
+template <int D, int WR, bool TREE>
+__global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attention_kernel(const Call a) {
+  constexpr int WK = 4 / WR, NKT = WR == 4 ? 2 : 1, KT = 32 * NKT * WK;
+  constexpr int PITCH = D * 2, TILE = KT * PITCH, NI = TILE / 4096, RPI = 1024 / PITCH;   // loads of a wave per tile, rows of one load
+  constexpr int KS = D / 16, DT = D / 32;
+  using L = Tile<D>;
+  extern __shared__ __align__(1024) uint8_t lds[];     // K[2], V[2]; the waves' sums at the end of a segment
+  __shared__ float s_m[4][32], s_l[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / WK, wk = wave % WK;
+  const unsigned lds0 = (unsigned)(size_t)lds;
+
+  const uint32_t per = a.Hkv * a.row_blocks;
+  const Plan plan = plan_of<KT, TREE>(a);
+  const uint32_t g = xcd_contiguous(blockIdx.x, gridDim.x);
+  uint32_t pos = g * plan.c;
+  const uint32_t end = min(pos + plan.c, plan.total);
+  if (g >= (plan.total + plan.c - 1) / plan.c) return;
+  const Place at = place_of<KT, TREE>(a, pos, true);
+  uint32_t b = at.b, tiles = at.tiles, unit = (pos - at.before) / tiles, tile = (pos - at.before) % tiles;
+
+  // addresses inside a tile
+  unsigned k_off[NI], v_off[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int r = (wave * NI + i) * RPI + lane / L::CHUNKS, c = lane % L::CHUNKS;
+    k_off[i] = r * PITCH + ((c ^ L::k_swizzle(r)) << 4);
+    v_off[i] = r * PITCH + ((c ^ L::v_swizzle(r)) << 4);
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  _Float16* to = (_Float16*)out + (size_t)item * D;
-  to[lane] = (_Float16)(o0 * inv);
-  if constexpr (D == 128) to[lane + 64] = (_Float16)(o1 * inv);
-  if (stats && lane == 0) stats[((size_t)b * Hq + h) * T + t] = m * 1.4426950408889634f + __builtin_amdgcn_logf(l);
+  const int k_at = L::k_at(wk * NKT * 32 + n, h);      // + 32 PITCH per 32 keys; step s of 16 channels enters by XOR
+  // transpose loads: lane i of 16 addresses the 8-byte piece i % 4 of the 32-byte run of channels that its group will own, in row i / 4
+  const int grp = lane >> 4, gi = lane & 15;
+  int tr_off[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    tr_off[dt] = L::v_at(wk * NKT * 32 + 4 * (grp >> 1) + (gi >> 2), 4 * dt + ((grp & 1) << 1) + ((gi & 3) >> 1)) + ((gi & 1) << 3);
+
+  for (;;) {
+    // ---- one segment: tiles [tile, last) of this unit
+    const uint32_t last = min(tiles, tile + (end - pos));
+    const uint32_t head = unit / a.row_blocks, block = unit % a.row_blocks;
+    const uint32_t length = (uint32_t)a.lengths[b];
+    const uint32_t cached = (length + KT - 1) / KT;    // tiles of the cache
+    const size_t cache = ((size_t)b * a.Hkv + head) * a.max_len * D;
+    auto issue = [&](uint32_t t, int buf) {
+      const unsigned bytes = uniform(min((uint32_t)KT, length - t * KT)) * PITCH;   // (rows past the length arrive as zeros)
+      const v4i dk = buffer_of((const uint8_t*)(a.k_cache + cache + (size_t)t * KT * D), bytes);
+      const v4i dv = buffer_of((const uint8_t*)(a.v_cache + cache + (size_t)t * KT * D), bytes);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) load_rows_to_lds(dk, k_off[i], lds0 + buf * TILE + (wave * NI + i) * 1024);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) load_rows_to_lds(dv, v_off[i], lds0 + (2 + buf) * TILE + (wave * NI + i) * 1024);
+    };
+    const uint32_t cached_last = min(last, cached);
+    if (tile < cached_last) issue(tile, 0);
+
+    // this lane's query as B operand: channels 16 s + 8 h .. + 7 (rows past the last repeat it; they are not used)
+    const uint32_t row = min((block * WR + wr) * 32 + n, a.rows - 1), token = row / a.rep;
+    h8 qf[KS];
+    {
+      const size_t at_token = (size_t)b * a.T + token;
+      const __half* src = a.q + (at_token * a.Hq + head * a.rep + row % a.rep) * D + 8 * h;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qf[s] = *(const h8*)(src + 16 * s);
+      if constexpr (TREE) {
+#pragma unroll
+        for (int s = 0; s < KS / 2; ++s)
+          rotate8(qf[s], qf[s + KS / 2], a.cos + at_token * D, a.sin + at_token * D, 16 * s + 8 * h, D / 2);
+      }
+    }
+
+    v16f o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+    float m_run = kLowest, l_run = 0.f;                // running maximum (scaled, base 2) and this lane's share of the sum
+
+    // register r of 32-key tile kt: key key0 + 32 kt + 8 (r / 4) + r % 4 of the tile
+    const uint32_t key0 = wk * NKT * 32 + 4 * h;
+    auto compute = [&](int buf, uint32_t t, bool masked) {
+      v16f st[NKT];
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[kt][r] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const h8 kf = *(const h8*)(lds + buf * TILE + kt * 32 * PITCH + (k_at ^ (s << 5)));
+          st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], st[kt], 0, 0, 0);
+        }
+      }
+      if (masked) {                                    // a tile of the tree, or the last of the cache
+        if (TREE && t >= cached) {
+          const uint8_t* seen = a.mask + (size_t)b * a.mask_stride + (size_t)token * a.T;
+#pragma unroll
+          for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const uint32_t j = (t - cached) * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3);
+              if (!(j < a.T && seen[min(j, a.T - 1)])) st[kt][r] = -INFINITY;
+            }
+        } else {
+#pragma unroll
+          for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (t * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3) >= length) st[kt][r] = -INFINITY;
+        }
+      }
+      if constexpr (!TREE) {                           // scores for the weights' launch
+        if ((block * WR + wr) * 32 + n < a.rows) {
+          float* to = a.scores + ((size_t)b * a.Hq + head * a.rep + row) * a.score_pitch;
+#pragma unroll
+          for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              const uint32_t j = t * KT + key0 + 32 * kt + 8 * q4;
+              const v4f x = {st[kt][4 * q4] * a.scale_log2, st[kt][4 * q4 + 1] * a.scale_log2, st[kt][4 * q4 + 2] * a.scale_log2,
+                             st[kt][4 * q4 + 3] * a.scale_log2};
+              if (j < length) *(v4f*)(to + j) = x;
+            }
+        }
+      }
+      float top = st[0][0];
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, st[kt][r]);
+      const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_int(top), __float_as_int(top), false, false);
+      top = fmaxf(__int_as_float(halves[0]), __int_as_float(halves[1])) * a.scale_log2;
+      const float m_new = fmaxf(m_run, top);
+      if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+        m_run = m_new;
+      }
+      float sum = 0.f;
+      h8 pb[NKT][2];
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][r], a.scale_log2, -m_run));
+          sum += p;
+          pb[kt][r >> 3][r & 7] = (_Float16)p;
+        }
+      l_run += sum;
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const uint8_t* v = lds + (2 + buf) * TILE + tr_off[dt] + (2 * kt + ks) * (16 * PITCH);
+            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)v);
+            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(v + 8 * PITCH));
+            const h8 vf = __builtin_bit_cast(h8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[kt][ks], o[dt], 0, 0, 0);
+          }
+    };
+
+    int buf = 0;
+    for (uint32_t t = tile; t < cached_last; ++t, buf ^= 1) {
+      wait_vmcnt<0>();
+      __syncthreads();                                 // this tile has landed, and everybody has read the one before it
+      if (t + 1 < cached_last) issue(t + 1, buf ^ 1);
+      compute(buf, t, (t + 1) * KT > length);
+    }
+    if constexpr (TREE) {
+      for (uint32_t t = max(tile, cached); t < last; ++t) {
+        __syncthreads();                               // (the buffers have been read)
+        constexpr int PAIRS = L::CHUNKS / 2;
+        for (uint32_t i = tid; i < KT * PAIRS; i += 256) {
+          const uint32_t r = i / PAIRS, c = i % PAIRS, j = (t - cached) * KT + r;
+          h8 k0 = {}, k1 = {}, v0 = {}, v1 = {};
+          if (j < a.T) {
+            const size_t at_token = (size_t)b * a.T + j, src = (at_token * a.Hkv + head) * D + 8 * c;
+            k0 = *(const h8*)(a.k_new + src), k1 = *(const h8*)(a.k_new + src + D / 2);
+            v0 = *(const h8*)(a.v_new + src), v1 = *(const h8*)(a.v_new + src + D / 2);
+            rotate8(k0, k1, a.cos + at_token * D, a.sin + at_token * D, 8 * c, D / 2);
+            if (block == 0) {
+              const size_t to = cache + ((size_t)length + j) * D + 8 * c;
+              *(h8*)(a.k_cache + to) = k0, *(h8*)(a.k_cache + to + D / 2) = k1;
+              *(h8*)(a.v_cache + to) = v0, *(h8*)(a.v_cache + to + D / 2) = v1;
+            }
+          }
+          *(h8*)(lds + L::k_at(r, c)) = k0, *(h8*)(lds + L::k_at(r, c + PAIRS)) = k1;
+          *(h8*)(lds + 2 * TILE + L::v_at(r, c)) = v0, *(h8*)(lds + 2 * TILE + L::v_at(r, c + PAIRS)) = v1;
+        }
+        __syncthreads();
+        compute(0, t, true);
+      }
+    }
+
+    // ---- the waves that share rows meet, then the segment's piece goes out: [row group][register quad][lane], maxima and sums behind
+    float l_all = l_run + lane_xor_f<32>(l_run);
+    float* piece = a.partials + (size_t)(g + b * per + unit) * kPiece<D, WR>;
+    __syncthreads();
+    if constexpr (WK > 1) {
+      if (h == 0) s_m[wave][n] = m_run, s_l[wave][n] = l_all;
+      __syncthreads();
+      float m_all = s_m[wr * WK][n];
+#pragma unroll
+      for (int k = 1; k < WK; ++k) m_all = fmaxf(m_all, s_m[wr * WK + k][n]);
+      l_all = 0.f;
+#pragma unroll
+      for (int k = 0; k < WK; ++k) l_all += s_l[wr * WK + k][n] * __builtin_amdgcn_exp2f(s_m[wr * WK + k][n] - m_all);
+      const float mine = __builtin_amdgcn_exp2f(m_run - m_all);
+      v4f* all = (v4f*)lds;                            // [wave][quad][lane]
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          all[(wave * DT * 4 + dt * 4 + q4) * 64 + lane] =
+              v4f{o[dt][4 * q4] * mine, o[dt][4 * q4 + 1] * mine, o[dt][4 * q4 + 2] * mine, o[dt][4 * q4 + 3] * mine};
+      __syncthreads();
+      constexpr int QUADS = DT * 4 / WK;               // of this wave
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) {
+        const int quad = wk * QUADS + i;
+        v4f x = all[(wr * WK * DT * 4 + quad) * 64 + lane];
+#pragma unroll
+        for (int k = 1; k < WK; ++k) x += all[((wr * WK + k) * DT * 4 + quad) * 64 + lane];
+        ((v4f*)piece)[(wr * DT * 4 + quad) * 64 + lane] = x;
+      }
+      m_run = m_all;
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          ((v4f*)piece)[(wr * DT * 4 + dt * 4 + q4) * 64 + lane] = v4f{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
+    }
+    if (wk == 0 && h == 0) ((v2f*)(piece + 32 * WR * D))[wr * 32 + n] = v2f{m_run, l_all};
+
+    // ---- the next unit
+    pos += last - tile;
+    if (pos >= end) return;
+    tile = 0;
+    if (++unit == per) {
+      unit = 0;
+      do {
+        ++b;
+        tiles = uniform(tiles_of<KT, TREE>(a, b));
+      } while (tiles == 0 && b + 1 < a.B);
+      if (tiles == 0) return;                          // (not reached: there are tiles left)
+    }
+    __syncthreads();                                   // the sums have been read: the buffers are free
+  }
+}
+
+// The segments of a unit: workgroups first .. last of the first launch
+struct Segments {
+  uint32_t first, count;                               // pieces first .. first + count - 1
+};
+template <int KT, bool TREE>
+__device__ __forceinline__ Segments segments_of(const Call& a, const Plan& plan, const Place& at, uint32_t unit) {
+  if (at.tiles == 0) return {0, 0};
+  const uint32_t from = at.before + unit * at.tiles, first = from / plan.c, last = (from + at.tiles - 1) / plan.c;
+  return {first + at.b * (a.Hkv * a.row_blocks) + unit, last - first + 1};   // (piece g + unit: either grows from one piece to the next)
+}
+
+// Workgroup (b, unit, row group, 32 channels): the pieces' sums weighted and added, out as fp16.  For attention weights, workgroups
+// behind those: (b, head, 256 slots), the stored scores -> probabilities, summed over the rows, added to the weights.
+template <int D, int WR, bool TREE>
+__global__ __launch_bounds__(256) void cache_combine_kernel(const Call a) {
+  constexpr int WK = 4 / WR, NKT = WR == 4 ? 2 : 1, KT = 32 * NKT * WK, DT = D / 32;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t per = a.Hkv * a.row_blocks, outs = a.B * per * WR * DT;
+  const Plan plan = plan_of<KT, TREE>(a);
+  if (blockIdx.x < outs) {
+    const uint32_t dt = blockIdx.x % DT, wr = blockIdx.x / DT % WR, bu = blockIdx.x / (DT * WR), unit = bu % per;
+    const uint32_t head = unit / a.row_blocks, row = ((unit % a.row_blocks) * WR + wr) * 32 + n;
+    const Place at = place_of<KT, TREE>(a, bu / per, false);
+    const Segments seg = segments_of<KT, TREE>(a, plan, at, unit);
+    const float* piece = a.partials + (size_t)seg.first * kPiece<D, WR>;
+    const uint32_t of_row = 32 * WR * D + (wr * 32 + n) * 2, of_sum = ((wr * DT * 4 + dt * 4 + wave) * 64 + lane) * 4;
+    float m = kLowest;
+    for (uint32_t i = 0; i < seg.count; ++i) m = fmaxf(m, piece[(size_t)i * kPiece<D, WR> + of_row]);
+    float l = 0.f;
+    v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t i = 0; i < seg.count; ++i) {
+      const float* p = piece + (size_t)i * kPiece<D, WR>;
+      const v2f ml = *(const v2f*)(p + of_row);
+      const float w = __builtin_amdgcn_exp2f(ml[0] - m);
+      l = __builtin_fmaf(w, ml[1], l);
+      x += *(const v4f*)(p + of_sum) * w;
+    }
+    if (row < a.rows) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;       // (a query that sees nothing: zeros)
+      const h4 y = {(_Float16)(x[0] * inv), (_Float16)(x[1] * inv), (_Float16)(x[2] * inv), (_Float16)(x[3] * inv)};
+      __half* to = a.out + (((size_t)(bu / per) * a.T + row / a.rep) * a.Hq + head * a.rep + row % a.rep) * D;
+      *(h4*)(to + 32 * dt + 8 * wave + 4 * h) = y;
+    }
+    return;
+  }
+  if constexpr (!TREE) {
+    __shared__ v2f stats[64];
+    const uint32_t blocks = (a.max_len + 255) / 256, bg = (blockIdx.x - outs) / blocks, j = (blockIdx.x - outs) % blocks * 256 + tid;
+    const uint32_t b = bg / a.Hkv, head = bg % a.Hkv;
+    const Place at = place_of<KT, TREE>(a, b, false);
+    const long long length = a.lengths[b];
+    if (at.tiles == 0 || (long long)(j - tid) >= length) return;
+    float sum = 0.f;
+    for (uint32_t r0 = 0; r0 < a.rows; r0 += 64) {
+      __syncthreads();
+      // a wave takes every fourth row, a lane of it every 64th segment
+      for (uint32_t r = r0 + wave; r < min(a.rows, r0 + 64); r += 4) {
+        const Segments seg = segments_of<KT, TREE>(a, plan, at, head * a.row_blocks + r / (32 * WR));
+        const float* piece = a.partials + (size_t)seg.first * kPiece<D, WR> + 32 * WR * D + r % (32 * WR) * 2;
+        float m = kLowest, l = 0.f;
+        for (uint32_t i = lane; i < seg.count; i += 64) m = fmaxf(m, piece[(size_t)i * kPiece<D, WR>]);
+        m = wave_max(m);
+        for (uint32_t i = lane; i < seg.count; i += 64) {
+          const v2f ml = *(const v2f*)(piece + (size_t)i * kPiece<D, WR>);
+          l = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[0] - m), ml[1], l);
+        }
+        l = wave_sum(l);
+        if (lane == 0) stats[r - r0] = v2f{m, l > 0.f ? 1.f / l : 0.f};
+      }
+      __syncthreads();
+      if (j < length) {
+        const float* s = a.scores + ((size_t)b * a.Hq + head * a.rep + r0) * a.score_pitch + j;
+        for (uint32_t r = 0; r < min(a.rows - r0, 64u); ++r)
+          sum = __builtin_fmaf(__builtin_amdgcn_exp2f(s[(size_t)r * a.score_pitch] - stats[r][0]), stats[r][1], sum);
+      }
+    }
+    if (j < length) a.weights[(size_t)bg * a.max_len + j] += sum;
+  }
 }
 
 // weights[b, g, j] += the probabilities of slot j over all queries of key / value head g: one lane per slot
-template <int D>
 __global__ __launch_bounds__(64) void slot_weights_kernel(const __half* __restrict__ q, const __half* __restrict__ k_cache,
-                                                          const long long* __restrict__ lengths, const float* __restrict__ stats,
-                                                          float* __restrict__ weights, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t past,
-                                                          uint32_t max_len, uint32_t blocks, float scale) {
+                                                          const float* __restrict__ stats, float* __restrict__ weights, uint32_t T, uint32_t Hq,
+                                                          uint32_t Hkv, uint32_t past, uint32_t max_len, uint32_t blocks, float scale) {
+  constexpr int D = 128;
   __shared__ float qs[D];
   const uint32_t bg = blockIdx.x / blocks, b = bg / Hkv, g = bg % Hkv, rep = Hq / Hkv;
   const uint32_t j = blockIdx.x % blocks * 64 + threadIdx.x;
-  const long long n = lengths ? lengths[b] : (long long)past + T;
-  if (n <= 0 || n > max_len || blockIdx.x % blocks * 64 >= n) return;
   const __half* key = k_cache + ((size_t)bg * max_len + min(j, max_len - 1)) * D;
   float sum = 0.f, part = 0.f;                         // (in two levels: thousands of small terms one by one lose digits)
   for (uint32_t t = 0; t < T; ++t) {
@@ -137,19 +485,76 @@ __global__ __launch_bounds__(64) void slot_weights_kernel(const __half* __restri
       __syncthreads();
       for (int c = threadIdx.x; c < D; c += 64) qs[c] = (float)((const _Float16*)q)[item * D + c];
       __syncthreads();
-      if (lengths ? j < n : j <= past + t) {
-        part += __builtin_amdgcn_exp2f(score<D>(qs, key, scale * 1.4426950408889634f) - stats[((size_t)b * Hq + g * rep + r) * T + t]);
+      if (j <= past + t) {
+        float s = 0.f;
+        for (int c = 0; c < D; c += 8) {
+          const h8 x = *(const h8*)(key + c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s = __builtin_fmaf(qs[c + e], (float)x[e], s);
+        }
+        part += __builtin_amdgcn_exp2f(s * (scale * 1.4426950408889634f) - stats[((size_t)b * Hq + g * rep + r) * T + t]);
       }
     }
   }
-  if (j < n) weights[(size_t)bg * max_len + j] += sum + part;
+  if (j < past + T) weights[(size_t)bg * max_len + j] += sum + part;
 }
 
 int check_heads(const char* what, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, float scale) {
   if (head_dim != 128 && head_dim != 64) return fail(FLH_EINVAL, "%s: head_dim (%u) must be 64 or 128", what, head_dim);
   if (Hq == 0 || Hkv == 0 || Hq % Hkv) return fail(FLH_EINVAL, "%s: %u query heads do not divide over %u key / value heads", what, Hq, Hkv);
-  if (!(scale > 0.f) || scale > 1e30f) return fail(FLH_EINVAL, "%s: the scale must be positive and finite", what);
+  if (!(scale > 0.f) || scale > 1e15f) return fail(FLH_EINVAL, "%s: the scale must be positive and at most 1e15", what);
   return FLH_OK;
+}
+
+// How many groups of 32 rows a workgroup holds: all of the rows up to 128, so that K and V are read once.
+int row_groups(uint64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+
+// Workgroups of the first launch: as many as are resident (one per compute unit where the tiles fill its LDS, else two), so that every
+// piece of work ends at about the same time.
+uint32_t work_groups(uint32_t head_dim, int wr) { return head_dim == 128 && wr == 1 ? 256 : 512; }
+
+uint64_t units_of(uint32_t B, uint32_t Hkv, uint64_t rows) { return (uint64_t)B * Hkv * ((rows + 32 * row_groups(rows) - 1) / (32 * row_groups(rows))); }
+
+size_t partial_bytes(uint32_t B, uint64_t rows, uint32_t Hkv, uint32_t head_dim) {
+  const int wr = row_groups(rows);
+  return (work_groups(head_dim, wr) + units_of(B, Hkv, rows)) * (size_t)(32 * wr) * (head_dim + 2) * sizeof(float);
+}
+
+template <int D, int WR, bool TREE>
+int launch_rows(Call& a, hipStream_t stream) {
+  constexpr int WK = 4 / WR, NKT = WR == 4 ? 2 : 1, KT = 32 * NKT * WK;
+  constexpr size_t smem = 4 * (size_t)KT * D * 2;
+  static_assert(WK == 1 || smem >= 4 * 32 * D * 4, "the waves' sums reuse the tiles");
+  a.row_blocks = (a.rows + 32 * WR - 1) / (32 * WR);
+  a.groups = work_groups(D, WR);
+  a.least = WR;                                        // (a piece of partial results has half the bytes of WR tiles)
+  static LdsGrant grant;
+  if (int rc = reserve_lds((const void*)cache_attention_kernel<D, WR, TREE>, smem, grant, "cache attention")) return rc;
+  hipLaunchKernelGGL((cache_attention_kernel<D, WR, TREE>), dim3(a.groups), dim3(256), smem, stream, a);
+  if (int rc = check_launch("cache attention")) return rc;
+  const uint64_t outs = (uint64_t)a.B * a.Hkv * a.row_blocks * WR * (D / 32), sums = TREE ? 0 : (uint64_t)a.B * a.Hkv * ((a.max_len + 255) / 256);
+  hipLaunchKernelGGL((cache_combine_kernel<D, WR, TREE>), dim3((unsigned)(outs + sums)), dim3(256), 0, stream, a);
+  return check_launch("cache attention (combine)");
+}
+
+template <bool TREE>
+int launch_call(Call& a, uint32_t head_dim, hipStream_t stream) {
+  auto go = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    switch (row_groups(a.rows)) {
+      case 1: return launch_rows<D, 1, TREE>(a, stream);
+      case 2: return launch_rows<D, 2, TREE>(a, stream);
+      default: return launch_rows<D, 4, TREE>(a, stream);
+    }
+  };
+  return head_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{});
+}
+
+// tiles, rows and elements that fit the kernels' 32-bit counts
+bool too_large(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
+  const uint64_t rows = (uint64_t)T * (Hq / Hkv), units = units_of(B, Hkv, rows);
+  return rows > (1u << 24) || max_len > (1u << 30) || units > (1u << 24) || units * ((uint64_t)max_len / 64 + 8) > 0x7FFFFFFFull ||
+         (uint64_t)B * Hkv * max_len * head_dim > (1ull << 40) || (uint64_t)B * T * Hq * head_dim > (1ull << 36);
 }
 
 }  // namespace
@@ -157,10 +562,8 @@ int check_heads(const char* what, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, 
 
 using namespace flh;
 
-constexpr uint32_t kMaxNodes = 256;
-
 extern "C" size_t flh_tree_attention_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim) {
-  return 16;
+  return Hkv ? partial_bytes(B, (uint64_t)T * (Hq / Hkv), Hkv, head_dim) : 0;
 }
 
 extern "C" int flh_tree_attention_f16(const flh_half* q, const flh_half* k_new, const flh_half* v_new, const flh_half* cos,
@@ -174,50 +577,26 @@ extern "C" int flh_tree_attention_f16(const flh_half* q, const flh_half* k_new, 
   if (int rc = check_heads("tree_attention", Hq, Hkv, head_dim, scale)) return rc;
   if (T > kMaxNodes) return fail(FLH_EINVAL, "tree_attention: %u nodes (at most %u)", T, kMaxNodes);
   if (B == 0 || T == 0) return FLH_OK;
+  if (too_large(B, T, Hq, Hkv, head_dim, max_len)) return fail(FLH_EINVAL, "tree_attention: problem too large");
   const size_t need = flh_tree_attention_workspace_bytes(B, T, Hq, Hkv, head_dim);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return fail(FLH_EINVAL, "tree_attention: a 16-byte aligned workspace of %zu bytes is required", need);
-  if ((uint64_t)B * T * Hq * head_dim > 0x7FFFFFFFull || (uint64_t)B * Hkv * max_len * head_dim > (1ull << 40) || max_len > (1u << 30))
-    return fail(FLH_EINVAL, "tree_attention: problem too large");
-  const hipStream_t st = (hipStream_t)stream;
-  const uint64_t lanes = (uint64_t)B * T * Hkv * (head_dim / 2);
-  hipLaunchKernelGGL(tree_write_kernel, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, (const __half*)k_new, (const __half*)v_new,
-                     (const __half*)cos, (const __half*)sin, (const long long*)lengths, (__half*)k_cache, (__half*)v_cache, B, T, Hkv,
-                     head_dim, max_len);
-  if (int rc = check_launch("tree_attention (write)")) return rc;
-  auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3(B * T * Hq), dim3(64), 0, st, (const __half*)q, (const __half*)cos, (const __half*)sin, (const __half*)k_cache,
-                       (const __half*)v_cache, (const long long*)lengths, mask, mask_per_sequence ? T * T : 0u, (__half*)out, (float*)nullptr,
-                       T, Hq, Hkv, max_len, scale);
-  };
-  if (head_dim == 128) go(query_attention_kernel<128>);
-  else go(query_attention_kernel<64>);
-  return check_launch("tree_attention");
+  Call a = {};
+  a.q = (const __half*)q, a.k_new = (const __half*)k_new, a.v_new = (const __half*)v_new, a.cos = (const __half*)cos, a.sin = (const __half*)sin;
+  a.lengths = (const long long*)lengths, a.mask = mask, a.mask_stride = mask_per_sequence ? T * T : 0;
+  a.k_cache = (__half*)k_cache, a.v_cache = (__half*)v_cache, a.out = (__half*)out, a.partials = (float*)workspace;
+  a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.rows = T * a.rep, a.max_len = max_len;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return launch_call<true>(a, head_dim, (hipStream_t)stream);
 }
-
-extern "C" size_t flh_decode_attention_weights_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
-  return (size_t)B * Hq * 4 + 16;
-}
-
-extern "C" size_t flh_prefill_attention_weights_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq) { return (size_t)B * T * Hq * 4 + 16; }
 
 namespace {
-template <int D>
-int launch_weights(const __half* q, const __half* k, const __half* v, const long long* lengths, __half* out, float* weights, uint32_t B,
-                   uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t past, uint32_t max_len, float scale, void* ws, hipStream_t st) {
-  if (lengths) {
-    hipLaunchKernelGGL(query_attention_kernel<D>, dim3(B * T * Hq), dim3(64), 0, st, q, (const __half*)nullptr, (const __half*)nullptr, k, v,
-                       lengths, (const uint8_t*)nullptr, 0u, out, (float*)ws, T, Hq, Hkv, max_len, scale);
-    if (int rc = check_launch("attention_weights")) return rc;
-  } else if (int rc = prefill_attention(q, k, v, out, (float*)ws, B, T, Hq, Hkv, D, past, max_len, scale, st)) {
-    return rc;
-  }
-  const uint32_t blocks = (max_len + 63) / 64;
-  hipLaunchKernelGGL(slot_weights_kernel<D>, dim3(B * Hkv * blocks), dim3(64), 0, st, q, k, lengths, (const float*)ws, weights, T, Hq, Hkv, past,
-                     max_len, blocks, scale);
-  return check_launch("attention_weights (sums)");
-}
+uint32_t score_pitch(uint32_t max_len) { return (max_len + 3) / 4 * 4; }
 }  // namespace
+
+extern "C" size_t flh_decode_attention_weights_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
+  return Hkv ? partial_bytes(B, Hq / Hkv, Hkv, head_dim) + (size_t)B * Hq * score_pitch(max_len) * sizeof(float) : 0;
+}
 
 extern "C" int flh_decode_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, const int64_t* lengths,
                                                 flh_half* out, float* weights, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
@@ -226,17 +605,20 @@ extern "C" int flh_decode_attention_weights_f16(const flh_half* q, const flh_hal
   if (misaligned16(q, k_cache, v_cache, out, weights)) return fail(FLH_EINVAL, "decode_attention_weights: tensors must be 16-byte aligned");
   if (int rc = check_heads("decode_attention_weights", Hq, Hkv, head_dim, scale)) return rc;
   if (B == 0 || max_len == 0) return FLH_OK;
-  if ((uint64_t)B * Hq * head_dim > 0x7FFFFFFFull || (uint64_t)B * Hkv * ((max_len + 63) / 64) > 0x7FFFFFFFull || max_len > (1u << 30))
-    return fail(FLH_EINVAL, "decode_attention_weights: problem too large");
+  if (too_large(B, 1, Hq, Hkv, head_dim, max_len)) return fail(FLH_EINVAL, "decode_attention_weights: problem too large");
   const size_t need = flh_decode_attention_weights_workspace_bytes(B, Hq, Hkv, head_dim, max_len);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return fail(FLH_EINVAL, "decode_attention_weights: a 16-byte aligned workspace of %zu bytes is required", need);
-  auto go = [&](auto d) {
-    return launch_weights<decltype(d)::value>((const __half*)q, (const __half*)k_cache, (const __half*)v_cache, (const long long*)lengths,
-                                              (__half*)out, weights, B, 1, Hq, Hkv, 0, max_len, scale, workspace, (hipStream_t)stream);
-  };
-  return head_dim == 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 64>{});
+  Call a = {};
+  a.q = (const __half*)q, a.lengths = (const long long*)lengths, a.out = (__half*)out, a.weights = weights;
+  a.k_cache = (__half*)k_cache, a.v_cache = (__half*)v_cache;   // (only read)
+  a.partials = (float*)workspace, a.scores = (float*)workspace + partial_bytes(B, Hq / Hkv, Hkv, head_dim) / sizeof(float);
+  a.B = B, a.T = 1, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.rows = a.rep, a.max_len = max_len, a.score_pitch = score_pitch(max_len);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return launch_call<false>(a, head_dim, (hipStream_t)stream);
 }
+
+extern "C" size_t flh_prefill_attention_weights_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq) { return (size_t)B * T * Hq * 4 + 16; }
 
 extern "C" int flh_prefill_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, flh_half* out,
                                                  float* weights, uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
@@ -253,6 +635,12 @@ extern "C" int flh_prefill_attention_weights_f16(const flh_half* q, const flh_ha
   const size_t need = flh_prefill_attention_weights_workspace_bytes(B, T, Hq);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return fail(FLH_EINVAL, "prefill_attention_weights: a 16-byte aligned workspace of %zu bytes is required", need);
-  return launch_weights<128>((const __half*)q, (const __half*)k_cache, (const __half*)v_cache, nullptr, (__half*)out, weights, B, T, Hq, Hkv, past,
-                             max_len, scale, workspace, (hipStream_t)stream);
+  float* stats = (float*)workspace;
+  if (int rc = prefill_attention((const __half*)q, (const __half*)k_cache, (const __half*)v_cache, (__half*)out, stats, B, T, Hq, Hkv, head_dim,
+                                 past, max_len, scale, (hipStream_t)stream))
+    return rc;
+  const uint32_t blocks = (past + T + 63) / 64;
+  hipLaunchKernelGGL(slot_weights_kernel, dim3(B * Hkv * blocks), dim3(64), 0, (hipStream_t)stream, (const __half*)q, (const __half*)k_cache, stats,
+                     weights, T, Hq, Hkv, past, max_len, blocks, scale);
+  return check_launch("prefill_attention_weights");
 }

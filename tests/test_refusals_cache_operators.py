@@ -27,7 +27,7 @@ def tree(at=None, value=None, mask_per_sequence=0, B=2, T=8, Hq=8, Hkv=2, d=128,
     (dict(at=0, value=None), b"null pointer"), (dict(at=6, value=None), b"null pointer"), (dict(at=5, value=None), b"null pointer"),
     (dict(at=0, value=ODD), b"16-byte aligned"), (dict(at=9, value=ODD), b"16-byte aligned"), (dict(at=3, value=ODD), b"16-byte aligned"),
     (dict(d=96), b"head_dim (96) must be 64 or 128"), (dict(Hq=7), b"do not divide"), (dict(Hkv=0), b"do not divide"),
-    (dict(T=257), b"257 nodes"), (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"),
+    (dict(T=257), b"257 nodes"), (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"), (dict(scale=1e16), b"scale"),
     (dict(B=1 << 20, T=256), b"too large"), (dict(ws=None), b"workspace"), (dict(ws=ODD), b"workspace"), (dict(ws_bytes=8), b"workspace")])
 def test_tree_attention(more, message):
     call("flh_tree_attention_f16", tree(**more), message)
