@@ -87,7 +87,7 @@ _SIG = {
     "flh_tree_commit": (_c.c_int, [_PTR, _PTR, _c.c_int] + [_PTR] * 6 + [_c.c_int, _PTR, _PTR] + [_c.c_uint32] * 5 + [_PTR]),
     "flh_decode_attention_weights_workspace_bytes": (_c.c_size_t, [_c.c_uint32] * 5),
     "flh_decode_attention_weights_f16": (_c.c_int, [_PTR] * 6 + [_c.c_uint32] * 5 + [_c.c_float, _PTR, _c.c_size_t, _PTR]),
-    "flh_prefill_attention_weights_workspace_bytes": (_c.c_size_t, [_c.c_uint32] * 3),
+    "flh_prefill_attention_weights_workspace_bytes": (_c.c_size_t, [_c.c_uint32] * 5),
     "flh_prefill_attention_weights_f16": (_c.c_int, [_PTR] * 5 + [_c.c_uint32] * 7 + [_c.c_float, _PTR, _c.c_size_t, _PTR]),
     "flh_evict_kv_cache": (_c.c_int, [_c.c_int] + [_PTR] * 7 + [_c.c_uint32] * 6 + [_PTR]),
     "flh_add_rmsnorm_rotate_quant_i4": (_c.c_int, [_PTR, _PTR, _PTR, _PTR, _c.c_float, _PTR, _PTR, _c.c_uint32, _c.c_uint32,

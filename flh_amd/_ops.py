@@ -850,7 +850,7 @@ def prefill_attention_weights(q, k_cache, v_cache, past, weights, scale=None, wo
     out = torch.empty((B, T, Hq * d), dtype=torch.float16, device=q.device)
     if B == 0 or T == 0:
         return out
-    workspace = _attention_workspace("flh_prefill_attention_weights", q, workspace, B, T, Hq)
+    workspace = _attention_workspace("flh_prefill_attention_weights", q, workspace, B, T, Hq, Hkv, past)
     _run("flh_prefill_attention_weights_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
          weights.data_ptr(), B, T, Hq, Hkv, d, past, max_len, float(scale if scale is not None else d ** -0.5),
          workspace.data_ptr(), workspace.numel(), _stream(q))

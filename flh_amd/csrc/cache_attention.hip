@@ -468,35 +468,132 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const Call a) {
   }
 }
 
-// weights[b, g, j] += the probabilities of slot j over all queries of key / value head g: one lane per slot
-__global__ __launch_bounds__(64) void slot_weights_kernel(const __half* __restrict__ q, const __half* __restrict__ k_cache,
-                                                          const float* __restrict__ stats, float* __restrict__ weights, uint32_t T, uint32_t Hq,
-                                                          uint32_t Hkv, uint32_t past, uint32_t max_len, uint32_t blocks, float scale) {
-  constexpr int D = 128;
-  __shared__ float qs[D];
-  const uint32_t bg = blockIdx.x / blocks, b = bg / Hkv, g = bg % Hkv, rep = Hq / Hkv;
-  const uint32_t j = blockIdx.x % blocks * 64 + threadIdx.x;
-  const __half* key = k_cache + ((size_t)bg * max_len + min(j, max_len - 1)) * D;
-  float sum = 0.f, part = 0.f;                         // (in two levels: thousands of small terms one by one lose digits)
-  for (uint32_t t = 0; t < T; ++t) {
-    if (t % 32 == 0) sum += part, part = 0.f;
-    for (uint32_t r = 0; r < rep; ++r) {
-      const size_t item = ((size_t)b * T + t) * Hq + g * rep + r;
-      __syncthreads();
-      for (int c = threadIdx.x; c < D; c += 64) qs[c] = (float)((const _Float16*)q)[item * D + c];
-      __syncthreads();
-      if (j <= past + t) {
-        float s = 0.f;
-        for (int c = 0; c < D; c += 8) {
-          const h8 x = *(const h8*)(key + c);
+// ---- the weights of a prompt -----------------------------------------------------------------------------------------
+// weights[b, g, j] += sum over heads of g and queries t of exp2(scale_log2 q . K[j] - lse): the scores of one more product, whose rows
+// are queries and whose columns are slots, S = Q K^T on v_mfma_f32_32x32x16_f16 -- a lane owns a column, so that the sum over the queries
+// stays in its registers.  A workgroup has 256 slots (64 per wave, whose keys it keeps in registers) and a chunk of the queries, 64 of
+// one head at a time through LDS; of several chunks each writes its sums, and a second launch adds them in their order.
+// Bound by the exponentials next to the MFMAs: one per 128 multiply-adds.
+constexpr int kSlots = 256, kQueries = 64;
+
+struct Columns {
+  const __half *q, *k;
+  const float* lse;                                    // [B, Hq, T]
+  float *weights, *parts;                              // parts [chunk][b][g][pitch]
+  uint32_t T, Hq, Hkv, rep, past, max_len, blocks, chunks, chunk, pitch;   // chunk: queries of one, a multiple of 64
+  float scale_log2;
+};
+
+__global__ __launch_bounds__(256, 2) void column_weights_kernel(const Columns a) {
+  constexpr int D = 128, PITCH = 2 * D, TILE = kQueries * PITCH, KS = D / 16;
+  using L = Tile<D>;
+  __shared__ __align__(1024) uint8_t lds[2 * TILE];
+  __shared__ __align__(16) float lse[2][kQueries];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t block = blockIdx.x % a.blocks, units = gridDim.x / (a.blocks * a.chunks);
+  const uint32_t bg = blockIdx.x / a.blocks % units, chunk = blockIdx.x / a.blocks / units, b = bg / a.Hkv, g = bg % a.Hkv;
+  const uint32_t total = a.past + a.T, j0 = block * kSlots, mine = j0 + wave * 64;
+  // queries of the chunk that see a slot of the block: from the first tile of 64 that ends behind its first slot
+  const uint32_t t_end = min(a.T, (chunk + 1) * a.chunk);
+  uint32_t t0 = chunk * a.chunk;
+  if (j0 > a.past) t0 = max(t0, (j0 - a.past) / kQueries * kQueries);
+  const uint32_t steps = t0 < t_end ? (t_end - t0 + kQueries - 1) / kQueries * a.rep : 0;
+  float sum[2] = {0.f, 0.f};
+  if (steps) {
+    // this lane's slots as B operand: channels 16 s + 8 h .. + 7 (slots past the last repeat it; they are not used)
+    h8 kf[2][KS];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s = __builtin_fmaf(qs[c + e], (float)x[e], s);
+    for (int ct = 0; ct < 2; ++ct) {
+      const __half* src = a.k + ((size_t)bg * a.max_len + min(mine + ct * 32 + n, total - 1)) * D + 8 * h;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[ct][s] = *(const h8*)(src + 16 * s);
+    }
+    // loads of a tile: four rows each, four of a wave
+    const size_t stride = (size_t)a.Hq * PITCH;        // bytes from one token's query to the next
+    unsigned off[4];
+    uint32_t off_row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      off_row[i] = (wave * 4 + i) * 4 + lane / L::CHUNKS;
+      off[i] = ((lane % L::CHUNKS) ^ L::k_swizzle(off_row[i])) << 4;
+    }
+    const unsigned lds0 = (unsigned)(size_t)lds, lse0 = (unsigned)(size_t)&lse[0][0];
+    const uint8_t* queries = (const uint8_t*)(a.q + ((size_t)b * a.T * a.Hq + g * a.rep) * D);
+    const float* of_heads = a.lse + ((size_t)b * a.Hq + g * a.rep) * a.T;
+    auto issue = [&](uint32_t step, int buf) {         // (rows past the last query repeat it; their probabilities are dropped)
+      const uint32_t t = t0 + step / a.rep * kQueries, head = step % a.rep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        load_to_lds16(queries + min(t + off_row[i], a.T - 1) * stride + head * PITCH + off[i], lds0 + buf * TILE + (wave * 4 + i) * 1024);
+      if (wave == 0) load_to_lds4(of_heads + (size_t)head * a.T + min(t + lane, a.T - 1), lse0 + buf * kQueries * 4);
+    };
+    const int q_at = L::k_at(n, h);
+    auto compute = [&](uint32_t step, int buf) {
+      const uint32_t t = t0 + step / a.rep * kQueries;
+      if (mine > a.past + t + kQueries - 1 || mine >= total) return;   // (none of the wave's slots is seen)
+      const bool masked = t + kQueries > t_end || mine + 63 > a.past + t;
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+        v16f st[2];
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) st[ct][r] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const h8 qf = *(const h8*)(lds + buf * TILE + rt * 32 * PITCH + (q_at ^ (s << 5)));
+          st[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf, kf[0][s], st[0], 0, 0, 0);
+          st[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf, kf[1][s], st[1], 0, 0, 0);
         }
-        part += __builtin_amdgcn_exp2f(s * (scale * 1.4426950408889634f) - stats[((size_t)b * Hq + g * rep + r) * T + t]);
+        // register r: query t + 32 rt + 8 (r / 4) + 4 h + r % 4
+        v4f e[4];
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) e[q4] = *(const v4f*)&lse[buf][rt * 32 + 8 * q4 + 4 * h];
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+          float p[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[ct][r], a.scale_log2, -e[r >> 2][r & 3]));
+          if (masked) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const uint32_t q = t + rt * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+              if (q >= t_end || mine + ct * 32 + n > a.past + q) p[r] = 0.f;
+            }
+          }
+          float part = 0.f;                            // (in levels: thousands of small terms one by one lose digits)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) part += (p[4 * q4] + p[4 * q4 + 1]) + (p[4 * q4 + 2] + p[4 * q4 + 3]);
+          sum[ct] += part;
+        }
       }
+    };
+    issue(0, 0);
+    for (uint32_t step = 0; step < steps; ++step) {
+      wait_vmcnt<0>();
+      __syncthreads();                                 // this tile has landed, and everybody has read the one before it
+      if (step + 1 < steps) issue(step + 1, (step + 1) & 1);
+      compute(step, step & 1);
     }
   }
-  if (j < past + T) weights[(size_t)bg * max_len + j] += sum + part;
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    const float all = sum[ct] + lane_xor_f<32>(sum[ct]);
+    const uint32_t j = mine + ct * 32 + n;
+    if (h == 0 && j < total) {
+      if (a.chunks == 1) a.weights[(size_t)bg * a.max_len + j] += all;
+      else a.parts[((size_t)chunk * units + bg) * a.pitch + j] = all;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void column_sums_kernel(const Columns a, uint32_t units) {
+  const uint32_t bg = blockIdx.x / a.blocks, j = blockIdx.x % a.blocks * kSlots + threadIdx.x;
+  if (j >= a.past + a.T) return;
+  float sum = 0.f;
+  for (uint32_t c = 0; c < a.chunks; ++c) sum += a.parts[((size_t)c * units + bg) * a.pitch + j];
+  a.weights[(size_t)bg * a.max_len + j] += sum;
 }
 
 int check_heads(const char* what, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, float scale) {
@@ -618,7 +715,26 @@ extern "C" int flh_decode_attention_weights_f16(const flh_half* q, const flh_hal
   return launch_call<false>(a, head_dim, (hipStream_t)stream);
 }
 
-extern "C" size_t flh_prefill_attention_weights_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq) { return (size_t)B * T * Hq * 4 + 16; }
+namespace {
+// Chunks of queries: enough that the launch has about eight workgroups per compute unit (half of them see nothing of their slots).
+void cut_columns(Columns& a, uint32_t B) {
+  a.blocks = (a.past + a.T + kSlots - 1) / kSlots;
+  const uint64_t units = (uint64_t)B * a.Hkv * a.blocks, tiles = (a.T + kQueries - 1) / kQueries;
+  const uint64_t wanted = units >= 2048 ? 1 : (2048 + units - 1) / units, chunks = wanted < tiles ? wanted : tiles;
+  a.chunk = (uint32_t)((tiles + chunks - 1) / chunks) * kQueries;
+  a.chunks = (a.T + a.chunk - 1) / a.chunk;
+  a.pitch = a.blocks * kSlots;
+}
+size_t lse_floats(uint32_t B, uint32_t T, uint32_t Hq) { return ((size_t)B * T * Hq + 3) / 4 * 4; }
+}  // namespace
+
+extern "C" size_t flh_prefill_attention_weights_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t past) {
+  if (B == 0 || T == 0 || Hkv == 0) return 0;
+  Columns a = {};
+  a.T = T, a.Hkv = Hkv, a.past = past;
+  cut_columns(a, B);
+  return (lse_floats(B, T, Hq) + (a.chunks > 1 ? (size_t)a.chunks * B * Hkv * a.pitch : 0)) * sizeof(float);
+}
 
 extern "C" int flh_prefill_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, flh_half* out,
                                                  float* weights, uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
@@ -630,17 +746,23 @@ extern "C" int flh_prefill_attention_weights_f16(const flh_half* q, const flh_ha
   if (head_dim != 128) return fail(FLH_EINVAL, "prefill_attention_weights: head_dim (%u) must be 128", head_dim);
   if ((uint64_t)past + T > max_len) return fail(FLH_EINVAL, "prefill_attention_weights: past (%u) + T (%u) exceeds the cache length %u", past, T, max_len);
   if (B == 0 || T == 0) return FLH_OK;
-  if ((uint64_t)B * T * Hq > 0x7FFFFFFFull || (uint64_t)B * Hkv * ((max_len + 63) / 64) > 0x7FFFFFFFull || max_len > (1u << 30))
+  if ((uint64_t)B * T * Hq > 0x7FFFFFFFull || max_len > (1u << 30) || (uint64_t)B * Hkv * ((uint64_t)max_len / kSlots + 1) > (1u << 24))
     return fail(FLH_EINVAL, "prefill_attention_weights: problem too large");
-  const size_t need = flh_prefill_attention_weights_workspace_bytes(B, T, Hq);
+  const size_t need = flh_prefill_attention_weights_workspace_bytes(B, T, Hq, Hkv, past);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return fail(FLH_EINVAL, "prefill_attention_weights: a 16-byte aligned workspace of %zu bytes is required", need);
-  float* stats = (float*)workspace;
-  if (int rc = prefill_attention((const __half*)q, (const __half*)k_cache, (const __half*)v_cache, (__half*)out, stats, B, T, Hq, Hkv, head_dim,
-                                 past, max_len, scale, (hipStream_t)stream))
+  Columns a = {};
+  a.q = (const __half*)q, a.k = (const __half*)k_cache, a.weights = weights;
+  a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.past = past, a.max_len = max_len, a.scale_log2 = scale * 1.4426950408889634f;
+  a.lse = (float*)workspace, a.parts = (float*)workspace + lse_floats(B, T, Hq);
+  cut_columns(a, B);
+  const hipStream_t st = (hipStream_t)stream;
+  if (int rc = prefill_attention(a.q, a.k, (const __half*)v_cache, (__half*)out, (float*)workspace, B, T, Hq, Hkv, head_dim, past, max_len, scale, st))
     return rc;
-  const uint32_t blocks = (past + T + 63) / 64;
-  hipLaunchKernelGGL(slot_weights_kernel, dim3(B * Hkv * blocks), dim3(64), 0, (hipStream_t)stream, (const __half*)q, (const __half*)k_cache, stats,
-                     weights, T, Hq, Hkv, past, max_len, blocks, scale);
-  return check_launch("prefill_attention_weights");
+  const uint32_t units = B * Hkv;
+  hipLaunchKernelGGL(column_weights_kernel, dim3(units * a.blocks * a.chunks), dim3(256), 0, st, a);
+  if (int rc = check_launch("prefill_attention_weights")) return rc;
+  if (a.chunks == 1) return FLH_OK;
+  hipLaunchKernelGGL(column_sums_kernel, dim3(units * a.blocks), dim3(256), 0, st, a, units);
+  return check_launch("prefill_attention_weights (sums)");
 }

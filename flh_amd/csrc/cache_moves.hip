@@ -22,61 +22,81 @@ struct Caches {
 };
 
 // ---- tree commit ---------------------------------------------------------------------------------------------------
-// One wave per sequence walks the tree from node 0: the next node is the lowest child whose token the model has chosen.  Lane i looks
-// at the nodes i, i + 64, ...; children come behind their parent, so the walk ends after at most T steps.
-__global__ __launch_bounds__(64) void tree_walk_kernel(const long long* __restrict__ tokens, const long long* __restrict__ parents,
-                                                       uint32_t parents_stride, const long long* __restrict__ chosen,
-                                                       const long long* __restrict__ lengths, long long* __restrict__ path,
-                                                       long long* __restrict__ accepted, long long* __restrict__ next,
-                                                       long long* __restrict__ new_lengths, uint32_t T, uint32_t max_len) {
+// A wave walks the tree of its sequence from node 0: the next node is the lowest child whose token the model has chosen.  Lane i holds
+// the nodes i, i + 64, ... in registers; children come behind their parent, so the walk ends after at most T steps.
+struct Tree {
+  const long long *tokens, *parents, *chosen, *lengths;
+  long long *path, *accepted, *next, *new_lengths;
+  uint32_t parents_stride, T, max_len;
+};
+
+__device__ __forceinline__ long long of_lane(long long v, int l) {
+  return (long long)((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, l));
+}
+
+// The accepted nodes into `path` (LDS), their number back; `want` is the token behind the last.
+__device__ __forceinline__ uint32_t walk(const Tree& t, uint32_t b, uint16_t* path, long long& want) {
   constexpr int N = kMaxNodes / 64;
-  const uint32_t b = blockIdx.x;
-  const int lane = threadIdx.x;
-  const long long n = lengths[b];
-  const bool active = n >= 0 && n + T <= max_len;
-  long long tok[N], par[N];
+  const int lane = threadIdx.x & 63;
+  long long tok[N], par[N], cho[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const uint32_t c = i * 64 + lane;
-    tok[i] = c < T ? tokens[(size_t)b * T + c] : 0;
-    par[i] = c < T ? parents[(size_t)b * parents_stride + c] : -1;
+    const bool have = c < t.T;
+    tok[i] = have ? t.tokens[(size_t)b * t.T + c] : 0;
+    par[i] = have ? t.parents[(size_t)b * t.parents_stride + c] : -1;
+    cho[i] = have ? t.chosen[(size_t)b * t.T + c] : 0;
   }
   uint32_t node = 0, count = 0;
-  long long want = active ? chosen[(size_t)b * T] : -1;
-  if (active) {
-    for (;;) {
-      if (lane == 0) path[(size_t)b * T + count] = node;
-      ++count;
-      uint32_t found = T;
+  for (;;) {
+    if (lane == 0) path[count] = (uint16_t)node;
+    ++count;
+    const int l = (int)(node & 63);
+    want = of_lane(cho[0], l);
 #pragma unroll
-      for (int i = N - 1; i >= 0; --i) {
-        const uint32_t c = i * 64 + lane;
-        const unsigned long long hit = __ballot(c < T && c > node && par[i] == (long long)node && tok[i] == want);
-        if (hit) found = i * 64 + __builtin_ctzll(hit);
-      }
-      if (found == T) break;
-      node = found;
-      want = chosen[(size_t)b * T + node];
+    for (int i = 1; i < N; ++i)
+      if (node >> 6 == (uint32_t)i) want = of_lane(cho[i], l);
+    uint32_t found = t.T;
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) {
+      const uint32_t c = i * 64 + lane;
+      const unsigned long long hit = __ballot(c < t.T && c > node && par[i] == (long long)node && tok[i] == want);
+      if (hit) found = i * 64 + __builtin_ctzll(hit);
     }
+    if (found == t.T) return count;
+    node = (uint32_t)__builtin_amdgcn_readfirstlane((int)found);
   }
-  for (uint32_t i = count + lane; i < T; i += 64) path[(size_t)b * T + i] = -1;
-  if (lane == 0) accepted[b] = count, next[b] = want, new_lengths[b] = n + count;
 }
 
-// One workgroup per (layer, key or value, sequence, head): the accepted rows through LDS, so that no row is overwritten unread.
-__global__ __launch_bounds__(256) void tree_move_kernel(Caches caches, const long long* __restrict__ path,
-                                                        const long long* __restrict__ accepted, const long long* __restrict__ lengths,
-                                                        uint32_t T, uint32_t Hkv, uint32_t pieces, uint32_t max_len) {
+// One workgroup per (sequence, head), layer, and 16 chunks of 16 bytes of the keys' or the values' rows: it walks the tree for itself
+// (one launch instead of two; the walk is a microsecond), then moves the accepted rows through LDS, so that none is overwritten unread.
+__global__ __launch_bounds__(256) void tree_commit_kernel(Caches caches, Tree t, bool first, uint32_t Hkv, uint32_t pieces) {
   extern __shared__ __align__(16) v4i rows[];
+  __shared__ uint16_t path[kMaxNodes];
+  __shared__ uint32_t s_count;
   const uint32_t bg = blockIdx.x, b = bg / Hkv, layer = blockIdx.y;
-  const uint32_t count = (uint32_t)accepted[b];
-  if (count < 2) return;
-  v4i* cache = (v4i*)(blockIdx.z ? caches.v[layer] : caches.k[layer]) + ((size_t)bg * max_len + (size_t)lengths[b]) * pieces;
-  // node 0 stays where it is
-  for (uint32_t i = threadIdx.x; i < (count - 1) * pieces; i += 256)
-    rows[i] = cache[(size_t)path[(size_t)b * T + 1 + i / pieces] * pieces + i % pieces];
+  const long long n = t.lengths[b];
+  const bool active = n >= 0 && n + t.T <= t.max_len;
+  const bool tells = first && bg % Hkv == 0 && layer == 0 && blockIdx.z == 0;
+  if (threadIdx.x < 64) {
+    long long want = -1;
+    const uint32_t count = active ? walk(t, b, path, want) : 0;
+    if (threadIdx.x == 0) {
+      s_count = count;
+      if (tells) t.accepted[b] = count, t.next[b] = want, t.new_lengths[b] = n + count;
+    }
+  }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < (count - 1) * pieces; i += 256) cache[pieces + i] = rows[i];
+  const uint32_t count = s_count;
+  if (tells)
+    for (uint32_t i = threadIdx.x; i < t.T; i += 256) t.path[(size_t)b * t.T + i] = i < count ? (long long)path[i] : -1;
+  if (count < 2 || !caches.k[layer]) return;
+  const uint32_t slice = blockIdx.z >> 1, c0 = slice * 16, width = min(16u, pieces - c0);
+  v4i* cache = (v4i*)(blockIdx.z & 1 ? caches.v[layer] : caches.k[layer]) + ((size_t)bg * t.max_len + (size_t)n) * pieces + c0;
+  // node 0 stays where it is
+  for (uint32_t i = threadIdx.x; i < (count - 1) * width; i += 256) rows[i] = cache[(size_t)path[1 + i / width] * pieces + i % width];
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < (count - 1) * width; i += 256) cache[(size_t)(1 + i / width) * pieces + i % width] = rows[i];
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------------
@@ -87,90 +107,153 @@ __device__ __forceinline__ unsigned rank_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One workgroup per (layer, sequence, head): the (budget - recent)-th largest weight of the slots in front of the latest, digit by
-// digit, then the slots above it and the first of those at it, in order.
-__global__ __launch_bounds__(256) void evict_select_kernel(const float* __restrict__ weights, const long long* __restrict__ lengths,
-                                                           long long* __restrict__ kept, float* __restrict__ new_weights,
-                                                           long long* __restrict__ new_lengths, uint32_t Hkv, uint32_t max_len,
-                                                           uint32_t budget, uint32_t recent) {
-  __shared__ unsigned count[256], part[2][4];
+constexpr int kSelectThreads = 512, kSelectWaves = kSelectThreads / 64, kDigits = 2048;
+constexpr uint32_t kStagedSlots = 16384;               // weights of a head that are read once, into LDS
+
+// One workgroup per (layer, sequence, head): the (budget - recent)-th largest weight of the slots in front of the latest, in three digits
+// of eleven bits (the first holds the sign, the exponent and two bits of the fraction: few weights share one), then the slots above
+// it and the first of those at it, in order: every wave counts those of its own range of slots, then writes them.
+template <bool STAGED>
+__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const float* __restrict__ weights, const long long* __restrict__ lengths,
+                                                                      long long* __restrict__ kept, float* __restrict__ new_weights,
+                                                                      long long* __restrict__ new_lengths, uint32_t Hkv, uint32_t max_len,
+                                                                      uint32_t budget, uint32_t recent) {
+  extern __shared__ float staged[];
+  __shared__ unsigned count[kDigits], part[2][kSelectWaves];
   __shared__ unsigned s_digit, s_rest;
   const uint32_t bg = blockIdx.x, b = bg / Hkv;
   const size_t unit = (size_t)blockIdx.y * gridDim.x + bg;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long len = lengths[b];
   const bool valid = len >= 0 && len <= max_len;
   const uint32_t n = valid ? (uint32_t)len : 0;
-  const float* w = weights + unit * max_len;
+  const float* from = weights + unit * max_len;
   float* nw = new_weights + unit * max_len;
   long long* list = kept + unit * budget;
   if (blockIdx.y == 0 && bg % Hkv == 0 && tid == 0) new_lengths[b] = valid && n > budget ? budget : len;
   if (n <= budget) {                                   // (a length that is none: as it is, nothing kept)
-    for (uint32_t i = tid; i < budget; i += 256) list[i] = i < n ? (long long)i : -1;
-    for (uint32_t i = tid; i < max_len; i += 256) nw[i] = i < n ? w[i] : 0.f;
+    for (uint32_t i = tid; i < budget; i += kSelectThreads) list[i] = i < n ? (long long)i : -1;
+    for (uint32_t i = tid; i < max_len; i += kSelectThreads) nw[i] = i < n ? from[i] : 0.f;
     return;
   }
+  if constexpr (STAGED) {
+    for (uint32_t i = tid; i < n; i += kSelectThreads) staged[i] = from[i];
+  }
+  auto w = [&](uint32_t i) { return STAGED ? staged[i] : from[i]; };
   const uint32_t old = n - recent;                     // slots that are chosen from
   unsigned prefix = 0, mask = 0, rest = budget - recent;
-  for (int shift = 24; shift >= 0 && rest; shift -= 8) {
-    count[tid] = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const unsigned digits = pass == 2 ? 1023 : 2047;
+    if (rest == 0) break;                              // (nothing but the latest)
+    for (int i = tid; i < kDigits; i += kSelectThreads) count[i] = 0;
     __syncthreads();
-    for (uint32_t i = tid; i < old; i += 256) {
-      const unsigned r = rank_of(w[i]);
-      if ((r & mask) == prefix) atomicAdd(&count[(r >> shift) & 255], 1u);
+    for (uint32_t i = tid; i < old; i += kSelectThreads) {
+      const unsigned r = rank_of(w(i));
+      if ((r & mask) == prefix) atomicAdd(&count[(r >> shift) & digits], 1u);
     }
     __syncthreads();
-    if (tid == 0) {
-      unsigned left = rest;
-      int d = 255;
-      while (count[d] < left) left -= count[d], --d;
-      s_digit = d, s_rest = left;
+    // sums from the largest digit down: thread t has the four digits below 2048 - 4 t
+    unsigned c[4], sum = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum += c[k] = count[kDigits - 1 - 4 * tid - k];
+    unsigned up = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const unsigned x = __shfl_up(up, d);
+      up += lane >= d ? x : 0;
+    }
+    if (lane == 63) part[0][wave] = up;
+    __syncthreads();
+    for (int k = 0; k < wave; ++k) up += part[0][k];
+    unsigned before = up - sum;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (before < rest && before + c[k] >= rest) s_digit = kDigits - 1 - 4 * tid - k, s_rest = rest - before;
+      before += c[k];
     }
     __syncthreads();
-    prefix |= s_digit << shift, mask |= 255u << shift, rest = s_rest;
+    prefix |= s_digit << shift, mask |= digits << shift, rest = s_rest;
   }
   // above the threshold, or one of the first `rest` at it, or one of the latest
   const bool none = budget == recent;
-  unsigned above = 0, equal = 0;                       // of the slots so far
-  for (uint32_t i0 = 0; i0 < n; i0 += 256) {
-    const uint32_t i = i0 + tid;
-    const float wi = i < n ? w[i] : 0.f;
-    const unsigned r = rank_of(wi);
-    const bool late = i >= old && i < n, up = late || (i < old && !none && r > prefix), at = i < old && !none && r == prefix;
-    const unsigned long long ups = __ballot(up), ats = __ballot(at);
-    __syncthreads();
-    if (lane == 0) part[0][wave] = __popcll(ups), part[1][wave] = __popcll(ats);
-    __syncthreads();
-    unsigned a = above, e = equal;
-    for (int k = 0; k < wave; ++k) a += part[0][k], e += part[1][k];
-    const unsigned long long below = (1ull << lane) - 1;
-    a += __popcll(ups & below), e += __popcll(ats & below);
-    if (up || (at && e < rest)) {
-      const unsigned to = a + min(e, rest);
-      list[to] = i, nw[to] = wi;
-    }
-    for (int k = 0; k < 4; ++k) above += part[0][k], equal += part[1][k];
+  const uint32_t share = ((n + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64, i0 = wave * share, i1 = min(n, i0 + share);
+  auto look = [&](uint32_t i, unsigned long long& ups, unsigned long long& ats) {
+    const unsigned r = i < i1 ? rank_of(w(i)) : 0;
+    ups = __ballot(i < i1 && (i >= old || (!none && r > prefix)));
+    ats = __ballot(i < i1 && i < old && !none && r == prefix);
+  };
+  unsigned long long ups, ats;
+  unsigned above = 0, equal = 0;
+  for (uint32_t i = i0; i < i1; i += 64) {
+    look(i + lane, ups, ats);
+    above += __popcll(ups), equal += __popcll(ats);
   }
-  for (uint32_t i = budget + tid; i < max_len; i += 256) nw[i] = 0.f;
+  __syncthreads();
+  if (lane == 0) part[0][wave] = above, part[1][wave] = equal;
+  __syncthreads();
+  above = equal = 0;
+  for (int k = 0; k < wave; ++k) above += part[0][k], equal += part[1][k];
+  const unsigned long long mine = 1ull << lane, below = mine - 1;
+  for (uint32_t i = i0; i < i1; i += 64) {
+    look(i + lane, ups, ats);
+    const unsigned a = above + __popcll(ups & below), e = equal + __popcll(ats & below);
+    if ((ups & mine) || ((ats & mine) && e < rest)) {
+      const unsigned to = a + min(e, rest);
+      list[to] = i + lane, nw[to] = w(i + lane);
+    }
+    above += __popcll(ups), equal += __popcll(ats);
+  }
+  for (uint32_t i = budget + tid; i < max_len; i += kSelectThreads) nw[i] = 0.f;
 }
 
-// One workgroup per (layer, sequence, head) of keys or values; slots move down only, in order, 16 rows at a time.
+// One workgroup per (layer, sequence, head) of keys or values, or per slice of their rows' chunks where those alone are few workgroups.  A
+// row moves to a lower slot, and rows keep their order: a batch of rows may be written once it and those before it are read, by all
+// waves, and the next batch may be requested before that (its rows lie behind everything that is written until then).
+constexpr int kMovePieces = 8;                         // of a thread per batch
+
 __global__ __launch_bounds__(256) void evict_move_kernel(Caches caches, const long long* __restrict__ lengths,
-                                                         const long long* __restrict__ kept, uint32_t Hkv, uint32_t pieces,
+                                                         const long long* __restrict__ kept, uint32_t Hkv, uint32_t pieces, uint32_t width,
                                                          uint32_t max_len, uint32_t budget) {
-  const uint32_t bg = blockIdx.x, layer = blockIdx.y;
+  const uint32_t bg = blockIdx.x, layer = blockIdx.y, slice = blockIdx.z >> 1;
   const long long len = lengths[bg / Hkv];
-  if (len <= budget || len > max_len) return;
+  if (len <= (long long)budget || len > max_len) return;
   const long long* list = kept + ((size_t)layer * gridDim.x + bg) * budget;
-  v4i* cache = (v4i*)(blockIdx.z ? caches.v[layer] : caches.k[layer]) + (size_t)bg * max_len * pieces;
-  const uint64_t all = (uint64_t)budget * pieces;
-  for (uint64_t i0 = 0; i0 < all; i0 += 256) {
-    const uint64_t i = i0 + threadIdx.x;
-    v4i x = {0, 0, 0, 0};
-    if (i < all) x = cache[(size_t)list[i / pieces] * pieces + i % pieces];
-    asm volatile("" : "+v"(x));                        // (the row has arrived)
-    __syncthreads();                                   // every row of these is read before one of them is written
-    if (i < all) cache[i] = x;
+  v4i* cache = (v4i*)(blockIdx.z & 1 ? caches.v[layer] : caches.k[layer]) + (size_t)bg * max_len * pieces + slice * width;
+  const uint32_t all = budget * width;
+  constexpr uint32_t BATCH = 256 * kMovePieces;
+  v4i x[2][kMovePieces];
+  auto request = [&](uint32_t first, v4i(&y)[kMovePieces]) __attribute__((always_inline)) {
+    uint32_t row[kMovePieces];
+#pragma unroll
+    for (int k = 0; k < kMovePieces; ++k) {
+      const uint32_t i = min(first + k * 256 + threadIdx.x, all - 1);
+      row[k] = (uint32_t)list[i / width];
+    }
+#pragma unroll
+    for (int k = 0; k < kMovePieces; ++k) {
+      const uint32_t i = min(first + k * 256 + threadIdx.x, all - 1);
+      y[k] = cache[(size_t)row[k] * pieces + i % width];
+    }
+  };
+  auto store = [&](uint32_t first, v4i(&y)[kMovePieces]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < kMovePieces; ++k) asm volatile("" : "+v"(y[k]));   // (the rows have arrived)
+    barrier_no_fence();
+#pragma unroll
+    for (int k = 0; k < kMovePieces; ++k) {
+      const uint32_t i = first + k * 256 + threadIdx.x;
+      if (i < all) cache[(size_t)(i / width) * pieces + i % width] = y[k];
+    }
+  };
+  request(0, x[0]);
+  for (uint32_t i = 0; i < all; i += 2 * BATCH) {
+    if (i + BATCH < all) request(i + BATCH, x[1]);
+    store(i, x[0]);
+    if (i + BATCH >= all) break;
+    if (i + 2 * BATCH < all) request(i + 2 * BATCH, x[0]);
+    store(i + BATCH, x[1]);
   }
 }
 
@@ -188,7 +271,7 @@ int check_caches(int layers, flh_half* const* k, flh_half* const* v, uint32_t B,
   if (layers < 0 || (layers && (!k || !v))) return fail(FLH_EINVAL, "%s: null pointer", what);
   if (Hkv == 0 || max_len == 0) return fail(FLH_EINVAL, "%s: heads and cache length must be positive", what);
   if (head_dim == 0 || head_dim % 8 || head_dim > 512) return fail(FLH_EINVAL, "%s: head_dim (%u) must be a multiple of 8, at most 512", what, head_dim);
-  if ((uint64_t)B * Hkv > 0x7FFFFFFFull || max_len > (1u << 30)) return fail(FLH_EINVAL, "%s: problem too large", what);
+  if ((uint64_t)B * Hkv > 0x7FFFFFFFull || max_len > (1u << 30) || (uint64_t)max_len * (head_dim / 8) > (1u << 31)) return fail(FLH_EINVAL, "%s: problem too large", what);
   Caches c;
   for (int l = 0; l < layers; l += kMaxLayers)
     if (int rc = take_caches(c, l, layers - l < kMaxLayers ? layers - l : kMaxLayers, k, v, what)) return rc;
@@ -221,21 +304,18 @@ extern "C" int flh_tree_commit(const int64_t* tokens, const int64_t* parents, in
   if (lengths == new_lengths) return fail(FLH_EINVAL, "tree_commit: the new lengths need memory of their own");
   if (int rc = check_caches(layers, k_caches, v_caches, B, Hkv, head_dim, max_len, "tree_commit")) return rc;
   if (B == 0) return FLH_OK;
-  const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(tree_walk_kernel, dim3(B), dim3(64), 0, st, (const long long*)tokens, (const long long*)parents,
-                     parents_per_sequence ? T : 0u, (const long long*)chosen, (const long long*)lengths, (long long*)path,
-                     (long long*)accepted, (long long*)next, (long long*)new_lengths, T, max_len);
-  if (int rc = check_launch("tree_commit (walk)")) return rc;
-  if (T == 1) return FLH_OK;
-  const size_t smem = (size_t)(T - 1) * head_dim * 2;
+  const uint32_t pieces = head_dim / 8;
+  const size_t smem = (size_t)(T - 1) * (pieces < 16 ? pieces : 16) * 16;
   static LdsGrant grant;
-  if (int rc = reserve_lds((const void*)tree_move_kernel, smem, grant, "tree_commit")) return rc;
-  for (int l = 0; l < layers; l += kMaxLayers) {
-    Caches c;
+  if (int rc = reserve_lds((const void*)tree_commit_kernel, smem, grant, "tree_commit")) return rc;
+  const Tree t = {(const long long*)tokens, (const long long*)parents, (const long long*)chosen, (const long long*)lengths, (long long*)path,
+                  (long long*)accepted,     (long long*)next,          (long long*)new_lengths,  parents_per_sequence ? T : 0u, T, max_len};
+  for (int l = 0; l == 0 || l < layers; l += kMaxLayers) {
+    Caches c = {};
     const int n = layers - l < kMaxLayers ? layers - l : kMaxLayers;
     if (int rc = take_caches(c, l, n, k_caches, v_caches, "tree_commit")) return rc;
-    hipLaunchKernelGGL(tree_move_kernel, dim3(B * Hkv, n, 2), dim3(256), smem, st, c, (const long long*)path, (const long long*)accepted,
-                       (const long long*)lengths, T, Hkv, head_dim / 8, max_len);
+    hipLaunchKernelGGL(tree_commit_kernel, dim3(B * Hkv, n ? n : 1, n ? 2 * ((pieces + 15) / 16) : 1), dim3(256), smem, (hipStream_t)stream, c, t,
+                       l == 0, Hkv, pieces);
     if (int rc = check_launch("tree_commit")) return rc;
   }
   return FLH_OK;
@@ -257,12 +337,23 @@ extern "C" int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_hal
     Caches c;
     const int n = layers - l < kMaxLayers ? layers - l : kMaxLayers;
     if (int rc = take_caches(c, l, n, k_caches, v_caches, "evict_kv_cache")) return rc;
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)units, n), dim3(256), 0, st, weights + l * units * max_len, (const long long*)lengths,
-                       (long long*)kept + l * units * budget, new_weights + l * units * max_len, (long long*)new_lengths, Hkv, max_len, budget,
-                       recent);
+    auto select = [&](auto kern, size_t smem) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)units, n), dim3(kSelectThreads), smem, st, weights + l * units * max_len, (const long long*)lengths,
+                         (long long*)kept + l * units * budget, new_weights + l * units * max_len, (long long*)new_lengths, Hkv, max_len,
+                         budget, recent);
+    };
+    if (max_len <= kStagedSlots) {
+      static LdsGrant grant;
+      if (int rc = reserve_lds((const void*)evict_select_kernel<true>, max_len * sizeof(float), grant, "evict_kv_cache")) return rc;
+      select(evict_select_kernel<true>, max_len * sizeof(float));
+    } else {
+      select(evict_select_kernel<false>, 0);
+    }
     if (int rc = check_launch("evict_kv_cache (select)")) return rc;
-    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)units, n, 2), dim3(256), 0, st, c, (const long long*)lengths,
-                       (const long long*)kept + l * units * budget, Hkv, head_dim / 8, max_len, budget);
+    // whole rows, or four slices of them where a launch would have fewer than two workgroups per compute unit
+    const uint32_t pieces = head_dim / 8, slices = pieces % 4 == 0 && units * n * 2 < 512 ? 4 : 1;
+    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)units, n, 2 * slices), dim3(256), 0, st, c, (const long long*)lengths,
+                       (const long long*)kept + l * units * budget, Hkv, pieces, pieces / slices, max_len, budget);
     if (int rc = check_launch("evict_kv_cache")) return rc;
   }
   return FLH_OK;

@@ -486,7 +486,7 @@ size_t flh_decode_attention_weights_workspace_bytes(uint32_t B, uint32_t Hq, uin
 int flh_decode_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, const int64_t* lengths,
                                      flh_half* out, float* weights, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
                                      uint32_t max_len, float scale, void* workspace, size_t workspace_bytes, void* stream);
-size_t flh_prefill_attention_weights_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq);
+size_t flh_prefill_attention_weights_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t past);
 int flh_prefill_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, flh_half* out, float* weights,
                                       uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t past,
                                       uint32_t max_len, float scale, void* workspace, size_t workspace_bytes, void* stream);
