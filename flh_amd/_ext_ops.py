@@ -6,6 +6,8 @@ ctypes route at decode sizes); everything else falls through to the ctypes ops o
 same C ABI of libflh_hip.so."""
 import importlib
 
+import torch
+
 from . import _lib
 from . import _ops
 
@@ -33,6 +35,9 @@ gemm_f6_swiglu = _ext.gemm_f6_swiglu
 gemm_f6_dequant_multi = _ext.gemm_f6_dequant_multi
 prefill_attention = _ext.prefill_attention
 rope_kv_cache_ = _ext.rope_kv_cache_
+tree_attention = _ext.tree_attention
+decode_attention_weights = _ext.decode_attention_weights
+prefill_attention_weights = _ext.prefill_attention_weights
 rotate_quantize_gemm_i4 = _ext.rotate_quantize_gemm_i4
 rotate_quantize_gemm_i4_multi = _ext.rotate_quantize_gemm_i4_multi
 rmsnorm_rotate_quantize_gemm_i4_multi = _ext.rmsnorm_rotate_quantize_gemm_i4_multi
@@ -76,6 +81,18 @@ def add_rmsnorm_rotate_and_quantize_i4(x, add, weight, eps, hadamard=True, clip_
 def rotate_and_quantize_f6(x, hadamard=True, clip_ratio=1.0, norm_weight=None, eps=None, add=None, weights=None):
     mode = _ops._f6_mode(x, hadamard, eps, add) if x.dim() == 2 else 0
     return tuple(_ext.rotate_and_quantize_f6_mode(x, mode, clip_ratio, norm_weight, eps, add, weights))
+
+
+def _layers(caches):
+    return [caches] if isinstance(caches, torch.Tensor) else caches
+
+
+def tree_commit_(tokens, parents, chosen, lengths, k_caches, v_caches):
+    return tuple(_ext.tree_commit_(tokens, parents, chosen, lengths, _layers(k_caches), _layers(v_caches)))
+
+
+def evict_kv_cache_(k_caches, v_caches, weights, lengths, budget, recent):
+    return tuple(_ext.evict_kv_cache_(_layers(k_caches), _layers(v_caches), weights, lengths, int(budget), int(recent)))
 
 
 def __getattr__(name):        # ops the extension does not wrap (one matrix's encoding, int32 output, tuning hook, ...)

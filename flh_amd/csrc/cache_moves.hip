@@ -68,16 +68,18 @@ __device__ __forceinline__ uint32_t walk(const Tree& t, uint32_t b, uint16_t* pa
   }
 }
 
-// One workgroup per (sequence, head), layer, and 16 chunks of 16 bytes of the keys' or the values' rows: it walks the tree for itself
-// (one launch instead of two; the walk is a microsecond), then moves the accepted rows through LDS, so that none is overwritten unread.
+// What moves at once: (keys or values, head, up to 16 chunks of 16 bytes of a row).  One workgroup has sixteen of them, of one sequence and
+// layer: it walks the tree for itself (one launch instead of two; the walk is a microsecond), then reads the accepted rows of as many as fit
+// its registers, and writes them when all have arrived, so that none is overwritten unread.
+constexpr uint32_t kMoves = 16, kHeld = 16;            // of a workgroup; chunks in a thread's registers
+
 __global__ __launch_bounds__(256) void tree_commit_kernel(Caches caches, Tree t, bool first, uint32_t Hkv, uint32_t pieces) {
-  extern __shared__ __align__(16) v4i rows[];
   __shared__ uint16_t path[kMaxNodes];
   __shared__ uint32_t s_count;
-  const uint32_t bg = blockIdx.x, b = bg / Hkv, layer = blockIdx.y;
+  const uint32_t b = blockIdx.x, layer = blockIdx.y;
   const long long n = t.lengths[b];
   const bool active = n >= 0 && n + t.T <= t.max_len;
-  const bool tells = first && bg % Hkv == 0 && layer == 0 && blockIdx.z == 0;
+  const bool tells = first && layer == 0 && blockIdx.z == 0;
   if (threadIdx.x < 64) {
     long long want = -1;
     const uint32_t count = active ? walk(t, b, path, want) : 0;
@@ -91,12 +93,31 @@ __global__ __launch_bounds__(256) void tree_commit_kernel(Caches caches, Tree t,
   if (tells)
     for (uint32_t i = threadIdx.x; i < t.T; i += 256) t.path[(size_t)b * t.T + i] = i < count ? (long long)path[i] : -1;
   if (count < 2 || !caches.k[layer]) return;
-  const uint32_t slice = blockIdx.z >> 1, c0 = slice * 16, width = min(16u, pieces - c0);
-  v4i* cache = (v4i*)(blockIdx.z & 1 ? caches.v[layer] : caches.k[layer]) + ((size_t)bg * t.max_len + (size_t)n) * pieces + c0;
-  // node 0 stays where it is
-  for (uint32_t i = threadIdx.x; i < (count - 1) * width; i += 256) rows[i] = cache[(size_t)path[1 + i / width] * pieces + i % width];
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < (count - 1) * width; i += 256) cache[(size_t)(1 + i / width) * pieces + i % width] = rows[i];
+  const uint32_t slices = (pieces + 15) / 16, end = min((blockIdx.z + 1) * kMoves, 2 * Hkv * slices);
+  const uint32_t rows = count - 1, width = min(16u, pieces), each = rows * width;   // (node 0 stays where it is)
+  const uint32_t batch = max(1u, kHeld * 256 / each);  // (255 rows of 16 chunks fit)
+  for (uint32_t u0 = blockIdx.z * kMoves; u0 < end; u0 += batch) {
+    const uint32_t all = min(batch, end - u0) * each;
+    v4i x[kHeld];
+    v4i* to[kHeld];
+#pragma unroll
+    for (uint32_t k = 0; k < kHeld; ++k) {
+      const uint32_t i = k * 256 + threadIdx.x;
+      to[k] = nullptr;
+      if (i >= all) continue;
+      const uint32_t u = u0 + i / each, r = i % each / width, head = (u >> 1) / slices, c = (u >> 1) % slices * 16 + i % width;
+      if (c >= pieces) continue;
+      v4i* cache = (v4i*)(u & 1 ? caches.v[layer] : caches.k[layer]) + (((size_t)b * Hkv + head) * t.max_len + (size_t)n) * pieces + c;
+      to[k] = cache + (size_t)(r + 1) * pieces;
+      x[k] = cache[(size_t)path[r + 1] * pieces];
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kHeld; ++k) asm volatile("" : "+v"(x[k]));   // (the rows have arrived)
+    barrier_no_fence();
+#pragma unroll
+    for (uint32_t k = 0; k < kHeld; ++k)
+      if (to[k]) *to[k] = x[k];
+  }
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------------
@@ -304,18 +325,15 @@ extern "C" int flh_tree_commit(const int64_t* tokens, const int64_t* parents, in
   if (lengths == new_lengths) return fail(FLH_EINVAL, "tree_commit: the new lengths need memory of their own");
   if (int rc = check_caches(layers, k_caches, v_caches, B, Hkv, head_dim, max_len, "tree_commit")) return rc;
   if (B == 0) return FLH_OK;
-  const uint32_t pieces = head_dim / 8;
-  const size_t smem = (size_t)(T - 1) * (pieces < 16 ? pieces : 16) * 16;
-  static LdsGrant grant;
-  if (int rc = reserve_lds((const void*)tree_commit_kernel, smem, grant, "tree_commit")) return rc;
+  const uint32_t pieces = head_dim / 8, moves = 2 * Hkv * ((pieces + 15) / 16);
   const Tree t = {(const long long*)tokens, (const long long*)parents, (const long long*)chosen, (const long long*)lengths, (long long*)path,
                   (long long*)accepted,     (long long*)next,          (long long*)new_lengths,  parents_per_sequence ? T : 0u, T, max_len};
   for (int l = 0; l == 0 || l < layers; l += kMaxLayers) {
     Caches c = {};
     const int n = layers - l < kMaxLayers ? layers - l : kMaxLayers;
     if (int rc = take_caches(c, l, n, k_caches, v_caches, "tree_commit")) return rc;
-    hipLaunchKernelGGL(tree_commit_kernel, dim3(B * Hkv, n ? n : 1, n ? 2 * ((pieces + 15) / 16) : 1), dim3(256), smem, (hipStream_t)stream, c, t,
-                       l == 0, Hkv, pieces);
+    hipLaunchKernelGGL(tree_commit_kernel, dim3(B, n ? n : 1, n ? (moves + kMoves - 1) / kMoves : 1), dim3(256), 0, (hipStream_t)stream, c, t, l == 0,
+                       Hkv, pieces);
     if (int rc = check_launch("tree_commit")) return rc;
   }
   return FLH_OK;

@@ -14,8 +14,11 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <algorithm>
 #include <cmath>
+#include <map>
 #include <mutex>
+#include <utility>
 #include <vector>
 
 #include "../../include/flh_hip.h"
@@ -152,6 +155,181 @@ Tensor prefill_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v
                                (uint32_t)d, (uint32_t)past, (uint32_t)max_len,
                                (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)d)), stream_of(q)));
   return out;
+}
+
+// ---- caches whose sequences have lengths of their own (the checks of _ops.py) ----------------------------------------------
+void check_cache_pair(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, int64_t batch, int64_t d) {
+  for (const Tensor* t : {&q, &k_cache, &v_cache})
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kFloat16 && t->is_contiguous() && t->device() == q.device(),
+                "tensors must be contiguous float16 CUDA tensors on one device");
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes() && k_cache.size(0) == batch && k_cache.size(3) == d,
+              "caches must be [B, Hkv, max_len, d]");
+}
+
+void check_lengths(const Tensor& lengths, int64_t batch, const c10::Device& device) {
+  TORCH_CHECK(lengths.is_cuda() && lengths.scalar_type() == torch::kInt64 && lengths.is_contiguous() && lengths.dim() == 1 &&
+                  lengths.size(0) == batch && lengths.device() == device,
+              "lengths must be a contiguous int64 CUDA tensor [B]");
+}
+
+void check_weights(const Tensor& weights, at::IntArrayRef shape, const c10::Device& device) {
+  TORCH_CHECK(weights.is_cuda() && weights.scalar_type() == torch::kFloat32 && weights.is_contiguous() && weights.sizes() == shape &&
+                  weights.device() == device,
+              "weights must be a contiguous float32 CUDA tensor ", shape);
+}
+
+// The caller's workspace (checked), or one kept per (device, stream) and grown as needed: launches of one stream run in order.  A captured
+// graph keeps the pointer it was recorded with, so under capture the caller has to bring one that it owns.
+Tensor attention_workspace(const Tensor& q, const c10::optional<Tensor>& given, size_t need) {
+  if (given.has_value()) {
+    TORCH_CHECK(given->is_cuda() && given->scalar_type() == torch::kUInt8 && given->is_contiguous() && given->device() == q.device() &&
+                    (size_t)given->numel() >= need,
+                "workspace: ", need, " bytes of uint8 needed");
+    return *given;
+  }
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing((hipStream_t)stream_of(q), &status) == hipSuccess && status == hipStreamCaptureStatusNone,
+              "pass `workspace` (a tensor that outlives the graph) when capturing");
+  static std::mutex mu;
+  static auto* kept = new std::map<std::pair<int, void*>, Tensor>;   // (never destroyed: the device may be gone by then)
+  std::lock_guard<std::mutex> lock(mu);
+  Tensor& w = (*kept)[{q.device().index(), stream_of(q)}];
+  if (!w.defined() || (size_t)w.numel() < need)
+    w = torch::empty({(int64_t)std::max(need, (size_t)1 << 20)}, q.options().dtype(torch::kUInt8));
+  return w;
+}
+
+float scale_of(const c10::optional<double>& scale, int64_t d) { return (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)d)); }
+
+Tensor tree_attention(const Tensor& q, const Tensor& k_new, const Tensor& v_new, const Tensor& cos, const Tensor& sin, const Tensor& lengths,
+                      const Tensor& mask, Tensor k_cache, Tensor v_cache, const c10::optional<double>& scale,
+                      const c10::optional<Tensor>& workspace) {
+  TORCH_CHECK(q.dim() == 4 && k_new.dim() == 4, "q [B, T, Hq, d] and k_new, v_new [B, T, Hkv, d] expected");
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), d = q.size(3), Hkv = k_new.size(2);
+  check_cache_pair(q, k_cache, v_cache, B, d);
+  for (const Tensor* t : {&k_new, &v_new, &cos, &sin})
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kFloat16 && t->is_contiguous() && t->device() == q.device(),
+                "tensors must be contiguous float16 CUDA tensors on one device");
+  const int64_t rows[] = {B, T, Hkv, d}, rotary[] = {B, T, d};
+  TORCH_CHECK(k_new.sizes() == at::IntArrayRef(rows) && v_new.sizes() == k_new.sizes() && k_cache.size(1) == Hkv,
+              "q [B, T, Hq, d] and k_new, v_new [B, T, Hkv, d] expected");
+  TORCH_CHECK(cos.sizes() == at::IntArrayRef(rotary) && sin.sizes() == cos.sizes(), "cos / sin must be [B, T, d]");
+  check_lengths(lengths, B, q.device());
+  const int64_t each[] = {B, T, T}, one[] = {T, T};
+  TORCH_CHECK(mask.is_cuda() && mask.scalar_type() == torch::kBool && mask.is_contiguous() && mask.device() == q.device() &&
+                  (mask.sizes() == at::IntArrayRef(one) || mask.sizes() == at::IntArrayRef(each)),
+              "mask must be a contiguous bool CUDA tensor [T, T] or [B, T, T]");
+  TORCH_CHECK(d == 64 || d == 128, "head_dim must be 64 or 128");
+  TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "Hq must be a multiple of Hkv");
+  TORCH_CHECK(T <= 256, "at most 256 nodes");
+  Tensor out = torch::empty({B, T, Hq * d}, q.options());
+  if (B == 0 || T == 0) return out;
+  Launch l(q);
+  Tensor ws = attention_workspace(q, workspace, flh_tree_attention_workspace_bytes(B, T, Hq, Hkv, d));
+  ok(flh_tree_attention_f16(h(q), h(k_new), h(v_new), h(cos), h(sin), lengths.data_ptr<int64_t>(), u8(mask), mask.dim() == 3, hm(k_cache),
+                            hm(v_cache), hm(out), B, T, Hq, Hkv, d, k_cache.size(2), scale_of(scale, d), ws.data_ptr(), ws.numel(),
+                            stream_of(q)));
+  return out;
+}
+
+Tensor decode_attention_weights(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths, Tensor weights,
+                                const c10::optional<double>& scale, const c10::optional<Tensor>& workspace) {
+  TORCH_CHECK(q.dim() == 3, "q [B, Hq, d] expected");
+  const int64_t B = q.size(0), Hq = q.size(1), d = q.size(2);
+  check_cache_pair(q, k_cache, v_cache, B, d);
+  const int64_t Hkv = k_cache.size(1), max_len = k_cache.size(2);
+  check_lengths(lengths, B, q.device());
+  check_weights(weights, {B, Hkv, max_len}, q.device());
+  TORCH_CHECK(d == 64 || d == 128, "head_dim must be 64 or 128");
+  TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "Hq must be a multiple of Hkv");
+  TORCH_CHECK(max_len > 0, "the caches have no slots");
+  Tensor out = torch::empty_like(q);
+  if (B == 0) return out;
+  Launch l(q);
+  Tensor ws = attention_workspace(q, workspace, flh_decode_attention_weights_workspace_bytes(B, Hq, Hkv, d, max_len));
+  ok(flh_decode_attention_weights_f16(h(q), h(k_cache), h(v_cache), lengths.data_ptr<int64_t>(), hm(out), weights.data_ptr<float>(), B, Hq, Hkv, d,
+                                      max_len, scale_of(scale, d), ws.data_ptr(), ws.numel(), stream_of(q)));
+  return out;
+}
+
+Tensor prefill_attention_weights(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, int64_t past, Tensor weights,
+                                 const c10::optional<double>& scale, const c10::optional<Tensor>& workspace) {
+  TORCH_CHECK(q.dim() == 4, "q [B, T, Hq, d] and caches [B, Hkv, max_len, d] expected");
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), d = q.size(3);
+  check_cache_pair(q, k_cache, v_cache, B, d);
+  const int64_t Hkv = k_cache.size(1), max_len = k_cache.size(2);
+  check_weights(weights, {B, Hkv, max_len}, q.device());
+  TORCH_CHECK(d == 128, "head_dim must be 128");
+  TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "Hq must be a multiple of Hkv");
+  TORCH_CHECK(past >= 0 && past + T <= max_len, "past + T must fit the cache");
+  Tensor out = torch::empty({B, T, Hq * d}, q.options());
+  if (B == 0 || T == 0) return out;
+  Launch l(q);
+  Tensor ws = attention_workspace(q, workspace, flh_prefill_attention_weights_workspace_bytes(B, T, Hq, Hkv, past));
+  ok(flh_prefill_attention_weights_f16(h(q), h(k_cache), h(v_cache), hm(out), weights.data_ptr<float>(), B, T, Hq, Hkv, d, past, max_len,
+                                       scale_of(scale, d), ws.data_ptr(), ws.numel(), stream_of(q)));
+  return out;
+}
+
+struct CacheList {   // the layers' caches and their common shape
+  std::vector<flh_half*> k, v;
+  int64_t B, Hkv, max_len, d;
+  CacheList(const std::vector<Tensor>& ks, const std::vector<Tensor>& vs, const c10::Device& device) {
+    TORCH_CHECK(!ks.empty() && ks.size() == vs.size(), "one key and one value cache per layer");
+    const at::IntArrayRef shape = ks[0].sizes();
+    TORCH_CHECK(shape.size() == 4 && shape[1] > 0 && shape[2] > 0, "caches must be [B, Hkv, max_len, d]");
+    for (const auto* list : {&ks, &vs})
+      for (const Tensor& t : *list) {
+        TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kFloat16 && t.is_contiguous() && t.device() == device && t.sizes() == shape,
+                    "caches must be contiguous float16 CUDA tensors of one shape on one device");
+        (list == &ks ? k : v).push_back((flh_half*)t.data_ptr());
+      }
+    B = shape[0], Hkv = shape[1], max_len = shape[2], d = shape[3];
+    TORCH_CHECK(d > 0 && d % 8 == 0 && d <= 512, "head_dim must be a multiple of 8, at most 512");
+  }
+};
+
+std::vector<Tensor> tree_commit_(const Tensor& tokens, const Tensor& parents, const Tensor& chosen, const Tensor& lengths,
+                                 const std::vector<Tensor>& k_caches, const std::vector<Tensor>& v_caches) {
+  TORCH_CHECK(tokens.dim() == 2, "tokens [B, T] expected");
+  const int64_t B = tokens.size(0), T = tokens.size(1);
+  for (const Tensor* t : {&tokens, &parents, &chosen})
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kInt64 && t->is_contiguous() && t->device() == tokens.device(),
+                "tokens, parents and chosen must be contiguous int64 CUDA tensors on one device");
+  TORCH_CHECK(((parents.dim() == 1 && parents.size(0) == T) || parents.sizes() == tokens.sizes()) && chosen.sizes() == tokens.sizes(),
+              "parents [T] or [B, T], chosen [B, T] expected");
+  TORCH_CHECK(T >= 1 && T <= 256, "1 to 256 nodes");
+  check_lengths(lengths, B, tokens.device());
+  const CacheList c(k_caches, v_caches, tokens.device());
+  TORCH_CHECK(c.B == B, "caches must be [B, Hkv, max_len, d]");
+  Tensor path = torch::empty_like(tokens), accepted = torch::empty_like(lengths), next = torch::empty_like(lengths),
+         new_lengths = torch::empty_like(lengths);
+  if (B) {
+    Launch l(tokens);
+    ok(flh_tree_commit(tokens.data_ptr<int64_t>(), parents.data_ptr<int64_t>(), parents.dim() == 2, chosen.data_ptr<int64_t>(),
+                       lengths.data_ptr<int64_t>(), path.data_ptr<int64_t>(), accepted.data_ptr<int64_t>(), next.data_ptr<int64_t>(),
+                       new_lengths.data_ptr<int64_t>(), (int)c.k.size(), c.k.data(), c.v.data(), B, T, c.Hkv, c.d, c.max_len,
+                       stream_of(tokens)));
+  }
+  return {path, accepted, next, new_lengths};
+}
+
+std::vector<Tensor> evict_kv_cache_(const std::vector<Tensor>& k_caches, const std::vector<Tensor>& v_caches, const Tensor& weights,
+                                    const Tensor& lengths, int64_t budget, int64_t recent) {
+  const CacheList c(k_caches, v_caches, weights.device());
+  const int64_t layers = (int64_t)c.k.size();
+  check_weights(weights, {layers, c.B, c.Hkv, c.max_len}, weights.device());
+  check_lengths(lengths, c.B, weights.device());
+  TORCH_CHECK(budget >= 1 && budget <= c.max_len && recent >= 0 && recent <= budget, "the budget must be in 1 .. max_len, recent at most that");
+  Tensor kept = torch::empty({layers, c.B, c.Hkv, budget}, lengths.options()), new_weights = torch::empty_like(weights),
+         new_lengths = torch::empty_like(lengths);
+  if (c.B) {
+    Launch l(weights);
+    ok(flh_evict_kv_cache((int)layers, c.k.data(), c.v.data(), weights.data_ptr<float>(), lengths.data_ptr<int64_t>(), kept.data_ptr<int64_t>(),
+                          new_weights.data_ptr<float>(), new_lengths.data_ptr<int64_t>(), c.B, c.Hkv, c.d, c.max_len, budget, recent,
+                          stream_of(weights)));
+  }
+  return {kept, new_weights, new_lengths};
 }
 
 // gate and up projection of a SwiGLU MLP in one launch: fp16(fp16(silu(gate)) * up)
@@ -1029,6 +1207,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("residual"), py::arg("group_size") = 128, py::arg("out") = py::none());
   m.def("prefill_attention", &prefill_attention, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("past"),
         py::arg("scale") = py::none());
+  m.def("tree_attention", &tree_attention, py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("cos"), py::arg("sin"), py::arg("lengths"),
+        py::arg("mask"), py::arg("k_cache"), py::arg("v_cache"), py::arg("scale") = py::none(), py::arg("workspace") = py::none());
+  m.def("decode_attention_weights", &decode_attention_weights, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("lengths"),
+        py::arg("weights"), py::arg("scale") = py::none(), py::arg("workspace") = py::none());
+  m.def("prefill_attention_weights", &prefill_attention_weights, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("past"),
+        py::arg("weights"), py::arg("scale") = py::none(), py::arg("workspace") = py::none());
+  m.def("tree_commit_", &tree_commit_);
+  m.def("evict_kv_cache_", &evict_kv_cache_);
   m.def("rotate_quantize_gemm_i4", &rotate_quantize_gemm_i4, py::arg("x"), py::arg("B"), py::arg("B_scale"));
   m.def("rotate_quantize_gemm_i4_multi", &rotate_quantize_gemm_i4_multi, py::arg("x"), py::arg("Bs"), py::arg("B_scales"));
   m.def("rope_kv_cache_", &rope_kv_cache_, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cos"), py::arg("sin"),
