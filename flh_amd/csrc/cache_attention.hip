@@ -480,27 +480,34 @@ struct Columns {
   const __half *q, *k;
   const float* lse;                                    // [B, Hq, T]
   float *weights, *parts;                              // parts [chunk][b][g][pitch]
-  uint32_t T, Hq, Hkv, rep, past, max_len, blocks, chunks, chunk, pitch;   // chunk: queries of one, a multiple of 64
+  uint32_t T, Hq, Hkv, rep, past, max_len, blocks, chunks, chunk, pitch, pairs;   // chunk: queries of one, a multiple of 64
   float scale_log2;
+  // blocks of slots that some query of chunk c sees; pairs: their sum over the chunks
+  __host__ __device__ uint32_t live_blocks(uint32_t c) const {
+    const uint32_t last = c + 1 < chunks ? (c + 1) * chunk : T;
+    return (past + last - 1) / kSlots + 1;
+  }
 };
 
 __global__ __launch_bounds__(256, 2) void column_weights_kernel(const Columns a) {
   constexpr int D = 128, PITCH = 2 * D, TILE = kQueries * PITCH, KS = D / 16;
   using L = Tile<D>;
   __shared__ __align__(1024) uint8_t lds[2 * TILE];
-  __shared__ __align__(16) float lse[2][kQueries];
+  __shared__ __align__(16) float lse[4][kQueries];      // (a tile's are read one tile later)
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t block = blockIdx.x % a.blocks, units = gridDim.x / (a.blocks * a.chunks);
-  const uint32_t bg = blockIdx.x / a.blocks % units, chunk = blockIdx.x / a.blocks / units, b = bg / a.Hkv, g = bg % a.Hkv;
+  // (a die takes a contiguous range, whose workgroups share queries and keys in its L2)
+  const uint32_t at = xcd_contiguous(blockIdx.x, gridDim.x), units = gridDim.x / a.pairs, bg = at / a.pairs, b = bg / a.Hkv, g = bg % a.Hkv;
+  uint32_t chunk = 0, block = at % a.pairs;
+  for (; block >= a.live_blocks(chunk); ++chunk) block -= a.live_blocks(chunk);
   const uint32_t total = a.past + a.T, j0 = block * kSlots, mine = j0 + wave * 64;
   // queries of the chunk that see a slot of the block: from the first tile of 64 that ends behind its first slot
   const uint32_t t_end = min(a.T, (chunk + 1) * a.chunk);
   uint32_t t0 = chunk * a.chunk;
   if (j0 > a.past) t0 = max(t0, (j0 - a.past) / kQueries * kQueries);
-  const uint32_t steps = t0 < t_end ? (t_end - t0 + kQueries - 1) / kQueries * a.rep : 0;
+  const uint32_t steps = (t_end - t0 + kQueries - 1) / kQueries * a.rep;   // (not zero: the chunk sees the block)
   float sum[2] = {0.f, 0.f};
-  if (steps) {
+  {
     // this lane's slots as B operand: channels 16 s + 8 h .. + 7 (slots past the last repeat it; they are not used)
     h8 kf[2][KS];
 #pragma unroll
@@ -511,13 +518,8 @@ __global__ __launch_bounds__(256, 2) void column_weights_kernel(const Columns a)
     }
     // loads of a tile: four rows each, four of a wave
     const size_t stride = (size_t)a.Hq * PITCH;        // bytes from one token's query to the next
-    unsigned off[4];
-    uint32_t off_row[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      off_row[i] = (wave * 4 + i) * 4 + lane / L::CHUNKS;
-      off[i] = ((lane % L::CHUNKS) ^ L::k_swizzle(off_row[i])) << 4;
-    }
+    const uint32_t my_row = wave * 16 + lane / L::CHUNKS;   // + 4 i
+    const unsigned my_off = ((lane % L::CHUNKS) ^ (lane / L::CHUNKS)) << 4;   // (the swizzle by row 16 wave + 4 i + lane / 16: XOR 4 i)
     const unsigned lds0 = (unsigned)(size_t)lds, lse0 = (unsigned)(size_t)&lse[0][0];
     const uint8_t* queries = (const uint8_t*)(a.q + ((size_t)b * a.T * a.Hq + g * a.rep) * D);
     const float* of_heads = a.lse + ((size_t)b * a.Hq + g * a.rep) * a.T;
@@ -525,57 +527,79 @@ __global__ __launch_bounds__(256, 2) void column_weights_kernel(const Columns a)
       const uint32_t t = t0 + step / a.rep * kQueries, head = step % a.rep;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        load_to_lds16(queries + min(t + off_row[i], a.T - 1) * stride + head * PITCH + off[i], lds0 + buf * TILE + (wave * 4 + i) * 1024);
-      if (wave == 0) load_to_lds4(of_heads + (size_t)head * a.T + min(t + lane, a.T - 1), lse0 + buf * kQueries * 4);
+        load_to_lds16(queries + min(t + my_row + 4 * i, a.T - 1) * stride + head * PITCH + (my_off ^ (i << 6)), lds0 + buf * TILE + (wave * 4 + i) * 1024);
+      if (wave == 0) load_to_lds4(of_heads + (size_t)head * a.T + min(t + lane, a.T - 1), lse0 + (step & 3) * kQueries * 4);
     };
+    // A tile of 32 queries: the MFMAs of its scores, and between them the exponentials of the tile before it (P: parity of the scores'
+    // registers).  Four fragments of Q are on their way or in use at a time, those of the next tile among them.
     const int q_at = L::k_at(n, h);
-    auto compute = [&](uint32_t step, int buf) {
-      const uint32_t t = t0 + step / a.rep * kQueries;
-      if (mine > a.past + t + kQueries - 1 || mine >= total) return;   // (none of the wave's slots is seen)
-      const bool masked = t + kQueries > t_end || mine + 63 > a.past + t;
+    v16f st[2][2];
+    v4f e[4];                                          // log2 sums of the tile before
+    h8 f[4];
+    auto read_q = [&](int s, int buf, int rt) { return *(const h8*)(lds + buf * TILE + rt * 32 * PITCH + (q_at ^ (s << 5))); };
+    auto read_e = [&](uint32_t step, int rt) {         // register r of a tile: query 8 (r / 4) + 4 h + r % 4
 #pragma unroll
-      for (int rt = 0; rt < 2; ++rt) {
-        v16f st[2];
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) st[ct][r] = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const h8 qf = *(const h8*)(lds + buf * TILE + rt * 32 * PITCH + (q_at ^ (s << 5)));
-          st[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf, kf[0][s], st[0], 0, 0, 0);
-          st[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf, kf[1][s], st[1], 0, 0, 0);
-        }
-        // register r: query t + 32 rt + 8 (r / 4) + 4 h + r % 4
-        v4f e[4];
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) e[q4] = *(const v4f*)&lse[buf][rt * 32 + 8 * q4 + 4 * h];
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-          float p[16];
-#pragma unroll
-          for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[ct][r], a.scale_log2, -e[r >> 2][r & 3]));
-          if (masked) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const uint32_t q = t + rt * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
-              if (q >= t_end || mine + ct * 32 + n > a.past + q) p[r] = 0.f;
-            }
-          }
-          float part = 0.f;                            // (in levels: thousands of small terms one by one lose digits)
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) part += (p[4 * q4] + p[4 * q4 + 1]) + (p[4 * q4 + 2] + p[4 * q4 + 3]);
-          sum[ct] += part;
-        }
-      }
+      for (int q4 = 0; q4 < 4; ++q4) e[q4] = *(const v4f*)&lse[step & 3][rt * 32 + 8 * q4 + 4 * h];
     };
+    auto mask = [&](auto p_, uint32_t q0) {            // scores of the tile from query q0 on that are none
+      constexpr int P = decltype(p_)::value;
+      if (q0 + 32 <= t_end && mine + 63 <= a.past + q0) return;
+      asm volatile("" ::: "memory");                   // (a branch of its own: few tiles need it)
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t q = q0 + 8 * (r >> 2) + 4 * h + (r & 3);
+          if (q >= t_end || mine + ct * 32 + n > a.past + q) st[P][ct][r] = -INFINITY;
+        }
+    };
+    auto tile = [&](auto p_, auto products_, uint32_t step) {
+      constexpr int P = decltype(p_)::value;
+      constexpr bool PRODUCTS = decltype(products_)::value;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};            // (sums in levels: thousands of small terms one by one lose digits)
+      static_for<16>([&](auto j_) {
+        constexpr int j = decltype(j_)::value, s = j >> 1, ct = j & 1;
+        if constexpr (PRODUCTS) {
+          if constexpr (P == 1 && j == 8) {            // the second half has its fragments; from here on the next tiles' are read
+            wait_vmcnt<0>();
+            wait_lgkmcnt0();
+            __syncthreads();                           // the next 64 queries have landed, and everybody has read these
+            if (step + 2 < steps) issue(step + 2, step & 1);
+          }
+          const v16f zero = {};
+          st[P][ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[s & 3], kf[ct][s], j < 2 ? zero : st[P][ct], 0, 0, 0);
+          if constexpr (ct == 1) f[s & 3] = s < 4 ? read_q(s + 4, step & 1, P) : read_q(s - 4, (step + P) & 1, P ^ 1);
+        }
+        constexpr int c = j >> 3, r = (2 * j) & 15;
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[P ^ 1][c][r], a.scale_log2, -e[r >> 2][r & 3]));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[P ^ 1][c][r + 1], a.scale_log2, -e[r >> 2][(r & 3) + 1]));
+        part[2 * c] += p0, part[2 * c + 1] += p1;
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      sum[0] += part[0] + part[1], sum[1] += part[2] + part[3];
+    };
+    constexpr std::integral_constant<int, 0> first{};
+    constexpr std::integral_constant<int, 1> second{};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[1][0][r] = st[1][1][r] = -INFINITY;   // (in front of the first tile: nothing)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) e[q4] = v4f{0.f, 0.f, 0.f, 0.f};
     issue(0, 0);
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (steps > 1) issue(1, 1);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) f[s] = read_q(s, 0, 0);
     for (uint32_t step = 0; step < steps; ++step) {
-      wait_vmcnt<0>();
-      __syncthreads();                                 // this tile has landed, and everybody has read the one before it
-      if (step + 1 < steps) issue(step + 1, (step + 1) & 1);
-      compute(step, step & 1);
+      const uint32_t t = t0 + step / a.rep * kQueries;
+      tile(first, std::true_type{}, step);
+      mask(first, t);
+      read_e(step, 0);
+      tile(second, std::true_type{}, step);
+      mask(second, t + 32);
+      read_e(step, 1);
     }
+    tile(first, std::false_type{}, 0);
   }
 #pragma unroll
   for (int ct = 0; ct < 2; ++ct) {
@@ -592,7 +616,9 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const Columns a, uint3
   const uint32_t bg = blockIdx.x / a.blocks, j = blockIdx.x % a.blocks * kSlots + threadIdx.x;
   if (j >= a.past + a.T) return;
   float sum = 0.f;
-  for (uint32_t c = 0; c < a.chunks; ++c) sum += a.parts[((size_t)c * units + bg) * a.pitch + j];
+  uint32_t c = 0;
+  while (blockIdx.x % a.blocks >= a.live_blocks(c)) ++c;   // (the first that sees the block; the last sees all)
+  for (; c < a.chunks; ++c) sum += a.parts[((size_t)c * units + bg) * a.pitch + j];
   a.weights[(size_t)bg * a.max_len + j] += sum;
 }
 
@@ -724,6 +750,8 @@ void cut_columns(Columns& a, uint32_t B) {
   a.chunk = (uint32_t)((tiles + chunks - 1) / chunks) * kQueries;
   a.chunks = (a.T + a.chunk - 1) / a.chunk;
   a.pitch = a.blocks * kSlots;
+  a.pairs = 0;
+  for (uint32_t c = 0; c < a.chunks; ++c) a.pairs += a.live_blocks(c);
 }
 size_t lse_floats(uint32_t B, uint32_t T, uint32_t Hq) { return ((size_t)B * T * Hq + 3) / 4 * 4; }
 }  // namespace
@@ -760,7 +788,7 @@ extern "C" int flh_prefill_attention_weights_f16(const flh_half* q, const flh_ha
   if (int rc = prefill_attention(a.q, a.k, (const __half*)v_cache, (__half*)out, (float*)workspace, B, T, Hq, Hkv, head_dim, past, max_len, scale, st))
     return rc;
   const uint32_t units = B * Hkv;
-  hipLaunchKernelGGL(column_weights_kernel, dim3(units * a.blocks * a.chunks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(column_weights_kernel, dim3(units * a.pairs), dim3(256), 0, st, a);
   if (int rc = check_launch("prefill_attention_weights")) return rc;
   if (a.chunks == 1) return FLH_OK;
   hipLaunchKernelGGL(column_sums_kernel, dim3(units * a.blocks), dim3(256), 0, st, a, units);
