@@ -35,70 +35,109 @@ struct Call {
   float scale_log2;
 };
 
-// The work of a call is one list of tiles of KT keys: for every sequence, every key / value head and every block of 32 WR query rows, the
-// tiles of the cache and then those of the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more
-// than the rounding of c, however the lengths differ, and nothing of it has to be known on the host.
-struct Plan {
-  uint32_t c, total;                                   // tiles of a workgroup, of all
-};
-
+// The work of a call is one list of tiles of KT keys: for every sequence and every key / value head, the tiles of the cache and then those of
+// the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more than the rounding of c, however the
+// lengths differ, and nothing of it has to be known on the host.  More than 32 WR query rows of a head are blocks of that many with a
+// workgroup each, next to each other, so that the second one finds the keys and values in its die's L2 (8 x 64 nodes of 32 / 8 heads behind
+// 8192 tokens, two blocks: 124 us when the blocks were units of the list, whose keys and values came from memory twice).
 template <int KT, bool TREE>
-__device__ __forceinline__ uint32_t tiles_of(const Call& a, uint32_t b) {
-  if (b >= a.B) return 0;
-  const long long n = a.lengths[b];
+__device__ __forceinline__ uint32_t tiles_for(const Call& a, long long n) {
   if (TREE) return n < 0 || n + a.T > a.max_len ? 0 : ((uint32_t)n + KT - 1) / KT + (a.T + KT - 1) / KT;
   return n <= 0 || n > a.max_len ? 0 : ((uint32_t)n + KT - 1) / KT;
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
 __device__ __forceinline__ uint32_t scan_up(uint32_t v) {   // inclusive sums over the wave's lanes
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t x = __shfl_up(v, d);
-    v += lane >= d ? x : 0;
-  }
-  return v;
+  v = add_dpp<0x111, 0xF>(v);                          // row_shr:1, 2, 4, 8 inside the rows of sixteen
+  v = add_dpp<0x112, 0xF>(v);
+  v = add_dpp<0x114, 0xF>(v);
+  v = add_dpp<0x118, 0xF>(v);
+  v = add_dpp<0x142, 0xA>(v);                          // row_bcast:15 into rows 1 and 3
+  return add_dpp<0x143, 0xC>(v);                       // row_bcast:31 into rows 2 and 3
 }
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
 
-template <int KT, bool TREE>
-__device__ __forceinline__ Plan plan_of(const Call& a) {
-  const int lane = threadIdx.x & 63;
-  uint32_t tiles = 0;
-  for (uint32_t b0 = 0; b0 < a.B; b0 += 64) tiles += (uint32_t)__shfl(scan_up(tiles_of<KT, TREE>(a, b0 + lane)), 63);
-  const uint32_t total = uniform(tiles) * (a.Hkv * a.row_blocks);
-  return {max(a.least, (total + a.groups - 1) / a.groups), total};
-}
-
-// tiles (over all heads and row blocks) in front of sequence `of`, or of the sequence that holds tile `of` (of_tile) and that sequence
+// A sequence: its slots taken, the tiles of one of its units, and those of all sequences before it
 struct Place {
-  uint32_t b, before, tiles;
+  uint32_t b, length, tiles, before;
 };
+
+// The sequences' tiles, 64 of them in the lanes at a time (the usual batch: one load and one scan for everything below)
 template <int KT, bool TREE>
-__device__ __forceinline__ Place place_of(const Call& a, uint32_t of, bool of_tile) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t per = a.Hkv * a.row_blocks;
-  uint32_t before = 0;
-  for (uint32_t b0 = 0;; b0 += 64) {
-    const uint32_t mine = tiles_of<KT, TREE>(a, b0 + lane) * per, up = scan_up(mine);
-    const unsigned long long hit = __ballot(of_tile ? before + up > of : b0 + lane == of);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      return {uniform(b0 + l), uniform(before + (uint32_t)__shfl(up - mine, l)), uniform((uint32_t)__shfl(mine, l) / per)};
-    }
-    before += (uint32_t)__shfl(up, 63);
-    if (b0 + 64 >= a.B) return {a.B, before, 0};       // (not reached: the tile is in the list, the sequence below B)
+struct Plan {
+  uint32_t c, total;                                   // tiles of a workgroup, of all
+  long long n;                                         // of the last 64 sequences looked at: lane's length, tiles, inclusive sum
+  uint32_t tiles, up, first, before;                   // .. the first of them, tiles before it
+
+  __device__ __forceinline__ void look(const Call& a, uint32_t b0) {
+    const uint32_t b = b0 + (threadIdx.x & 63);
+    n = b < a.B ? a.lengths[b] : -1;
+    tiles = tiles_for<KT, TREE>(a, n);
+    up = scan_up(tiles * a.Hkv);
+    first = b0;
   }
-}
+  __device__ __forceinline__ explicit Plan(const Call& a) {
+    total = 0;
+    for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+      look(a, b0);
+      before = total;
+      total += from_lane(up, 63);
+    }
+    c = max(a.least, (total + a.groups - 1) / a.groups);
+  }
+  __device__ __forceinline__ Place in_lane(const Call& a, int l) const {
+    const uint32_t t = from_lane(tiles, l);
+    return {first + l, from_lane((uint32_t)n, l), t, before + from_lane(up, l) - t * a.Hkv};
+  }
+  // the sequence b
+  __device__ __forceinline__ Place of(const Call& a, uint32_t b) {
+    if (b - first >= 64) {
+      before = 0;
+      for (uint32_t b0 = 0;; b0 += 64) {
+        look(a, b0);
+        if (b - b0 < 64) break;
+        before += from_lane(up, 63);
+      }
+    }
+    return in_lane(a, b - first);
+  }
+  // the sequence that holds tile `pos` (below total)
+  __device__ __forceinline__ Place at(const Call& a, uint32_t pos) {
+    if (a.B > 64) {
+      before = 0;
+      for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+        look(a, b0);
+        if (before + from_lane(up, 63) > pos) break;
+        before += from_lane(up, 63);
+      }
+    }
+    return in_lane(a, __builtin_ctzll(__ballot(before + up > pos)));
+  }
+};
 
 // floats of one piece of partial results: 32 WR rows of D sums, their maxima and sums
 template <int D, int WR>
 constexpr uint32_t kPiece = 32 * WR * (D + 2);
 
-// 1 KiB: lane i's 16 bytes at voff go to lds_base + 16 i
+// The thread's index anew: addresses that are made of it here are not computed in front of the loops and kept in registers across them
+__device__ __forceinline__ int thread_again() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// 1 KiB: lane i's 16 bytes at voff go to lds_base + 16 i (NT: past the caches)
+template <bool NT>
 __device__ __forceinline__ void load_rows_to_lds(const v4i& d, unsigned voff, unsigned lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_base), "v"(voff), "s"(d) : "memory", "m0");
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds_base), "v"(voff), "s"(d) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_base), "v"(voff), "s"(d) : "memory", "m0");
 }
 
 // Rows of D channels in LDS, 16-byte chunks XOR-swizzled by the row: K so that the 16 rows of a fragment read fall into different
@@ -113,14 +152,31 @@ struct Tile {
 };
 
 // (x0, x1): eight channels and their partners half a head further; the rotary embedding in float32, rounded once
-__device__ __forceinline__ void rotate8(h8& x0, h8& x1, const __half* cos, const __half* sin, int c, int half) {
+// (LOW: and what that leaves, rounded as well)
+template <bool LOW>
+__device__ __forceinline__ void rotate8(h8& x0, h8& x1, h8& l0, h8& l1, const __half* cos, const __half* sin, int c, int half) {
   const h8 c0 = *(const h8*)(cos + c), c1 = *(const h8*)(cos + c + half), s0 = *(const h8*)(sin + c), s1 = *(const h8*)(sin + c + half);
   const h8 a = x0, b = x1;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    x0[e] = (_Float16)round_here((float)a[e] * (float)c0[e] - (float)b[e] * (float)s0[e]);
-    x1[e] = (_Float16)round_here((float)b[e] * (float)c1[e] + (float)a[e] * (float)s1[e]);
+    const float y0 = round_here((float)a[e] * (float)c0[e] - (float)b[e] * (float)s0[e]);
+    const float y1 = round_here((float)b[e] * (float)c1[e] + (float)a[e] * (float)s1[e]);
+    x0[e] = (_Float16)y0, x1[e] = (_Float16)y1;
+    if constexpr (LOW) l0[e] = (_Float16)(y0 - (float)x0[e]), l1[e] = (_Float16)(y1 - (float)x1[e]);
   }
+}
+
+// zero for every value that is infinite or a NaN; whether there was one
+__device__ __forceinline__ bool finite8(h8& x) {
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = (float)x[e];
+    const bool is = !(v - v == 0.f);
+    odd |= is;
+    x[e] = is ? (_Float16)0.f : x[e];
+  }
+  return odd;
 }
 
 // The four waves of a workgroup are WR groups of 32 query rows (the queries of a key / value head: row t rep + i is head i of token t) times
@@ -130,35 +186,31 @@ __device__ __forceinline__ void rotate8(h8& x0, h8& x1, const __half* cos, const
 //   rounded to fp16 for the second product.
 // K and V of the cache come by direct-to-LDS loads, the next tile during the present one.  The tree's own tiles are staged by hand:
 // the keys have to be rotated, and go to the cache as well.
-template <int D, int WR, bool TREE>
+template <int D, int WR, bool TREE, bool NT>
 __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attention_kernel(const Call a) {
   constexpr int WK = 4 / WR, NKT = WR == 4 ? 2 : 1, KT = 32 * NKT * WK;
   constexpr int PITCH = D * 2, TILE = KT * PITCH, NI = TILE / 4096, RPI = 1024 / PITCH;   // loads of a wave per tile, rows of one load
-  constexpr int KS = D / 16, DT = D / 32;
+  constexpr int KS = D / 16, DT = D / 32, NF = NKT * KS;   // NF: fragments of K, and of V, that a wave reads per tile
   using L = Tile<D>;
   extern __shared__ __align__(1024) uint8_t lds[];     // K[2], V[2]; the waves' sums at the end of a segment
   __shared__ float s_m[4][32], s_l[4][32];
+  __shared__ unsigned s_odd[4];                        // rows of a tree's tile whose values are not all finite
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / WK, wk = wave % WK;
   const unsigned lds0 = (unsigned)(size_t)lds;
 
-  const uint32_t per = a.Hkv * a.row_blocks;
-  const Plan plan = plan_of<KT, TREE>(a);
-  const uint32_t g = xcd_contiguous(blockIdx.x, gridDim.x);
+  Plan<KT, TREE> plan(a);
+  const uint32_t index = xcd_contiguous(blockIdx.x, gridDim.x), g = index / a.row_blocks, block = index % a.row_blocks;
   uint32_t pos = g * plan.c;
   const uint32_t end = min(pos + plan.c, plan.total);
   if (g >= (plan.total + plan.c - 1) / plan.c) return;
-  const Place at = place_of<KT, TREE>(a, pos, true);
-  uint32_t b = at.b, tiles = at.tiles, unit = (pos - at.before) / tiles, tile = (pos - at.before) % tiles;
+  Place at = plan.at(a, pos);
+  uint32_t head = (pos - at.before) / at.tiles, tile = (pos - at.before) % at.tiles;
 
-  // addresses inside a tile
-  unsigned k_off[NI], v_off[NI];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int r = (wave * NI + i) * RPI + lane / L::CHUNKS, c = lane % L::CHUNKS;
-    k_off[i] = r * PITCH + ((c ^ L::k_swizzle(r)) << 4);
-    v_off[i] = r * PITCH + ((c ^ L::v_swizzle(r)) << 4);
-  }
+  // addresses inside a tile: row wave NI RPI + lane / CHUNKS of the first load, RPI rows further each (V's swizzle is the same there, K's
+  // differs in the bits of 4 i)
+  const int first_row = wave * NI * RPI + lane / L::CHUNKS;
+  const unsigned k_off = L::k_at(first_row, lane % L::CHUNKS), v_off = L::v_at(first_row, lane % L::CHUNKS);
   const int k_at = L::k_at(wk * NKT * 32 + n, h);      // + 32 PITCH per 32 keys; step s of 16 channels enters by XOR
   // transpose loads: lane i of 16 addresses the 8-byte piece i % 4 of the 32-byte run of channels that its group will own, in row i / 4
   const int grp = lane >> 4, gi = lane & 15;
@@ -168,36 +220,41 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
     tr_off[dt] = L::v_at(wk * NKT * 32 + 4 * (grp >> 1) + (gi >> 2), 4 * dt + ((grp & 1) << 1) + ((gi & 3) >> 1)) + ((gi & 1) << 3);
 
   for (;;) {
-    // ---- one segment: tiles [tile, last) of this unit
-    const uint32_t last = min(tiles, tile + (end - pos));
-    const uint32_t head = unit / a.row_blocks, block = unit % a.row_blocks;
-    const uint32_t length = (uint32_t)a.lengths[b];
+    // ---- one segment: tiles [tile, last) of this sequence and head
+    const uint32_t b = at.b, length = at.length, last = min(at.tiles, tile + (end - pos));
     const uint32_t cached = (length + KT - 1) / KT;    // tiles of the cache
     const size_t cache = ((size_t)b * a.Hkv + head) * a.max_len * D;
+    auto rows_from = [&](const __half* from, uint32_t t) {   // (rows past the length arrive as zeros)
+      return buffer_of((const uint8_t*)(from + cache + (size_t)t * KT * D), uniform(min((uint32_t)KT, length - t * KT)) * PITCH);
+    };
     auto issue = [&](uint32_t t, int buf) {
-      const unsigned bytes = uniform(min((uint32_t)KT, length - t * KT)) * PITCH;   // (rows past the length arrive as zeros)
-      const v4i dk = buffer_of((const uint8_t*)(a.k_cache + cache + (size_t)t * KT * D), bytes);
-      const v4i dv = buffer_of((const uint8_t*)(a.v_cache + cache + (size_t)t * KT * D), bytes);
+      const v4i dk = rows_from(a.k_cache, t), dv = rows_from(a.v_cache, t);
+      unsigned k = k_off, v = v_off;
+      asm volatile("" : "+v"(k), "+v"(v));             // (offsets kept across the tiles are registers there are not)
 #pragma unroll
-      for (int i = 0; i < NI; ++i) load_rows_to_lds(dk, k_off[i], lds0 + buf * TILE + (wave * NI + i) * 1024);
+      for (int i = 0; i < NI; ++i)
+        load_rows_to_lds<NT>(dk, (k ^ ((i & (D == 128 ? 3 : 1)) << 6)) + i * 1024, lds0 + buf * TILE + (wave * NI + i) * 1024);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) load_rows_to_lds(dv, v_off[i], lds0 + (2 + buf) * TILE + (wave * NI + i) * 1024);
+      for (int i = 0; i < NI; ++i) load_rows_to_lds<NT>(dv, v + i * 1024, lds0 + (2 + buf) * TILE + (wave * NI + i) * 1024);
     };
     const uint32_t cached_last = min(last, cached);
     if (tile < cached_last) issue(tile, 0);
 
     // this lane's query as B operand: channels 16 s + 8 h .. + 7 (rows past the last repeat it; they are not used)
-    const uint32_t row = min((block * WR + wr) * 32 + n, a.rows - 1), token = row / a.rep;
-    h8 qf[KS];
+    auto row_of = [&](int thread) { return min((block * WR + wr) * 32 + (thread & 31), a.rows - 1); };
+    h8 qf[KS], ql[TREE ? KS : 1];
     {
-      const size_t at_token = (size_t)b * a.T + token;
+      const int me = thread_again();
+      const uint32_t row = row_of(me), h = me >> 5 & 1;
+      const size_t at_token = (size_t)b * a.T + row / a.rep;
       const __half* src = a.q + (at_token * a.Hq + head * a.rep + row % a.rep) * D + 8 * h;
 #pragma unroll
       for (int s = 0; s < KS; ++s) qf[s] = *(const h8*)(src + 16 * s);
       if constexpr (TREE) {
 #pragma unroll
-        for (int s = 0; s < KS / 2; ++s)
-          rotate8(qf[s], qf[s + KS / 2], a.cos + at_token * D, a.sin + at_token * D, 16 * s + 8 * h, D / 2);
+        for (int s = 0; s < KS / 2; ++s) {
+          rotate8<true>(qf[s], qf[s + KS / 2], ql[s], ql[s + KS / 2], a.cos + at_token * D, a.sin + at_token * D, 16 * s + 8 * h, D / 2);
+        }
       }
     }
 
@@ -206,73 +263,90 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
-    float m_run = kLowest, l_run = 0.f;                // running maximum (scaled, base 2) and this lane's share of the sum
+    float m_run = kLowest, sum = 0.f;                  // running maximum (scaled, base 2) and this lane's share of the sum
 
     // register r of 32-key tile kt: key key0 + 32 kt + 8 (r / 4) + r % 4 of the tile
     const uint32_t key0 = wk * NKT * 32 + 4 * h;
-    auto compute = [&](int buf, uint32_t t, bool masked) {
-      v16f st[NKT];
-#pragma unroll
-      for (int kt = 0; kt < NKT; ++kt) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[kt][r] = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const h8 kf = *(const h8*)(lds + buf * TILE + kt * 32 * PITCH + (k_at ^ (s << 5)));
-          st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], st[kt], 0, 0, 0);
-        }
-      }
-      if (masked) {                                    // a tile of the tree, or the last of the cache
-        if (TREE && t >= cached) {
-          const uint8_t* seen = a.mask + (size_t)b * a.mask_stride + (size_t)token * a.T;
-#pragma unroll
-          for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const uint32_t j = (t - cached) * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3);
-              if (!(j < a.T && seen[min(j, a.T - 1)])) st[kt][r] = -INFINITY;
-            }
-        } else {
-#pragma unroll
-          for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (t * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3) >= length) st[kt][r] = -INFINITY;
-        }
-      }
-      if constexpr (!TREE) {                           // scores for the weights' launch
-        if ((block * WR + wr) * 32 + n < a.rows) {
-          float* to = a.scores + ((size_t)b * a.Hq + head * a.rep + row) * a.score_pitch;
-#pragma unroll
-          for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              const uint32_t j = t * KT + key0 + 32 * kt + 8 * q4;
-              const v4f x = {st[kt][4 * q4] * a.scale_log2, st[kt][4 * q4 + 1] * a.scale_log2, st[kt][4 * q4 + 2] * a.scale_log2,
-                             st[kt][4 * q4 + 3] * a.scale_log2};
-              if (j < length) *(v4f*)(to + j) = x;
-            }
-        }
-      }
-      float top = st[0][0];
+    v16f st[NKT];
+    h8 pb[NKT][2];
+    auto read_k = [&](int j, int buf) { return *(const h8*)(lds + buf * TILE + j % NKT * 32 * PITCH + (k_at ^ ((j / NKT) << 5))); };
+    auto read_v = [&](int j, int buf) {                // (channel tile j % DT of the 16 keys j / DT)
+      const uint8_t* v = lds + (2 + buf) * TILE + tr_off[j % DT] + j / DT * (16 * PITCH);
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)v);
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(v + 8 * PITCH));
+      return __builtin_bit_cast(h8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto clear = [&]() {
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, st[kt][r]);
+        for (int r = 0; r < 16; ++r) st[kt][r] = 0.f;
+    };
+    auto score = [&](int j, h8 kf) {
+      st[j % NKT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[j / NKT], st[j % NKT], 0, 0, 0);
+      if constexpr (TREE) st[j % NKT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[j / NKT], st[j % NKT], 0, 0, 0);
+    };
+    auto weigh = [&](int j, h8 vf) {
+      o[j % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[j / DT / 2][j / DT % 2], o[j % DT], 0, 0, 0);
+    };
+    // scores that the queries do not see: those behind the cache's last slot, those that the mask of the tree leaves out
+    auto mask_cached = [&](uint32_t t) {
+      if ((t + 1) * KT <= length) return;
+      asm volatile("" ::: "memory");                   // (a branch of its own: few tiles need it)
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (t * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3) >= length) st[kt][r] = -INFINITY;
+    };
+    auto mask_tree = [&](uint32_t t) {
+      const uint32_t token = row_of(thread_again()) / a.rep;
+      const uint8_t* seen = a.mask + (size_t)b * a.mask_stride + (size_t)token * a.T;
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t j = (t - cached) * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3);
+          if (!(j < a.T && seen[min(j, a.T - 1)])) st[kt][r] = -INFINITY;
+        }
+    };
+    auto keep_scores = [&](uint32_t t) {               // for the weights' launch
+      if ((block * WR + wr) * 32 + n < a.rows) {
+        float* to = a.scores + ((size_t)b * a.Hq + head * a.rep + row_of(thread_again())) * a.score_pitch;
+#pragma unroll
+        for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const uint32_t j = t * KT + key0 + 32 * kt + 8 * q4;
+            const v4f x = {st[kt][4 * q4] * a.scale_log2, st[kt][4 * q4 + 1] * a.scale_log2, st[kt][4 * q4 + 2] * a.scale_log2,
+                           st[kt][4 * q4 + 3] * a.scale_log2};
+            if (j < length) *(v4f*)(to + j) = x;
+          }
+      }
+    };
+    auto softmax = [&]() {                             // st -> pb; running maximum and sum, and the sums of values with them
+      float mx[2 * NKT];
+#pragma unroll
+      for (int c = 0; c < 2 * NKT; ++c) {
+        mx[c] = fmaxf(st[c >> 1][8 * (c & 1)], st[c >> 1][8 * (c & 1) + 1]);
+#pragma unroll
+        for (int r = 2; r < 8; ++r) mx[c] = fmaxf(mx[c], st[c >> 1][8 * (c & 1) + r]);
+      }
+      float top = fmaxf(mx[0], mx[1]);
+      if constexpr (NKT == 2) top = fmaxf(top, fmaxf(mx[2], mx[3]));
       const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_int(top), __float_as_int(top), false, false);
-      top = fmaxf(__int_as_float(halves[0]), __int_as_float(halves[1])) * a.scale_log2;
+      top = fmaxf(__int_as_float(halves[0]), __int_as_float(halves[1])) * a.scale_log2;   // (the scale is positive)
       const float m_new = fmaxf(m_run, top);
+      // rescale what has been added up -- unless no lane's maximum moved (the common case after the first tiles)
       if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-        l_run *= alpha;
+        sum *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
         m_run = m_new;
       }
-      float sum = 0.f;
-      h8 pb[NKT][2];
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
@@ -281,57 +355,74 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
           sum += p;
           pb[kt][r >> 3][r & 7] = (_Float16)p;
         }
-      l_run += sum;
+    };
+    auto compute = [&](int buf, auto mask) {
+      clear();
 #pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
+      for (int j = 0; j < NF; ++j) score(j, read_k(j, buf));
+      mask();
+      softmax();
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const uint8_t* v = lds + (2 + buf) * TILE + tr_off[dt] + (2 * kt + ks) * (16 * PITCH);
-            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)v);
-            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(v + 8 * PITCH));
-            const h8 vf = __builtin_bit_cast(h8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[kt][ks], o[dt], 0, 0, 0);
-          }
+      for (int j = 0; j < NF; ++j) weigh(j, read_v(j, buf));
     };
 
-    int buf = 0;
-    for (uint32_t t = tile; t < cached_last; ++t, buf ^= 1) {
+    for (uint32_t t = tile; t < cached_last; ++t) {
+      const int buf = (t - tile) & 1;
       wait_vmcnt<0>();
       __syncthreads();                                 // this tile has landed, and everybody has read the one before it
       if (t + 1 < cached_last) issue(t + 1, buf ^ 1);
-      compute(buf, t, (t + 1) * KT > length);
+      compute(buf, [&]() { mask_cached(t); });
+      if constexpr (!TREE) keep_scores(t);
     }
     if constexpr (TREE) {
       for (uint32_t t = max(tile, cached); t < last; ++t) {
+        if (tid < 4) s_odd[tid] = 0;
         __syncthreads();                               // (the buffers have been read)
         constexpr int PAIRS = L::CHUNKS / 2;
-        for (uint32_t i = tid; i < KT * PAIRS; i += 256) {
+        for (uint32_t i = thread_again(); i < KT * PAIRS; i += 256) {
           const uint32_t r = i / PAIRS, c = i % PAIRS, j = (t - cached) * KT + r;
           h8 k0 = {}, k1 = {}, v0 = {}, v1 = {};
           if (j < a.T) {
             const size_t at_token = (size_t)b * a.T + j, src = (at_token * a.Hkv + head) * D + 8 * c;
             k0 = *(const h8*)(a.k_new + src), k1 = *(const h8*)(a.k_new + src + D / 2);
             v0 = *(const h8*)(a.v_new + src), v1 = *(const h8*)(a.v_new + src + D / 2);
-            rotate8(k0, k1, a.cos + at_token * D, a.sin + at_token * D, 8 * c, D / 2);
+            h8 none;
+            rotate8<false>(k0, k1, none, none, a.cos + at_token * D, a.sin + at_token * D, 8 * c, D / 2);
             if (block == 0) {
               const size_t to = cache + ((size_t)length + j) * D + 8 * c;
               *(h8*)(a.k_cache + to) = k0, *(h8*)(a.k_cache + to + D / 2) = k1;
               *(h8*)(a.v_cache + to) = v0, *(h8*)(a.v_cache + to + D / 2) = v1;
             }
           }
+          // an infinite value or a NaN times the zero of a query that does not see it is a NaN: zero here, and added below
+          if (finite8(v0) | finite8(v1)) atomicOr(&s_odd[r >> 5], 1u << (r & 31));
           *(h8*)(lds + L::k_at(r, c)) = k0, *(h8*)(lds + L::k_at(r, c + PAIRS)) = k1;
           *(h8*)(lds + 2 * TILE + L::v_at(r, c)) = v0, *(h8*)(lds + 2 * TILE + L::v_at(r, c + PAIRS)) = v1;
         }
         __syncthreads();
-        compute(0, t, true);
+        compute(0, [&]() { mask_tree(t); });
+#pragma unroll
+        for (int w = 0; w < KT / 32; ++w)
+          for (unsigned odd = uniform(s_odd[w]); odd && w / NKT == wk; odd &= odd - 1) {
+            const uint32_t j = (t - cached) * KT + 32 * w + __builtin_ctz(odd);
+            const int me = thread_again();
+            if (!a.mask[(size_t)b * a.mask_stride + (size_t)(row_of(me) / a.rep) * a.T + j]) continue;
+            const _Float16* v = (const _Float16*)a.v_new + (((size_t)b * a.T + j) * a.Hkv + head) * D + 4 * (me >> 5 & 1);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const float x = (float)v[32 * dt + 8 * (r >> 2) + (r & 3)];
+                o[dt][r] += x - x == 0.f ? 0.f : x;
+              }
+          }
       }
     }
 
     // ---- the waves that share rows meet, then the segment's piece goes out: [row group][register quad][lane], maxima and sums behind
-    float l_all = l_run + lane_xor_f<32>(l_run);
-    float* piece = a.partials + (size_t)(g + b * per + unit) * kPiece<D, WR>;
+    const int me = thread_again(), lane = me & 63, n = me & 31, h = me >> 5 & 1;
+    float l_all = sum + lane_xor_f<32>(sum);
+    float* piece = a.partials + ((size_t)(g + b * a.Hkv + head) * a.row_blocks + block) * kPiece<D, WR>;
     __syncthreads();
     if constexpr (WK > 1) {
       if (h == 0) s_m[wave][n] = m_run, s_l[wave][n] = l_all;
@@ -370,31 +461,30 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
     }
     if (wk == 0 && h == 0) ((v2f*)(piece + 32 * WR * D))[wr * 32 + n] = v2f{m_run, l_all};
 
-    // ---- the next unit
+    // ---- the next head
     pos += last - tile;
     if (pos >= end) return;
     tile = 0;
-    if (++unit == per) {
-      unit = 0;
+    if (++head == a.Hkv) {
+      head = 0;
       do {
-        ++b;
-        tiles = uniform(tiles_of<KT, TREE>(a, b));
-      } while (tiles == 0 && b + 1 < a.B);
-      if (tiles == 0) return;                          // (not reached: there are tiles left)
+        if (at.b + 1 == a.B) return;                   // (not reached: there are tiles left)
+        at = plan.of(a, at.b + 1);
+      } while (at.tiles == 0);
     }
     __syncthreads();                                   // the sums have been read: the buffers are free
   }
 }
 
-// The segments of a unit: workgroups first .. last of the first launch
+// The segments of a sequence's head: pieces first .. first + count - 1, each as often as there are row blocks
 struct Segments {
-  uint32_t first, count;                               // pieces first .. first + count - 1
+  uint32_t first, count;
 };
 template <int KT, bool TREE>
-__device__ __forceinline__ Segments segments_of(const Call& a, const Plan& plan, const Place& at, uint32_t unit) {
+__device__ __forceinline__ Segments segments_of(const Call& a, const Plan<KT, TREE>& plan, const Place& at, uint32_t head) {
   if (at.tiles == 0) return {0, 0};
-  const uint32_t from = at.before + unit * at.tiles, first = from / plan.c, last = (from + at.tiles - 1) / plan.c;
-  return {first + at.b * (a.Hkv * a.row_blocks) + unit, last - first + 1};   // (piece g + unit: either grows from one piece to the next)
+  const uint32_t from = at.before + head * at.tiles, first = from / plan.c, last = (from + at.tiles - 1) / plan.c;
+  return {first + at.b * a.Hkv + head, last - first + 1};   // (piece g + b Hkv + head: either grows from one piece to the next)
 }
 
 // Workgroup (b, unit, row group, 32 channels): the pieces' sums weighted and added, out as fp16.  For attention weights, workgroups
@@ -404,31 +494,47 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const Call a) {
   constexpr int WK = 4 / WR, NKT = WR == 4 ? 2 : 1, KT = 32 * NKT * WK, DT = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t per = a.Hkv * a.row_blocks, outs = a.B * per * WR * DT;
-  const Plan plan = plan_of<KT, TREE>(a);
+  const uint32_t outs = a.B * a.Hkv * a.row_blocks * WR * DT;
+  const size_t stride = (size_t)a.row_blocks * kPiece<D, WR>;   // from one piece of a row block to its next
+  Plan<KT, TREE> plan(a);
   if (blockIdx.x < outs) {
-    const uint32_t dt = blockIdx.x % DT, wr = blockIdx.x / DT % WR, bu = blockIdx.x / (DT * WR), unit = bu % per;
-    const uint32_t head = unit / a.row_blocks, row = ((unit % a.row_blocks) * WR + wr) * 32 + n;
-    const Place at = place_of<KT, TREE>(a, bu / per, false);
-    const Segments seg = segments_of<KT, TREE>(a, plan, at, unit);
-    const float* piece = a.partials + (size_t)seg.first * kPiece<D, WR>;
+    const uint32_t dt = blockIdx.x % DT, wr = blockIdx.x / DT % WR, block = blockIdx.x / (DT * WR) % a.row_blocks;
+    const uint32_t bg = blockIdx.x / (DT * WR * a.row_blocks), b = bg / a.Hkv, head = bg % a.Hkv, row = (block * WR + wr) * 32 + n;
+    const Place at = plan.of(a, b);
+    const Segments seg = segments_of(a, plan, at, head);
+    const float* piece = a.partials + (size_t)seg.first * stride + block * kPiece<D, WR>;
     const uint32_t of_row = 32 * WR * D + (wr * 32 + n) * 2, of_sum = ((wr * DT * 4 + dt * 4 + wave) * 64 + lane) * 4;
-    float m = kLowest;
-    for (uint32_t i = 0; i < seg.count; ++i) m = fmaxf(m, piece[(size_t)i * kPiece<D, WR> + of_row]);
-    float l = 0.f;
+    float m = kLowest, l = 0.f;
     v4f x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (uint32_t i = 0; i < seg.count; ++i) {
-      const float* p = piece + (size_t)i * kPiece<D, WR>;
-      const v2f ml = *(const v2f*)(p + of_row);
-      const float w = __builtin_amdgcn_exp2f(ml[0] - m);
-      l = __builtin_fmaf(w, ml[1], l);
-      x += *(const v4f*)(p + of_sum) * w;
+    for (uint32_t i0 = 0; i0 < seg.count; i0 += 8) {   // eight pieces on their way at a time
+      v2f ml[8];
+      v4f y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* p = piece + min(i0 + i, seg.count - 1) * stride;
+        ml[i] = *(const v2f*)(p + of_row);
+        y[i] = *(const v4f*)(p + of_sum);
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= seg.count) ml[i] = v2f{kLowest, 0.f}, y[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        top = fmaxf(top, ml[i][0]);
+      }
+      const float keep = __builtin_amdgcn_exp2f(m - top);
+      l *= keep, x *= keep;
+      m = top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __builtin_amdgcn_exp2f(ml[i][0] - m);
+        l = __builtin_fmaf(w, ml[i][1], l);
+        x += y[i] * w;
+      }
     }
     if (row < a.rows) {
       const float inv = l > 0.f ? 1.f / l : 0.f;       // (a query that sees nothing: zeros)
       const h4 y = {(_Float16)(x[0] * inv), (_Float16)(x[1] * inv), (_Float16)(x[2] * inv), (_Float16)(x[3] * inv)};
-      __half* to = a.out + (((size_t)(bu / per) * a.T + row / a.rep) * a.Hq + head * a.rep + row % a.rep) * D;
+      __half* to = a.out + (((size_t)b * a.T + row / a.rep) * a.Hq + head * a.rep + row % a.rep) * D;
       *(h4*)(to + 32 * dt + 8 * wave + 4 * h) = y;
     }
     return;
@@ -437,34 +543,45 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const Call a) {
     __shared__ v2f stats[64];
     const uint32_t blocks = (a.max_len + 255) / 256, bg = (blockIdx.x - outs) / blocks, j = (blockIdx.x - outs) % blocks * 256 + tid;
     const uint32_t b = bg / a.Hkv, head = bg % a.Hkv;
-    const Place at = place_of<KT, TREE>(a, b, false);
-    const long long length = a.lengths[b];
-    if (at.tiles == 0 || (long long)(j - tid) >= length) return;
+    const Place at = plan.of(a, b);
+    const uint32_t length = at.length;
+    if (at.tiles == 0 || j - tid >= length) return;
+    float* to = a.weights + (size_t)bg * a.max_len + min(j, a.max_len - 1);
+    const float old = *to;
+    const Segments seg = segments_of(a, plan, at, head);
     float sum = 0.f;
     for (uint32_t r0 = 0; r0 < a.rows; r0 += 64) {
       __syncthreads();
       // a wave takes every fourth row, a lane of it every 64th segment
       for (uint32_t r = r0 + wave; r < min(a.rows, r0 + 64); r += 4) {
-        const Segments seg = segments_of<KT, TREE>(a, plan, at, head * a.row_blocks + r / (32 * WR));
-        const float* piece = a.partials + (size_t)seg.first * kPiece<D, WR> + 32 * WR * D + r % (32 * WR) * 2;
+        const float* piece = a.partials + (size_t)seg.first * stride + r / (32 * WR) * kPiece<D, WR> + 32 * WR * D + r % (32 * WR) * 2;
         float m = kLowest, l = 0.f;
-        for (uint32_t i = lane; i < seg.count; i += 64) m = fmaxf(m, piece[(size_t)i * kPiece<D, WR>]);
-        m = wave_max(m);
         for (uint32_t i = lane; i < seg.count; i += 64) {
-          const v2f ml = *(const v2f*)(piece + (size_t)i * kPiece<D, WR>);
-          l = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[0] - m), ml[1], l);
+          const v2f ml = *(const v2f*)(piece + i * stride);
+          const float top = fmaxf(m, ml[0]);
+          l = l * __builtin_amdgcn_exp2f(m - top) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - top);
+          m = top;
         }
-        l = wave_sum(l);
+        const float top = wave_max(m);
+        l = wave_sum(l * __builtin_amdgcn_exp2f(m - top));
+        m = top;
         if (lane == 0) stats[r - r0] = v2f{m, l > 0.f ? 1.f / l : 0.f};
       }
       __syncthreads();
       if (j < length) {
         const float* s = a.scores + ((size_t)b * a.Hq + head * a.rep + r0) * a.score_pitch + j;
-        for (uint32_t r = 0; r < min(a.rows - r0, 64u); ++r)
-          sum = __builtin_fmaf(__builtin_amdgcn_exp2f(s[(size_t)r * a.score_pitch] - stats[r][0]), stats[r][1], sum);
+        const uint32_t rows = min(a.rows - r0, 64u);
+        for (uint32_t r = 0; r < rows; r += 4) {
+          float x[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) x[i] = s[(size_t)min(r + i, rows - 1) * a.score_pitch];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i)
+            if (r + i < rows) sum = __builtin_fmaf(__builtin_amdgcn_exp2f(x[i] - stats[r + i][0]), stats[r + i][1], sum);
+        }
       }
     }
-    if (j < length) a.weights[(size_t)bg * a.max_len + j] += sum;
+    if (j < length) *to = old + sum;
   }
 }
 
@@ -636,11 +753,14 @@ int row_groups(uint64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 // piece of work ends at about the same time.
 uint32_t work_groups(uint32_t head_dim, int wr) { return head_dim == 128 && wr == 1 ? 256 : 512; }
 
-uint64_t units_of(uint32_t B, uint32_t Hkv, uint64_t rows) { return (uint64_t)B * Hkv * ((rows + 32 * row_groups(rows) - 1) / (32 * row_groups(rows))); }
+uint32_t row_blocks_of(uint64_t rows) { return (uint32_t)((rows + 32 * row_groups(rows) - 1) / (32 * row_groups(rows))); }
+uint32_t groups_of(uint32_t head_dim, uint64_t rows) {   // of one row block
+  return (work_groups(head_dim, row_groups(rows)) + row_blocks_of(rows) - 1) / row_blocks_of(rows);
+}
 
 size_t partial_bytes(uint32_t B, uint64_t rows, uint32_t Hkv, uint32_t head_dim) {
   const int wr = row_groups(rows);
-  return (work_groups(head_dim, wr) + units_of(B, Hkv, rows)) * (size_t)(32 * wr) * (head_dim + 2) * sizeof(float);
+  return rows ? (groups_of(head_dim, rows) + (size_t)B * Hkv) * row_blocks_of(rows) * (32 * wr) * (head_dim + 2) * sizeof(float) : 0;
 }
 
 template <int D, int WR, bool TREE>
@@ -648,13 +768,22 @@ int launch_rows(Call& a, hipStream_t stream) {
   constexpr int WK = 4 / WR, NKT = WR == 4 ? 2 : 1, KT = 32 * NKT * WK;
   constexpr size_t smem = 4 * (size_t)KT * D * 2;
   static_assert(WK == 1 || smem >= 4 * 32 * D * 4, "the waves' sums reuse the tiles");
-  a.row_blocks = (a.rows + 32 * WR - 1) / (32 * WR);
-  a.groups = work_groups(D, WR);
+  a.row_blocks = row_blocks_of(a.rows);
+  a.groups = groups_of(D, a.rows);
   a.least = WR;                                        // (a piece of partial results has half the bytes of WR tiles)
-  static LdsGrant grant;
-  if (int rc = reserve_lds((const void*)cache_attention_kernel<D, WR, TREE>, smem, grant, "cache attention")) return rc;
-  hipLaunchKernelGGL((cache_attention_kernel<D, WR, TREE>), dim3(a.groups), dim3(256), smem, stream, a);
-  if (int rc = check_launch("cache attention")) return rc;
+  auto go = [&](auto kern, LdsGrant& grant) {
+    if (int rc = reserve_lds((const void*)kern, smem, grant, "cache attention")) return rc;
+    hipLaunchKernelGGL(kern, dim3(a.groups * a.row_blocks), dim3(256), smem, stream, a);
+    return check_launch("cache attention");
+  };
+  static LdsGrant grant, grant_nt;
+  // A decode step reads its caches once: past the last-level cache (256 MB) if they do not fit it beside what else a step reads.  us: 16 x 4000
+  // slots of 32 / 8 heads (268 MB of caches) 55.4 -> 49.8; 8 x 1000 of 32 / 32 (134 MB) 32.2 -> 32.7
+  if (!TREE && WR == 1 && (uint64_t)a.B * a.Hkv * a.max_len * D * 4 > (192ull << 20)) {
+    if (int rc = go(cache_attention_kernel<D, WR, TREE, !TREE && WR == 1>, grant_nt)) return rc;
+  } else if (int rc = go(cache_attention_kernel<D, WR, TREE, false>, grant)) {
+    return rc;
+  }
   const uint64_t outs = (uint64_t)a.B * a.Hkv * a.row_blocks * WR * (D / 32), sums = TREE ? 0 : (uint64_t)a.B * a.Hkv * ((a.max_len + 255) / 256);
   hipLaunchKernelGGL((cache_combine_kernel<D, WR, TREE>), dim3((unsigned)(outs + sums)), dim3(256), 0, stream, a);
   return check_launch("cache attention (combine)");
@@ -675,8 +804,10 @@ int launch_call(Call& a, uint32_t head_dim, hipStream_t stream) {
 
 // tiles, rows and elements that fit the kernels' 32-bit counts
 bool too_large(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
-  const uint64_t rows = (uint64_t)T * (Hq / Hkv), units = units_of(B, Hkv, rows);
-  return rows > (1u << 24) || max_len > (1u << 30) || units > (1u << 24) || units * ((uint64_t)max_len / 64 + 8) > 0x7FFFFFFFull ||
+  const uint64_t rows = (uint64_t)T * (Hq / Hkv);
+  if (rows > (1u << 24)) return true;
+  const uint64_t units = (uint64_t)B * Hkv * row_blocks_of(rows);
+  return max_len > (1u << 30) || units > (1u << 24) || units * ((uint64_t)max_len / 64 + 8) > 0x7FFFFFFFull ||
          (uint64_t)B * Hkv * max_len * head_dim > (1ull << 40) || (uint64_t)B * T * Hq * head_dim > (1ull << 36);
 }
 

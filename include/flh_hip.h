@@ -455,8 +455,8 @@ int flh_decode_attention_f16_static(const flh_half* q, const flh_half* k_cache, 
  *   out [B, T, Hq * d] fp16.  Hq a multiple of Hkv, d 64 or 128.
  * The rotation x cos + rotate_half(x) sin is computed in float32 and rounded once; softmax statistics and sums in float32,
  * probabilities rounded to fp16 for the second product.  A node that sees nothing gets zeros.  A sequence whose length is negative
- * or above max_len - T takes no part: zeros as output, its cache untouched.  What a query does not see may hold anything, except
- * that the values v_new of the tree itself must be finite.
+ * or above max_len - T takes no part: zeros as output, its cache untouched.  What a query does not see may hold anything,
+ * infinities and NaN among it.
  * workspace: 16-byte aligned, flh_tree_attention_workspace_bytes(...) bytes, contents irrelevant; launches that share one must not
  * overlap. */
 size_t flh_tree_attention_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim);

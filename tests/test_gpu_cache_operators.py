@@ -120,7 +120,7 @@ def run_tree(ops, case, **more):
     out = ops.tree_attention(*dev, **more)
     torch.cuda.synchronize()
     for a, b in zip(dev[:7], before):
-        assert torch.equal(a, b)
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     return out, dev[7], dev[8]
 
 
@@ -179,6 +179,34 @@ def test_tree_attention_workspace_scale_and_peaks(ops):
     check_tree(ops, case, scale=0.01)
     flat = (case[0] * 0, *case[1:])
     check_tree(ops, flat)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,d", [(9, 4, 2, 128), (40, 4, 1, 64), (70, 2, 1, 128), (20, 2, 1, 128)])
+def test_tree_values_that_some_queries_do_not_see(ops, T, Hq, Hkv, d):
+    """Keys and values of the tree that are infinite or NaN reach the queries that see them, and no others."""
+    gen = torch.Generator().manual_seed(T)
+    case = list(tree_case(gen, 1, T, Hq, Hkv, d, [37], 256, "tree"))
+    mask = case[6]
+    odd = [T - 1, T // 2, T // 3]
+    ref_case = [t.clone() for t in case]
+    case[1][0, odd[0]] = float("nan")                                  # a key
+    case[2][0, odd[1], :, 3] = float("inf")                            # one channel of the values
+    case[2][0, odd[2], :, d - 5] = float("nan")
+    ref_case[6][:, odd[0]] = False                                     # (queries that see the key are not compared)
+    out, _, vc = run_tree(ops, case)
+    got = out.cpu().double().view(1, T, Hq, d)
+    ref, tol, _, _ = tree_oracle(ref_case)
+    for t in range(T):
+        if mask[t, odd[0]]:
+            assert torch.isnan(got[0, t]).all()
+            continue
+        skip = [c for j, c in ((odd[1], 3), (odd[2], d - 5)) if mask[t, j]]
+        for j, c in ((odd[1], 3), (odd[2], d - 5)):
+            if mask[t, j]:
+                assert not torch.isfinite(got[0, t, :, c]).any()
+        rest = [c for c in range(d) if c not in skip]
+        assert ((got[0, t] - ref[0, t]).abs() <= tol[0, 0])[:, rest].all()
+    assert torch.isinf(vc[0, :, 37 + odd[1], 3]).all() and torch.isnan(vc[0, :, 37 + odd[2], d - 5]).all()
 
 
 def test_tree_attention_zero_sizes(ops):
