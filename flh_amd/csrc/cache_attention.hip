@@ -46,19 +46,6 @@ __device__ __forceinline__ uint32_t tiles_for(const Call& a, long long n) {
   return n <= 0 || n > a.max_len ? 0 : ((uint32_t)n + KT - 1) / KT;
 }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
-  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ uint32_t scan_up(uint32_t v) {   // inclusive sums over the wave's lanes
-  v = add_dpp<0x111, 0xF>(v);                          // row_shr:1, 2, 4, 8 inside the rows of sixteen
-  v = add_dpp<0x112, 0xF>(v);
-  v = add_dpp<0x114, 0xF>(v);
-  v = add_dpp<0x118, 0xF>(v);
-  v = add_dpp<0x142, 0xA>(v);                          // row_bcast:15 into rows 1 and 3
-  return add_dpp<0x143, 0xC>(v);                       // row_bcast:31 into rows 2 and 3
-}
-
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 __device__ __forceinline__ uint32_t from_lane(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
 
@@ -78,7 +65,7 @@ struct Plan {
     const uint32_t b = b0 + (threadIdx.x & 63);
     n = b < a.B ? a.lengths[b] : -1;
     tiles = tiles_for<KT, TREE>(a, n);
-    up = scan_up(tiles * a.Hkv);
+    up = wave_scan(tiles * a.Hkv);
     first = b0;
   }
   __device__ __forceinline__ explicit Plan(const Call& a) {

@@ -158,7 +158,14 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const floa
     return;
   }
   if constexpr (STAGED) {
-    for (uint32_t i = tid; i < n; i += kSelectThreads) staged[i] = from[i];
+    for (uint32_t i0 = 0; i0 < n; i0 += 8 * kSelectThreads) {   // eight on their way at a time
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = from[min(i0 + k * kSelectThreads + tid, n - 1)];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (const uint32_t i = i0 + k * kSelectThreads + tid; i < n) staged[i] = x[k];
+    }
   }
   auto w = [&](uint32_t i) { return STAGED ? staged[i] : from[i]; };
   const uint32_t old = n - recent;                     // slots that are chosen from
@@ -179,12 +186,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const floa
     unsigned c[4], sum = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum += c[k] = count[kDigits - 1 - 4 * tid - k];
-    unsigned up = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const unsigned x = __shfl_up(up, d);
-      up += lane >= d ? x : 0;
-    }
+    unsigned up = wave_scan(sum);
     if (lane == 63) part[0][wave] = up;
     __syncthreads();
     for (int k = 0; k < wave; ++k) up += part[0][k];

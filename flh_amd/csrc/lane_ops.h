@@ -63,4 +63,19 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// v of the lane `CTRL` names, where the rows of sixteen in ROWS have one there, added
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned add_dpp(unsigned v) {
+  return v + (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+// inclusive sums over the wavefront's lanes
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+  v = add_dpp<0x111, 0xF>(v);                          // row_shr:1, 2, 4, 8 inside the rows
+  v = add_dpp<0x112, 0xF>(v);
+  v = add_dpp<0x114, 0xF>(v);
+  v = add_dpp<0x118, 0xF>(v);
+  v = add_dpp<0x142, 0xA>(v);                          // row_bcast:15 into rows 1 and 3
+  return add_dpp<0x143, 0xC>(v);                       // row_bcast:31 into rows 2 and 3
+}
+
 }  // namespace flh

@@ -73,6 +73,28 @@ def _rotate_half(x):
     return torch.cat((-x[..., half:], x[..., :half]), dim=-1)
 
 
+class DraftTree:
+    """A tree of drafted tokens (nodes), the same for every sequence of a batch: `parents` names each node's parent, a lower index;
+    node 0 is the root, the last token that is certain (parent -1).  On the device: `parents` int64 [T], `mask` bool [T, T] (whether
+    node i sees node j: its ancestors and itself) and `depths` int64 [T], how far behind the sequence a node's position is."""
+
+    def __init__(self, parents, device="cuda"):
+        parents = [int(p) for p in parents]
+        if not 1 <= len(parents) <= 256:
+            raise ValueError("a tree has 1 to 256 nodes")
+        if parents[0] != -1 or any(not 0 <= p < i for i, p in enumerate(parents) if i):
+            raise ValueError("node 0 is the root (parent -1); every other node's parent is a lower index")
+        mask = torch.eye(len(parents), dtype=torch.bool)
+        for i, p in enumerate(parents[1:], 1):
+            mask[i] |= mask[p]
+        self.parents = torch.tensor(parents, dtype=torch.int64, device=device)
+        self.depths = (mask.sum(1) - 1).to(device)
+        self.mask = mask.to(device)
+
+    def __len__(self):
+        return self.parents.numel()
+
+
 class StaticKVCache:
     """Preallocated fp16 keys / values [layers][batch, kv_heads, max_len, head_dim].  `layer(i)` is what a decoder layer
     takes as `kv_cache`: new keys / values are written in place at `positions` and attention reads the first `kv_len`
@@ -83,7 +105,12 @@ class StaticKVCache:
     derived from it, not from `positions` (a device tensor the host does not read): other positions would let queries
     see slots that are not theirs to see, or leave the new keys outside what attention reads.  `advance(T)` sets both
     together.  For the same reason a captured graph serves ONE `kv_len` (it is a launch parameter, fixed at capture):
-    replaying it after overwriting `positions` does not move the range attention reads -- capture one graph per length."""
+    replaying it after overwriting `positions` does not move the range attention reads -- capture one graph per length.
+
+    Drafted tokens.  `begin_drafts()` gives every sequence a length of its own, `lengths` (device int64 [batch], from then on in
+    place of kv_len): steps over a DraftTree write the nodes' keys / values behind it without moving it, and `commit` moves the
+    accepted ones there and it with them.  A captured step serves every length.  A sequence whose tree does not fit (length above
+    max_len - T) or whose length has been set negative takes no part in a step."""
 
     def __init__(self, layers, batch, kv_heads, max_len, head_dim, device, dtype=torch.float16, q_heads=None):
         self.keys = [torch.zeros(batch, kv_heads, max_len, head_dim, dtype=dtype, device=device) for _ in range(layers)]
@@ -91,6 +118,8 @@ class StaticKVCache:
         self.max_len = max_len
         self.kv_len = 0
         self._positions = torch.arange(max_len, dtype=torch.int64, device=device)   # advance() hands out views of it
+        self.lengths = None                 # of the sequences, once drafts have begun
+        self._tree_workspaces = {}          # scratch of the steps over drafts, by size: captured graphs keep theirs
         # the decode-attention kernel's scratch (partial results of the chunks), shared by the layers: they run in
         # order on one stream.  Owned here so that a captured graph finds it allocated.
         q_heads = q_heads or kv_heads * 8
@@ -115,6 +144,8 @@ class StaticKVCache:
     def advance(self, t):
         """Make room for `t` new tokens behind what the cache holds: kv_len grows by t; returns the positions
         arange(kv_len - t, kv_len) (device int64 [t]) the step has to be run with."""
+        if self.lengths is not None:
+            raise ValueError("the sequences of this cache have lengths of their own: it grows by commit()")
         if t < 1 or self.kv_len + t > self.max_len:
             raise ValueError(f"cannot advance a cache of {self.max_len} slots holding {self.kv_len} by {t}")
         self.kv_len += t
@@ -122,6 +153,48 @@ class StaticKVCache:
 
     def layer(self, index):
         return StaticKVCache._Layer(self, index)
+
+    class _TreeLayer:
+        """One layer of the cache in a step over drafted tokens."""
+
+        def __init__(self, owner, index, tree):
+            self.owner, self.index, self.tree = owner, index, tree
+
+        def attend(self, q, k, v, cos, sin):
+            """q [B, T, Hq, d], k / v [B, T, Hkv, d] of the nodes as projected, cos / sin [B, T, d] -> [B, T, Hq * d]"""
+            keys, values = self.owner.keys[self.index], self.owner.values[self.index]
+            return _ops().tree_attention(q, k, v, cos, sin, self.owner.lengths, self.tree.mask, keys, values,
+                                         workspace=self.owner._tree_workspace(q, k))
+
+    def tree_layer(self, index, tree):
+        """What a decoder layer takes as `kv_cache` in a step over the nodes of `tree` (positions None, cos / sin [B, T, d])."""
+        if self.lengths is None:
+            raise ValueError("begin_drafts() first: a step over drafted tokens needs the sequences' own lengths")
+        return StaticKVCache._TreeLayer(self, index, tree)
+
+    def _tree_workspace(self, q, k):
+        from .. import _lib
+        need = int(_lib.load().flh_tree_attention_workspace_bytes(q.size(0), q.size(1), q.size(2), k.size(2), q.size(3)))
+        ws = self._tree_workspaces.get(need)
+        if ws is None:
+            ws = self._tree_workspaces[need] = torch.empty(need, dtype=torch.uint8, device=q.device)
+        return ws
+
+    def begin_drafts(self):
+        """From here on the sequences have lengths of their own (all kv_len at first): steps over drafted tokens and commit()."""
+        if self.lengths is None:
+            self.lengths = torch.full((self.keys[0].size(0),), self.kv_len, dtype=torch.int64, device=self.keys[0].device)
+        return self.lengths
+
+    def commit(self, tokens, tree, chosen):
+        """After a step over `tree`: tokens [B, T] its nodes' tokens, chosen [B, T] the token that the model picks behind each node
+        -> (path, accepted, next token) as tree_commit_; the accepted nodes' rows move behind the sequences in all layers, and
+        `lengths` (the same tensor) with them."""
+        if self.lengths is None:
+            raise ValueError("begin_drafts() first")
+        path, accepted, following, lengths = _ops().tree_commit_(tokens, tree.parents, chosen, self.lengths, self.keys, self.values)
+        self.lengths.copy_(lengths)
+        return path, accepted, following
 
 
 def _stock_call(module, cls):
@@ -349,7 +422,8 @@ class W4A4DecoderLayer(torch.nn.Module):
 
     def attention(self, x, cos, sin, kv_cache=None, positions=None):
         """x [B, T, hidden] fp16 (already the residual stream); cos / sin [T, head_dim] of the T new positions;
-        kv_cache: None, a pair (keys, values) [B, kv_heads, past, head_dim] that grows by concatenation, or one layer
+        kv_cache: None, a pair (keys, values) [B, kv_heads, past, head_dim] that grows by concatenation, one layer of a
+        StaticKVCache in a step over drafted tokens (`tree_layer`; cos / sin [B, T, head_dim], positions None), or one layer
         of a StaticKVCache together with `positions` (device int64 [T]: the slots the new tokens take, which must be
         arange(kv_len - T, kv_len) for the cache's kv_len, the number of slots attention reads -- see StaticKVCache).
         Causal over past + T positions."""
@@ -368,14 +442,20 @@ class W4A4DecoderLayer(torch.nn.Module):
         else:
             x, s, z, q = self._residual_norm_quant("attn_in", self.input_layernorm, "input_layernorm",
                                                    self.attn_quantizer1, x, add, qkv)
-            mode = self._qkv_rope_applies(b * t, q, s, cos, kv_cache, positions)
+            tree = isinstance(kv_cache, StaticKVCache._TreeLayer)
+            mode = None if tree else self._qkv_rope_applies(b * t, q, s, cos, kv_cache, positions)
             if mode:
                 return self._attention_after_fused_qkv(x, q, s, z, cos, sin, kv_cache, positions, fold_residual, mode)
             qs, ks, vs = self._project(qkv, q, s, z)
         self._tap("q_proj", qs), self._tap("k_proj", ks), self._tap("v_proj", vs)
         static = isinstance(kv_cache, StaticKVCache._Layer)
         out = None
-        if (static and t == 1 and self.head_dim in (64, 128) and self.num_heads // self.num_kv_heads in (1, 2, 4, 8)
+        if isinstance(kv_cache, StaticKVCache._TreeLayer):
+            # drafted tokens against a cache with lengths of its own: rotary embedding, cache write and attention in two launches
+            out = kv_cache.attend(qs.view(b, t, self.num_heads, self.head_dim), ks.view(b, t, self.num_kv_heads, self.head_dim),
+                                  vs.view(b, t, self.num_kv_heads, self.head_dim), cos, sin)
+            cache = kv_cache
+        elif (static and t == 1 and self.head_dim in (64, 128) and self.num_heads // self.num_kv_heads in (1, 2, 4, 8)
                 and positions is not None):
             # one new token against the cache: rotary embedding, cache write and chunked attention in two launches
             keys, values = kv_cache.tensors()

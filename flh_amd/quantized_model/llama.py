@@ -290,6 +290,8 @@ class W4A4LlamaModel(torch.nn.Module):
         positions == arange(kv_len - T, kv_len) (what cache.advance(T) returns; see StaticKVCache for why nothing else
         is meaningful).  Returns logits [B, T, vocab] fp16 (or the final hidden state)."""
         if cache is not None:
+            if cache.lengths is not None:
+                raise ValueError("the sequences of this cache have lengths of their own: tree_step() (a tree of one node for one token)")
             t = input_ids.size(1)
             if positions.numel() != t or not 0 < t <= cache.kv_len <= cache.max_len:
                 raise ValueError(f"a step over {t} tokens needs {t} positions and a cache with {t} <= kv_len "
@@ -302,6 +304,28 @@ class W4A4LlamaModel(torch.nn.Module):
         for i, layer in enumerate(self.layers):
             x, pending, _ = layer.forward_deferred(x, pending, cos, sin, cache.layer(i) if cache is not None else None,
                                                    positions)
+        x = self._final_norm(x, pending)
+        return x if return_hidden else self._head(x)
+
+    def tree_step(self, input_ids, tree, cache, return_hidden=False):
+        """One step over drafted tokens: input_ids [B, T] int64, the tokens of the nodes of `tree` (a DraftTree), behind what
+        `cache` holds of each sequence (cache.begin_drafts() after the prompt) -> logits [B, T, vocab] fp16 (or the final hidden
+        state), row i those of the token behind node i.  The nodes' keys and values are in the cache behind cache.lengths; `cache.commit`
+        keeps the accepted ones.  Can be captured into a graph (after one eager step): it serves every length."""
+        b, t = input_ids.shape
+        if t != len(tree):
+            raise ValueError(f"{t} tokens for a tree of {len(tree)} nodes")
+        if cache.lengths is None:
+            raise ValueError("cache.begin_drafts() first")
+        if input_ids.size(0) != cache.lengths.numel():
+            raise ValueError(f"{b} sequences for a cache of {cache.lengths.numel()}")
+        # (a sequence that takes no part has no position: any row of the table will do)
+        positions = (cache.lengths[:, None] + tree.depths).clamp(0, cache.max_len - 1).reshape(-1)
+        x, cos, sin = self._look_up(input_ids, positions, cache)
+        cos, sin = cos.view(b, t, -1), sin.view(b, t, -1)
+        pending = None
+        for i, layer in enumerate(self.layers):
+            x, pending, _ = layer.forward_deferred(x, pending, cos, sin, cache.tree_layer(i, tree))
         x = self._final_norm(x, pending)
         return x if return_hidden else self._head(x)
 
