@@ -39,17 +39,18 @@ struct Call {
 // the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more than the rounding of c, however the
 // lengths differ, and nothing of it has to be known on the host.  More than 32 WR query rows of a head are blocks of that many with a
 // workgroup each, next to each other, so that the second one finds the keys and values in its die's L2 (8 x 64 nodes of 32 / 8 heads behind
-// 8192 tokens, two blocks: 124 us when the blocks were units of the list, whose keys and values came from memory twice).
+// 8192 tokens, two blocks, with the queries' high halves alone: 131 us with the blocks as units of the list, whose keys and values then
+// come from memory twice, 126 so).
 template <int KT, bool TREE>
 __device__ __forceinline__ uint32_t tiles_for(const Call& a, long long n) {
-  if (TREE) return n < 0 || n + a.T > a.max_len ? 0 : ((uint32_t)n + KT - 1) / KT + (a.T + KT - 1) / KT;
+  if (TREE) return n < 0 || n > (long long)a.max_len - a.T ? 0 : ((uint32_t)n + KT - 1) / KT + (a.T + KT - 1) / KT;
   return n <= 0 || n > a.max_len ? 0 : ((uint32_t)n + KT - 1) / KT;
 }
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 __device__ __forceinline__ uint32_t from_lane(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
 
-// A sequence: its slots taken, the tiles of one of its units, and those of all sequences before it
+// A sequence: its slots taken, the tiles of one of its heads, and those of all sequences before it
 struct Place {
   uint32_t b, length, tiles, before;
 };
@@ -173,6 +174,16 @@ __device__ __forceinline__ bool finite8(h8& x) {
 //   rounded to fp16 for the second product.
 // K and V of the cache come by direct-to-LDS loads, the next tile during the present one.  The tree's own tiles are staged by hand:
 // the keys have to be rotated, and go to the cache as well.
+//
+// A rotated query is rounded to fp16 as the cached keys are, but its rounding is kept as a second fp16 value with MFMAs of its own (ql): it
+// moves every score by 2^-11 of its size, twice the error of the result's own rounding (4.3e-4 against 2.1e-4 of the 2-norm).  That costs
+// 26.7 -> 28.6 us (2 x 63 nodes of 64 channels behind 5001 tokens), 126 -> 141 (8 x 64 of 128 behind 8192, where the MFMAs bound the launch).
+//
+// What bounds it: memory up to about 64 rows of a head (decode with weights, 16 x up to 4000 slots of 32 / 8 heads: 209 MB in 41 us, 5.1 TB/s,
+// where a large copy reads and writes 4.9), the MFMAs from there on (8 x 64 behind 8192: 104 Gflop with the low halves in 119 us = 0.87
+// PFLOP/s, where an 8192^3 product of the vendor's reaches 1.14).  Short calls are latencies: the lengths, then the queries and the first
+// tile, then the pieces in the second launch (1 x 8 behind 120: 8 + 3 us).  Not taken: fragments read during the MFMAs before them, as in
+// the prefill kernel (no gain, 131 against 130 us, or spills); tiles of a wave of its own two ahead without barriers (58.4 against 58.9 us).
 template <int D, int WR, bool TREE, bool NT>
 __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attention_kernel(const Call a) {
   constexpr int WK = 4 / WR, NKT = WR == 4 ? 2 : 1, KT = 32 * NKT * WK;
@@ -181,7 +192,7 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
   using L = Tile<D>;
   extern __shared__ __align__(1024) uint8_t lds[];     // K[2], V[2]; the waves' sums at the end of a segment
   __shared__ float s_m[4][32], s_l[4][32];
-  __shared__ unsigned s_odd[4];                        // rows of a tree's tile whose values are not all finite
+  __shared__ unsigned s_odd[2][4];                     // rows of a tree's tile whose values are not all finite, by the tile's parity
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / WK, wk = wave % WK;
   const unsigned lds0 = (unsigned)(size_t)lds;
@@ -363,7 +374,7 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
     }
     if constexpr (TREE) {
       for (uint32_t t = max(tile, cached); t < last; ++t) {
-        if (tid < 4) s_odd[tid] = 0;
+        if (tid < 4) s_odd[t & 1][tid] = 0;            // (last read two tiles ago)
         __syncthreads();                               // (the buffers have been read)
         constexpr int PAIRS = L::CHUNKS / 2;
         for (uint32_t i = thread_again(); i < KT * PAIRS; i += 256) {
@@ -382,7 +393,7 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
             }
           }
           // an infinite value or a NaN times the zero of a query that does not see it is a NaN: zero here, and added below
-          if (finite8(v0) | finite8(v1)) atomicOr(&s_odd[r >> 5], 1u << (r & 31));
+          if (finite8(v0) | finite8(v1)) atomicOr(&s_odd[t & 1][r >> 5], 1u << (r & 31));
           *(h8*)(lds + L::k_at(r, c)) = k0, *(h8*)(lds + L::k_at(r, c + PAIRS)) = k1;
           *(h8*)(lds + 2 * TILE + L::v_at(r, c)) = v0, *(h8*)(lds + 2 * TILE + L::v_at(r, c + PAIRS)) = v1;
         }
@@ -390,7 +401,7 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
         compute(0, [&]() { mask_tree(t); });
 #pragma unroll
         for (int w = 0; w < KT / 32; ++w)
-          for (unsigned odd = uniform(s_odd[w]); odd && w / NKT == wk; odd &= odd - 1) {
+          for (unsigned odd = uniform(s_odd[t & 1][w]); odd && w / NKT == wk; odd &= odd - 1) {
             const uint32_t j = (t - cached) * KT + 32 * w + __builtin_ctz(odd);
             const int me = thread_again();
             if (!a.mask[(size_t)b * a.mask_stride + (size_t)(row_of(me) / a.rep) * a.T + j]) continue;
@@ -474,7 +485,7 @@ __device__ __forceinline__ Segments segments_of(const Call& a, const Plan<KT, TR
   return {first + at.b * a.Hkv + head, last - first + 1};   // (piece g + b Hkv + head: either grows from one piece to the next)
 }
 
-// Workgroup (b, unit, row group, 32 channels): the pieces' sums weighted and added, out as fp16.  For attention weights, workgroups
+// Workgroup (b, head, row block, row group, 32 channels): the pieces' sums weighted and added, out as fp16.  For attention weights, workgroups
 // behind those: (b, head, 256 slots), the stored scores -> probabilities, summed over the rows, added to the weights.
 template <int D, int WR, bool TREE>
 __global__ __launch_bounds__(256) void cache_combine_kernel(const Call a) {

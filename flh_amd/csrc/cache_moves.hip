@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void tree_commit_kernel(Caches caches, Tree t,
   __shared__ uint32_t s_count;
   const uint32_t b = blockIdx.x, layer = blockIdx.y;
   const long long n = t.lengths[b];
-  const bool active = n >= 0 && n + t.T <= t.max_len;
+  const bool active = n >= 0 && n <= (long long)t.max_len - t.T;
   const bool tells = first && layer == 0 && blockIdx.z == 0;
   if (threadIdx.x < 64) {
     long long want = -1;

@@ -72,6 +72,7 @@ def tree_case(gen, B, T, Hq, Hkv, d, lengths, max_len, kind, qscale=1.0):
     mask = random_mask(gen, kind, B, T)
     kc, vc = normal(gen, B, Hkv, max_len, d), normal(gen, B, Hkv, max_len, d)
     for b, n in enumerate(lengths):                                    # what lies behind a sequence is not looked at
+        n = min(n, max_len)
         kc[b, :, max(n, 0):] = float("nan")
         vc[b, :, max(n, 0):] = float("inf") if b % 2 else float("nan")
     return q, k, v, angle.cos().half(), angle.sin().half(), torch.tensor(lengths), mask, kc, vc
@@ -150,6 +151,7 @@ TREES = [
     (2, 33, 4, 4, 64, [0, 65], 128, "random"),                         # rows that see nothing at all
     (2, 63, 16, 4, 64, [1000, 777], 1063, "tree-each"),
     (4, 5, 12, 4, 64, [-1, 100, 124, 123], 128, "tree"),               # no sequence, and one whose tree does not fit
+    (4, 3, 4, 2, 128, [2 ** 63 - 1, -2 ** 63, 7, 2 ** 32 + 5], 64, "tree"),
     (1, 64, 32, 4, 128, [2049], 2200, "tree"),
     (1, 256, 2, 1, 128, [70], 400, "random-each"),
     (2, 100, 3, 1, 64, [31, 32], 200, "tree"),
@@ -181,7 +183,7 @@ def test_tree_attention_workspace_scale_and_peaks(ops):
     check_tree(ops, flat)
 
 
-@pytest.mark.parametrize("T,Hq,Hkv,d", [(9, 4, 2, 128), (40, 4, 1, 64), (70, 2, 1, 128), (20, 2, 1, 128)])
+@pytest.mark.parametrize("T,Hq,Hkv,d", [(9, 4, 2, 128), (40, 4, 1, 64), (70, 2, 1, 128), (20, 2, 1, 128), (200, 1, 1, 64), (219, 1, 1, 128)])
 def test_tree_values_that_some_queries_do_not_see(ops, T, Hq, Hkv, d):
     """Keys and values of the tree that are infinite or NaN reach the queries that see them, and no others."""
     gen = torch.Generator().manual_seed(T)
@@ -316,6 +318,8 @@ def test_tree_commit(ops, B, T, layers, Hkv, d, max_len, per_sequence):
     lengths = [int(x) for x in rng.integers(0, max_len - T + 1, B)]
     if B > 2:
         lengths[1], lengths[2] = -1, max_len - T + 1
+    if B > 3:
+        lengths[3] = 2 ** 63 - 1
     caches = [normal(gen, B, Hkv, max_len, d) for _ in range(2 * layers)]
     path, accepted, following, new, ref = commit_oracle(tokens, parents, chosen, lengths, caches, max_len)
     dev = [torch.from_numpy(x).cuda() for x in (tokens, parents, chosen)]
@@ -353,7 +357,7 @@ def weights_tolerance(size, d, n, rows, added, total):
 
 
 @pytest.mark.parametrize("B,Hq,Hkv,d,lengths,max_len", [(1, 32, 8, 128, [2048], 2048), (3, 8, 8, 128, [1, 64, 65], 100),
-                                                        (4, 16, 4, 64, [0, 777, -3, 1001], 1000), (2, 12, 4, 64, [333, 31], 400),
+                                                        (4, 16, 4, 64, [0, 777, -3, 1001], 1000), (3, 4, 2, 128, [2 ** 63 - 1, 30, 2 ** 32 + 1], 64), (2, 12, 4, 64, [333, 31], 400),
                                                         (5, 64, 2, 128, [129, 500, 2, 1023, 1024], 1024), (1, 3, 1, 128, [4500], 4501),
                                                         (66, 2, 2, 64, [i for i in range(66)], 70), (1, 128, 1, 128, [300], 320)])
 def test_decode_attention_weights(ops, B, Hq, Hkv, d, lengths, max_len):
@@ -362,7 +366,7 @@ def test_decode_attention_weights(ops, B, Hq, Hkv, d, lengths, max_len):
     q = normal(gen, B, Hq, d, scale=2.0)
     kc, vc = normal(gen, B, Hkv, max_len, d), normal(gen, B, Hkv, max_len, d)
     for b, n in enumerate(lengths):
-        kc[b, :, max(n, 0):], vc[b, :, max(n, 0):] = float("nan"), float("inf")
+        kc[b, :, max(min(n, max_len), 0):], vc[b, :, max(min(n, max_len), 0):] = float("nan"), float("inf")
     weights = torch.rand(B, Hkv, max_len, generator=gen)
     args = [q.cuda(), kc.cuda(), vc.cuda(), torch.tensor(lengths).cuda()]
     dev = weights.cuda()
@@ -473,7 +477,7 @@ def evict_oracle(caches, weights, lengths, budget, recent, max_len):
 @pytest.mark.parametrize("L,B,Hkv,d,max_len,lengths,budget,recent,kind",
                          [(1, 1, 1, 128, 64, [64], 32, 4, "random"), (2, 3, 2, 128, 300, [300, 100, 257], 100, 100, "random"),
                           (3, 2, 2, 64, 700, [513, 700], 511, 0, "ties"), (130, 1, 1, 8, 40, [33], 17, 5, "ties"),
-                          (1, 4, 1, 128, 64, [-1, 0, 65, 10], 10, 3, "random"), (2, 2, 2, 128, 1025, [1025, 1024], 1024, 7, "equal"),
+                          (1, 4, 1, 128, 64, [-1, 0, 65, 10], 10, 3, "random"), (1, 2, 1, 64, 64, [2 ** 63 - 1, 2 ** 32 + 9], 10, 3, "random"), (2, 2, 2, 128, 1025, [1025, 1024], 1024, 7, "equal"),
                           (1, 1, 2, 128, 2100, [2100], 1, 0, "random"), (1, 2, 1, 24, 500, [400, 500], 130, 20, "odd"),
                           (1, 1, 1, 128, 5000, [4999], 2500, 100, "front"), (1, 1, 1, 64, 9000, [9000], 4500, 1, "log")])
 def test_evict(ops, L, B, Hkv, d, max_len, lengths, budget, recent, kind):
