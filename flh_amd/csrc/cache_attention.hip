@@ -31,12 +31,12 @@ struct Call {
   const uint8_t* mask;
   __half *k_cache, *v_cache, *out;
   float *partials, *scores, *weights;                  // scores, weights: attention weights only
-  uint32_t mask_stride, B, T, Hq, Hkv, rep, rows, row_blocks, max_len, score_pitch, groups, least;
+  uint32_t mask_stride, B, T, Hq, Hkv, rep, rows, row_blocks, max_len, score_pitch, groups;
   float scale_log2;
 };
 
 // The work of a call is one list of tiles of KT keys: for every sequence and every key / value head, the tiles of the cache and then those of
-// the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more than the rounding of c, however the
+// the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more than the rounding of c (one tile at least: 4 x 40 nodes of 32 / 8 heads behind up to 300, four tiles at least 34.1 us, one 26.4), however the
 // lengths differ, and nothing of it has to be known on the host.  More than 32 WR query rows of a head are blocks of that many with a
 // workgroup each, next to each other, so that the second one finds the keys and values in its die's L2 (8 x 64 nodes of 32 / 8 heads behind
 // 8192 tokens, two blocks, with the queries' high halves alone: 131 us with the blocks as units of the list, whose keys and values then
@@ -76,7 +76,7 @@ struct Plan {
       before = total;
       total += from_lane(up, 63);
     }
-    c = max(a.least, (total + a.groups - 1) / a.groups);
+    c = max(1u, (total + a.groups - 1) / a.groups);
   }
   __device__ __forceinline__ Place in_lane(const Call& a, int l) const {
     const uint32_t t = from_lane(tiles, l);
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
     auto weigh = [&](int j, h8 vf) {
       o[j % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[j / DT / 2][j / DT % 2], o[j % DT], 0, 0, 0);
     };
-    // scores that the queries do not see: those behind the cache's last slot, those that the mask of the tree leaves out
+    // scores that the queries do not see: those behind the cache's last slot
     auto mask_cached = [&](uint32_t t) {
       if ((t + 1) * KT <= length) return;
       asm volatile("" ::: "memory");                   // (a branch of its own: few tiles need it)
@@ -296,17 +296,6 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (t * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3) >= length) st[kt][r] = -INFINITY;
-    };
-    auto mask_tree = [&](uint32_t t) {
-      const uint32_t token = row_of(thread_again()) / a.rep;
-      const uint8_t* seen = a.mask + (size_t)b * a.mask_stride + (size_t)token * a.T;
-#pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const uint32_t j = (t - cached) * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3);
-          if (!(j < a.T && seen[min(j, a.T - 1)])) st[kt][r] = -INFINITY;
-        }
     };
     auto keep_scores = [&](uint32_t t) {               // for the weights' launch
       if ((block * WR + wr) * 32 + n < a.rows) {
@@ -376,6 +365,17 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
       for (uint32_t t = max(tile, cached); t < last; ++t) {
         if (tid < 4) s_odd[t & 1][tid] = 0;            // (last read two tiles ago)
         __syncthreads();                               // (the buffers have been read)
+        // the mask's bytes of this lane's query and keys, requested in front of what takes their time to arrive
+        uint8_t seen[NKT][16];
+        {
+          const int me = thread_again();
+          const uint8_t* from = a.mask + (size_t)b * a.mask_stride + (size_t)(row_of(me) / a.rep) * a.T;
+          const uint32_t first = (t - cached) * KT + wk * NKT * 32 + 4 * (me >> 5 & 1);
+#pragma unroll
+          for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) seen[kt][r] = from[min(first + 32 * kt + 8 * (r >> 2) + (r & 3), a.T - 1)];
+        }
         constexpr int PAIRS = L::CHUNKS / 2;
         for (uint32_t i = thread_again(); i < KT * PAIRS; i += 256) {
           const uint32_t r = i / PAIRS, c = i % PAIRS, j = (t - cached) * KT + r;
@@ -398,7 +398,13 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
           *(h8*)(lds + 2 * TILE + L::v_at(r, c)) = v0, *(h8*)(lds + 2 * TILE + L::v_at(r, c + PAIRS)) = v1;
         }
         __syncthreads();
-        compute(0, [&]() { mask_tree(t); });
+        compute(0, [&]() {
+#pragma unroll
+          for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (!seen[kt][r] || (t - cached) * KT + key0 + 32 * kt + 8 * (r >> 2) + (r & 3) >= a.T) st[kt][r] = -INFINITY;
+        });
 #pragma unroll
         for (int w = 0; w < KT / 32; ++w)
           for (unsigned odd = uniform(s_odd[t & 1][w]); odd && w / NKT == wk; odd &= odd - 1) {
@@ -768,7 +774,6 @@ int launch_rows(Call& a, hipStream_t stream) {
   static_assert(WK == 1 || smem >= 4 * 32 * D * 4, "the waves' sums reuse the tiles");
   a.row_blocks = row_blocks_of(a.rows);
   a.groups = groups_of(D, a.rows);
-  a.least = WR;                                        // (a piece of partial results has half the bytes of WR tiles)
   auto go = [&](auto kern, LdsGrant& grant) {
     if (int rc = reserve_lds((const void*)kern, smem, grant, "cache attention")) return rc;
     hipLaunchKernelGGL(kern, dim3(a.groups * a.row_blocks), dim3(256), smem, stream, a);

@@ -359,7 +359,8 @@ def weights_tolerance(size, d, n, rows, added, total):
 @pytest.mark.parametrize("B,Hq,Hkv,d,lengths,max_len", [(1, 32, 8, 128, [2048], 2048), (3, 8, 8, 128, [1, 64, 65], 100),
                                                         (4, 16, 4, 64, [0, 777, -3, 1001], 1000), (3, 4, 2, 128, [2 ** 63 - 1, 30, 2 ** 32 + 1], 64), (2, 12, 4, 64, [333, 31], 400),
                                                         (5, 64, 2, 128, [129, 500, 2, 1023, 1024], 1024), (1, 3, 1, 128, [4500], 4501),
-                                                        (66, 2, 2, 64, [i for i in range(66)], 70), (1, 128, 1, 128, [300], 320)])
+                                                        (66, 2, 2, 64, [i for i in range(66)], 70), (1, 128, 1, 128, [300], 320),
+                                                        (2, 320, 1, 64, [70, 33], 80)])
 def test_decode_attention_weights(ops, B, Hq, Hkv, d, lengths, max_len):
     gen = torch.Generator().manual_seed(B + Hq)
     print(f"case decode weights B={B} Hq={Hq} Hkv={Hkv} d={d} max={max_len}", flush=True)
@@ -517,6 +518,41 @@ def test_evict_a_single_pair_of_tensors(ops):
     assert n.tolist() == [20] and tuple(kept.shape) == (1, 1, 2, 20)
     at = kept[0][..., None].expand(1, 2, 20, 64)
     assert torch.equal(k[:, :, :20], kk.gather(2, at)) and torch.equal(v[:, :, :20], vv.gather(2, at))
+
+
+# ---------------------------------------------------------------------------------------------------- sizes
+def test_offsets_beyond_32_bits(ops):
+    """A cache whose last heads lie more than 4 GiB behind its start, against the same slots in a small one: the same bits."""
+    gen = torch.Generator().manual_seed(8)
+    B, T, Hq, Hkv, d, n, small, large = 1, 6, 34, 17, 128, 100, 128, 1 << 20
+    case = [t.cuda() for t in tree_case(gen, B, T, Hq, Hkv, d, [n], small, "tree")]
+    big = [torch.empty(B, Hkv, large, d, dtype=torch.float16, device="cuda") for _ in range(2)]
+    for b, s in zip(big, case[7:]):
+        b[:, :, :small] = s
+    assert big[0].stride(1) * (Hkv - 1) * 2 >= 2 ** 32
+
+    def same():
+        return all(equal_bits(b[:, :, :small], s) for b, s in zip(big, case[7:]))
+    assert torch.equal(ops.tree_attention(*case[:7], *big), ops.tree_attention(*case))
+    assert same()
+    parents, tokens = torch.tensor([-1, 0, 0, 1, 2, 4]).cuda(), torch.arange(6)[None].cuda()
+    chosen = torch.tensor([[2, 9, 4, 9, 5, 9]]).cuda()
+    got = ops.tree_commit_(tokens, parents, chosen, case[5], *big)
+    ref = ops.tree_commit_(tokens, parents, chosen, case[5], *case[7:])
+    assert all(torch.equal(a, b) for a, b in zip(got, ref)) and got[1].tolist() == [4] and same()
+    q = normal(gen, B, Hq, d).cuda()
+    w = torch.rand(B, Hkv, small, generator=gen).cuda()
+    wide = torch.zeros(B, Hkv, large, device="cuda")
+    wide[:, :, :small] = w
+    assert torch.equal(ops.decode_attention_weights(q, *big, got[3], wide), ops.decode_attention_weights(q, *case[7:], got[3], w))
+    assert torch.equal(wide[:, :, :small], w)
+    qs = normal(gen, B, 40, Hq, d).cuda()
+    assert torch.equal(ops.prefill_attention_weights(qs, *big, 60, wide), ops.prefill_attention_weights(qs, *case[7:], 60, w))
+    assert torch.equal(wide[:, :, :small], w)
+    got = ops.evict_kv_cache_(*big, wide[None], got[3], 50, 9)         # (weights of more slots than are staged at once)
+    ref = ops.evict_kv_cache_(*case[7:], w[None], ref[3], 50, 9)
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1][..., :small], ref[1]) and torch.equal(got[2], ref[2]) and same()
+    assert not got[1][..., small:].any()
 
 
 # ---------------------------------------------------------------------------------------------------- together
