@@ -31,13 +31,12 @@ struct Call {
   const uint8_t* mask;
   __half *k_cache, *v_cache, *out;
   float *partials, *scores, *weights;                  // scores, weights: attention weights only
-  uint32_t mask_stride, B, T, Hq, Hkv, rep, rows, row_blocks, max_len, score_pitch, groups;
+  uint32_t mask_stride, B, T, Hq, Hkv, rep, rows, row_blocks, max_len, score_pitch, groups, few;
   float scale_log2;
 };
 
 // The work of a call is one list of tiles of KT keys: for every sequence and every key / value head, the tiles of the cache and then those of
-// the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more than the rounding of c (one tile at least: 4 x 40 nodes of 32 / 8 heads behind up to 300, four tiles at least 34.1 us, one 26.4), however the
-// lengths differ, and nothing of it has to be known on the host.  More than 32 WR query rows of a head are blocks of that many with a
+// the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more than the rounding of c, however the lengths differ, and nothing of it has to be known on the host.  More than 32 WR query rows of a head are blocks of that many with a
 // workgroup each, next to each other, so that the second one finds the keys and values in its die's L2 (8 x 64 nodes of 32 / 8 heads behind
 // 8192 tokens, two blocks, with the queries' high halves alone: 131 us with the blocks as units of the list, whose keys and values then
 // come from memory twice, 126 so).
@@ -76,7 +75,8 @@ struct Plan {
       before = total;
       total += from_lane(up, 63);
     }
-    c = max(1u, (total + a.groups - 1) / a.groups);
+    const uint32_t groups = total <= a.few * 8 ? a.few : a.groups;
+    c = max(1u, (total + groups - 1) / groups);
   }
   __device__ __forceinline__ Place in_lane(const Call& a, int l) const {
     const uint32_t t = from_lane(tiles, l);
@@ -198,10 +198,11 @@ __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attent
   const unsigned lds0 = (unsigned)(size_t)lds;
 
   Plan<KT, TREE> plan(a);
-  const uint32_t index = xcd_contiguous(blockIdx.x, gridDim.x), g = index / a.row_blocks, block = index % a.row_blocks;
+  const uint32_t used = (plan.total + plan.c - 1) / plan.c * a.row_blocks;   // workgroups that have work: the first ones, on all dies
+  if (blockIdx.x >= used) return;
+  const uint32_t index = xcd_contiguous(blockIdx.x, used), g = index / a.row_blocks, block = index % a.row_blocks;
   uint32_t pos = g * plan.c;
   const uint32_t end = min(pos + plan.c, plan.total);
-  if (g >= (plan.total + plan.c - 1) / plan.c) return;
   Place at = plan.at(a, pos);
   uint32_t head = (pos - at.before) / at.tiles, tile = (pos - at.before) % at.tiles;
 
@@ -753,9 +754,13 @@ int check_heads(const char* what, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, 
 // How many groups of 32 rows a workgroup holds: all of the rows up to 128, so that K and V are read once.
 int row_groups(uint64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 
-// Workgroups of the first launch: as many as are resident (one per compute unit where the tiles fill its LDS, else two), so that every
-// piece of work ends at about the same time.
-uint32_t work_groups(uint32_t head_dim, int wr) { return head_dim == 128 && wr == 1 ? 256 : 512; }
+// Workgroups of the first launch that have work: as many as are resident (one per compute unit where the tiles fill its LDS, else two), so
+// that every piece of work ends at about the same time -- but one per compute unit up to eight tiles each: two hide each other's waits
+// only over several tiles, and more of them write more pieces.  us, two -> one: 2 x 32 nodes of 32 / 8 heads behind 4000 (4 tiles) 31.5 ->
+// 25.6, 4 x 40 behind 300 (2) 26.2 -> 22.9, 1 x 16 behind 2000 (2) 24.3 -> 20.3, 8 x 20 of 64 channels behind 700 20.3 -> 19.5;  2 x 63 of
+// 64 channels behind 5001 (9) 26.7 -> 28.5, 8 x 64 behind 8192 (65) 140 -> 151.
+constexpr uint32_t kUnits = 256;
+uint32_t work_groups(uint32_t head_dim, int wr) { return head_dim == 128 && wr == 1 ? kUnits : 2 * kUnits; }
 
 uint32_t row_blocks_of(uint64_t rows) { return (uint32_t)((rows + 32 * row_groups(rows) - 1) / (32 * row_groups(rows))); }
 uint32_t groups_of(uint32_t head_dim, uint64_t rows) {   // of one row block
@@ -774,6 +779,7 @@ int launch_rows(Call& a, hipStream_t stream) {
   static_assert(WK == 1 || smem >= 4 * 32 * D * 4, "the waves' sums reuse the tiles");
   a.row_blocks = row_blocks_of(a.rows);
   a.groups = groups_of(D, a.rows);
+  a.few = (kUnits + a.row_blocks - 1) / a.row_blocks;
   auto go = [&](auto kern, LdsGrant& grant) {
     if (int rc = reserve_lds((const void*)kern, smem, grant, "cache attention")) return rc;
     hipLaunchKernelGGL(kern, dim3(a.groups * a.row_blocks), dim3(256), smem, stream, a);
