@@ -180,9 +180,9 @@ __device__ __forceinline__ bool finite8(h8& x) {
 // 26.7 -> 28.6 us (2 x 63 nodes of 64 channels behind 5001 tokens), 126 -> 141 (8 x 64 of 128 behind 8192, where the MFMAs bound the launch).
 //
 // What bounds it: memory up to about 64 rows of a head (decode with weights, 16 x up to 4000 slots of 32 / 8 heads: 209 MB in 41 us, 5.1 TB/s,
-// where a large copy reads and writes 4.9), the MFMAs from there on (8 x 64 behind 8192: 104 Gflop with the low halves in 119 us = 0.87
+// where a large copy reads and writes 4.9), the MFMAs from there on (8 x 64 behind 8192: 104 Gflop with the low halves in 117 us = 0.89
 // PFLOP/s, where an 8192^3 product of the vendor's reaches 1.14).  Short calls are latencies: the lengths, then the queries and the first
-// tile, then the pieces in the second launch (1 x 8 behind 120: 8 + 3 us).  Not taken: fragments read during the MFMAs before them, as in
+// tile, then the pieces in the second launch (1 x 8 behind 120: 9 + 3 us).  Not taken: fragments read during the MFMAs before them, as in
 // the prefill kernel (no gain, 131 against 130 us, or spills); tiles of a wave of its own two ahead without barriers (58.4 against 58.9 us).
 template <int D, int WR, bool TREE, bool NT>
 __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attention_kernel(const Call a) {
