@@ -35,11 +35,12 @@ struct Call {
   float scale_log2;
 };
 
-// The work of a call is one list of tiles of KT keys: for every sequence and every key / value head, the tiles of the cache and then those of
-// the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more than the rounding of c, however the lengths differ, and nothing of it has to be known on the host.  More than 32 WR query rows of a head are blocks of that many with a
-// workgroup each, next to each other, so that the second one finds the keys and values in its die's L2 (8 x 64 nodes of 32 / 8 heads behind
-// 8192 tokens, two blocks, with the queries' high halves alone: 131 us with the blocks as units of the list, whose keys and values then
-// come from memory twice, 126 so).
+// The work of a call is one list of tiles of KT keys: for every sequence and every key / value head, the tiles of the cache and then
+// those of the tree.  Workgroup g takes the tiles [g c, g c + c): no workgroup has more than another by more than the rounding of c,
+// however the lengths differ, and nothing of it has to be known on the host.  More than 32 WR query rows of a head are blocks of that
+// many with a workgroup each, next to each other, so that the second one finds the keys and values in its die's L2 (8 x 64 nodes of 32
+// / 8 heads behind 8192 tokens, two blocks, with the queries' high halves alone: 131 us with the blocks as units of the list, whose
+// keys and values then come from memory twice, 126 so).
 template <int KT, bool TREE>
 __device__ __forceinline__ uint32_t tiles_for(const Call& a, long long n) {
   if (TREE) return n < 0 || n > (long long)a.max_len - a.T ? 0 : ((uint32_t)n + KT - 1) / KT + (a.T + KT - 1) / KT;

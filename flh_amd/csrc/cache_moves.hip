@@ -370,7 +370,9 @@ extern "C" int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_hal
       select(evict_select_kernel<false>, 0);
     }
     if (int rc = check_launch("evict_kv_cache (select)")) return rc;
-    // whole rows, or four slices of them where a launch would have fewer than two workgroups per compute unit
+    // Whole rows, or four slices of them where a launch would have fewer than two workgroups per compute unit.  us for both launches, other
+    // sides: halves of rows up to four workgroups per unit 157 -> 260 (20 layers x 3 x 3000 slots, 8 heads of 64 channels), eighths and
+    // sixteenths up to half a workgroup 28.4 -> 24.8 and 26.0 (1 layer x 4000, heads of 128), 14.0 -> 15.0 and 15.0 (4 x 1100)
     const uint32_t pieces = head_dim / 8, slices = pieces % 4 == 0 && units * n * 2 < 512 ? 4 : 1;
     hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)units, n, 2 * slices), dim3(256), 0, st, c, (const long long*)lengths,
                        (const long long*)kept + l * units * budget, Hkv, pieces, pieces / slices, max_len, budget);
