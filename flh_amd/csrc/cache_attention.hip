@@ -815,7 +815,7 @@ int launch_call(Call& a, uint32_t head_dim, hipStream_t stream) {
 // tiles, rows and elements that fit the kernels' 32-bit counts
 bool too_large(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
   const uint64_t rows = (uint64_t)T * (Hq / Hkv);
-  if (rows > (1u << 24)) return true;
+  if (rows > (1u << 24) || (uint64_t)B * Hkv > (1u << 24)) return true;   // (the products below then fit 64 bits)
   const uint64_t units = (uint64_t)B * Hkv * row_blocks_of(rows);
   return max_len > (1u << 30) || units > (1u << 24) || units * ((uint64_t)max_len / 64 + 8) > 0x7FFFFFFFull ||
          (uint64_t)B * Hkv * max_len * head_dim > (1ull << 40) || (uint64_t)B * T * Hq * head_dim > (1ull << 36);
@@ -826,8 +826,10 @@ bool too_large(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_
 
 using namespace flh;
 
+// (sizes that the call itself refuses need no bytes: their counts do not fit the arithmetic)
 extern "C" size_t flh_tree_attention_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim) {
-  return Hkv ? partial_bytes(B, (uint64_t)T * (Hq / Hkv), Hkv, head_dim) : 0;
+  if (Hkv == 0 || head_dim > 128 || too_large(B, T, Hq, Hkv, head_dim, 0)) return 0;
+  return partial_bytes(B, (uint64_t)T * (Hq / Hkv), Hkv, head_dim);
 }
 
 extern "C" int flh_tree_attention_f16(const flh_half* q, const flh_half* k_new, const flh_half* v_new, const flh_half* cos,
@@ -859,7 +861,8 @@ uint32_t score_pitch(uint32_t max_len) { return (max_len + 3) / 4 * 4; }
 }  // namespace
 
 extern "C" size_t flh_decode_attention_weights_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
-  return Hkv ? partial_bytes(B, Hq / Hkv, Hkv, head_dim) + (size_t)B * Hq * score_pitch(max_len) * sizeof(float) : 0;
+  if (Hkv == 0 || head_dim > 128 || too_large(B, 1, Hq, Hkv, head_dim, max_len)) return 0;
+  return partial_bytes(B, Hq / Hkv, Hkv, head_dim) + (size_t)B * Hq * score_pitch(max_len) * sizeof(float);
 }
 
 extern "C" int flh_decode_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, const int64_t* lengths,
@@ -895,10 +898,16 @@ void cut_columns(Columns& a, uint32_t B) {
   for (uint32_t c = 0; c < a.chunks; ++c) a.pairs += a.live_blocks(c);
 }
 size_t lse_floats(uint32_t B, uint32_t T, uint32_t Hq) { return ((size_t)B * T * Hq + 3) / 4 * 4; }
+
+// queries, and blocks of slots of a cache of `slots`, that fit the kernels' 32-bit counts
+bool too_many_columns(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint64_t slots) {
+  const uint64_t rows = (uint64_t)B * T, units = (uint64_t)B * Hkv;
+  return rows > 0x7FFFFFFFull || rows * Hq > 0x7FFFFFFFull || slots > (1u << 30) || units > (1u << 24) || units * (slots / kSlots + 1) > (1u << 24);
+}
 }  // namespace
 
 extern "C" size_t flh_prefill_attention_weights_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t past) {
-  if (B == 0 || T == 0 || Hkv == 0) return 0;
+  if (B == 0 || T == 0 || Hkv == 0 || too_many_columns(B, T, Hq, Hkv, (uint64_t)past + T)) return 0;
   Columns a = {};
   a.T = T, a.Hkv = Hkv, a.past = past;
   cut_columns(a, B);
@@ -915,8 +924,7 @@ extern "C" int flh_prefill_attention_weights_f16(const flh_half* q, const flh_ha
   if (head_dim != 128) return fail(FLH_EINVAL, "prefill_attention_weights: head_dim (%u) must be 128", head_dim);
   if ((uint64_t)past + T > max_len) return fail(FLH_EINVAL, "prefill_attention_weights: past (%u) + T (%u) exceeds the cache length %u", past, T, max_len);
   if (B == 0 || T == 0) return FLH_OK;
-  if ((uint64_t)B * T * Hq > 0x7FFFFFFFull || max_len > (1u << 30) || (uint64_t)B * Hkv * ((uint64_t)max_len / kSlots + 1) > (1u << 24))
-    return fail(FLH_EINVAL, "prefill_attention_weights: problem too large");
+  if (too_many_columns(B, T, Hq, Hkv, max_len)) return fail(FLH_EINVAL, "prefill_attention_weights: problem too large");
   const size_t need = flh_prefill_attention_weights_workspace_bytes(B, T, Hq, Hkv, past);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return fail(FLH_EINVAL, "prefill_attention_weights: a 16-byte aligned workspace of %zu bytes is required", need);
