@@ -817,6 +817,8 @@ bool too_large(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_
   const uint64_t rows = (uint64_t)T * (Hq / Hkv);
   if (rows > (1u << 24) || (uint64_t)B * Hkv > (1u << 24)) return true;   // (the products below then fit 64 bits)
   const uint64_t units = (uint64_t)B * Hkv * row_blocks_of(rows);
+  // the joining launch: workgroups of 32 rows and channels, and (attention weights) of 256 slots
+  if (too_many_items(units * row_groups(rows) * (head_dim / 32) + (uint64_t)B * Hkv * (((uint64_t)max_len + 255) / 256), 256)) return true;
   return max_len > (1u << 30) || units > (1u << 24) || units * ((uint64_t)max_len / 64 + 8) > 0x7FFFFFFFull ||
          (uint64_t)B * Hkv * max_len * head_dim > (1ull << 40) || (uint64_t)B * T * Hq * head_dim > (1ull << 36);
 }
@@ -902,7 +904,7 @@ size_t lse_floats(uint32_t B, uint32_t T, uint32_t Hq) { return ((size_t)B * T *
 // queries, and blocks of slots of a cache of `slots`, that fit the kernels' 32-bit counts
 bool too_many_columns(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint64_t slots) {
   const uint64_t rows = (uint64_t)B * T, units = (uint64_t)B * Hkv;
-  return rows > 0x7FFFFFFFull || rows * Hq > 0x7FFFFFFFull || slots > (1u << 30) || units > (1u << 24) || units * (slots / kSlots + 1) > (1u << 24);
+  return rows > 0x7FFFFFFFull || rows * Hq > 0x7FFFFFFFull || slots > (1u << 30) || units > (1u << 24) || too_many_items(units * (slots / kSlots + 1), 256);
 }
 }  // namespace
 

@@ -326,6 +326,7 @@ extern "C" int flh_tree_commit(const int64_t* tokens, const int64_t* parents, in
   if (T == 0 || T > kMaxNodes) return fail(FLH_EINVAL, "tree_commit: %u nodes (1 to %u)", T, kMaxNodes);
   if (lengths == new_lengths) return fail(FLH_EINVAL, "tree_commit: the new lengths need memory of their own");
   if (int rc = check_caches(layers, k_caches, v_caches, B, Hkv, head_dim, max_len, "tree_commit")) return rc;
+  if (too_many_items(B, 256)) return fail(FLH_EINVAL, "tree_commit: problem too large");
   if (B == 0) return FLH_OK;
   const uint32_t pieces = head_dim / 8, moves = 2 * Hkv * ((pieces + 15) / 16);
   const Tree t = {(const long long*)tokens, (const long long*)parents, (const long long*)chosen, (const long long*)lengths, (long long*)path,
@@ -353,6 +354,7 @@ extern "C" int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_hal
   if (B == 0) return FLH_OK;
   const hipStream_t st = (hipStream_t)stream;
   const size_t units = (size_t)B * Hkv;
+  if (too_many_items(units, kSelectThreads)) return fail(FLH_EINVAL, "evict_kv_cache: problem too large");
   for (int l = 0; l < layers; l += kMaxLayers) {
     Caches c;
     const int n = layers - l < kMaxLayers ? layers - l : kMaxLayers;

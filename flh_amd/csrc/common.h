@@ -34,6 +34,9 @@ int reserve_lds(const void* kernel, size_t bytes, LdsGrant& grant, const char* w
 template <typename... P>
 inline bool misaligned16(P... p) { return (((uintptr_t)p | ...) & 15) != 0; }
 
+// whether a launch's work items along one axis pass what it counts them in (32 bits)
+inline bool too_many_items(uint64_t workgroups, uint32_t threads) { return workgroups * threads > 0xFFFFFFFFull; }
+
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));

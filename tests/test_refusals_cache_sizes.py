@@ -1,4 +1,6 @@
 """Sizes at the C entries of the operators on caches that their 32-bit counts do not hold (no device here: nothing is launched)."""
+import ctypes
+
 import pytest
 
 from flh_amd import _lib
@@ -27,3 +29,20 @@ def test_workspace_sizes_of_calls_that_are_refused(name, args):
     ("flh_decode_attention_weights_workspace_bytes", (2, 8, 2, 64, 101), 2 * 8 * 104 * 4 + 2 * 2 * 32 * 66 * 4)])
 def test_workspace_sizes_of_calls_that_run(name, args, least):
     assert least <= getattr(_lib.load(), name)(*args) < 2 ** 30
+
+
+OK, BIG = 0x10000, 1 << 60
+CACHES = ((ctypes.c_void_p * 1)(1 << 50), (ctypes.c_void_p * 1)(1 << 56))
+
+
+@pytest.mark.parametrize("name,args", [
+    ("flh_tree_attention_f16", (*[OK] * 7, 0, OK, OK, OK, 1 << 20, 1, 4, 4, 128, 64, 0.1, OK, BIG, None)),
+    ("flh_decode_attention_weights_f16", (*[OK] * 6, 1 << 20, 4, 4, 128, 64, 0.1, OK, BIG, None)),
+    ("flh_decode_attention_weights_f16", (*[OK] * 6, 1 << 21, 4, 4, 64, 256, 0.1, OK, BIG, None)),
+    ("flh_prefill_attention_weights_f16", (*[OK] * 5, 1 << 22, 1, 4, 4, 128, 0, 64, 0.1, OK, BIG, None)),
+    ("flh_tree_commit", (OK, OK, 0, OK, 2 * OK, OK, OK, OK, 3 * OK, 1, *CACHES, 1 << 24, 8, 2, 8, 16, None)),
+    ("flh_evict_kv_cache", (1, *CACHES, OK, OK, OK, 2 * OK, 2 * OK, 1 << 22, 2, 8, 16, 8, 4, None))])
+def test_launches_of_more_items_than_32_bits_count(name, args):
+    """Refused in front of the first launch, not by the runtime behind the one that has written the caches."""
+    lib = _lib.load()
+    assert getattr(lib, name)(*args) == -1 and b"too large" in lib.flh_last_error(), lib.flh_last_error()
