@@ -871,6 +871,7 @@ def _cache_lists(k_caches, v_caches, device):
     for t_ in ks + vs:
         _check(t_.is_cuda and t_.dtype == torch.float16 and t_.is_contiguous() and t_.device == device and t_.shape == shape,
                "caches must be contiguous float16 CUDA tensors of one shape on one device")
+    _check(max(shape) < 2 ** 31, "caches: problem too large")      # (the C ABI takes sizes of 32 bits)
     _check(shape[3] > 0 and shape[3] % 8 == 0 and shape[3] <= 512, "head_dim must be a multiple of 8, at most 512")
     pointers = [(ctypes.c_void_p * len(ts))(*[t_.data_ptr() for t_ in ts]) for ts in (ks, vs)]
     return pointers, len(ks), tuple(shape)

@@ -285,6 +285,7 @@ struct CacheList {   // the layers' caches and their common shape
         (list == &ks ? k : v).push_back((flh_half*)t.data_ptr());
       }
     B = shape[0], Hkv = shape[1], max_len = shape[2], d = shape[3];
+    TORCH_CHECK(std::max({B, Hkv, max_len, d}) < (1ll << 31), "caches: problem too large");   // (the C ABI takes sizes of 32 bits)
     TORCH_CHECK(d > 0 && d % 8 == 0 && d <= 512, "head_dim must be a multiple of 8, at most 512");
   }
 };
