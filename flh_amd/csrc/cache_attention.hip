@@ -612,6 +612,38 @@ struct Columns {
   }
 };
 
+// A query whose log2 sum is no number has no probabilities either: every slot that it sees gets NaN.  In the kernel's tiles so do
+// slots that it does not see (-inf less NaN).  Columns that are NaN come here, which a launch without such a query never does: slot j's
+// sum over the queries t0 .. t_end - 1, two lanes a slot.  (Told apart in the loop's tiles it is 1-2 % of every launch -- 285 -> 288.5 us
+// for 4096 tokens, 79 -> 80.7 for 4 x 700 behind 100 -- or registers that spill.)
+__device__ __forceinline__ float numbers_of_column(const Columns& a, uint32_t b, uint32_t g, uint32_t j, uint32_t t0, uint32_t t_end) {
+  constexpr int D = 128;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const float* lse = a.lse + ((size_t)b * a.Hq + g * a.rep) * a.T;
+  uint32_t seen = 0;                                   // past the latest such query
+  for (uint32_t head = 0; head < a.rep; ++head)
+    for (uint32_t t = t0 + lane; t < t_end; t += 64) {
+      const float x = lse[(size_t)head * a.T + t];
+      if (!(x - x == 0.f)) seen = max(seen, t + 1);
+    }
+  for (int o = 32; o; o >>= 1) seen = max(seen, (uint32_t)__shfl_xor((int)seen, o));
+  if (j < a.past + seen || j >= a.past + a.T) return NAN;   // (past the last slot: not used)
+  const __half* key = a.k + (((size_t)b * a.Hkv + g) * a.max_len + j) * D;
+  float sum = 0.f;
+  for (uint32_t head = 0; head < a.rep; ++head)
+    for (uint32_t t = max(t0, j > a.past ? j - a.past : 0) + h; t < t_end; t += 2) {
+      const __half* query = a.q + (((size_t)b * a.T + t) * a.Hq + g * a.rep + head) * D;
+      float s = 0.f;
+      for (int c = 0; c < D; c += 8) {
+        const h8 x = *(const h8*)(query + c), y = *(const h8*)(key + c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = __builtin_fmaf((float)x[i], (float)y[i], s);
+      }
+      sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale_log2, -lse[(size_t)head * a.T + t]));
+    }
+  return sum + __shfl_xor(sum, 32);
+}
+
 __global__ __launch_bounds__(256, 2) void column_weights_kernel(const Columns a) {
   constexpr int D = 128, PITCH = 2 * D, TILE = kQueries * PITCH, KS = D / 16;
   using L = Tile<D>;
@@ -726,8 +758,12 @@ __global__ __launch_bounds__(256, 2) void column_weights_kernel(const Columns a)
   }
 #pragma unroll
   for (int ct = 0; ct < 2; ++ct) {
-    const float all = sum[ct] + lane_xor_f<32>(sum[ct]);
+    float all = sum[ct] + lane_xor_f<32>(sum[ct]);
     const uint32_t j = mine + ct * 32 + n;
+    if (__ballot(all != all)) {
+      const float number = numbers_of_column(a, b, g, j, chunk * a.chunk, t_end);
+      all = all != all ? number : all;
+    }
     if (h == 0 && j < total) {
       if (a.chunks == 1) a.weights[(size_t)bg * a.max_len + j] += all;
       else a.parts[((size_t)chunk * units + bg) * a.pitch + j] = all;
