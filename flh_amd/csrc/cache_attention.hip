@@ -571,7 +571,7 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const Call a) {
         const float top = wave_max(m);
         l = wave_sum(l * __builtin_amdgcn_exp2f(m - top));
         m = top;
-        if (lane == 0) stats[r - r0] = v2f{m, l > 0.f ? 1.f / l : 0.f};
+        if (lane == 0) stats[r - r0] = v2f{m, l == 0.f ? 0.f : 1.f / l};   // (a sum of NaN: no weight of the row is a number)
       }
       __syncthreads();
       if (j < length) {

@@ -41,3 +41,21 @@ def test_a_prompt_with_one_odd_query(ops, B, T, Hq, Hkv, past, odd, value):
             spoilt = past + odd + 1 if b == 0 and g == Hkv - 1 else 0
             assert torch.isnan(got[b, g, :spoilt]).all()
             assert ((got[b, g, spoilt:n].double() - total[spoilt:]).abs() <= tol[spoilt:]).all()
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,d,n,slot", [(2, 8, 2, 128, 300, 5), (1, 4, 4, 64, 1000, 999), (1, 70, 1, 128, 130, 64)])
+def test_a_decode_step_over_a_key_that_is_no_number(ops, B, Hq, Hkv, d, n, slot):
+    gen = torch.Generator().manual_seed(n)
+    print(f"case decode weights, odd key B={B} Hq={Hq} Hkv={Hkv} d={d} {n} {slot}", flush=True)
+    q, kc, vc = normal(gen, B, Hq, d), normal(gen, B, Hkv, n + 7, d), normal(gen, B, Hkv, n + 7, d)
+    kc[0, 0, slot, 3] = float("nan")
+    weights = torch.rand(B, Hkv, n + 7, generator=gen)
+    dev, clean = weights.cuda(), weights.cuda()
+    lengths = torch.tensor([n] * B).cuda()
+    out = ops.decode_attention_weights(q.cuda(), kc.cuda(), vc.cuda(), lengths, dev)
+    kc[0, 0, slot, 3] = 0
+    ref = ops.decode_attention_weights(q.cuda(), kc.cuda(), vc.cuda(), lengths, clean)
+    assert torch.isnan(out[0, :Hq // Hkv]).all() and torch.isnan(dev[0, 0, :n]).all()
+    dev[0, 0, :n] = clean[0, 0, :n]                                    # everything else has the bits it has without the NaN
+    out[0, :Hq // Hkv] = ref[0, :Hq // Hkv]
+    assert torch.equal(dev, clean) and torch.equal(out, ref)
