@@ -907,7 +907,8 @@ extern "C" int flh_decode_attention_weights_f16(const flh_half* q, const flh_hal
                                                 flh_half* out, float* weights, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
                                                 uint32_t max_len, float scale, void* workspace, size_t workspace_bytes, void* stream) {
   if (!q || !k_cache || !v_cache || !lengths || !out || !weights) return fail(FLH_EINVAL, "decode_attention_weights: null pointer");
-  if (misaligned16(q, k_cache, v_cache, out, weights)) return fail(FLH_EINVAL, "decode_attention_weights: tensors must be 16-byte aligned");
+  if (misaligned16(q, k_cache, v_cache, out)) return fail(FLH_EINVAL, "decode_attention_weights: tensors must be 16-byte aligned");
+  if ((uintptr_t)weights & 3) return fail(FLH_EINVAL, "decode_attention_weights: the weights must be 4-byte aligned");
   if (int rc = check_heads("decode_attention_weights", Hq, Hkv, head_dim, scale)) return rc;
   if (B == 0 || max_len == 0) return FLH_OK;
   if (too_large(B, 1, Hq, Hkv, head_dim, max_len)) return fail(FLH_EINVAL, "decode_attention_weights: problem too large");
@@ -957,7 +958,8 @@ extern "C" int flh_prefill_attention_weights_f16(const flh_half* q, const flh_ha
                                                  uint32_t past, uint32_t max_len, float scale, void* workspace, size_t workspace_bytes,
                                                  void* stream) {
   if (!q || !k_cache || !v_cache || !out || !weights) return fail(FLH_EINVAL, "prefill_attention_weights: null pointer");
-  if (misaligned16(q, k_cache, v_cache, out, weights)) return fail(FLH_EINVAL, "prefill_attention_weights: tensors must be 16-byte aligned");
+  if (misaligned16(q, k_cache, v_cache, out)) return fail(FLH_EINVAL, "prefill_attention_weights: tensors must be 16-byte aligned");
+  if ((uintptr_t)weights & 3) return fail(FLH_EINVAL, "prefill_attention_weights: the weights must be 4-byte aligned");
   if (int rc = check_heads("prefill_attention_weights", Hq, Hkv, head_dim, scale)) return rc;
   if (head_dim != 128) return fail(FLH_EINVAL, "prefill_attention_weights: head_dim (%u) must be 128", head_dim);
   if ((uint64_t)past + T > max_len) return fail(FLH_EINVAL, "prefill_attention_weights: past (%u) + T (%u) exceeds the cache length %u", past, T, max_len);

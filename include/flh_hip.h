@@ -479,6 +479,7 @@ int flh_tree_commit(const int64_t* tokens, const int64_t* parents, int parents_p
 
 /* Attention that also adds up how much each cache slot is looked at:
  *   weights[b, g, j] += sum of the probabilities of slot j over the queries of key / value head g,  float32 [B, Hkv, max_len].
+ * (aligned as floats are: one layer's part of what flh_evict_kv_cache takes will do).
  * decode: one query per sequence, q, out [B, Hq, d], over the slots 0 .. lengths[b] - 1 (the new token's key and value among them; a
  * length of zero, a negative one or one above max_len: zeros, no weights); d 64 or 128.  prefill: flh_prefill_attention_f16 (d = 128, the
  * same output bits), each query over the slots it sees.  Sums are taken in a fixed order: the same call gives the same bits. */

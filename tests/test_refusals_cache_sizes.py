@@ -46,3 +46,13 @@ def test_launches_of_more_items_than_32_bits_count(name, args):
     """Refused in front of the first launch, not by the runtime behind the one that has written the caches."""
     lib = _lib.load()
     assert getattr(lib, name)(*args) == -1 and b"too large" in lib.flh_last_error(), lib.flh_last_error()
+
+
+@pytest.mark.parametrize("name,args", [
+    ("flh_decode_attention_weights_f16", (OK, OK, OK, OK, OK, "weights", 1, 8, 2, 128, 64, 0.1, OK, 4, None)),
+    ("flh_prefill_attention_weights_f16", (OK, OK, OK, OK, "weights", 1, 4, 8, 2, 128, 0, 64, 0.1, OK, 4, None))])
+def test_sums_of_weights_are_aligned_as_floats(name, args):
+    lib = _lib.load()
+    for at, message in ((OK + 2, b"4-byte aligned"), (OK + 4, b"workspace"), (OK + 8, b"workspace")):
+        assert getattr(lib, name)(*(at if x == "weights" else x for x in args)) == -1
+        assert message in lib.flh_last_error(), lib.flh_last_error()
