@@ -5,7 +5,9 @@ the C ABI in include/flh_hip.h.  torch is used only for device memory and the cu
 stream.  Beyond the nine reference ops it exports the whole-row rotate+quantise op and
 the generalised GEMM (per-token x per-channel scales, int32 output).
 """
+import contextlib
 import ctypes
+import threading
 
 import torch
 
@@ -641,6 +643,7 @@ def rope_kv_cache_(q, k, v, cos, sin, positions, k_cache, v_cache):
 
 
 _attention_workspaces = {}      # (device index, stream handle) -> uint8 tensor: launches of one stream run in order
+_attention_locks = {}           # ... -> lock held while a call launches
 
 
 def prefill_attention(q, k_cache, v_cache, past, scale=None):
@@ -680,6 +683,19 @@ def _default_attention_workspace(q, need):
     return workspace
 
 
+@contextlib.contextmanager
+def _attention_workspace(q, need, workspace):
+    """The caller's workspace (checked), or the default one.  Two threads may launch on one stream, and ctypes gives the interpreter
+    up during a call: the lock keeps a call's two or three launches, which hand results on through the default workspace, together."""
+    if workspace is not None:
+        _check(workspace.is_cuda and workspace.dtype == torch.uint8 and workspace.is_contiguous()
+               and workspace.device == q.device and workspace.numel() >= need, f"workspace: {need} bytes of uint8 needed")
+        yield workspace
+        return
+    with _attention_locks.setdefault((q.device.index, _stream(q)), threading.Lock()):
+        yield _default_attention_workspace(q, need)
+
+
 def decode_attention(q, k_cache, v_cache, kv_len, scale=None, workspace=None):
     """One new token per sequence against the first `kv_len` slots of a preallocated cache: q [B, Hq, d] fp16,
     k_cache / v_cache [B, Hkv, max_len, d] fp16 -> [B, Hq, d] fp16 = softmax(q K^T * scale) V with float32 scores,
@@ -699,14 +715,10 @@ def decode_attention(q, k_cache, v_cache, kv_len, scale=None, workspace=None):
     if B == 0:
         return out
     need = int(_lib.load().flh_decode_attention_workspace_bytes(B, Hq, d, int(kv_len)))
-    if workspace is None:
-        workspace = _default_attention_workspace(q, need)
-    else:
-        _check(workspace.is_cuda and workspace.dtype == torch.uint8 and workspace.is_contiguous()
-               and workspace.device == q.device and workspace.numel() >= need, f"workspace: {need} bytes of uint8 needed")
-    _run("flh_decode_attention_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), B, Hq,
-         Hkv, d, int(kv_len), max_len, float(scale if scale is not None else d ** -0.5), workspace.data_ptr(),
-         workspace.numel(), _stream(q))
+    with _attention_workspace(q, need, workspace) as ws:
+        _run("flh_decode_attention_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), B, Hq,
+             Hkv, d, int(kv_len), max_len, float(scale if scale is not None else d ** -0.5), ws.data_ptr(),
+             ws.numel(), _stream(q))
     return out
 
 
@@ -742,15 +754,11 @@ def decode_attention_rope(q, k_new, v_new, cos, sin, positions, k_cache, v_cache
     if B == 0:
         return result
     need = int(_lib.load().flh_decode_attention_workspace_bytes(B, Hq, d, int(kv_len)))
-    if workspace is None:
-        workspace = _default_attention_workspace(q, need)
-    else:
-        _check(workspace.is_cuda and workspace.dtype == torch.uint8 and workspace.is_contiguous()
-               and workspace.device == q.device and workspace.numel() >= need, f"workspace: {need} bytes of uint8 needed")
-    _run("flh_decode_attention_rope_group_quant_i4" if quantize else "flh_decode_attention_rope_f16", q.device, q.data_ptr(),
-         k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), k_cache.data_ptr(),
-         v_cache.data_ptr(), *(t.data_ptr() for t in out), B, Hq, Hkv, d, int(kv_len), max_len,
-         float(scale if scale is not None else d ** -0.5), workspace.data_ptr(), workspace.numel(), _stream(q))
+    with _attention_workspace(q, need, workspace) as ws:
+        _run("flh_decode_attention_rope_group_quant_i4" if quantize else "flh_decode_attention_rope_f16", q.device, q.data_ptr(),
+             k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), k_cache.data_ptr(),
+             v_cache.data_ptr(), *(t.data_ptr() for t in out), B, Hq, Hkv, d, int(kv_len), max_len,
+             float(scale if scale is not None else d ** -0.5), ws.data_ptr(), ws.numel(), _stream(q))
     return result
 
 
@@ -765,15 +773,6 @@ def _check_cache_pair(q, k_cache, v_cache, batch, d):
 def _check_lengths(lengths, batch, device):
     _check(lengths.is_cuda and lengths.dtype == torch.int64 and lengths.is_contiguous() and tuple(lengths.shape) == (batch,)
            and lengths.device == device, "lengths must be a contiguous int64 CUDA tensor [B]")
-
-
-def _attention_workspace(name, q, workspace, *sizes):
-    need = int(getattr(_lib.load(), name + "_workspace_bytes")(*sizes))
-    if workspace is None:
-        return _default_attention_workspace(q, need)
-    _check(workspace.is_cuda and workspace.dtype == torch.uint8 and workspace.is_contiguous()
-           and workspace.device == q.device and workspace.numel() >= need, f"workspace: {need} bytes of uint8 needed")
-    return workspace
 
 
 def tree_attention(q, k_new, v_new, cos, sin, lengths, mask, k_cache, v_cache, scale=None, workspace=None):
@@ -803,11 +802,12 @@ def tree_attention(q, k_new, v_new, cos, sin, lengths, mask, k_cache, v_cache, s
     out = torch.empty((B, T, Hq * d), dtype=torch.float16, device=q.device)
     if B == 0 or T == 0:
         return out
-    workspace = _attention_workspace("flh_tree_attention", q, workspace, B, T, Hq, Hkv, d)
-    _run("flh_tree_attention_f16", q.device, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-         lengths.data_ptr(), mask.data_ptr(), int(mask.dim() == 3), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), B, T, Hq,
-         Hkv, d, k_cache.size(2), float(scale if scale is not None else d ** -0.5), workspace.data_ptr(), workspace.numel(),
-         _stream(q))
+    need = int(_lib.load().flh_tree_attention_workspace_bytes(B, T, Hq, Hkv, d))
+    with _attention_workspace(q, need, workspace) as ws:
+        _run("flh_tree_attention_f16", q.device, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+             lengths.data_ptr(), mask.data_ptr(), int(mask.dim() == 3), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), B, T, Hq,
+             Hkv, d, k_cache.size(2), float(scale if scale is not None else d ** -0.5), ws.data_ptr(), ws.numel(),
+             _stream(q))
     return out
 
 
@@ -828,10 +828,11 @@ def decode_attention_weights(q, k_cache, v_cache, lengths, weights, scale=None, 
     out = torch.empty_like(q)
     if B == 0:
         return out
-    workspace = _attention_workspace("flh_decode_attention_weights", q, workspace, B, Hq, Hkv, d, max_len)
-    _run("flh_decode_attention_weights_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
-         out.data_ptr(), weights.data_ptr(), B, Hq, Hkv, d, max_len, float(scale if scale is not None else d ** -0.5),
-         workspace.data_ptr(), workspace.numel(), _stream(q))
+    need = int(_lib.load().flh_decode_attention_weights_workspace_bytes(B, Hq, Hkv, d, max_len))
+    with _attention_workspace(q, need, workspace) as ws:
+        _run("flh_decode_attention_weights_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
+             out.data_ptr(), weights.data_ptr(), B, Hq, Hkv, d, max_len, float(scale if scale is not None else d ** -0.5),
+             ws.data_ptr(), ws.numel(), _stream(q))
     return out
 
 
@@ -850,10 +851,11 @@ def prefill_attention_weights(q, k_cache, v_cache, past, weights, scale=None, wo
     out = torch.empty((B, T, Hq * d), dtype=torch.float16, device=q.device)
     if B == 0 or T == 0:
         return out
-    workspace = _attention_workspace("flh_prefill_attention_weights", q, workspace, B, T, Hq, Hkv, past)
-    _run("flh_prefill_attention_weights_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
-         weights.data_ptr(), B, T, Hq, Hkv, d, past, max_len, float(scale if scale is not None else d ** -0.5),
-         workspace.data_ptr(), workspace.numel(), _stream(q))
+    need = int(_lib.load().flh_prefill_attention_weights_workspace_bytes(B, T, Hq, Hkv, past))
+    with _attention_workspace(q, need, workspace) as ws:
+        _run("flh_prefill_attention_weights_f16", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+             weights.data_ptr(), B, T, Hq, Hkv, d, past, max_len, float(scale if scale is not None else d ** -0.5),
+             ws.data_ptr(), ws.numel(), _stream(q))
     return out
 
 
