@@ -910,7 +910,9 @@ def evict_kv_cache_(k_caches, v_caches, weights, lengths, budget, recent):
     largest weights (equal ones: the lowest slot; NaN counts as largest), for every layer and key / value head by itself.  k_caches
     / v_caches: a tensor or a list of them, [B, Hkv, max_len, d], compacted in place in the slots' order (rows behind the budget
     stay as they were); weights float32 [layers, B, Hkv, max_len]; lengths [B] int64.  -> (kept [layers, B, Hkv, budget] int64,
-    -1 behind the last slot of a shorter sequence; the kept slots' weights, zeros behind, shaped as `weights`; the new lengths)."""
+    -1 behind the last slot of a shorter sequence; the kept slots' weights, zeros behind, shaped as `weights`; the new lengths).
+    A sequence whose length is negative or above max_len: nothing kept or moved, zeros as new weights (the old ones are still in
+    `weights`), its length as it was."""
     pointers, layers, shape = _cache_lists(k_caches, v_caches, weights.device)
     B, Hkv, max_len, d = shape
     _check_weights(weights, (layers, B, Hkv, max_len), weights.device)

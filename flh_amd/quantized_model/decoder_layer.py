@@ -110,15 +110,21 @@ class StaticKVCache:
     Drafted tokens.  `begin_drafts()` gives every sequence a length of its own, `lengths` (device int64 [batch], from then on in
     place of kv_len): steps over a DraftTree write the nodes' keys / values behind it without moving it, and `commit` moves the
     accepted ones there and it with them.  A captured step serves every length.  A sequence whose tree does not fit (length above
-    max_len - T) or whose length has been set negative takes no part in a step."""
+    max_len - T) or whose length has been set negative takes no part in a step.
 
-    def __init__(self, layers, batch, kv_heads, max_len, head_dim, device, dtype=torch.float16, q_heads=None):
+    A bounded cache.  `evict` cuts the sequences' slots; the positions of what follows go on counting (the kept keys stay rotated as
+    they were): `cut` (device int64 [batch]) is how many slots each sequence has lost, its next position lengths + cut.  The rotary
+    table has `max_positions` rows then, which the cache has to be made with; a sequence whose tree passes them takes no part."""
+
+    def __init__(self, layers, batch, kv_heads, max_len, head_dim, device, dtype=torch.float16, q_heads=None, max_positions=None):
+        if max_positions is not None and max_positions < max_len:
+            raise ValueError(f"max_positions ({max_positions}) below max_len ({max_len})")
         self.keys = [torch.zeros(batch, kv_heads, max_len, head_dim, dtype=dtype, device=device) for _ in range(layers)]
         self.values = [torch.zeros_like(k) for k in self.keys]
-        self.max_len = max_len
+        self.max_len, self.max_positions = max_len, max_positions
         self.kv_len = 0
         self._positions = torch.arange(max_len, dtype=torch.int64, device=device)   # advance() hands out views of it
-        self.lengths = None                 # of the sequences, once drafts have begun
+        self.lengths = self.cut = None      # of the sequences, once drafts have begun (cut: with max_positions)
         self._tree_workspaces = {}          # scratch of the steps over drafts, by size: captured graphs keep theirs
         # the decode-attention kernel's scratch (partial results of the chunks), shared by the layers: they run in
         # order on one stream.  Owned here so that a captured graph finds it allocated.
@@ -157,20 +163,31 @@ class StaticKVCache:
     class _TreeLayer:
         """One layer of the cache in a step over drafted tokens."""
 
-        def __init__(self, owner, index, tree):
-            self.owner, self.index, self.tree = owner, index, tree
+        def __init__(self, owner, index, tree, lengths):
+            self.owner, self.index, self.tree, self.lengths = owner, index, tree, lengths
 
         def attend(self, q, k, v, cos, sin):
             """q [B, T, Hq, d], k / v [B, T, Hkv, d] of the nodes as projected, cos / sin [B, T, d] -> [B, T, Hq * d]"""
             keys, values = self.owner.keys[self.index], self.owner.values[self.index]
-            return _ops().tree_attention(q, k, v, cos, sin, self.owner.lengths, self.tree.mask, keys, values,
+            return _ops().tree_attention(q, k, v, cos, sin, self.lengths, self.tree.mask, keys, values,
                                          workspace=self.owner._tree_workspace(q, k))
 
-    def tree_layer(self, index, tree):
-        """What a decoder layer takes as `kv_cache` in a step over the nodes of `tree` (positions None, cos / sin [B, T, d])."""
+    def tree_layer(self, index, tree, lengths=None):
+        """What a decoder layer takes as `kv_cache` in a step over the nodes of `tree` (positions None, cos / sin [B, T, d]); `lengths`:
+        step_lengths(T), if the caller has it for all layers."""
+        return StaticKVCache._TreeLayer(self, index, tree, self.step_lengths(len(tree)) if lengths is None else lengths)
+
+    def step_lengths(self, t):
+        """`lengths` in a step over t nodes: -1 where the positions of a sequence that has been cut pass the rotary table."""
         if self.lengths is None:
             raise ValueError("begin_drafts() first: a step over drafted tokens needs the sequences' own lengths")
-        return StaticKVCache._TreeLayer(self, index, tree)
+        if self.cut is None:
+            return self.lengths
+        return torch.where(self.lengths + self.cut > self.max_positions - t, -1, self.lengths)
+
+    def next_positions(self):
+        """The position behind each sequence: the root's of its next tree."""
+        return self.lengths if self.cut is None else self.lengths + self.cut
 
     def _tree_workspace(self, q, k):
         from .. import _lib
@@ -184,6 +201,7 @@ class StaticKVCache:
         """From here on the sequences have lengths of their own (all kv_len at first): steps over drafted tokens and commit()."""
         if self.lengths is None:
             self.lengths = torch.full((self.keys[0].size(0),), self.kv_len, dtype=torch.int64, device=self.keys[0].device)
+            self.cut = torch.zeros_like(self.lengths) if self.max_positions is not None else None
         return self.lengths
 
     def commit(self, tokens, tree, chosen):
@@ -192,9 +210,25 @@ class StaticKVCache:
         `lengths` (the same tensor) with them."""
         if self.lengths is None:
             raise ValueError("begin_drafts() first")
-        path, accepted, following, lengths = _ops().tree_commit_(tokens, tree.parents, chosen, self.lengths, self.keys, self.values)
-        self.lengths.copy_(lengths)
+        path, accepted, following, _ = _ops().tree_commit_(tokens, tree.parents, chosen, self.step_lengths(tokens.size(1)), self.keys,
+                                                           self.values)
+        self.lengths.add_(accepted)         # (none of a sequence that takes no part)
         return path, accepted, following
+
+    def evict(self, weights, budget, recent):
+        """Cut every sequence of more than `budget` slots to that many, as evict_kv_cache_ does: weights float32 [layers, batch, kv_heads,
+        max_len], the sums that attention weights have been added up in -> (kept, the kept slots' weights).  `lengths` and `cut` (the
+        same tensors) move on.  A sequence that takes no part (length negative or above max_len) keeps its slots and its sums."""
+        if self.lengths is None:
+            raise ValueError("begin_drafts() first: sequences are cut to lengths of their own")
+        if self.cut is None:
+            raise ValueError("a cache to be cut is made with max_positions: the positions behind a cut go on counting")
+        kept, left, lengths = _ops().evict_kv_cache_(self.keys, self.values, weights, self.lengths, budget, recent)
+        out = (self.lengths < 0) | (self.lengths > self.max_len)
+        left = torch.where(out[:, None, None], weights, left)
+        self.cut.add_(self.lengths - lengths)
+        self.lengths.copy_(lengths)
+        return kept, left
 
 
 def _stock_call(module, cls):

@@ -234,10 +234,12 @@ class W4A4LlamaModel(torch.nn.Module):
         for layer in self.layers:
             layer.set_six_bit(six_bit)
 
-    def new_cache(self, batch, max_len):
+    def new_cache(self, batch, max_len, max_positions=None):
+        """`max_positions`: of a cache that is cut on the way (StaticKVCache.evict), the positions that its sequences may reach."""
         s = self.shape
         dev = self.embed_tokens.weight.device
-        return StaticKVCache(s.num_layers, batch, s.num_kv_heads, max_len, s.head_dim, dev, q_heads=s.num_heads)
+        return StaticKVCache(s.num_layers, batch, s.num_kv_heads, max_len, s.head_dim, dev, q_heads=s.num_heads,
+                             max_positions=max_positions)
 
     def embed(self, input_ids):
         x = self.embed_tokens(input_ids)
@@ -246,7 +248,7 @@ class W4A4LlamaModel(torch.nn.Module):
         return x
 
     def _rotary(self, positions, cache):
-        """cos / sin [T, head_dim] of `positions`.  With a static cache the table of all its slots is computed once and
+        """cos / sin [T, head_dim] of `positions`.  With a static cache the table of all its positions is computed once and
         the step's rows are gathered from it (two small launches instead of the dozen that build a table), the same
         values either way."""
         if cache is None:
@@ -257,7 +259,7 @@ class W4A4LlamaModel(torch.nn.Module):
     def _rotary_table(self, cache, device):
         table = getattr(cache, "rotary_table", None)
         if table is None:
-            table = rotary_tables(torch.arange(cache.max_len, device=device), self.shape.head_dim, self.shape.rope_theta)
+            table = rotary_tables(torch.arange(cache.max_positions or cache.max_len, device=device), self.shape.head_dim, self.shape.rope_theta)
             cache.rotary_table = table
         return table
 
@@ -320,12 +322,12 @@ class W4A4LlamaModel(torch.nn.Module):
         if input_ids.size(0) != cache.lengths.numel():
             raise ValueError(f"{b} sequences for a cache of {cache.lengths.numel()}")
         # (a sequence that takes no part has no position: any row of the table will do)
-        positions = (cache.lengths[:, None] + tree.depths).clamp(0, cache.max_len - 1).reshape(-1)
+        positions = (cache.next_positions()[:, None] + tree.depths).clamp(0, (cache.max_positions or cache.max_len) - 1).reshape(-1)
         x, cos, sin = self._look_up(input_ids, positions, cache)
         cos, sin = cos.view(b, t, -1), sin.view(b, t, -1)
-        pending = None
+        pending, lengths = None, cache.step_lengths(t)
         for i, layer in enumerate(self.layers):
-            x, pending, _ = layer.forward_deferred(x, pending, cos, sin, cache.tree_layer(i, tree))
+            x, pending, _ = layer.forward_deferred(x, pending, cos, sin, cache.tree_layer(i, tree, lengths))
         x = self._final_norm(x, pending)
         return x if return_hidden else self._head(x)
 

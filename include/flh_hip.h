@@ -497,7 +497,8 @@ int flh_prefill_attention_weights_f16(const flh_half* q, const flh_half* k_cache
  * that stay move to the slots 0 .. budget - 1 in their order; rows behind are left as they were.
  *   weights [layers, B, Hkv, max_len] float32 (as the calls above add them up);  kept [layers, B, Hkv, budget] int64 the slots that stay
  *   (-1 behind the last of a shorter sequence);  new_weights [layers, B, Hkv, max_len] their weights, zeros behind;
- *   new_lengths [B] = min(lengths, budget) (a length that is negative or above max_len stays, nothing kept).
+ *   new_lengths [B] = min(lengths, budget) (a length that is negative or above max_len stays: nothing kept, its new weights are zeros -- the
+ *   old ones are still in `weights`).
  * new_weights and new_lengths need memory of their own. */
 int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_half* const* v_caches, const float* weights, const int64_t* lengths,
                        int64_t* kept, float* new_weights, int64_t* new_lengths, uint32_t B, uint32_t Hkv, uint32_t head_dim,
