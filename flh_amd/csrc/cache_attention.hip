@@ -885,6 +885,8 @@ extern "C" int flh_tree_attention_f16(const flh_half* q, const flh_half* k_new, 
   const size_t need = flh_tree_attention_workspace_bytes(B, T, Hq, Hkv, head_dim);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return fail(FLH_EINVAL, "tree_attention: a 16-byte aligned workspace of %zu bytes is required", need);
+  const uint64_t cache = (uint64_t)B * Hkv * max_len * head_dim * 2;
+  if (overlap(k_cache, cache, v_cache, cache)) return fail(FLH_EINVAL, "tree_attention: the caches share memory");
   Call a = {};
   a.q = (const __half*)q, a.k_new = (const __half*)k_new, a.v_new = (const __half*)v_new, a.cos = (const __half*)cos, a.sin = (const __half*)sin;
   a.lengths = (const long long*)lengths, a.mask = mask, a.mask_stride = mask_per_sequence ? T * T : 0;
@@ -968,6 +970,9 @@ extern "C" int flh_prefill_attention_weights_f16(const flh_half* q, const flh_ha
   const size_t need = flh_prefill_attention_weights_workspace_bytes(B, T, Hq, Hkv, past);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return fail(FLH_EINVAL, "prefill_attention_weights: a 16-byte aligned workspace of %zu bytes is required", need);
+  const uint64_t queries = (uint64_t)B * T * Hq * head_dim * 2;
+  if (overlap(q, queries, out, queries))               // (the sums read the queries behind the attention)
+    return fail(FLH_EINVAL, "prefill_attention_weights: the output needs memory of its own");
   Columns a = {};
   a.q = (const __half*)q, a.k = (const __half*)k_cache, a.weights = weights;
   a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.past = past, a.max_len = max_len, a.scale_log2 = scale * 1.4426950408889634f;

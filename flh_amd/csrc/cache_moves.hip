@@ -6,6 +6,7 @@
 // Both are bound by the rows' bytes (each read and written once) and, for one sequence, by the launches.  Caches are compacted in
 // place: a copy would take as much memory again.
 #include <algorithm>
+#include <initializer_list>
 #include <new>
 #include <vector>
 
@@ -312,6 +313,21 @@ int check_caches(int layers, flh_half* const* k, flh_half* const* v, uint32_t B,
   return FLH_OK;
 }
 
+// Outputs in memory of their own: workgroups read the inputs while others write.
+struct Piece {
+  const void* at;
+  uint64_t bytes;
+};
+int check_outputs(std::initializer_list<Piece> outputs, std::initializer_list<Piece> inputs, const char* what) {
+  for (const Piece* o = outputs.begin(); o != outputs.end(); ++o) {
+    for (const Piece& i : inputs)
+      if (overlap(o->at, o->bytes, i.at, i.bytes)) return fail(FLH_EINVAL, "%s: an output shares memory with an input", what);
+    for (const Piece* p = outputs.begin(); p != o; ++p)
+      if (overlap(o->at, o->bytes, p->at, p->bytes)) return fail(FLH_EINVAL, "%s: two outputs share memory", what);
+  }
+  return FLH_OK;
+}
+
 }  // namespace
 }  // namespace flh
 
@@ -327,6 +343,10 @@ extern "C" int flh_tree_commit(const int64_t* tokens, const int64_t* parents, in
   if (lengths == new_lengths) return fail(FLH_EINVAL, "tree_commit: the new lengths need memory of their own");
   if (int rc = check_caches(layers, k_caches, v_caches, B, Hkv, head_dim, max_len, "tree_commit")) return rc;
   if (too_many_items(B, 256)) return fail(FLH_EINVAL, "tree_commit: problem too large");
+  const uint64_t nodes = (uint64_t)B * T * 8, each = (uint64_t)B * 8;
+  if (int rc = check_outputs({{path, nodes}, {accepted, each}, {next, each}, {new_lengths, each}},
+                             {{tokens, nodes}, {parents, parents_per_sequence ? nodes : T * 8ull}, {chosen, nodes}, {lengths, each}}, "tree_commit"))
+    return rc;
   if (B == 0) return FLH_OK;
   const uint32_t pieces = head_dim / 8, moves = 2 * Hkv * ((pieces + 15) / 16);
   const Tree t = {(const long long*)tokens, (const long long*)parents, (const long long*)chosen, (const long long*)lengths, (long long*)path,
@@ -355,6 +375,10 @@ extern "C" int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_hal
   const hipStream_t st = (hipStream_t)stream;
   const size_t units = (size_t)B * Hkv;
   if (too_many_items(units, kSelectThreads)) return fail(FLH_EINVAL, "evict_kv_cache: problem too large");
+  const uint64_t heads = (uint64_t)layers * units;
+  if (int rc = check_outputs({{kept, heads * budget * 8}, {new_weights, heads * max_len * 4}, {new_lengths, B * 8ull}},
+                             {{weights, heads * max_len * 4}, {lengths, B * 8ull}}, "evict_kv_cache"))
+    return rc;
   for (int l = 0; l < layers; l += kMaxLayers) {
     Caches c;
     const int n = layers - l < kMaxLayers ? layers - l : kMaxLayers;

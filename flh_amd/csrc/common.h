@@ -34,6 +34,11 @@ int reserve_lds(const void* kernel, size_t bytes, LdsGrant& grant, const char* w
 template <typename... P>
 inline bool misaligned16(P... p) { return (((uintptr_t)p | ...) & 15) != 0; }
 
+// whether two pieces of memory share a byte
+inline bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
+  return na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 // whether a launch's work items along one axis pass what it counts them in (32 bits)
 inline bool too_many_items(uint64_t workgroups, uint32_t threads) { return workgroups * threads > 0xFFFFFFFFull; }
 

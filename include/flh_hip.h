@@ -469,7 +469,7 @@ int flh_tree_attention_f16(const flh_half* q, const flh_half* k_new, const flh_h
  * (a lower index; node 0 is the root, the last token that was certain), chosen [B, T] int64 the token that the model picks behind
  * each node.  From node 0 on, the lowest child whose token is chosen[node] is accepted, until there is none:
  *   path [B, T] int64 the accepted nodes in order, -1 behind them;  accepted [B] their number;  next [B] chosen[last node];
- *   new_lengths [B] = lengths + accepted (memory of its own),
+ *   new_lengths [B] = lengths + accepted (all four in memory of their own),
  * and in every layer's caches [B, Hkv, max_len, head_dim] the rows of slots lengths + path[i] move to lengths + i; all other rows stay.  A
  * sequence whose length is negative or above max_len - T: nothing accepted or moved, next -1, its length as it was. */
 int flh_tree_commit(const int64_t* tokens, const int64_t* parents, int parents_per_sequence, const int64_t* chosen,
@@ -482,7 +482,8 @@ int flh_tree_commit(const int64_t* tokens, const int64_t* parents, int parents_p
  * (aligned as floats are: one layer's part of what flh_evict_kv_cache takes will do).
  * decode: one query per sequence, q, out [B, Hq, d], over the slots 0 .. lengths[b] - 1 (the new token's key and value among them; a
  * length of zero, a negative one or one above max_len: zeros, no weights); d 64 or 128.  prefill: flh_prefill_attention_f16 (d = 128, the
- * same output bits), each query over the slots it sees.  Sums are taken in a fixed order: the same call gives the same bits. */
+ * same output bits), each query over the slots it sees.  Sums are taken in a fixed order: the same call gives the same bits.  A prompt's output
+ * needs memory of its own (the queries are read again behind it). */
 size_t flh_decode_attention_weights_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len);
 int flh_decode_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, const int64_t* lengths,
                                      flh_half* out, float* weights, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
@@ -499,7 +500,7 @@ int flh_prefill_attention_weights_f16(const flh_half* q, const flh_half* k_cache
  *   (-1 behind the last of a shorter sequence);  new_weights [layers, B, Hkv, max_len] their weights, zeros behind;
  *   new_lengths [B] = min(lengths, budget) (a length that is negative or above max_len stays: nothing kept, its new weights are zeros -- the
  *   old ones are still in `weights`).
- * new_weights and new_lengths need memory of their own. */
+ * kept, new_weights and new_lengths need memory of their own. */
 int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_half* const* v_caches, const float* weights, const int64_t* lengths,
                        int64_t* kept, float* new_weights, int64_t* new_lengths, uint32_t B, uint32_t Hkv, uint32_t head_dim,
                        uint32_t max_len, uint32_t budget, uint32_t recent, void* stream);

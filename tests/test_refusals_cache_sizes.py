@@ -56,3 +56,41 @@ def test_sums_of_weights_are_aligned_as_floats(name, args):
     for at, message in ((OK + 2, b"4-byte aligned"), (OK + 4, b"workspace"), (OK + 8, b"workspace")):
         assert getattr(lib, name)(*(at if x == "weights" else x for x in args)) == -1
         assert message in lib.flh_last_error(), lib.flh_last_error()
+
+
+AT = [(i + 2) << 32 for i in range(12)]                                # places far from one another
+
+
+@pytest.mark.parametrize("k,v", [(AT[0], AT[0]), (AT[0], AT[0] + 16), (AT[0] + 2 * 2 * 64 * 128 * 2 - 16, AT[0])])
+def test_the_caches_of_a_tree_share_no_memory(k, v):
+    lib = _lib.load()
+    assert lib.flh_tree_attention_f16(*[OK] * 7, 0, k, v, OK, 2, 8, 8, 2, 128, 64, 0.1, OK, BIG, None) == -1
+    assert b"share memory" in lib.flh_last_error()
+
+
+@pytest.mark.parametrize("shift", [0, 16, 1 * 4 * 8 * 128 * 2 - 16, -16])
+def test_the_output_of_a_prompt_with_weights_is_not_its_queries(shift):
+    lib = _lib.load()
+    assert lib.flh_prefill_attention_weights_f16(AT[0], AT[1], AT[2], AT[0] + shift, AT[3], 1, 4, 8, 2, 128, 0, 64, 0.1, OK, BIG, None) == -1
+    assert b"memory of its own" in lib.flh_last_error()
+
+
+@pytest.mark.parametrize("one,other,shift,message", [(4, 0, 0, b"with an input"), (4, 2, 8, b"with an input"), (5, 1, 56, b"with an input"),
+                                                     (6, 3, 8, b"with an input"), (4, 3, -8, b"with an input"),
+                                                     (5, 4, 8, b"two outputs"), (6, 5, 0, b"two outputs"), (7, 6, 8, b"two outputs")])
+def test_the_outputs_of_a_commit_are_in_memory_of_their_own(one, other, shift, message):
+    at = AT[:8]                                                        # tokens, parents, chosen, lengths; path, accepted, next, new lengths
+    at[one] = at[other] + shift
+    lib = _lib.load()
+    assert lib.flh_tree_commit(*at[:2], 0, *at[2:], 1, *CACHES, 2, 8, 2, 8, 16, None) == -1
+    assert message in lib.flh_last_error(), lib.flh_last_error()
+
+
+@pytest.mark.parametrize("one,other,shift,message", [(2, 0, 0, b"with an input"), (3, 0, 4, b"with an input"), (4, 1, 8, b"with an input"),
+                                                     (3, 2, 8, b"two outputs"), (4, 3, 0, b"two outputs")])
+def test_the_outputs_of_an_eviction_are_in_memory_of_their_own(one, other, shift, message):
+    at = AT[:5]                                                        # weights, lengths; kept, new weights, new lengths
+    at[one] = at[other] + shift
+    lib = _lib.load()
+    assert lib.flh_evict_kv_cache(1, *CACHES, *at, 2, 2, 8, 16, 8, 4, None) == -1
+    assert message in lib.flh_last_error(), lib.flh_last_error()
