@@ -912,7 +912,8 @@ extern "C" int flh_decode_attention_weights_f16(const flh_half* q, const flh_hal
   if (misaligned16(q, k_cache, v_cache, out)) return fail(FLH_EINVAL, "decode_attention_weights: tensors must be 16-byte aligned");
   if ((uintptr_t)weights & 3) return fail(FLH_EINVAL, "decode_attention_weights: the weights must be 4-byte aligned");
   if (int rc = check_heads("decode_attention_weights", Hq, Hkv, head_dim, scale)) return rc;
-  if (B == 0 || max_len == 0) return FLH_OK;
+  if (max_len == 0) return fail(FLH_EINVAL, "decode_attention_weights: the caches have no slots");
+  if (B == 0) return FLH_OK;
   if (too_large(B, 1, Hq, Hkv, head_dim, max_len)) return fail(FLH_EINVAL, "decode_attention_weights: problem too large");
   const size_t need = flh_decode_attention_weights_workspace_bytes(B, Hq, Hkv, head_dim, max_len);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)

@@ -94,3 +94,10 @@ def test_the_outputs_of_an_eviction_are_in_memory_of_their_own(one, other, shift
     lib = _lib.load()
     assert lib.flh_evict_kv_cache(1, *CACHES, *at, 2, 2, 8, 16, 8, 4, None) == -1
     assert message in lib.flh_last_error(), lib.flh_last_error()
+
+
+def test_a_decode_step_over_caches_without_slots_is_refused():
+    """(zeros are documented where there is nothing to see: success without writing them is not that)"""
+    lib = _lib.load()
+    assert lib.flh_decode_attention_weights_f16(*AT[:6], 2, 8, 2, 128, 0, 0.1, OK, BIG, None) == -1
+    assert b"no slots" in lib.flh_last_error()
