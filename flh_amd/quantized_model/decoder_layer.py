@@ -158,6 +158,8 @@ class StaticKVCache:
         return self._positions[self.kv_len - t:self.kv_len]
 
     def layer(self, index):
+        if self.lengths is not None:        # (attention would read kv_len slots of every sequence)
+            raise ValueError("the sequences of this cache have lengths of their own: tree_layer()")
         return StaticKVCache._Layer(self, index)
 
     class _TreeLayer:
