@@ -12,8 +12,8 @@ PARENTS = [-1, 0, 0, 1, 1, 2, 5, 6]
 T, SLOTS = len(PARENTS), 160
 
 
-def make(activation="group"):
-    return W4A4LlamaModel.random_init(SHAPE, activation=activation, weight_group_size=128, fused=True, device="cuda", seed=3)
+def make(activation="group", shape=SHAPE):
+    return W4A4LlamaModel.random_init(shape, activation=activation, weight_group_size=128, fused=True, device="cuda", seed=3)
 
 
 def prompted(model, length=100, **more):
@@ -134,6 +134,32 @@ def test_a_step_captured_in_front_of_a_cut_serves_behind_it():
         assert cache.next_positions().tolist() == [100 + 3 * 5, 100 + 5]
 
 
+def test_a_place_takes_a_new_prompt_as_chains():
+    """A finished sequence's place: its length (and cut) zero, the other one out of the steps; the prompt as chains of up to 256 tokens,
+    all accepted.  The first layer's rows have the bits that one chain of the whole prompt leaves."""
+    model = make()
+    cache, other = prompted(model, max_positions=400), prompted(model, max_positions=400)
+    cache.evict(sums(), 60, 10)
+    waiting = [c[1].clone() for c in cache.keys + cache.values]
+    ids = torch.randint(0, 512, (2, 120), device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    with torch.no_grad():
+        for c, pieces in ((cache, (70, 50)), (other, (120,))):
+            c.lengths.copy_(torch.tensor([0, -1]))
+            c.cut.zero_()
+            at = 0
+            for n in pieces:
+                chain, part = DraftTree(range(-1, n - 1)), ids[:, at:at + n].contiguous()
+                model.tree_step(part, chain, c)
+                _, accepted, _ = c.commit(part, chain, torch.cat((part[:, 1:], part[:, :1]), 1))
+                assert accepted.tolist() == [n, 0]
+                at += n
+            assert c.lengths.tolist() == [120, -1]
+    for a, b in zip((cache.keys[0], cache.values[0]), (other.keys[0], other.values[0])):
+        assert torch.equal(a[0, :, :120], b[0, :, :120])
+    for a, b in zip(waiting, cache.keys + cache.values):
+        assert torch.equal(a, b[1])
+
+
 def test_refusals():
     model = make()
     with pytest.raises(ValueError, match="below max_len"):
@@ -149,16 +175,19 @@ def test_refusals():
         cache.evict(sums()[:1].contiguous(), 40, 8)
 
 
+@pytest.mark.parametrize("batch,nodes,hidden", [(2, 4, 1024), (1, 1, 1024), (1, 1, 4096), (1, 2, 4096), (2, 1, 4096), (3, 1, 4096),
+                                                (1, 17, 4096), (3, 43, 1024), (1, 256, 1024), (2, 256, 1024)])
 @pytest.mark.parametrize("activation", ["group", "token"])
-def test_nodes_that_see_only_themselves_are_steps_of_one_token(activation):
-    """A node that sees nothing but itself attends to its own value, exactly: its logits have the bits of a first token's step."""
-    model = make(activation)
-    ids = torch.randint(0, 512, (2, 4), device="cuda", generator=torch.Generator("cuda").manual_seed(9))
-    tree = DraftTree([-1, 0, 0, 0])
-    tree.mask.copy_(torch.eye(4, dtype=torch.bool))
-    first, cache = model.new_cache(8, 16), model.new_cache(2, 16)
+def test_nodes_that_see_only_themselves_are_steps_of_one_token(activation, batch, nodes, hidden):
+    """A node that sees nothing but itself attends to its own value, exactly: its logits have the bits of a first token's step, whichever
+    launches a step of that many tokens takes."""
+    model = make(activation, LlamaShape(hidden, hidden // 128, hidden // 512, 2 * hidden, 1 if hidden > 1024 else 2, 512, 1e-5, 10000.0))
+    ids = torch.randint(0, 512, (batch, nodes), device="cuda", generator=torch.Generator("cuda").manual_seed(9))
+    tree = DraftTree([-1] + [0] * (nodes - 1))
+    tree.mask.copy_(torch.eye(nodes, dtype=torch.bool))
+    first, cache = model.new_cache(batch * nodes, 2), model.new_cache(batch, nodes)
     cache.begin_drafts()
     with torch.no_grad():
-        want = model(ids.view(8, 1), first.advance(1), first)
+        want = model(ids.view(-1, 1), first.advance(1), first)
         got = model.tree_step(ids, tree, cache)
-    assert torch.equal(got.view(8, 1, -1), want)
+    assert torch.equal(got.view(batch * nodes, 1, -1), want)
