@@ -180,11 +180,20 @@ __device__ __forceinline__ bool finite8(h8& x) {
 // moves every score by 2^-11 of its size, twice the error of the result's own rounding (4.3e-4 against 2.1e-4 of the 2-norm).  That costs
 // 26.7 -> 28.6 us (2 x 63 nodes of 64 channels behind 5001 tokens), 126 -> 141 (8 x 64 of 128 behind 8192, where the MFMAs bound the launch).
 //
-// What bounds it: memory up to about 64 rows of a head (decode with weights, 16 x up to 4000 slots of 32 / 8 heads: 209 MB in 41 us, 5.1 TB/s,
-// where a large copy reads and writes 4.9), the MFMAs from there on (8 x 64 behind 8192: 104 Gflop with the low halves in 117 us = 0.89
-// PFLOP/s, where an 8192^3 product of the vendor's reaches 1.14).  Short calls are latencies: the lengths, then the queries and the first
-// tile, then the pieces in the second launch (1 x 8 behind 120: 9 + 3 us).  Not taken: fragments read during the MFMAs before them, as in
-// the prefill kernel (no gain, 131 against 130 us, or spills); tiles of a wave of its own two ahead without barriers (58.4 against 58.9 us).
+// Probabilities are rounded to fp16 without a low half: independent errors of 2^-11 each, which a sum over many slots averages, next to the
+// result's own rounding of as much (2.104e-4 of the 2-norm against 2.069e-4 with float32 probabilities, 8 x 64 behind 8192; 2.144e-4
+// against 2.093e-4 over the 128 slots of 1 x 8 behind 120).  Low halves with MFMAs of their own give the float32 figure for 144 -> 164 us
+// (in a graph; 2 x 63: 26.8 -> 29.7, 4 x 26 behind 1500: 30.9 -> 31.5, decode 16 x 4000: 49.7 -> 50.4), and make an infinite cached value
+// NaN where a low half is zero.
+//
+// What bounds it: memory up to about 64 rows of a head (decode with weights, 16 x up to 4000 slots of 32 / 8 heads: 209 MB in 41 us,
+// 5.1 TB/s, where a large copy reads and writes 4.9), the MFMAs from there on (8 x 64 behind 8192: 104 Gflop with the low halves in
+// 128 us = 0.81 PFLOP/s, where an 8192^3 product of the vendor's reaches 1.14).  Short shares are ramps as much as tiles.  By a clock in
+// the kernel, us: 2 x 63 of 64 channels, five tiles of 64 keys a workgroup: workgroups start over 4.2, lengths and list 0.9, queries and
+// their rotation 1.7, the tiles 7.5, the piece 0.7; a share that ends one head and begins the next pays queries and piece again (the last
+// ends at 19).  1 x 8 behind 120: starts 2.4, list 0.7, queries 2.4, a cached tile 1.0, the tree's 1.9, the piece 1.2; then the second
+// launch (9 + 4 traced).  Not taken: fragments read during the MFMAs before them, as in the prefill kernel (no gain, 131 against 130 us,
+// or spills); tiles of a wave of its own two ahead without barriers (58.4 against 58.9 us).
 template <int D, int WR, bool TREE, bool NT>
 __global__ __launch_bounds__(256, D == 128 && WR == 1 ? 1 : 2) void cache_attention_kernel(const Call a) {
   constexpr int WK = 4 / WR, NKT = WR == 4 ? 2 : 1, KT = 32 * NKT * WK;

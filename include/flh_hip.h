@@ -481,9 +481,11 @@ int flh_tree_commit(const int64_t* tokens, const int64_t* parents, int parents_p
  *   weights[b, g, j] += sum of the probabilities of slot j over the queries of key / value head g,  float32 [B, Hkv, max_len].
  * (aligned as floats are: one layer's part of what flh_evict_kv_cache takes will do).
  * decode: one query per sequence, q, out [B, Hq, d], over the slots 0 .. lengths[b] - 1 (the new token's key and value among them; a
- * length of zero, a negative one or one above max_len: zeros, no weights); d 64 or 128.  prefill: flh_prefill_attention_f16 (d = 128, the
- * same output bits), each query over the slots it sees.  Sums are taken in a fixed order: the same call gives the same bits.  A prompt's output
- * needs memory of its own (the queries are read again behind it). */
+ * length of zero, a negative one or one above max_len: zeros, no weights); d 64 or 128; for the output probabilities are rounded to
+ * fp16 as above, where flh_decode_attention_f16 keeps them in float32 (the sums take them unrounded).  prefill: flh_prefill_attention_f16 (d = 128, the
+ * same output bits), each query over the slots it sees.  Sums are taken in a fixed order: the same call gives the same bits.  A query that has no
+ * probabilities (a NaN among its scores) makes the sums of all slots that it sees NaN, and no others.  A prompt's output needs memory
+ * of its own (the queries are read again behind it). */
 size_t flh_decode_attention_weights_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len);
 int flh_decode_attention_weights_f16(const flh_half* q, const flh_half* k_cache, const flh_half* v_cache, const int64_t* lengths,
                                      flh_half* out, float* weights, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
