@@ -14,7 +14,6 @@ class OnDevice(torch.Tensor):
     is_cuda = property(lambda self: True)
 
 
-
 def dev(*shape, dtype=torch.float16):
     return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
 
