@@ -38,6 +38,10 @@ rope_kv_cache_ = _ext.rope_kv_cache_
 tree_attention = _ext.tree_attention
 decode_attention_weights = _ext.decode_attention_weights
 prefill_attention_weights = _ext.prefill_attention_weights
+rope_quantize_kv_cache_ = _ext.rope_quantize_kv_cache_
+dequantize_kv_cache = _ext.dequantize_kv_cache
+decode_attention_rope_i4 = _ext.decode_attention_rope_i4
+prefill_attention_i4 = _ext.prefill_attention_i4
 rotate_quantize_gemm_i4 = _ext.rotate_quantize_gemm_i4
 rotate_quantize_gemm_i4_multi = _ext.rotate_quantize_gemm_i4_multi
 rmsnorm_rotate_quantize_gemm_i4_multi = _ext.rmsnorm_rotate_quantize_gemm_i4_multi

@@ -859,6 +859,115 @@ def prefill_attention_weights(q, k_cache, v_cache, past, weights, scale=None, wo
     return out
 
 
+def _check_halves(device, *tensors):
+    for t_ in tensors:
+        _check(t_.is_cuda and t_.dtype == torch.float16 and t_.is_contiguous() and t_.device == device,
+               "tensors must be contiguous float16 CUDA tensors on one device")
+
+
+def _check_cache_i4(device, batch, d, k_codes, k_scales, v_codes, v_scales):
+    """A layer's cache in 4 bits -> (Hkv, max_len)"""
+    for t_ in (k_codes, v_codes):
+        _check(t_.is_cuda and t_.dtype == torch.uint8 and t_.is_contiguous() and t_.device == device,
+               "codes must be contiguous uint8 CUDA tensors on one device")
+    _check_halves(device, k_scales, v_scales)
+    _check(k_codes.dim() == 4 and k_codes.shape == v_codes.shape and k_codes.size(0) == batch and k_codes.size(3) * 2 == d
+           and k_scales.shape == k_codes.shape[:3] and v_scales.shape == k_scales.shape,
+           "codes must be [B, Hkv, max_len, d / 2], scales [B, Hkv, max_len]")
+    _check(d in (64, 128), "head_dim must be 64 or 128")
+    _check(k_codes.size(1) > 0 and k_codes.size(2) > 0, "the caches have no heads or slots")
+    _check(max(k_codes.shape) < 2 ** 31, "caches: problem too large")     # (the C ABI takes sizes of 32 bits)
+    return k_codes.size(1), k_codes.size(2)
+
+
+def rope_quantize_kv_cache_(q, k, v, cos, sin, lengths, k_codes, k_scales, v_codes, v_scales):
+    """A block of T new tokens per sequence into a cache held in 4 bits: q [B, T, Hq, d], k / v [B, T, Hkv, d] fp16 as projected, cos / sin
+    [B, T, d] fp16 the rotary rows of the tokens' positions, lengths [B] int64 the slots taken.  Keys are turned by the rotary embedding and
+    the orthonormal Hadamard matrix of their head, keys and values quantised row by row (scale fp16(max / 7), codes -8 .. 7) and written to
+    the slots lengths[b] .. lengths[b] + T - 1 of k_codes / v_codes [B, Hkv, max_len, d / 2] uint8 and k_scales / v_scales [B, Hkv, max_len]
+    fp16.  -> the queries turned alike, [B, T, Hq, d] (q stays as it was).  A sequence whose length is negative or above max_len - T takes
+    no part: its cache stays as it was.  d in {64, 128}."""
+    _check(q.dim() == 4 and k.dim() == 4, "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected")
+    B, T, Hq, d = q.shape
+    _check_halves(q.device, q, k, v, cos, sin)
+    Hkv, max_len = _check_cache_i4(q.device, B, d, k_codes, k_scales, v_codes, v_scales)
+    _check(k.shape == (B, T, Hkv, d) and v.shape == k.shape, "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected")
+    _check(cos.shape == (B, T, d) and sin.shape == (B, T, d), "cos / sin must be [B, T, d]")
+    _check_lengths(lengths, B, q.device)
+    _check(Hq > 0 and max(q.shape) < 2 ** 31, "q must have heads, and less than 2^31 of anything")
+    out = torch.empty_like(q)
+    if B and T:
+        _run("flh_rope_quant_kv_cache_i4", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+             lengths.data_ptr(), out.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), B, T, Hq,
+             Hkv, d, max_len, _stream(q))
+    return out
+
+
+def dequantize_kv_cache(k_codes, k_scales, v_codes, v_scales, first, rows):
+    """Rows of a cache held in 4 bits as fp16: the slots first[b] .. first[b] + rows - 1 (first int64 [B] on the device) of every sequence ->
+    (keys, values) [B, Hkv, rows, d], keys with the Hadamard rotation undone (rotary embedding and all, as an fp16 cache holds them).  A slot outside
+    the cache gives zeros."""
+    _check(k_codes.dim() == 4, "codes must be [B, Hkv, max_len, d / 2], scales [B, Hkv, max_len]")
+    B, d, rows = k_codes.size(0), 2 * k_codes.size(3), int(rows)
+    Hkv, max_len = _check_cache_i4(k_codes.device, B, d, k_codes, k_scales, v_codes, v_scales)
+    _check_lengths(first, B, k_codes.device)
+    _check(0 <= rows < 2 ** 31, "rows must be in 0 .. 2^31 - 1")
+    keys, values = (torch.empty((B, Hkv, rows, d), dtype=torch.float16, device=k_codes.device) for _ in range(2))
+    if B and rows:
+        _run("flh_dequant_kv_cache_i4", k_codes.device, k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+             first.data_ptr(), keys.data_ptr(), values.data_ptr(), B, rows, Hkv, d, max_len, _stream(k_codes))
+    return keys, values
+
+
+def decode_attention_rope_i4(q, k_new, v_new, cos, sin, lengths, k_codes, k_scales, v_codes, v_scales, scale=None, workspace=None):
+    """One new token per sequence on a cache held in 4 bits, rotation, quantisation, cache write and attention in one pair of launches:
+    q [B, Hq, d], k_new / v_new [B, Hkv, d] fp16 as projected (left as they are), cos / sin [B, d], lengths [B] int64 the slots taken in
+    front of the token, which takes slot lengths[b] (the bytes of rope_quantize_kv_cache_) -> [B, Hq, d] fp16, attention over the slots
+    0 .. lengths[b] as they are held.  Hq a multiple of Hkv, d in {64, 128}.  A sequence whose length is negative or above max_len - 1
+    takes no part: zeros, its cache untouched.  `workspace` as in decode_attention."""
+    _check(q.dim() == 3, "q [B, Hq, d] expected")
+    B, Hq, d = q.shape
+    _check_halves(q.device, q, k_new, v_new, cos, sin)
+    Hkv, max_len = _check_cache_i4(q.device, B, d, k_codes, k_scales, v_codes, v_scales)
+    _check(k_new.shape == (B, Hkv, d) and v_new.shape == k_new.shape, "k_new / v_new [B, Hkv, d] expected")
+    _check(cos.shape == (B, d) and sin.shape == (B, d), "cos / sin must be [B, d]")
+    _check_lengths(lengths, B, q.device)
+    _check(Hq > 0 and Hq % Hkv == 0, "Hq must be a multiple of Hkv")
+    out = torch.empty_like(q)
+    if B == 0:
+        return out
+    need = int(_lib.load().flh_decode_attention_i4_workspace_bytes(B, Hq, Hkv, d, max_len))
+    with _attention_workspace(q, need, workspace) as ws:
+        _run("flh_decode_attention_rope_i4", q.device, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+             lengths.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), out.data_ptr(), B, Hq, Hkv, d,
+             max_len, float(scale if scale is not None else d ** -0.5), ws.data_ptr(), ws.numel(), _stream(q))
+    return out
+
+
+def prefill_attention_i4(q, lengths, k_codes, k_scales, v_codes, v_scales, scale=None, workspace=None):
+    """Causal attention of a block of T new tokens per sequence over a cache held in 4 bits that rope_quantize_kv_cache_ has written them
+    to: q [B, T, Hq, d] fp16 (its result), lengths [B] int64 the slots taken in front of the block; query t sees the slots
+    0 .. lengths[b] + t -> [B, T, Hq * d] fp16.  Hq a multiple of Hkv, d in {64, 128}.  A sequence whose length is negative or above
+    max_len - T: zeros.  `workspace` as in decode_attention (calls with many rows take none)."""
+    _check(q.dim() == 4, "q [B, T, Hq, d] expected")
+    B, T, Hq, d = q.shape
+    _check_halves(q.device, q)
+    Hkv, max_len = _check_cache_i4(q.device, B, d, k_codes, k_scales, v_codes, v_scales)
+    _check_lengths(lengths, B, q.device)
+    _check(Hq > 0 and Hq % Hkv == 0, "Hq must be a multiple of Hkv")
+    _check(max(q.shape) < 2 ** 31, "q: problem too large")
+    out = torch.empty((B, T, Hq * d), dtype=torch.float16, device=q.device)
+    if B == 0 or T == 0:
+        return out
+    need = int(_lib.load().flh_prefill_attention_i4_workspace_bytes(B, T, Hq, Hkv, d, max_len))
+    with contextlib.nullcontext() if need == 0 else _attention_workspace(q, need, workspace) as ws:
+        _run("flh_prefill_attention_i4", q.device, q.data_ptr(), lengths.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(),
+             v_codes.data_ptr(), v_scales.data_ptr(), out.data_ptr(), B, T, Hq, Hkv, d, max_len,
+             float(scale if scale is not None else d ** -0.5), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+             _stream(q))
+    return out
+
+
 def _check_weights(weights, shape, device):
     _check(weights.is_cuda and weights.dtype == torch.float32 and weights.is_contiguous() and tuple(weights.shape) == shape
            and weights.device == device, f"weights must be a contiguous float32 CUDA tensor {list(shape)}")

@@ -1,0 +1,473 @@
+// Attention of ONE new token per sequence over a key / value cache held in 4 bits (cache_i4.h) whose sequences have lengths of their own, with
+// the rotary embedding, the Hadamard rotation, the quantisation and the cache write of the new token inside:
+//
+//   s[j] = scale ks[j] (q . ck[j]),  p[j] = exp(s[j] - max s),  out = sum_j p[j] vs[j] cv[j] / sum_j p[j]
+//
+// over the slots 0 .. lengths[b], the new token's among them as it is held.  Codes enter both products as they are: a row's scale is one
+// factor of its score, or of its probability.
+//
+// Work: for every sequence and key / value head (or sixteen of its queries) the tiles of 64 keys form one list, cut into equal shares on the
+// device, one a workgroup, whose four waves take every fourth tile.  A share that spans two heads writes two pieces (reference, sum,
+// weighted codes); piece number = workgroup + head, unique because one of them grows from a piece to the next.  A second launch joins them.
+//
+// A wave works by itself: a tile's codes and scales come straight to LDS, the next tile's while it is worked on.  Matrix tiles have keys
+// (scores) or channels (output) as rows and the queries of the key / value head as their sixteen columns.  A lane's sixteen scores of a tile
+// are those that its operand of the second product takes, and the values' nibbles are read to match by the LDS transpose load for 4 bits.
+#include "cache_i4.h"
+
+namespace flh {
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4, kCols = 16, kStages = 2;
+
+struct Decode {
+  const __half *q, *k_new, *v_new, *cos, *sin;
+  const long long* lengths;
+  uint8_t *k_codes, *v_codes;
+  __half *k_scales, *v_scales, *out;
+  float* partials;
+  uint32_t B, Hq, Hkv, rep, blocks, max_len, groups;   // blocks: of sixteen queries, per key / value head
+  float scale_log2;
+};
+
+// tiles of a sequence whose new token takes slot n (none: it takes no part)
+__device__ __forceinline__ uint32_t tiles_of(const Decode& a, long long n) {
+  return n < 0 || n >= (long long)a.max_len ? 0u : (uint32_t)n / kTileKeys + 1;
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+
+struct Place {
+  uint32_t b, length, tiles, before;                   // a sequence, its slots taken, tiles of a head, tiles of the sequences before it
+};
+
+// The sequences' tiles, 64 sequences in the lanes at a time
+struct Shares {
+  uint32_t c, total, heads;                            // tiles of a workgroup, of all; heads of a sequence
+  uint32_t length, tiles, up, first, before;           // of the 64 last looked at
+
+  __device__ __forceinline__ void look(const Decode& a, uint32_t b0) {
+    const uint32_t b = b0 + (threadIdx.x & 63);
+    const long long n = b < a.B ? a.lengths[b] : -1;
+    tiles = tiles_of(a, n);
+    length = (uint32_t)n;
+    up = wave_scan(tiles * heads);
+    first = b0;
+  }
+  __device__ __forceinline__ explicit Shares(const Decode& a) {
+    heads = a.Hkv * a.blocks;
+    total = 0;
+    for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+      look(a, b0);
+      before = total;
+      total += lane_value(up, 63);
+    }
+    c = max(1u, (total + a.groups - 1) / a.groups);
+    if (c > kWaves) c = (c + kWaves - 1) / kWaves * kWaves;
+  }
+  __device__ __forceinline__ Place in_lane(int l) const {
+    const uint32_t t = lane_value(tiles, l);
+    return {first + l, lane_value(length, l), t, before + lane_value(up, l) - t * heads};
+  }
+  __device__ __forceinline__ Place of(const Decode& a, uint32_t b) {
+    if (b - first >= 64) {
+      before = 0;
+      for (uint32_t b0 = 0;; b0 += 64) {
+        look(a, b0);
+        if (b - b0 < 64) break;
+        before += lane_value(up, 63);
+      }
+    }
+    return in_lane(b - first);
+  }
+  // the sequence that holds tile `pos` (below total)
+  __device__ __forceinline__ Place at(const Decode& a, uint32_t pos) {
+    if (a.B > 64) {
+      before = 0;
+      for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+        look(a, b0);
+        if (before + lane_value(up, 63) > pos) break;
+        before += lane_value(up, 63);
+      }
+    }
+    return in_lane(__builtin_ctzll(__ballot(before + up > pos)));
+  }
+};
+
+template <int D>
+struct Layout {
+  static constexpr int kRowBytes = D / 2, kTile = kTileKeys * kRowBytes;      // a tile's codes
+  static constexpr int kLoads = kTile / 1024;                                // direct-to-LDS loads for them
+  static constexpr int kStage = 2 * kTile + 2 * kTileKeys * 4;               // K, V, their scales (a dword each)
+  static constexpr int kQPitch = D * 2 + 16;                                 // bytes of a query's halves
+  static constexpr int kPiece = D + 2;                                       // floats of a piece and query
+  // the waves' stages; the queries' high and low halves; their factors and biases; the new row's codes and scales
+  static constexpr int kQ = kWaves * kStages * kStage, kFactor = kQ + 2 * kCols * kQPitch, kNew = kFactor + 2 * kCols * 4,
+                       kBytes = kNew + 2 * kRowBytes + 16;
+  static_assert(kCols * kPiece * 4 <= kStages * kStage, "a wave's result takes the place of its stages");
+};
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
+  using L = Layout<D>;
+  extern __shared__ __align__(1024) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, kb = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned lds0 = (unsigned)(size_t)lds;
+  uint8_t* const mine = lds + wave * (kStages * L::kStage);
+  const unsigned mine0 = lds0 + wave * (kStages * L::kStage);
+  Shares shares(a);
+  uint32_t pos = blockIdx.x * shares.c;
+  const uint32_t end = min(shares.total, pos + shares.c);
+
+  // where a lane's sixteen bytes of a load come from (1 KiB of rows): chunks of sixteen bytes are permuted so that neither the rows of a
+  // score operand nor the sixteen keys of a transpose load fall on the same banks
+  unsigned k_src[L::kLoads], v_src[L::kLoads];
+#pragma unroll
+  for (int i = 0; i < L::kLoads; ++i) {
+    if constexpr (D == 128) {
+      k_src[i] = i * 1024 + (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) << 4);
+      v_src[i] = i * 1024 + (lane >> 2) * 64 + (((lane & 3) ^ i) << 4);
+    } else {
+      k_src[i] = i * 1024 + (lane >> 1) * 32 + (((lane & 1) ^ ((lane >> 4) & 1)) << 4);
+      v_src[i] = i * 1024 + (lane >> 1) * 32 + (((lane & 1) ^ ((lane >> 5) & 1)) << 4);
+    }
+  }
+  // byte of chunk `c` in row `r` of a tile as it lies in LDS
+  auto k_at = [](int r, int c) { return D == 128 ? r * 64 + ((c ^ ((r >> 2) & 3)) << 4) : r * 32 + ((c ^ ((r >> 3) & 1)) << 4); };
+  auto v_at = [](int r, int c) { return D == 128 ? r * 64 + ((c ^ ((r >> 4) & 3)) << 4) : r * 32 + ((c ^ ((r >> 4) & 1)) << 4); };
+
+  while (pos < end) {
+    const Place place = shares.at(a, pos);
+    const uint32_t unit = (pos - place.before) / place.tiles;                   // of the sequence's heads x blocks
+    const uint32_t head_start = place.before + unit * place.tiles;
+    const uint32_t first = pos - head_start, stop = min(place.tiles, first + (end - pos));
+    const uint32_t hkv = unit / a.blocks, q0 = (unit % a.blocks) * kCols, cols = min((uint32_t)kCols, a.rep - q0);
+    const uint32_t bh = place.b * a.Hkv + hkv, slot = place.length;
+    const bool has_new = stop == place.tiles;
+
+    // ---- the rows that are turned here: sixteen queries, the new key, the new value
+    constexpr int kLanes = HeadRow<D>::kLanes;
+    const uint32_t r = tid / kLanes, chunk = HeadRow<D>::chunk_of(tid % kLanes);
+    const bool is_q = r < cols, is_new = has_new && (r == kCols || r == kCols + 1), is_v = r == kCols + 1;
+    h8 x[2] = {}, c[2] = {}, s[2] = {};
+    if (is_q || is_new) {
+      const __half* src = is_q ? a.q + ((size_t)place.b * a.Hq + hkv * a.rep + q0 + r) * D : (is_v ? a.v_new : a.k_new) + (size_t)bh * D;
+      const __half *cs = a.cos + (size_t)place.b * D, *sn = a.sin + (size_t)place.b * D;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        x[i] = *(const h8*)(src + chunk * 8 + i * (D / 2));
+        c[i] = *(const h8*)(cs + chunk * 8 + i * (D / 2));
+        s[i] = *(const h8*)(sn + chunk * 8 + i * (D / 2));
+      }
+    }
+
+    const uint8_t* const k_base = a.k_codes + (size_t)bh * a.max_len * L::kRowBytes;
+    const uint8_t* const v_base = a.v_codes + (size_t)bh * a.max_len * L::kRowBytes;
+    const v4i k_rows = buffer_of(k_base, (slot + 1) * L::kRowBytes), v_rows = buffer_of(v_base, (slot + 1) * L::kRowBytes);
+    const v4i k_sc = buffer_of((const uint8_t*)(a.k_scales + (size_t)bh * a.max_len), (slot + 1) * 2);
+    const v4i v_sc = buffer_of((const uint8_t*)(a.v_scales + (size_t)bh * a.max_len), (slot + 1) * 2);
+    auto request = [&](uint32_t tile, int stage) {
+      const unsigned to = mine0 + stage * L::kStage, from = tile * L::kTile;
+#pragma unroll
+      for (int i = 0; i < L::kLoads; ++i) rows_to_lds(k_rows, from + k_src[i], to + i * 1024);
+#pragma unroll
+      for (int i = 0; i < L::kLoads; ++i) rows_to_lds(v_rows, from + v_src[i], to + L::kTile + i * 1024);
+      halves_to_lds(k_sc, (tile * kTileKeys + lane) * 2, to + 2 * L::kTile);
+      halves_to_lds(v_sc, (tile * kTileKeys + lane) * 2, to + 2 * L::kTile + kTileKeys * 4);
+    };
+    uint32_t tile = first + wave;
+    if (tile < stop) request(tile, 0);
+
+    HeadRow<D> row;
+    row.set(x[0], x[1]);
+    if (!is_v) {
+      row.turn(c[0], c[1], s[0], s[1]);
+      row.hadamard(chunk);
+      row.scale(HeadRow<D>::norm());
+    }
+    if (r < kCols) {
+      // a query as two fp16 values, its largest between 2^8 and 2^9
+      const unsigned top = row.top();
+      const unsigned e = min(254u, 262u - (top >> 23));
+      row.scale(__int_as_float((int)(e << 23)));
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        h8 high, low;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float y = row.v[8 * i + k];
+          const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
+          high[code_element(k)] = hi, low[code_element(k)] = lo;
+          sum += (float)hi + (float)lo;
+        }
+        *(h8*)(lds + L::kQ + r * L::kQPitch + (chunk + i * (D / 16)) * 16) = high;
+        *(h8*)(lds + L::kQ + (kCols + r) * L::kQPitch + (chunk + i * (D / 16)) * 16) = low;
+      }
+      sum += dpp_f<kDppQuadXor1>(sum);
+      sum += dpp_f<kDppQuadXor2>(sum);
+      if constexpr (kLanes == 8) sum += dpp_f<kDppRowHalfMirror>(sum);
+      if (chunk == 0) {
+        float* f = (float*)(lds + L::kFactor);
+        f[r] = __builtin_fmaxf(__int_as_float((int)((254u - e) << 23)) * kFromSubnormal * a.scale_log2, 1e-37f);   // (never zero: it meets -inf)
+        f[kCols + r] = -8.0f / kFromSubnormal * sum;
+      }
+    } else if (is_new) {
+      const RowCodes codes = quantise(row);
+      uint8_t* there = lds + L::kNew + (is_v ? L::kRowBytes : 0);
+      *(unsigned*)(there + chunk * 4) = codes.lo;
+      *(unsigned*)(there + D / 4 + chunk * 4) = codes.hi;
+      if (chunk == 0) *(unsigned*)(lds + L::kNew + 2 * L::kRowBytes + (is_v ? 4 : 0)) = __builtin_bit_cast(unsigned short, codes.scale);
+      if (q0 == 0) {
+        uint8_t* to = (is_v ? a.v_codes : a.k_codes) + ((size_t)bh * a.max_len + slot) * L::kRowBytes;
+        *(unsigned*)(to + chunk * 4) = codes.lo;
+        *(unsigned*)(to + D / 4 + chunk * 4) = codes.hi;
+        if (chunk == 0) ((_Float16*)(is_v ? a.v_scales : a.k_scales))[(size_t)bh * a.max_len + slot] = codes.scale;
+      }
+    }
+    __syncthreads();
+
+    // this lane's column: query `col`, channels of its quarter of the rows
+    constexpr int kSteps = D / 32;
+    h8 qh[kSteps], ql[kSteps];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      qh[j] = *(const h8*)(lds + L::kQ + col * L::kQPitch + (kb * kSteps + j) * 16);
+      ql[j] = *(const h8*)(lds + L::kQ + (kCols + col) * L::kQPitch + (kb * kSteps + j) * 16);
+    }
+    const float factor = ((const float*)(lds + L::kFactor))[col], bias = ((const float*)(lds + L::kFactor))[kCols + col];
+
+    float ref = kLowestRef, l = 0.f;
+    v4f o[D / 16], ob = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[i] = ob;
+
+    for (int stage = 0; tile < stop; tile += kWaves, stage ^= 1) {
+      if (tile + kWaves < stop) {
+        wait_lds();                                    // (what was read of the stage before)
+        request(tile + kWaves, stage ^ 1);
+        wait_vmcnt<2 * L::kLoads + 2>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      asm volatile("" ::: "memory");
+      uint8_t* const kt = mine + stage * L::kStage;
+      uint8_t* const vt = kt + L::kTile;
+      unsigned* const ks = (unsigned*)(vt + L::kTile);
+      unsigned* const vs = ks + kTileKeys;
+      const bool last = tile + 1 == place.tiles;
+      if (last) {                                      // the new row takes the place of what the cache held
+        const int n = slot % kTileKeys;
+        if (lane < L::kRowBytes / 16) *(v4i*)(kt + k_at(n, lane)) = *(const v4i*)(lds + L::kNew + lane * 16);
+        else if (lane >= 32 && lane < 32 + L::kRowBytes / 16)
+          *(v4i*)(vt + v_at(n, lane - 32)) = *(const v4i*)(lds + L::kNew + L::kRowBytes + (lane - 32) * 16);
+        else if (lane == 63) ks[n] = *(const unsigned*)(lds + L::kNew + 2 * L::kRowBytes), vs[n] = *(const unsigned*)(lds + L::kNew + 2 * L::kRowBytes + 4);
+        wait_lds();
+      }
+      // ---- scores: tile t of sixteen keys as rows, key 16 t + 4 kb + i in element i
+      v4f st[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        st[t] = v4f{bias, bias, bias, bias};
+        unsigned w[kSteps];
+        if constexpr (D == 128) *(v4i*)w = *(const v4i*)(kt + k_at(16 * t + col, kb));
+        else *(v2i*)w = *(const v2i*)(kt + k_at(16 * t + col, kb >> 1) + (kb & 1) * 8);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+          const h8 k = code_halves(w[j]);
+          st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[j], st[t], 0, 0, 0);
+          st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], st[t], 0, 0, 0);
+        }
+      }
+      // ---- softmax relative to a reference that also holds the values' largest scale back: p vs <= 2^15
+      unsigned v[4][4], big = 0;
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const v4i k4 = *(const v4i*)(ks + 16 * t + 4 * kb), v4 = *(const v4i*)(vs + 16 * t + 4 * kb);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[t][i] = (unsigned)v4[i];
+          big = max(big, v[t][i] & 0x7FFFu);
+          st[t][i] = times_half(st[t][i], (unsigned)k4[i]);
+          if (last && tile * kTileKeys + 16 * t + 4 * kb + i > slot) st[t][i] = -INFINITY;
+          top = __builtin_fmaxf(top, st[t][i]);
+        }
+      }
+      top = __builtin_fmaxf(top, lane_xor_f<16>(top));
+      top = __builtin_fmaxf(top, lane_xor_f<32>(top));
+      big = max(big, (unsigned)lane_xor_i<16>((int)big));
+      big = max(big, (unsigned)lane_xor_i<32>((int)big));
+      const float now = __builtin_fmaxf(ref, __builtin_fmaf(top, factor, (float)((int)(min(big, 0x7C00u) >> 10) - 29)));
+      if (__builtin_amdgcn_ballot_w64(now != ref) != 0) {
+        const float alpha = __builtin_amdgcn_exp2f(ref - now);
+        l *= alpha;
+        ob *= alpha;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
+        ref = now;
+      }
+      h8 p[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * u][i], factor, -ref));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * u + 1][i], factor, -ref));
+          l += p0 + p1;
+          const h2 w = pair_times_halves(p0, v[2 * u][i], p1, v[2 * u + 1][i]);
+          p[u][2 * i] = w[0], p[u][2 * i + 1] = w[1];
+        }
+      // ---- output: sixteen channels as rows; a lane's sixteen keys 16 t + 4 kb + i in nibble 4 t + i
+      const int key = 16 * (col >> 2) + 4 * kb + (col & 3);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(bias_halves(), p[u], ob, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i*)(vt + v_at(key, i >> 1) + (i & 1) * 8));
+        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_halves((unsigned)w[0]), p[0], o[i], 0, 0, 0);
+        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_halves((unsigned)w[1]), p[1], o[i], 0, 0, 0);
+      }
+    }
+
+    // ---- the waves' results into one piece
+    l += lane_xor_f<16>(l);
+    l += lane_xor_f<32>(l);
+    wait_lds();
+    float* const there = (float*)mine;                 // (its own stages: everything asked for has come)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) *(v4f*)(there + col * L::kPiece + 16 * i + 4 * kb) = (o[i] - ob) * kFromSubnormal;
+    if (kb == 0) there[col * L::kPiece + D] = ref, there[col * L::kPiece + D + 1] = l;
+    __syncthreads();
+    float* const piece = a.partials + ((size_t)(blockIdx.x + (size_t)place.b * shares.heads + unit) * kCols) * L::kPiece;
+    for (uint32_t i = tid; i < cols * D; i += kThreads) {
+      const uint32_t h = i / D, ch = i % D;
+      float m = kLowestRef, w[kWaves], sum = 0.f, total = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) m = __builtin_fmaxf(m, ((const float*)(lds + k * (kStages * L::kStage)))[h * L::kPiece + D]);
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) {
+        const float* from = (const float*)(lds + k * (kStages * L::kStage)) + h * L::kPiece;
+        w[k] = first + k < stop ? __builtin_amdgcn_exp2f(from[D] - m) : 0.f;
+        total += first + k < stop ? w[k] * from[ch] : 0.f;
+        sum += first + k < stop ? w[k] * from[D + 1] : 0.f;
+      }
+      piece[h * L::kPiece + ch] = total;
+      if (ch == 0) piece[h * L::kPiece + D] = m, piece[h * L::kPiece + D + 1] = sum;
+    }
+    __syncthreads();
+    pos += stop - first;
+  }
+}
+
+// one workgroup of four waves per (sequence, query head): its pieces, one wave every fourth, then the waves' sums in a fixed order
+template <int D>
+__global__ __launch_bounds__(256) void decode_i4_join_kernel(Decode a) {
+  constexpr int kPiece = D + 2;
+  __shared__ float sums[4][D], refs[4], ls[4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t b = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq;
+  Shares shares(a);
+  const Place place = shares.of(a, b);
+  const uint32_t hkv = hq / a.rep, in_head = hq % a.rep, unit = hkv * a.blocks + in_head / kCols, h = in_head % kCols;
+  float m = kLowestRef, l = 0.f, o[D / 64] = {};
+  if (place.tiles) {
+    const uint32_t start = place.before + unit * place.tiles;
+    const uint32_t g0 = start / shares.c, g1 = (start + place.tiles - 1) / shares.c;
+    for (uint32_t g = g0 + wave; g <= g1; g += 4) {
+      const float* piece = a.partials + ((size_t)(g + (size_t)b * shares.heads + unit) * kCols + h) * kPiece;
+      const float pm = piece[D], now = __builtin_fmaxf(m, pm);
+      const float old = __builtin_amdgcn_exp2f(m - now), w = __builtin_amdgcn_exp2f(pm - now);
+      l = l * old + w * piece[D + 1];
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) o[i] = o[i] * old + w * piece[lane + 64 * i];
+      m = now;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) sums[wave][lane + 64 * i] = o[i];
+  if (lane == 0) refs[wave] = m, ls[wave] = l;
+  __syncthreads();
+  if (tid < D) {
+    const float top = __builtin_fmaxf(__builtin_fmaxf(refs[0], refs[1]), __builtin_fmaxf(refs[2], refs[3]));
+    float all = 0.f, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = __builtin_amdgcn_exp2f(refs[k] - top);
+      all += w * ls[k], sum += w * sums[k][tid];
+    }
+    ((_Float16*)a.out)[(size_t)blockIdx.x * D + tid] = (_Float16)(place.tiles ? sum / all : 0.f);
+  }
+}
+
+constexpr uint32_t kGroups = 512;                      // two workgroups on each compute unit
+
+uint32_t blocks_of(uint32_t rep) { return (rep + kCols - 1) / kCols; }
+
+bool too_large(uint64_t B, uint64_t Hq, uint64_t Hkv, uint32_t head_dim, uint64_t max_len) {
+  const uint64_t heads = B * Hkv * blocks_of((uint32_t)(Hq / Hkv));
+  return B > 0x7FFFFFFFull || B * Hq > 0x7FFFFFull || heads > 0x7FFFFFull || max_len > (1u << 25) || heads * (max_len / kTileKeys + 1) > 0x7FFFFFFFull ||
+         B * Hkv * max_len > 1ull << 40;
+}
+
+}  // namespace
+}  // namespace flh
+
+using namespace flh;
+
+extern "C" size_t flh_decode_attention_i4_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
+  if (Hq == 0 || Hkv == 0 || Hq % Hkv || (head_dim != 128 && head_dim != 64) || max_len == 0 || too_large(B, Hq, Hkv, head_dim, max_len)) return 0;
+  const uint64_t heads = (uint64_t)B * Hkv * blocks_of(Hq / Hkv);
+  return (size_t)(kGroups + heads) * kCols * (head_dim + 2) * sizeof(float);
+}
+
+extern "C" int flh_decode_attention_rope_i4(const flh_half* q, const flh_half* k_new, const flh_half* v_new, const flh_half* cos,
+                                            const flh_half* sin, const int64_t* lengths, uint8_t* k_codes, flh_half* k_scales,
+                                            uint8_t* v_codes, flh_half* v_scales, flh_half* out, uint32_t B, uint32_t Hq, uint32_t Hkv,
+                                            uint32_t head_dim, uint32_t max_len, float scale, void* workspace, size_t workspace_bytes,
+                                            void* stream) {
+  const char* what = "decode_attention (4-bit cache)";
+  if (!q || !k_new || !v_new || !cos || !sin || !lengths || !k_codes || !k_scales || !v_codes || !v_scales || !out)
+    return fail(FLH_EINVAL, "%s: null pointer", what);
+  if (misaligned16(q, k_new, v_new, cos, sin, k_codes, v_codes, out)) return fail(FLH_EINVAL, "%s: tensors must be 16-byte aligned", what);
+  if (head_dim != 128 && head_dim != 64) return fail(FLH_EINVAL, "%s: head_dim (%u) must be 64 or 128", what, head_dim);
+  if (Hq == 0 || Hkv == 0 || Hq % Hkv) return fail(FLH_EINVAL, "%s: %u query heads do not divide over %u key / value heads", what, Hq, Hkv);
+  if (max_len == 0) return fail(FLH_EINVAL, "%s: the caches have no slots", what);
+  if (bad_scale(scale)) return fail(FLH_EINVAL, "%s: the scale must be positive and at most 1e15", what);
+  if (B == 0) return FLH_OK;
+  if (too_large(B, Hq, Hkv, head_dim, max_len)) return fail(FLH_EINVAL, "%s: problem too large", what);
+  const size_t need = flh_decode_attention_i4_workspace_bytes(B, Hq, Hkv, head_dim, max_len);
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
+    return fail(FLH_EINVAL, "%s: a 16-byte aligned workspace of %zu bytes is required", what, need);
+  const uint64_t slots = (uint64_t)B * Hkv * max_len, queries = (uint64_t)B * Hq * head_dim * 2, rows = (uint64_t)B * Hkv * head_dim * 2;
+  const struct { const void* at; uint64_t bytes; } held[6] = {{k_codes, slots * (head_dim / 2)}, {k_scales, slots * 2}, {v_codes, slots * (head_dim / 2)},
+                                                              {v_scales, slots * 2}, {workspace, need}, {out, queries}},
+      in[6] = {{k_new, rows}, {v_new, rows}, {cos, (uint64_t)B * head_dim * 2}, {sin, (uint64_t)B * head_dim * 2}, {lengths, (uint64_t)B * 8}, {q, queries}};
+  for (int i = 0; i < 6; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (overlap(held[i].at, held[i].bytes, held[j].at, held[j].bytes)) return fail(FLH_EINVAL, "%s: outputs, caches or workspace share memory", what);
+    // (the joining launch alone writes `out`, behind everything that reads the queries, keys and values; it reads the lengths itself)
+    for (int j = 0; j < 6; ++j)
+      if (overlap(held[i].at, held[i].bytes, in[j].at, in[j].bytes) && (i < 5 || j == 4))
+        return fail(FLH_EINVAL, "%s: an output shares memory with an input", what);
+  }
+  Decode a = {};
+  a.q = (const __half*)q, a.k_new = (const __half*)k_new, a.v_new = (const __half*)v_new, a.cos = (const __half*)cos, a.sin = (const __half*)sin;
+  a.lengths = (const long long*)lengths, a.k_codes = k_codes, a.v_codes = v_codes, a.k_scales = (__half*)k_scales, a.v_scales = (__half*)v_scales;
+  a.out = (__half*)out, a.partials = (float*)workspace;
+  a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.blocks = blocks_of(a.rep), a.max_len = max_len;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const uint64_t most = (uint64_t)B * Hkv * a.blocks * ((max_len - 1) / kTileKeys + 1);
+  a.groups = (uint32_t)(most < kGroups ? most : kGroups);
+  auto go = [&](auto kern, auto join, size_t smem, LdsGrant& grant) {
+    if (int rc = reserve_lds((const void*)kern, smem, grant, what)) return rc;
+    hipLaunchKernelGGL(kern, dim3(a.groups), dim3(kThreads), smem, (hipStream_t)stream, a);
+    if (int rc = check_launch(what)) return rc;
+    hipLaunchKernelGGL(join, dim3(B * Hq), dim3(256), 0, (hipStream_t)stream, a);
+    return check_launch(what);
+  };
+  static LdsGrant grant128, grant64;
+  return head_dim == 128 ? go(decode_i4_kernel<128>, decode_i4_join_kernel<128>, Layout<128>::kBytes, grant128)
+                         : go(decode_i4_kernel<64>, decode_i4_join_kernel<64>, Layout<64>::kBytes, grant64);
+}

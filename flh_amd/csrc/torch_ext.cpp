@@ -271,6 +271,114 @@ Tensor prefill_attention_weights(const Tensor& q, const Tensor& k_cache, const T
   return out;
 }
 
+// ---- caches held in 4 bits (the checks of _ops.py) ---------------------------------------------------------------------------
+void check_halves(const c10::Device& device, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kFloat16 && t->is_contiguous() && t->device() == device,
+                "tensors must be contiguous float16 CUDA tensors on one device");
+}
+
+int64_t largest(const Tensor& t) {
+  int64_t m = 0;
+  for (int64_t n : t.sizes()) m = std::max(m, n);
+  return m;
+}
+
+struct CacheI4 {   // a layer's cache and its sizes
+  uint8_t *k_codes, *v_codes;
+  flh_half *k_scales, *v_scales;
+  int64_t Hkv, max_len;
+  CacheI4(const c10::Device& device, int64_t batch, int64_t d, const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs) {
+    for (const Tensor* t : {&kc, &vc})
+      TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kUInt8 && t->is_contiguous() && t->device() == device,
+                  "codes must be contiguous uint8 CUDA tensors on one device");
+    check_halves(device, {&ks, &vs});
+    TORCH_CHECK(kc.dim() == 4 && kc.sizes() == vc.sizes() && kc.size(0) == batch && kc.size(3) * 2 == d && ks.sizes() == kc.sizes().slice(0, 3) &&
+                    vs.sizes() == ks.sizes(), "codes must be [B, Hkv, max_len, d / 2], scales [B, Hkv, max_len]");
+    TORCH_CHECK(d == 64 || d == 128, "head_dim must be 64 or 128");
+    Hkv = kc.size(1), max_len = kc.size(2);
+    TORCH_CHECK(Hkv > 0 && max_len > 0, "the caches have no heads or slots");
+    TORCH_CHECK(largest(kc) < (1ll << 31), "caches: problem too large");   // (the C ABI takes sizes of 32 bits)
+    k_codes = (uint8_t*)kc.data_ptr(), v_codes = (uint8_t*)vc.data_ptr();
+    k_scales = (flh_half*)ks.data_ptr(), v_scales = (flh_half*)vs.data_ptr();
+  }
+};
+
+Tensor rope_quantize_kv_cache_(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos, const Tensor& sin, const Tensor& lengths,
+                               Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales) {
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4, "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected");
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), d = q.size(3);
+  check_halves(q.device(), {&q, &k, &v, &cos, &sin});
+  const CacheI4 c(q.device(), B, d, k_codes, k_scales, v_codes, v_scales);
+  const int64_t rows[] = {B, T, c.Hkv, d}, rotary[] = {B, T, d};
+  TORCH_CHECK(k.sizes() == at::IntArrayRef(rows) && v.sizes() == k.sizes(), "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected");
+  TORCH_CHECK(cos.sizes() == at::IntArrayRef(rotary) && sin.sizes() == cos.sizes(), "cos / sin must be [B, T, d]");
+  check_lengths(lengths, B, q.device());
+  TORCH_CHECK(Hq > 0 && largest(q) < (1ll << 31), "q must have heads, and less than 2^31 of anything");
+  Tensor out = torch::empty_like(q);
+  if (B == 0 || T == 0) return out;
+  Launch l(q);
+  ok(flh_rope_quant_kv_cache_i4(h(q), h(k), h(v), h(cos), h(sin), lengths.data_ptr<int64_t>(), hm(out), c.k_codes, c.k_scales, c.v_codes,
+                                c.v_scales, B, T, Hq, c.Hkv, d, c.max_len, stream_of(q)));
+  return out;
+}
+
+std::pair<Tensor, Tensor> dequantize_kv_cache(const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
+                                              const Tensor& first, int64_t rows) {
+  TORCH_CHECK(k_codes.dim() == 4, "codes must be [B, Hkv, max_len, d / 2], scales [B, Hkv, max_len]");
+  const int64_t B = k_codes.size(0), d = 2 * k_codes.size(3);
+  const CacheI4 c(k_codes.device(), B, d, k_codes, k_scales, v_codes, v_scales);
+  check_lengths(first, B, k_codes.device());
+  TORCH_CHECK(rows >= 0 && rows < (1ll << 31), "rows must be in 0 .. 2^31 - 1");
+  Tensor keys = torch::empty({B, c.Hkv, rows, d}, k_scales.options()), values = torch::empty_like(keys);
+  if (B == 0 || rows == 0) return {keys, values};
+  Launch l(k_codes);
+  ok(flh_dequant_kv_cache_i4(c.k_codes, c.k_scales, c.v_codes, c.v_scales, first.data_ptr<int64_t>(), hm(keys), hm(values), B, rows, c.Hkv, d,
+                             c.max_len, stream_of(k_codes)));
+  return {keys, values};
+}
+
+Tensor decode_attention_rope_i4(const Tensor& q, const Tensor& k_new, const Tensor& v_new, const Tensor& cos, const Tensor& sin,
+                                const Tensor& lengths, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales,
+                                const c10::optional<double>& scale, const c10::optional<Tensor>& workspace) {
+  TORCH_CHECK(q.dim() == 3, "q [B, Hq, d] expected");
+  const int64_t B = q.size(0), Hq = q.size(1), d = q.size(2);
+  check_halves(q.device(), {&q, &k_new, &v_new, &cos, &sin});
+  const CacheI4 c(q.device(), B, d, k_codes, k_scales, v_codes, v_scales);
+  const int64_t rows[] = {B, c.Hkv, d}, rotary[] = {B, d};
+  TORCH_CHECK(k_new.sizes() == at::IntArrayRef(rows) && v_new.sizes() == k_new.sizes(), "k_new / v_new [B, Hkv, d] expected");
+  TORCH_CHECK(cos.sizes() == at::IntArrayRef(rotary) && sin.sizes() == cos.sizes(), "cos / sin must be [B, d]");
+  check_lengths(lengths, B, q.device());
+  TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0, "Hq must be a multiple of Hkv");
+  Tensor out = torch::empty_like(q);
+  if (B == 0) return out;
+  Launch l(q);
+  Tensor ws = attention_workspace(q, workspace, flh_decode_attention_i4_workspace_bytes(B, Hq, c.Hkv, d, c.max_len));
+  ok(flh_decode_attention_rope_i4(h(q), h(k_new), h(v_new), h(cos), h(sin), lengths.data_ptr<int64_t>(), c.k_codes, c.k_scales, c.v_codes,
+                                  c.v_scales, hm(out), B, Hq, c.Hkv, d, c.max_len, scale_of(scale, d), ws.data_ptr(), ws.numel(), stream_of(q)));
+  return out;
+}
+
+Tensor prefill_attention_i4(const Tensor& q, const Tensor& lengths, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes,
+                            const Tensor& v_scales, const c10::optional<double>& scale, const c10::optional<Tensor>& workspace) {
+  TORCH_CHECK(q.dim() == 4, "q [B, T, Hq, d] expected");
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), d = q.size(3);
+  check_halves(q.device(), {&q});
+  const CacheI4 c(q.device(), B, d, k_codes, k_scales, v_codes, v_scales);
+  check_lengths(lengths, B, q.device());
+  TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0, "Hq must be a multiple of Hkv");
+  TORCH_CHECK(largest(q) < (1ll << 31), "q: problem too large");
+  Tensor out = torch::empty({B, T, Hq * d}, q.options());
+  if (B == 0 || T == 0) return out;
+  Launch l(q);
+  const size_t need = flh_prefill_attention_i4_workspace_bytes(B, T, Hq, c.Hkv, d, c.max_len);
+  Tensor ws;
+  if (need) ws = attention_workspace(q, workspace, need);
+  ok(flh_prefill_attention_i4(h(q), lengths.data_ptr<int64_t>(), c.k_codes, c.k_scales, c.v_codes, c.v_scales, hm(out), B, T, Hq, c.Hkv, d,
+                              c.max_len, scale_of(scale, d), need ? ws.data_ptr() : nullptr, need ? ws.numel() : 0, stream_of(q)));
+  return out;
+}
+
 struct CacheList {   // the layers' caches and their common shape
   std::vector<flh_half*> k, v;
   int64_t B, Hkv, max_len, d;
@@ -1214,6 +1322,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("weights"), py::arg("scale") = py::none(), py::arg("workspace") = py::none());
   m.def("prefill_attention_weights", &prefill_attention_weights, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("past"),
         py::arg("weights"), py::arg("scale") = py::none(), py::arg("workspace") = py::none());
+  m.def("rope_quantize_kv_cache_", &rope_quantize_kv_cache_, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cos"), py::arg("sin"),
+        py::arg("lengths"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"));
+  m.def("dequantize_kv_cache", &dequantize_kv_cache, py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"),
+        py::arg("first"), py::arg("rows"));
+  m.def("decode_attention_rope_i4", &decode_attention_rope_i4, py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("cos"), py::arg("sin"),
+        py::arg("lengths"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("scale") = py::none(),
+        py::arg("workspace") = py::none());
+  m.def("prefill_attention_i4", &prefill_attention_i4, py::arg("q"), py::arg("lengths"), py::arg("k_codes"), py::arg("k_scales"),
+        py::arg("v_codes"), py::arg("v_scales"), py::arg("scale") = py::none(), py::arg("workspace") = py::none());
   m.def("tree_commit_", &tree_commit_);
   m.def("evict_kv_cache_", &evict_kv_cache_);
   m.def("rotate_quantize_gemm_i4", &rotate_quantize_gemm_i4, py::arg("x"), py::arg("B"), py::arg("B_scale"));

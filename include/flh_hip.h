@@ -507,6 +507,50 @@ int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_half* const* v
                        int64_t* kept, float* new_weights, int64_t* new_lengths, uint32_t B, uint32_t Hkv, uint32_t head_dim,
                        uint32_t max_len, uint32_t budget, uint32_t recent, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * A key / value cache held in 4 bits, its sequences with lengths of their own.  A layer's cache is k_codes, v_codes [B, Hkv, max_len,
+ * head_dim / 2] u8 (packed int4 as above) and k_scales, v_scales [B, Hkv, max_len] fp16, one scale per row of a head; head_dim 64 or 128: 0.52 or
+ * 0.53 byte per value instead of 2.  No counterpart in the reference (whose caches are fp16).  Keys are held as they are after the rotary
+ * embedding and the orthonormal Hadamard rotation of their head; queries are rotated alike.
+ *   r = x cos + rotate_half(x) sin;  y = H r / sqrt(d);  s = fp16(max |y| / 7) (0: 1);  code = clamp(rint(y / s), -8, 7)
+ * in float32 (butterflies in ascending stride order; values are quantised the same way without rotation).  A row that is not finite, or whose
+ * scale is not, is held as scale NaN with codes of zero.
+ *
+ * T new tokens per sequence: token t of sequence b takes slot lengths[b] + t.  q [B, T, Hq, d], k, v [B, T, Hkv, d] fp16 as projected; cos, sin
+ * [B, T, d];  q_out [B, T, Hq, d] = fp16(y) of the queries (may be q itself).  A sequence whose length is negative or above max_len - T takes no
+ * part: nothing is written to its cache. */
+int flh_rope_quant_kv_cache_i4(const flh_half* q, const flh_half* k, const flh_half* v, const flh_half* cos, const flh_half* sin,
+                               const int64_t* lengths, flh_half* q_out, uint8_t* k_codes, flh_half* k_scales, uint8_t* v_codes,
+                               flh_half* v_scales, uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len,
+                               void* stream);
+
+/* Rows of such a cache back as fp16: keys, values [B, Hkv, rows, d] = slots first[b] .. first[b] + rows - 1 (first [B] int64 on the
+ * device), keys with the Hadamard rotation undone.  A slot outside the cache gives zeros. */
+int flh_dequant_kv_cache_i4(const uint8_t* k_codes, const flh_half* k_scales, const uint8_t* v_codes, const flh_half* v_scales,
+                            const int64_t* first, flh_half* keys, flh_half* values, uint32_t B, uint32_t rows, uint32_t Hkv,
+                            uint32_t head_dim, uint32_t max_len, void* stream);
+
+/* A decode step on it: q [B, Hq, d], k_new, v_new [B, Hkv, d] as projected, cos, sin [B, d]; the new token's key and value go to slot
+ * lengths[b] (the bytes of flh_rope_quant_kv_cache_i4), and out [B, Hq, d] is attention over the slots 0 .. lengths[b], the new one as it
+ * is held among them.  Hq a multiple of Hkv.  A sequence whose length is negative or above max_len - 1: zeros, its cache untouched.  Softmax
+ * statistics and sums in float32, probabilities (times their value's scale) rounded to fp16 for the second product.  workspace: 16-byte
+ * aligned, contents irrelevant; launches that share one must not overlap. */
+size_t flh_decode_attention_i4_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len);
+int flh_decode_attention_rope_i4(const flh_half* q, const flh_half* k_new, const flh_half* v_new, const flh_half* cos, const flh_half* sin,
+                                 const int64_t* lengths, uint8_t* k_codes, flh_half* k_scales, uint8_t* v_codes, flh_half* v_scales,
+                                 flh_half* out, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len, float scale,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal attention of T new tokens per sequence that flh_rope_quant_kv_cache_i4 has written behind the lengths: q [B, T, Hq, d] its q_out;
+ * query t of sequence b sees the slots 0 .. lengths[b] + t.  out [B, T, Hq * d].  Hq a multiple of Hkv; a sequence whose length is negative or above
+ * max_len - T: zeros.  What a query does not see may hold anything.  Roundings as above; workspace as above (0 bytes for calls whose rows fill
+ * the chip: NULL then). */
+size_t flh_prefill_attention_i4_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len);
+int flh_prefill_attention_i4(const flh_half* q, const int64_t* lengths, const uint8_t* k_codes, const flh_half* k_scales,
+                             const uint8_t* v_codes, const flh_half* v_scales, flh_half* out, uint32_t B, uint32_t T, uint32_t Hq,
+                             uint32_t Hkv, uint32_t head_dim, uint32_t max_len, float scale, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
 #ifdef __cplusplus
 }
 #endif
