@@ -2,13 +2,14 @@
 // t sits in slot lengths[b] + t and sees the slots up to its own.  Queries as the cache's writer leaves them (rotated like the keys), token-major
 // [B, T, Hq, D]; output [B, T, Hq * D].
 //
-// The rows of a key / value head are its T x rep queries, token by token: one workgroup = 4 waves = 128 of them, 32 per wave, so that heads that
-// share keys share the work of bringing them.  Both products run on v_mfma_f32_32x32x16_f16 in transposed form (a lane owns one query):
+// The rows of a key / value head are its T x rep queries, token by token: a workgroup has 32 of them, so that heads that share keys share the
+// work of bringing them, and its four waves take every fourth tile of 64 keys each, by themselves, without a barrier.  Both products run on
+// v_mfma_f32_32x32x16_f16 in transposed form (a lane owns one query):
 //
 //   S^T[key, query] = sum_d ck[key, d] Q[query, d]      O^T[d, query] += sum_key cv[key, d] (p vs)[query, key]
 //
-// with the codes as they are held (code_halves), keys' scales multiplied into the scores and values' into the probabilities.  Tiles of 64 keys,
-// three in LDS as packed codes (8 KiB each) by direct-to-LDS loads; values are transposed by the LDS load for 4 bits.
+// with the codes as they are held (code_halves), keys' scales multiplied into the scores and values' into the probabilities.  A tile comes to
+// LDS as packed codes (8 KiB) by direct-to-LDS loads, the next one while it is worked on; values are transposed by the LDS load for 4 bits.
 //
 // Few rows: the tiles of a block are split over several workgroups, whose pieces (reference, sum, weighted codes) a second launch joins.
 #include "cache_i4.h"
@@ -16,7 +17,7 @@
 namespace flh {
 namespace {
 
-constexpr int kThreads = 256, kBlockRows = 128, kStages = 3;
+constexpr int kThreads = 256, kWaves = 4, kBlockRows = 32, kStages = 2;
 
 struct Prefill {
   const __half* q;
@@ -25,308 +26,360 @@ struct Prefill {
   const __half *k_scales, *v_scales;
   __half* out;
   float* pieces;
-  uint32_t B, T, Hq, Hkv, rep, max_len, rows, blocks, splits;   // rows of a key / value head, blocks of 128 of them
+  uint32_t B, T, Hq, Hkv, rep, max_len, rows, blocks, splits;   // rows of a key / value head, blocks of 32 of them
   float scale_log2;
 };
 
-// floats of a piece: 128 rows of D sums, their references and sums of exponentials
+// The tiles of a block are split only as far as every workgroup has kSplitTiles: known on the device alone, like the lengths
+constexpr uint32_t kSplitTiles = 8;
+__device__ __forceinline__ uint32_t splits_for(const Prefill& a, uint32_t tiles) {
+  return max(1u, min(a.splits, (tiles + kSplitTiles - 1) / kSplitTiles));
+}
+// tiles with a slot that a query of the block sees (none: the sequence takes no part)
+__device__ __forceinline__ uint32_t tiles_of(const Prefill& a, long long length, uint32_t block) {
+  if (length < 0 || length > (long long)a.max_len - (long long)a.T) return 0;
+  return ((uint32_t)length + (min((block + 1) * kBlockRows, a.rows) - 1) / a.rep) / kTileKeys + 1;
+}
+
+// floats of a piece: 32 rows of D sums, their references and sums of exponentials
 template <int D>
 constexpr uint32_t kPieceFloats = kBlockRows * (D + 2);
 
 template <int D>
 struct Layout {
-  static constexpr int kRowBytes = D / 2, kTile = kTileKeys * kRowBytes, kStage = 2 * kTile + 2 * kTileKeys * 4;
-  static constexpr int kOutPitch = D * 2 + 16;
-  static constexpr int kBig = kStages * kStage, kBytes0 = kBig + 16;
-  static constexpr int kBytes = kBytes0 > kBlockRows * kOutPitch ? kBytes0 : kBlockRows * kOutPitch;
+  static constexpr int kRowBytes = D / 2, kTile = kTileKeys * kRowBytes, kLoads = kTile / 1024;
+  static constexpr int kStage = 2 * kTile + 2 * kTileKeys * 4;
+  // a wave's result: rows of D floats and their reference and sum, 16 bytes further each so that the lanes of a store meet other banks
+  static constexpr int kPitch = D + 4;
+  static constexpr int kWave = kStages * kStage > (kBlockRows * kPitch + 2 * kBlockRows) * 4 ? kStages * kStage : (kBlockRows * kPitch + 2 * kBlockRows) * 4;
+  static constexpr int kBytes = kWaves * kWave;
 };
 
-template <int D>
+// what is made of it here is not made in front of the branch that it is needed behind
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// KW: waves that share 32 rows and take every fourth tile (4), or waves with rows of their own (1)
+template <int D, int KW>
 __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
   using L = Layout<D>;
   extern __shared__ __align__(1024) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned lds0 = (unsigned)(size_t)lds;
+  uint8_t* const mine = lds + wave * L::kWave;
+  const unsigned mine0 = (unsigned)(size_t)mine;
   // every die takes a contiguous range of (sequence, key / value head) pairs; within one the long blocks (late queries) come first
   const unsigned w = xcd_contiguous(blockIdx.x, gridDim.x);
-  const uint32_t split = w % a.splits, block = a.blocks - 1 - w / a.splits % a.blocks, bh = w / a.splits / a.blocks;
+  uint32_t split, block, bh;
+  if constexpr (KW == 1) {                             // (one workgroup for four blocks, one piece each)
+    const uint32_t quads = (a.blocks + 3) / 4;
+    split = 0, bh = w / quads, block = (quads - 1 - w % quads) * 4 + wave;
+    if (block >= a.blocks) return;
+  } else {
+    split = w % a.splits, block = a.blocks - 1 - w / a.splits % a.blocks, bh = w / a.splits / a.blocks;
+  }
   const uint32_t b = bh / a.Hkv, hkv = bh % a.Hkv;
   const long long len = a.lengths[b];
-  const bool takes_part = len >= 0 && len <= (long long)a.max_len - (long long)a.T;
-  const uint32_t length = takes_part ? (uint32_t)len : 0u;
+  const uint32_t tiles = tiles_of(a, len, block), splits = KW == 1 ? 1 : splits_for(a, tiles);
+  if (split >= splits) return;
+  const uint32_t length = tiles ? (uint32_t)len : 0u;
 
-  const uint32_t first_row = block * kBlockRows + wave * 32;
-  const uint32_t row = min(first_row + n, a.rows - 1);                 // (rows past the end repeat the last one; never stored)
+  const uint32_t first_row = block * kBlockRows, live_rows = min((uint32_t)kBlockRows, a.rows - first_row);
+  const uint32_t row = first_row + min((uint32_t)n, live_rows - 1);    // (rows past the end repeat the last one; never stored)
   const uint32_t t = row / a.rep, head = hkv * a.rep + row % a.rep;
   const size_t q_at = (((size_t)b * a.T + t) * a.Hq + head) * D;
   const int limit = (int)(length + t);                                 // the last slot that the lane's query sees
-  const uint32_t last_row = min(block * kBlockRows + kBlockRows, a.rows) - 1;
-  const uint32_t slots = length + last_row / a.rep + 1;                // slots that any query of the block sees
-  const uint32_t all_tiles = takes_part ? (slots + kTileKeys - 1) / kTileKeys : 0;
-  const uint32_t tile0 = (uint32_t)((uint64_t)all_tiles * split / a.splits), tile1 = (uint32_t)((uint64_t)all_tiles * (split + 1) / a.splits);
-  // tiles with a slot that some query of the wave sees
-  const uint32_t wave_slots = length + min(first_row + 31, a.rows - 1) / a.rep + 1;
-  const uint32_t live = __builtin_amdgcn_readfirstlane(first_row < a.rows ? (wave_slots + kTileKeys - 1) / kTileKeys : 0);
-  const uint32_t whole = __builtin_amdgcn_readfirstlane((length + min(first_row, a.rows - 1) / a.rep + 1) / kTileKeys);   // tiles all of them see whole
+  const uint32_t slots = length + (first_row + live_rows - 1) / a.rep + 1;   // slots that any of them sees
+  const uint32_t tile0 = (uint32_t)((uint64_t)tiles * split / splits), tile1 = (uint32_t)((uint64_t)tiles * (split + 1) / splits);
+  const uint32_t whole = (length + first_row / a.rep + 1) / kTileKeys;       // tiles that all of them see whole
 
   const v4i k_rows = buffer_of(a.k_codes + (size_t)bh * a.max_len * L::kRowBytes, slots * L::kRowBytes);
   const v4i v_rows = buffer_of(a.v_codes + (size_t)bh * a.max_len * L::kRowBytes, slots * L::kRowBytes);
   const v4i k_sc = buffer_of((const uint8_t*)(a.k_scales + (size_t)bh * a.max_len), slots * 2);
   const v4i v_sc = buffer_of((const uint8_t*)(a.v_scales + (size_t)bh * a.max_len), slots * 2);
-
-  // codes: 1 KiB a load, wave w takes its 16 rows of either (D = 64: 32 rows, two waves for keys, two for values); chunks of sixteen bytes are
-  // permuted so that neither the rows of a score operand nor the sixteen keys of a transpose load fall on the same banks
+  // chunks of sixteen bytes are permuted so that neither the rows of a score operand nor the sixteen keys of a transpose load fall on the
+  // same banks
   unsigned k_src, v_src;
   if constexpr (D == 128) {
-    k_src = wave * 1024 + (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) << 4);
-    v_src = wave * 1024 + (lane >> 2) * 64 + (((lane & 3) ^ ((2 * wave + (lane >> 5)) & 3)) << 4);
+    k_src = (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) << 4);
+    v_src = (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 5)) << 4);      // (and 2 i of load i)
   } else {
-    k_src = v_src = (wave & 1) * 1024 + (lane >> 1) * 32 + (((lane & 1) ^ ((lane >> 4) & 1)) << 4);
+    k_src = v_src = (lane >> 1) * 32 + (((lane & 1) ^ ((lane >> 4) & 1)) << 4);
   }
   auto k_at = [](int r, int c) { return D == 128 ? r * 64 + ((c ^ ((r >> 2) & 3)) << 4) : r * 32 + ((c ^ ((r >> 3) & 1)) << 4); };
   auto v_at = [](int r, int c) { return D == 128 ? r * 64 + ((c ^ ((r >> 3) & 3)) << 4) : r * 32 + ((c ^ ((r >> 3) & 1)) << 4); };
-  auto request = [&](uint32_t tile, uint32_t stage) {
-    const unsigned to = lds0 + stage * L::kStage, from = tile * L::kTile;
-    if constexpr (D == 128) {
-      rows_to_lds(k_rows, from + k_src, to + wave * 1024);
-      rows_to_lds(v_rows, from + v_src, to + L::kTile + wave * 1024);
-    } else {
-      if (wave < 2) rows_to_lds(k_rows, from + k_src, to + wave * 1024);
-      else rows_to_lds(v_rows, from + v_src, to + L::kTile + (wave - 2) * 1024);
-    }
-    if (wave == 0) halves_to_lds(k_sc, (tile * kTileKeys + lane) * 2, to + 2 * L::kTile);
-    if (wave == 1) halves_to_lds(v_sc, (tile * kTileKeys + lane) * 2, to + 2 * L::kTile + kTileKeys * 4);
-  };
-  // the exponent of a tile's largest value scale, into LDS by one wave, a step ahead of its use
-  float* const bigs = (float*)(lds + L::kBig);
-  auto find_big = [&](uint32_t stage, uint32_t slot_of_it) {
-    const unsigned v = *(const unsigned*)(lds + stage * L::kStage + 2 * L::kTile + kTileKeys * 4 + lane * 4) & 0x7FFFu;
-    const float e = wave_max((float)(min(v, 0x7C00u) >> 10));
-    if (lane == 0) bigs[slot_of_it] = e - 29.0f;
+  auto request = [&](uint32_t tile, int stage) {
+    const unsigned to = mine0 + stage * L::kStage, from = tile * L::kTile;
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) rows_to_lds(k_rows, from + i * 1024 + k_src, to + i * 1024);
+    halves_to_lds(k_sc, (tile * kTileKeys + lane) * 2, to + 2 * L::kTile);
+    halves_to_lds(v_sc, (tile * kTileKeys + lane) * 2, to + 2 * L::kTile + kTileKeys * 4);
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i)
+      rows_to_lds(v_rows, from + i * 1024 + (D == 128 ? v_src ^ ((2 * i & 3) << 4) : v_src), to + L::kTile + i * 1024);
   };
 
   // this lane's query as operand: half h holds the channels of its half of a row's bytes, eight a step
   constexpr int kSteps = D / 16;
+  h8 x[kSteps];
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) x[j] = *(const h8*)(a.q + q_at + h * (D / 2) + 8 * j);
+  asm volatile("" ::: "memory");
+  uint32_t tile = tile0 + (KW == 1 ? 0 : wave);
+  if (tile < tile1) request(tile, 0);
+  if (tile + KW < tile1) request(tile + KW, 1);
   h8 qf[kSteps];
-  float factor, bias;
-  {
-    const __half* src = a.q + q_at + h * (D / 2);
-    h8 x[kSteps];
-    unsigned top = 0;
+  float bias = 0.f;
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      x[j] = *(const h8*)(src + 8 * j);
+  for (int j = 0; j < kSteps; ++j) {
+    qf[j] = __builtin_shufflevector(x[j], x[j], 0, 4, 1, 5, 2, 6, 3, 7);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, (unsigned)__float_as_int((float)x[j][e]) & 0x7FFFFFFFu);
-    }
-    top = max(top, (unsigned)lane_xor_i<32>((int)top));
-    // largest between 2^8 and 2^9 (a power of two: exact)
-    const unsigned e2 = min(254u, 262u - (top >> 23));
-    const float f = __int_as_float((int)(e2 << 23));
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const _Float16 y = (_Float16)((float)x[j][e] * f);
-        qf[j][code_element(e)] = y;
-        sum += (float)y;
-      }
-    sum += lane_xor_f<32>(sum);
-    bias = -8.0f / kFromSubnormal * sum;
-    factor = __builtin_fmaxf(__int_as_float((int)((254u - e2) << 23)) * kFromSubnormal * a.scale_log2, 1e-37f);   // (never zero: it meets -inf)
+    for (int e = 0; e < 4; ++e) bias = __builtin_amdgcn_fdot2(h2{qf[j][2 * e], qf[j][2 * e + 1]}, h2{(_Float16)1.0f, (_Float16)1.0f}, bias, false);
   }
+  bias = -8.0f / kFromSubnormal * (bias + lane_xor_f<32>(bias));
+  const float factor = kFromSubnormal * a.scale_log2;
 
-  v16f o[D / 32], ob;
+  v16f o[D / 32];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) ob[r] = 0.f;
+  for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) o[i] = ob;
-  float ref = kLowestRef, l = 0.f;
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  float ref = kLowestRef, l = 0.f, weights = 0.f;      // .. and the sum of the weights as the second product takes them
+  const int g = lane >> 4, gi = lane & 15;
+  const int key = 8 * (gi >> 2) + 4 * (g >> 1) + (gi & 3);             // the row that the lane addresses in a transpose load
 
-  if (tile0 < tile1) {
-    request(tile0, 0);
-    if (tile0 + 1 < tile1) request(tile0 + 1, 1);
-    wait_vmcnt<0>();
-    __syncthreads();
-    if (wave == 2) find_big(0, 0);
-  }
-  uint32_t stage = 0;
-  for (uint32_t tile = tile0; tile < tile1; ++tile) {
-    wait_vmcnt<0>();
-    __syncthreads();   // this tile and the next have come, everybody is done with the one before
-    const uint32_t next = stage == 2 ? 0 : stage + 1, third = next == 2 ? 0 : next + 1;
-    if (tile + 2 < tile1) request(tile + 2, third);
-    if (tile + 1 < tile1 && wave == 2) find_big(next, (tile + 1 - tile0) & 1);
-    const uint8_t* const kt = lds + stage * L::kStage;
+  bool set_reference = true;
+  for (int stage = 0; tile < tile1; tile += KW, stage ^= 1) {
+    if (tile + KW < tile1) wait_vmcnt<2 * L::kLoads + 2>();
+    else wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    const uint8_t* const kt = mine + stage * L::kStage;
     const uint8_t* const vt = kt + L::kTile;
-    const unsigned* const ks = (const unsigned*)(vt + L::kTile);
-    const unsigned* const vs = ks + kTileKeys;
-    stage = next;
-    if (tile >= live) continue;
-    // ---- scores of two tiles of 32 keys: element r of tile kt: key 32 kt + 8 (r / 4) + 4 h + r % 4
+    unsigned* const ks = (unsigned*)(mine + stage * L::kStage + 2 * L::kTile);
+    unsigned* const vs = ks + kTileKeys;
+    // ---- scores of two tiles of 32 keys: element r of tile i: key 32 i + 8 (r / 4) + 4 h + r % 4
     v16f st[2];
+    unsigned c[2][kSteps];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[i][r] = bias;
-      unsigned c[kSteps];
 #pragma unroll
-      for (int j = 0; j < kSteps / 4; ++j) *(v4i*)(c + 4 * j) = *(const v4i*)(kt + k_at(32 * i + n, h * (kSteps / 4) + j));
-#pragma unroll
-      for (int j = 0; j < kSteps; ++j) st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(code_halves(c[j]), qf[j], st[i], 0, 0, 0);
+      for (int j = 0; j < kSteps / 4; ++j) *(v4i*)(c[i] + 4 * j) = *(const v4i*)(kt + k_at(32 * i + n, h * (kSteps / 4) + j));
     }
-    float top = -INFINITY;
+    // the scales for all queries at once: keys' as the scores take them, values' in pairs of keys 8 apart, as the weights are packed
+    const unsigned k_raw = ks[lane], v_raw = vs[lane];
+    ks[lane] = __builtin_bit_cast(unsigned, low_half(k_raw) * factor);
+    ((unsigned short*)vs)[2 * (lane >> 4) * 8 + 2 * (lane & 7) + ((lane >> 3) & 1)] = (unsigned short)v_raw;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) st[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(code_halves(c[i][j]), qf[j], st[i], 0, 0, 0);
+    v2i cv[2][D / 32];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const v4i k4 = *(const v4i*)(ks + 32 * i + 8 * g + 4 * h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st[i][4 * g + e] = times_half(st[i][4 * g + e], (unsigned)k4[e]);
-      }
-    const bool masked = tile >= whole;
+      for (int dt = 0; dt < D / 32; ++dt)
+        cv[i][dt] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i*)(vt + v_at(32 * i + key, dt) + (g & 1) * 8));
     const int key0 = (int)(tile * kTileKeys) + 4 * h;
-    if (masked) {
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + 32 * i + 8 * (r >> 2) + (r & 3) > limit) st[i][r] = -INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, st[i][r]);
-    top = __builtin_fmaxf(top, lane_xor_f<32>(top));
-    const float now = __builtin_fmaxf(ref, __builtin_fmaf(top, factor, bigs[(tile - tile0) & 1]));
-    if (__builtin_amdgcn_ballot_w64(now != ref) != 0) {
-      const float alpha = __builtin_amdgcn_exp2f(ref - now);
-      l *= alpha;
-      ob *= alpha;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
-      ref = now;
-    }
-    // ---- probabilities with the values' scales, in pairs (r, r + 4) as the codes' halves come: p[i][u] is slots 16 u .. of tile i
+    // ---- probabilities, then weights, in pairs (r, r + 4) as the codes' halves come: p[i][u] is slots 16 u .. of tile i
     h8 p[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const v4i v0 = *(const v4i*)(vs + 32 * i + 16 * u + 4 * h), v1 = *(const v4i*)(vs + 32 * i + 16 * u + 8 + 4 * h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][8 * u + e], factor, -ref));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][8 * u + 4 + e], factor, -ref));
-          l += p0 + p1;
-          const h2 x = pair_times_halves(p0, (unsigned)v0[e], p1, (unsigned)v1[e]);
-          p[i][u][2 * e] = x[0], p[i][u][2 * e + 1] = x[1];
-        }
-      }
-    if (masked) {      // (a value that a query does not see may be NaN)
-      asm volatile("" ::: "memory");
+    float sum, added;
+    auto weigh = [&](auto masked_) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_)::value;
+      sum = added = 0.f;
+      const int from = opaque(key0);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + 32 * i + 8 * (r >> 2) + (r & 3) > limit) p[i][r >> 3][2 * (r & 3) + ((r >> 2) & 1)] = (_Float16)0.0f;
-    }
-    // ---- output: 32 channels as rows; the lane's sixteen keys 8 (r / 4) + 4 h + r % 4 of a tile of 32 in nibble r
-    const int g = lane >> 4, gi = lane & 15;
-    const int key = 8 * (gi >> 2) + 4 * (g >> 1) + (gi & 3);
+        for (int u = 0; u < 2; ++u) {
+          const v4i k0 = *(const v4i*)(ks + 32 * i + 16 * u + 4 * h), k1 = *(const v4i*)(ks + 32 * i + 16 * u + 8 + 4 * h);
+          const v4i v2 = *(const v4i*)(vs + 16 * i + 8 * u + 4 * h);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+          for (int e = 0; e < 4; ++e) {
+            const int a0 = k0[e], a1 = k1[e], vv = v2[e];
+            float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][8 * u + e], __int_as_float(a0), -ref));
+            float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][8 * u + 4 + e], __int_as_float(a1), -ref));
+            h2 w2 = pair_times_halves(p0, (unsigned)vv & 0xFFFFu, p1, (unsigned)vv >> 16);
+            if constexpr (MASKED) {                    // (a value that a query does not see may be NaN)
+              const int at = from + 32 * i + 16 * u + e;
+              if (at > limit) p0 = 0.f, w2[0] = (_Float16)0.0f;
+              if (at + 8 > limit) p1 = 0.f, w2[1] = (_Float16)0.0f;
+            }
+            sum += p0 + p1;
+            p[i][u][2 * e] = w2[0], p[i][u][2 * e + 1] = w2[1];
+            added = __builtin_amdgcn_fdot2(w2, h2{(_Float16)1.0f, (_Float16)1.0f}, added, false);
+          }
+        }
+    };
+    // A reference that holds the scores and the values' largest scale back: p vs < 2^11 when it is set, in the first tile and again where a weight
+    // leaves fp16's range, which few tiles' do
+    for (;;) {
+      if (set_reference) {
+        float top = -INFINITY;
+        const int from = opaque(key0);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) ob = __builtin_amdgcn_mfma_f32_32x32x16_f16(bias_halves(), p[i][u], ob, 0, 0, 0);
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        const v2i c = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i*)(vt + v_at(32 * i + key, dt) + (g & 1) * 8));
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(code_halves((unsigned)c[0]), p[i][0], o[dt], 0, 0, 0);
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(code_halves((unsigned)c[1]), p[i][1], o[dt], 0, 0, 0);
+          for (int k = 0; k < 4; ++k) {
+            const v4i k4 = *(const v4i*)(ks + 32 * i + 8 * k + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int f = k4[e];
+              const float y = st[i][4 * k + e] * __int_as_float(f);
+              top = __builtin_fmaxf(top, from + 32 * i + 8 * k + e > limit ? -INFINITY : y);
+            }
+          }
+        top = __builtin_fmaxf(top, lane_xor_f<32>(top));
+        const float most = wave_max((float)(min(v_raw & 0x7FFFu, 0x7C00u) >> 10));
+        const float now = __builtin_fmaxf(ref, top + (most - 25.0f));
+        const float alpha = __builtin_amdgcn_exp2f(ref - now);
+        l *= alpha, weights *= alpha;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+        ref = now;
       }
+      if (tile >= whole) weigh(std::true_type{});
+      else weigh(std::false_type{});
+      if (set_reference || __builtin_amdgcn_ballot_w64(!(added < INFINITY)) == 0) break;
+      set_reference = true;
+    }
+    set_reference = false;
+    l += sum, weights += added;
+    // ---- output: 32 channels as rows; the lane's sixteen keys 8 (r / 4) + 4 h + r % 4 of a tile of 32 in nibble r
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+          const int w8 = cv[i][dt][u];
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(code_halves((unsigned)w8), p[i][u], o[dt], 0, 0, 0);
+        }
+    if (tile + 2 * KW < tile1) {
+      wait_lds();                                      // (what was read of this stage)
+      request(tile + 2 * KW, stage);
     }
   }
 
+  // ---- the waves' results together
   l += lane_xor_f<32>(l);
-  if (a.splits > 1) {
-    float* piece = a.pieces + (((size_t)bh * a.blocks + block) * a.splits + split) * kPieceFloats<D>;
-    const uint32_t r0 = wave * 32 + n;
-    if (first_row + n < a.rows) {
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          v4f x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = (o[dt][4 * g + e] - ob[4 * g + e]) * kFromSubnormal;
-          *(v4f*)(piece + r0 * D + 32 * dt + 8 * g + 4 * h) = x;
-        }
-      if (h == 0) piece[kBlockRows * D + r0] = ref, piece[kBlockRows * (D + 1) + r0] = l;
-    }
-    return;
-  }
-  // ---- normalise, transpose through LDS, store whole rows (none for a sequence that takes no part: zeros)
-  const float inv = takes_part ? kFromSubnormal / l : 0.f;
-  __syncthreads();
-  uint8_t* stage_out = lds + wave * (32 * L::kOutPitch);
+  weights += lane_xor_f<32>(weights);
+  wait_lds();
+  float* const there = (float*)mine;                   // (its own stages: everything asked for has come)
+  const float eight = -8.0f * weights;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      h4 v;
+    for (int k = 0; k < 4; ++k) {
+      v4f y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (_Float16)((o[dt][4 * g + e] - ob[4 * g + e]) * inv);
-      *(h4*)(stage_out + n * L::kOutPitch + (32 * dt + 8 * g + 4 * h) * 2) = v;
+      for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[dt][4 * k + e], kFromSubnormal, eight);
+      *(v4f*)(there + n * L::kPitch + 32 * dt + 8 * k + 4 * h) = y;
     }
-  wait_lgkmcnt0();
-  __builtin_amdgcn_wave_barrier();
-  constexpr int kChunks = D / 8, kPerLoad = 64 / kChunks;
+  if constexpr (KW == 1) {
+    // its own rows: normalised on the way to the output, in whole rows
+    if (h == 0) there[kBlockRows * L::kPitch + n] = tiles ? 1.0f / l : 0.f;   // (a sequence that takes no part: zeros)
+    wait_lds();
+    constexpr int kChunks = D / 8;
+#pragma unroll 2
+    for (uint32_t i = lane; i < live_rows * kChunks; i += 64) {
+      const uint32_t r = i / kChunks, ch = i % kChunks * 8, at = first_row + r;
+      const float inv = there[kBlockRows * L::kPitch + r];
+      h8 z;
 #pragma unroll
-  for (int it = 0; it < 32 / kPerLoad; ++it) {
-    const uint32_t r = it * kPerLoad + lane / kChunks, c = lane % kChunks, global = first_row + r;
-    const v4i v = *(const v4i*)(stage_out + r * L::kOutPitch + c * 16);
-    if (global < a.rows)
-      *(v4i*)(a.out + (((size_t)b * a.T + global / a.rep) * a.Hq + hkv * a.rep + global % a.rep) * D + c * 8) = v;
+      for (int e = 0; e < 8; ++e) z[e] = (_Float16)(there[r * L::kPitch + ch + e] * inv);
+      *(h8*)(a.out + (((size_t)b * a.T + at / a.rep) * a.Hq + hkv * a.rep + at % a.rep) * D + ch) = z;
+    }
+    return;
+  }
+  if (h == 0) there[kBlockRows * L::kPitch + n] = ref, there[kBlockRows * L::kPitch + kBlockRows + n] = l;
+  __syncthreads();
+  // a thread: eight channels of a row at a time
+  constexpr int kChunks = D / 8;
+  for (uint32_t i = tid; i < live_rows * kChunks; i += kThreads) {
+    const uint32_t r = i / kChunks, ch = i % kChunks * 8;
+    float m = kLowestRef, wt[kWaves], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) m = __builtin_fmaxf(m, ((const float*)(lds + k * L::kWave))[kBlockRows * L::kPitch + r]);
+    float y[8] = {};
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+      const float* from = (const float*)(lds + k * L::kWave);
+      const float lk = from[kBlockRows * L::kPitch + kBlockRows + r];
+      wt[k] = __builtin_amdgcn_exp2f(from[kBlockRows * L::kPitch + r] - m);
+      if (lk == 0.f) continue;                         // (a wave without a tile, or one whose keys the query does not see)
+      sum += wt[k] * lk;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const v4f v = *(const v4f*)(from + r * L::kPitch + ch + e);
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) y[e + k4] += wt[k] * v[k4];
+      }
+    }
+    if (splits > 1) {
+      float* piece = a.pieces + (((size_t)bh * a.blocks + block) * a.splits + split) * kPieceFloats<D>;
+      *(v4f*)(piece + r * D + ch) = v4f{y[0], y[1], y[2], y[3]};
+      *(v4f*)(piece + r * D + ch + 4) = v4f{y[4], y[5], y[6], y[7]};
+      if (ch == 0) piece[kBlockRows * D + r] = m, piece[kBlockRows * (D + 1) + r] = sum;
+    } else {
+      const float inv = tiles ? 1.0f / sum : 0.f;      // (a sequence that takes no part: zeros)
+      h8 z;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = (_Float16)(y[e] * inv);
+      const uint32_t at = first_row + r;
+      *(h8*)(a.out + (((size_t)b * a.T + at / a.rep) * a.Hq + hkv * a.rep + at % a.rep) * D + ch) = z;
+    }
   }
 }
 
-// one wave per row: its pieces in their order
+// one wave per row: its pieces in their order, four at a time on the way
 template <int D>
 __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
   const int lane = threadIdx.x & 63;
-  const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item >= (uint64_t)a.B * a.Hkv * a.rows) return;
-  const uint32_t bh = (uint32_t)(item / a.rows), row = (uint32_t)(item % a.rows), b = bh / a.Hkv, hkv = bh % a.Hkv;
-  const uint32_t block = row / kBlockRows, r0 = row % kBlockRows;
-  const long long len = a.lengths[b];
-  const bool takes_part = len >= 0 && len <= (long long)a.max_len - (long long)a.T;
-  float m = kLowestRef, l = 0.f, o[D / 64] = {};
+  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= a.B * a.Hkv * a.rows) return;
+  const uint32_t bh = item / a.rows, row = item % a.rows, b = bh / a.Hkv, hkv = bh % a.Hkv;
+  const uint32_t block = row / kBlockRows, r = row % kBlockRows;
+  const uint32_t splits = splits_for(a, tiles_of(a, a.lengths[b], block));
+  if (splits == 1) return;                             // (its workgroup has stored the output)
   const float* base = a.pieces + ((size_t)bh * a.blocks + block) * a.splits * kPieceFloats<D>;
-  for (uint32_t s = 0; s < a.splits; ++s) {
-    const float* piece = base + (size_t)s * kPieceFloats<D>;
-    const float pm = piece[kBlockRows * D + r0], pl = piece[kBlockRows * (D + 1) + r0];
-    if (pl == 0.f) continue;                           // nothing of it is seen
-    const float now = __builtin_fmaxf(m, pm);
-    const float old = __builtin_amdgcn_exp2f(m - now), w = __builtin_amdgcn_exp2f(pm - now);
-    l = l * old + w * pl;
+  // lane s: piece s
+  const float* at = base + (size_t)min((uint32_t)lane, splits - 1) * kPieceFloats<D> + kBlockRows * D + r;
+  const bool have = (uint32_t)lane < splits;
+  const float pl = have ? at[kBlockRows] : 0.f;
+  const float pm = pl == 0.f ? kLowestRef : at[0];     // (nothing of it is seen)
+  const float m = wave_max(pm);
+  const float w = pl == 0.f ? 0.f : __builtin_amdgcn_exp2f(pm - m);
+  const float l = wave_sum(w * pl);
+  float o[D / 64] = {};
+#pragma unroll 4
+  for (uint32_t s = 0; s < splits; ++s) {
+    const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (int)s));
+    const bool seen = __builtin_amdgcn_readlane(__float_as_int(pl), (int)s) != 0;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] = o[i] * old + w * piece[r0 * D + lane + 64 * i];
-    m = now;
+    for (int i = 0; i < D / 64; ++i) {
+      const float v = base[(size_t)s * kPieceFloats<D> + r * D + lane + 64 * i];
+      o[i] += seen ? ws * v : 0.f;
+    }
   }
-  __half* dst = a.out + (((size_t)b * a.T + row / a.rep) * a.Hq + hkv * a.rep + row % a.rep) * D;
+  _Float16* dst = (_Float16*)(a.out + (((size_t)b * a.T + row / a.rep) * a.Hq + hkv * a.rep + row % a.rep) * D);
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) ((_Float16*)dst)[lane + 64 * i] = (_Float16)(takes_part ? o[i] / l : 0.f);
+  for (int i = 0; i < D / 64; ++i) dst[lane + 64 * i] = (_Float16)(o[i] / l);
 }
+
+// Blocks from which every wave has one of its own
+constexpr uint64_t kOwnRows = 4096;
 
 // Workgroups over which a block's tiles are split: as many as fill the chip, two a compute unit
 uint32_t splits_of(uint64_t groups, uint32_t max_len) {
   const uint64_t tiles = ((uint64_t)max_len + kTileKeys - 1) / kTileKeys;
+  const uint64_t most = (tiles + kSplitTiles - 1) / kSplitTiles;
   uint64_t s = 512 / groups;
-  if (s > 16) s = 16;
-  if (s > tiles) s = tiles;
+  if (s > 64) s = 64;
+  if (s > most) s = most;
   return s < 1 ? 1 : (uint32_t)s;
 }
 
@@ -380,7 +433,12 @@ extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* length
   a.scale_log2 = scale * 1.4426950408889634f;
   const uint64_t groups = (uint64_t)B * Hkv * a.blocks;
   a.splits = splits_of(groups, max_len);
-  auto go = [&](auto kern, auto join, size_t smem, LdsGrant& grant) {
+  auto go = [&](auto kern, auto rows, auto join, size_t smem, LdsGrant& grant, LdsGrant& rows_grant) {
+    if (groups >= kOwnRows) {
+      if (int rc = reserve_lds((const void*)rows, smem, rows_grant, what)) return rc;
+      hipLaunchKernelGGL(rows, dim3((unsigned)((uint64_t)B * Hkv * ((a.blocks + 3) / 4))), dim3(kThreads), smem, (hipStream_t)stream, a);
+      return check_launch(what);
+    }
     if (int rc = reserve_lds((const void*)kern, smem, grant, what)) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(groups * a.splits)), dim3(kThreads), smem, (hipStream_t)stream, a);
     if (int rc = check_launch(what)) return rc;
@@ -388,7 +446,7 @@ extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* length
     hipLaunchKernelGGL(join, dim3((unsigned)(((uint64_t)B * Hkv * a.rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
     return check_launch(what);
   };
-  static LdsGrant grant128, grant64;
-  return head_dim == 128 ? go(prefill_i4_kernel<128>, prefill_i4_join_kernel<128>, Layout<128>::kBytes, grant128)
-                         : go(prefill_i4_kernel<64>, prefill_i4_join_kernel<64>, Layout<64>::kBytes, grant64);
+  static LdsGrant grant128, grant64, rows128, rows64;
+  return head_dim == 128 ? go(prefill_i4_kernel<128, 4>, prefill_i4_kernel<128, 1>, prefill_i4_join_kernel<128>, Layout<128>::kBytes, grant128, rows128)
+                         : go(prefill_i4_kernel<64, 4>, prefill_i4_kernel<64, 1>, prefill_i4_join_kernel<64>, Layout<64>::kBytes, grant64, rows64);
 }
