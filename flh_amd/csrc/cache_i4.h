@@ -122,7 +122,7 @@ __device__ __forceinline__ RowCodes quantise(const HeadRow<D>& row) {
 }
 
 // Eight codes as an operand of the fp16 matrix instructions, without a conversion: code + 8 in bits 4 .. 7 of a half is the subnormal
-// (code + 8) 2^-20, which they multiply exactly; what the 8 adds is taken off with `bias_halves`, the same operand for codes of zero.  Elements are
+// (code + 8) 2^-20, which they multiply exactly; what the 8 adds, eight times the sum of the other operand, is taken off in float32.  Elements are
 // codes 0, 4 | 1, 5 | 2, 6 | 3, 7.  (Bits 0 .. 3 take two shifts less.  But products are lined up by the exponents of their operands, which for
 // a subnormal is that of 2^-14 whatever its bits: the sums lost the last ten bits of 24, in bits 4 .. 7 six.)
 constexpr unsigned kNibbles = 0x00F000F0u, kEight = 0x00800080u;
@@ -131,7 +131,6 @@ __device__ __forceinline__ h8 code_halves(unsigned w) {
                  (int)(((w >> 8) & kNibbles) ^ kEight)};
   return __builtin_bit_cast(h8, r);
 }
-__device__ __forceinline__ h8 bias_halves() { return __builtin_bit_cast(h8, (v4i{(int)kEight, (int)kEight, (int)kEight, (int)kEight})); }
 // the place of code e of eight among the elements of an operand
 __device__ __forceinline__ constexpr int code_element(int e) { return 2 * (e & 3) + (e >> 2); }
 
@@ -154,6 +153,12 @@ __device__ __forceinline__ void rows_to_lds(const v4i& d, unsigned voff, unsigne
 }
 __device__ __forceinline__ void halves_to_lds(const v4i& d, unsigned voff, unsigned lds_base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ushort %1, %2, 0 offen lds" ::"s"(lds_base), "v"(voff), "s"(d) : "memory", "m0");
+}
+
+// what is made of it here is not made in front of the branch that it is needed behind
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // every LDS operation of this wave has completed, and no memory operation crosses

@@ -37,36 +37,51 @@ __device__ __forceinline__ uint32_t tiles_of(const Decode& a, long long n) {
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
 
 struct Place {
-  uint32_t b, length, tiles, before;                   // a sequence, its slots taken, tiles of a head, tiles of the sequences before it
+  uint32_t b, length, tiles, entries, before;          // a sequence, its slots taken, tiles of a head, entries of a head, those of the sequences before
 };
 
-// The sequences' tiles, 64 sequences in the lanes at a time
+// How the work is shared.  Usually: the tiles of all heads are one list, a workgroup takes `c` of its entries.  With few tiles to a workgroup, where a
+// share of two heads would cost a second round of every latency: each head is cut into equal parts of at most c tiles, and the parts are the list, of
+// which a workgroup takes one (5 sequences of 778 slots, 32 heads: 13 tiles a head, 4 to a workgroup).  64 sequences in the lanes at a time.
 struct Shares {
-  uint32_t c, total, heads;                            // tiles of a workgroup, of all; heads of a sequence
-  uint32_t length, tiles, up, first, before;           // of the 64 last looked at
+  uint32_t c, total, heads;                            // .., entries of the list, heads of a sequence
+  bool parts;
+  uint32_t length, tiles, entries, up, first, before;  // of the 64 last looked at
 
   __device__ __forceinline__ void look(const Decode& a, uint32_t b0) {
     const uint32_t b = b0 + (threadIdx.x & 63);
     const long long n = b < a.B ? a.lengths[b] : -1;
-    tiles = tiles_of(a, n);
+    tiles = entries = tiles_of(a, n);
     length = (uint32_t)n;
-    up = wave_scan(tiles * heads);
+    up = wave_scan(entries * heads);
     first = b0;
   }
   __device__ __forceinline__ explicit Shares(const Decode& a) {
     heads = a.Hkv * a.blocks;
     total = 0;
+    parts = false;
     for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
       look(a, b0);
       before = total;
       total += lane_value(up, 63);
     }
-    c = max(1u, (total + a.groups - 1) / a.groups);
-    if (c > kWaves) c = (c + kWaves - 1) / kWaves * kWaves;
+    c = max((uint32_t)kWaves, (total + a.groups - 1) / a.groups);
+    const uint32_t all_heads = a.B * heads;
+    if (a.B <= 64 && all_heads < a.groups) {
+      // at most total / most + all_heads parts, which are no more than the workgroups
+      const uint32_t most = max((uint32_t)kWaves, (total + a.groups - all_heads - 1) / (a.groups - all_heads));
+      if (most <= 2 * kWaves) {
+        entries = (tiles + most - 1) / most;
+        up = wave_scan(entries * heads);
+        total = lane_value(up, 63), c = 1, parts = true;
+        return;
+      }
+    }
+    c = (c + kWaves - 1) / kWaves * kWaves;
   }
   __device__ __forceinline__ Place in_lane(int l) const {
-    const uint32_t t = lane_value(tiles, l);
-    return {first + l, lane_value(length, l), t, before + lane_value(up, l) - t * heads};
+    const uint32_t n = lane_value(entries, l);
+    return {first + l, lane_value(length, l), lane_value(tiles, l), n, before + lane_value(up, l) - n * heads};
   }
   __device__ __forceinline__ Place of(const Decode& a, uint32_t b) {
     if (b - first >= 64) {
@@ -79,7 +94,7 @@ struct Shares {
     }
     return in_lane(b - first);
   }
-  // the sequence that holds tile `pos` (below total)
+  // the sequence that holds entry `pos` (below total)
   __device__ __forceinline__ Place at(const Decode& a, uint32_t pos) {
     if (a.B > 64) {
       before = 0;
@@ -100,8 +115,8 @@ struct Layout {
   static constexpr int kStage = 2 * kTile + 2 * kTileKeys * 4;               // K, V, their scales (a dword each)
   static constexpr int kQPitch = D * 2 + 16;                                 // bytes of a query's halves
   static constexpr int kPiece = D + 2;                                       // floats of a piece and query
-  // the waves' stages; the queries' high and low halves; their factors and biases; the new row's codes and scales
-  static constexpr int kQ = kWaves * kStages * kStage, kFactor = kQ + 2 * kCols * kQPitch, kNew = kFactor + 2 * kCols * 4,
+  // the waves' stages; the queries' high and low halves; what their scores begin with; the new row's codes and scales
+  static constexpr int kQ = kWaves * kStages * kStage, kBias = kQ + 2 * kCols * kQPitch, kNew = kBias + kCols * 4,
                        kBytes = kNew + 2 * kRowBytes + 16;
   static_assert(kCols * kPiece * 4 <= kStages * kStage, "a wave's result takes the place of its stages");
 };
@@ -138,9 +153,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
 
   while (pos < end) {
     const Place place = shares.at(a, pos);
-    const uint32_t unit = (pos - place.before) / place.tiles;                   // of the sequence's heads x blocks
-    const uint32_t head_start = place.before + unit * place.tiles;
-    const uint32_t first = pos - head_start, stop = min(place.tiles, first + (end - pos));
+    const uint32_t unit = (pos - place.before) / place.entries;                 // of the sequence's heads x blocks
+    const uint32_t entry = pos - place.before - unit * place.entries;
+    const uint32_t first = shares.parts ? (uint32_t)((uint64_t)place.tiles * entry / place.entries) : entry;
+    const uint32_t stop = shares.parts ? (uint32_t)((uint64_t)place.tiles * (entry + 1) / place.entries) : min(place.tiles, first + (end - pos));
     const uint32_t hkv = unit / a.blocks, q0 = (unit % a.blocks) * kCols, cols = min((uint32_t)kCols, a.rep - q0);
     const uint32_t bh = place.b * a.Hkv + hkv, slot = place.length;
     const bool has_new = stop == place.tiles;
@@ -186,10 +202,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       row.scale(HeadRow<D>::norm());
     }
     if (r < kCols) {
-      // a query as two fp16 values, its largest between 2^8 and 2^9
-      const unsigned top = row.top();
-      const unsigned e = min(254u, 262u - (top >> 23));
-      row.scale(__int_as_float((int)(e << 23)));
+      // a query as two fp16 values
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -207,11 +220,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       sum += dpp_f<kDppQuadXor1>(sum);
       sum += dpp_f<kDppQuadXor2>(sum);
       if constexpr (kLanes == 8) sum += dpp_f<kDppRowHalfMirror>(sum);
-      if (chunk == 0) {
-        float* f = (float*)(lds + L::kFactor);
-        f[r] = __builtin_fmaxf(__int_as_float((int)((254u - e) << 23)) * kFromSubnormal * a.scale_log2, 1e-37f);   // (never zero: it meets -inf)
-        f[kCols + r] = -8.0f / kFromSubnormal * sum;
-      }
+      if (chunk == 0) ((float*)(lds + L::kBias))[r] = -8.0f / kFromSubnormal * sum;
     } else if (is_new) {
       const RowCodes codes = quantise(row);
       uint8_t* there = lds + L::kNew + (is_v ? L::kRowBytes : 0);
@@ -235,13 +244,14 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       qh[j] = *(const h8*)(lds + L::kQ + col * L::kQPitch + (kb * kSteps + j) * 16);
       ql[j] = *(const h8*)(lds + L::kQ + (kCols + col) * L::kQPitch + (kb * kSteps + j) * 16);
     }
-    const float factor = ((const float*)(lds + L::kFactor))[col], bias = ((const float*)(lds + L::kFactor))[kCols + col];
+    const float bias = ((const float*)(lds + L::kBias))[col], factor = kFromSubnormal * a.scale_log2;
+    const int key = 16 * (col >> 2) + 4 * kb + (col & 3);   // the row that the lane addresses in a transpose load
 
-    float ref = kLowestRef, l = 0.f;
-    v4f o[D / 16], ob = {0.f, 0.f, 0.f, 0.f};
+    float ref = kLowestRef, l = 0.f, weights = 0.f;    // .. and the sum of the weights as the second product takes them
+    v4f o[D / 16];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[i] = ob;
-
+    for (int i = 0; i < D / 16; ++i) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    bool set_reference = true;
     for (int stage = 0; tile < stop; tile += kWaves, stage ^= 1) {
       if (tile + kWaves < stop) {
         wait_lds();                                    // (what was read of the stage before)
@@ -264,6 +274,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
         else if (lane == 63) ks[n] = *(const unsigned*)(lds + L::kNew + 2 * L::kRowBytes), vs[n] = *(const unsigned*)(lds + L::kNew + 2 * L::kRowBytes + 4);
         wait_lds();
       }
+      // the scales for all queries at once: keys' as the scores take them, values' in pairs of keys 16 apart, as the weights are packed
+      const unsigned k_raw = ks[lane], v_raw = vs[lane];
+      ks[lane] = __builtin_bit_cast(unsigned, low_half(k_raw) * factor);
+      ((unsigned short*)vs)[(lane >> 5) * 32 + (lane & 15) * 2 + ((lane >> 4) & 1)] = (unsigned short)v_raw;
       // ---- scores: tile t of sixteen keys as rows, key 16 t + 4 kb + i in element i
       v4f st[4];
 #pragma unroll
@@ -279,49 +293,67 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
           st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], st[t], 0, 0, 0);
         }
       }
-      // ---- softmax relative to a reference that also holds the values' largest scale back: p vs <= 2^15
-      unsigned v[4][4], big = 0;
-      float top = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const v4i k4 = *(const v4i*)(ks + 16 * t + 4 * kb), v4 = *(const v4i*)(vs + 16 * t + 4 * kb);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[t][i] = (unsigned)v4[i];
-          big = max(big, v[t][i] & 0x7FFFu);
-          st[t][i] = times_half(st[t][i], (unsigned)k4[i]);
-          if (last && tile * kTileKeys + 16 * t + 4 * kb + i > slot) st[t][i] = -INFINITY;
-          top = __builtin_fmaxf(top, st[t][i]);
-        }
-      }
-      top = __builtin_fmaxf(top, lane_xor_f<16>(top));
-      top = __builtin_fmaxf(top, lane_xor_f<32>(top));
-      big = max(big, (unsigned)lane_xor_i<16>((int)big));
-      big = max(big, (unsigned)lane_xor_i<32>((int)big));
-      const float now = __builtin_fmaxf(ref, __builtin_fmaf(top, factor, (float)((int)(min(big, 0x7C00u) >> 10) - 29)));
-      if (__builtin_amdgcn_ballot_w64(now != ref) != 0) {
-        const float alpha = __builtin_amdgcn_exp2f(ref - now);
-        l *= alpha;
-        ob *= alpha;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
-        ref = now;
-      }
+      // ---- probabilities, then weights, in pairs (2 u, 2 u + 1) of tiles as the codes' halves come
       h8 p[2];
+      float sum, added;
+      auto weigh = [&](auto masked_) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        sum = added = 0.f;
+        const int left = MASKED ? opaque((int)(slot - tile * kTileKeys) - 4 * kb) : 0;   // the last of the lane's keys there is
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u) {
+          const v4i k0 = *(const v4i*)(ks + 32 * u + 4 * kb), k1 = *(const v4i*)(ks + 32 * u + 16 + 4 * kb);
+          const v4i v2 = *(const v4i*)(vs + 16 * u + 4 * kb);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * u][i], factor, -ref));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * u + 1][i], factor, -ref));
-          l += p0 + p1;
-          const h2 w = pair_times_halves(p0, v[2 * u][i], p1, v[2 * u + 1][i]);
-          p[u][2 * i] = w[0], p[u][2 * i + 1] = w[1];
+          for (int i = 0; i < 4; ++i) {
+            const int a0 = k0[i], a1 = k1[i], vv = v2[i];
+            float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * u][i], __int_as_float(a0), -ref));
+            float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * u + 1][i], __int_as_float(a1), -ref));
+            if constexpr (MASKED) {                    // (scales behind the sequence come as zeros: so do the weights)
+              if (32 * u + i > left) p0 = 0.f;
+              if (32 * u + 16 + i > left) p1 = 0.f;
+            }
+            const h2 w2 = pair_times_halves(p0, (unsigned)vv & 0xFFFFu, p1, (unsigned)vv >> 16);
+            sum += p0 + p1;
+            p[u][2 * i] = w2[0], p[u][2 * i + 1] = w2[1];
+            added = __builtin_amdgcn_fdot2(w2, h2{(_Float16)1.0f, (_Float16)1.0f}, added, false);
+          }
         }
-      // ---- output: sixteen channels as rows; a lane's sixteen keys 16 t + 4 kb + i in nibble 4 t + i
-      const int key = 16 * (col >> 2) + 4 * kb + (col & 3);
+      };
+      // A reference that holds the scores and the values' largest scale back: p vs < 2^11 when it is set, in the first tile and again where a
+      // weight leaves fp16's range, which few tiles' do
+      for (;;) {
+        if (set_reference) {
+          float top = -INFINITY;
+          const int left = opaque((int)(slot - tile * kTileKeys) - 4 * kb);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(bias_halves(), p[u], ob, 0, 0, 0);
+          for (int t = 0; t < 4; ++t) {
+            const v4i k4 = *(const v4i*)(ks + 16 * t + 4 * kb);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int f = k4[i];
+              const float y = st[t][i] * __int_as_float(f);
+              top = __builtin_fmaxf(top, 16 * t + i > left ? -INFINITY : y);
+            }
+          }
+          top = __builtin_fmaxf(top, lane_xor_f<16>(top));
+          top = __builtin_fmaxf(top, lane_xor_f<32>(top));
+          const float most = wave_max((float)(min(v_raw & 0x7FFFu, 0x7C00u) >> 10));
+          const float now = __builtin_fmaxf(ref, top + (most - 25.0f));
+          const float alpha = __builtin_amdgcn_exp2f(ref - now);
+          l *= alpha, weights *= alpha;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
+          ref = now;
+        }
+        if (last) weigh(std::true_type{});
+        else weigh(std::false_type{});
+        if (set_reference || __builtin_amdgcn_ballot_w64(!(added < INFINITY)) == 0) break;
+        set_reference = true;
+      }
+      set_reference = false;
+      l += sum, weights += added;
+      // ---- output: sixteen channels as rows; a lane's sixteen keys 16 t + 4 kb + i in nibble 4 t + i
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i*)(vt + v_at(key, i >> 1) + (i & 1) * 8));
@@ -333,10 +365,17 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
     // ---- the waves' results into one piece
     l += lane_xor_f<16>(l);
     l += lane_xor_f<32>(l);
+    weights += lane_xor_f<16>(weights);
+    weights += lane_xor_f<32>(weights);
     wait_lds();
     float* const there = (float*)mine;                 // (its own stages: everything asked for has come)
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) *(v4f*)(there + col * L::kPiece + 16 * i + 4 * kb) = (o[i] - ob) * kFromSubnormal;
+    for (int i = 0; i < D / 16; ++i) {
+      v4f y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[i][e], kFromSubnormal, -8.0f * weights);
+      *(v4f*)(there + col * L::kPiece + 16 * i + 4 * kb) = y;
+    }
     if (kb == 0) there[col * L::kPiece + D] = ref, there[col * L::kPiece + D + 1] = l;
     __syncthreads();
     float* const piece = a.partials + ((size_t)(blockIdx.x + (size_t)place.b * shares.heads + unit) * kCols) * L::kPiece;
@@ -356,48 +395,70 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       if (ch == 0) piece[h * L::kPiece + D] = m, piece[h * L::kPiece + D + 1] = sum;
     }
     __syncthreads();
-    pos += stop - first;
+    pos += shares.parts ? 1 : stop - first;
   }
 }
 
-// one workgroup of four waves per (sequence, query head): its pieces, one wave every fourth, then the waves' sums in a fixed order
+// n pieces, 4 K of them at a time: their references and sums one a lane, the weighted codes of every fourth one by this wave, all requested at once
+template <int D, int K>
+__device__ __forceinline__ void join_pieces(const float* base, size_t stride, uint32_t n, int wave, float (&o)[D / 64], float& l) {
+  const int lane = threadIdx.x & 63;
+  float m = kLowestRef;
+  for (uint32_t s0 = 0; s0 < n; s0 += 4 * K) {
+    const bool have = lane < 4 * K && s0 + lane < n;
+    const float* at = base + (size_t)min(s0 + lane, n - 1) * stride + D;
+    const float pm = at[0], pl = at[1];
+    float v[K][D / 64];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) v[k][i] = base[(size_t)min(s0 + wave + 4 * k, n - 1) * stride + lane + 64 * i];
+    const float now = __builtin_fmaxf(m, wave_max(have ? pm : kLowestRef)), old = __builtin_amdgcn_exp2f(m - now);
+    const float w = have ? __builtin_amdgcn_exp2f(pm - now) : 0.f;
+    l = l * old + (have ? w * pl : 0.f);
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) o[i] *= old;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (s0 + wave + 4 * k >= n) break;
+      const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), wave + 4 * k));
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) o[i] = __builtin_fmaf(wk, v[k][i], o[i]);
+    }
+    m = now;
+  }
+}
+
+// one workgroup of four waves per (sequence, query head): every wave its share of the pieces, then the waves' sums in a fixed order
 template <int D>
 __global__ __launch_bounds__(256) void decode_i4_join_kernel(Decode a) {
   constexpr int kPiece = D + 2;
-  __shared__ float sums[4][D], refs[4], ls[4];
+  __shared__ float sums[4][D];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t b = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq;
   Shares shares(a);
   const Place place = shares.of(a, b);
   const uint32_t hkv = hq / a.rep, in_head = hq % a.rep, unit = hkv * a.blocks + in_head / kCols, h = in_head % kCols;
-  float m = kLowestRef, l = 0.f, o[D / 64] = {};
+  float l = 0.f, o[D / 64] = {};
   if (place.tiles) {
-    const uint32_t start = place.before + unit * place.tiles;
-    const uint32_t g0 = start / shares.c, g1 = (start + place.tiles - 1) / shares.c;
-    for (uint32_t g = g0 + wave; g <= g1; g += 4) {
-      const float* piece = a.partials + ((size_t)(g + (size_t)b * shares.heads + unit) * kCols + h) * kPiece;
-      const float pm = piece[D], now = __builtin_fmaxf(m, pm);
-      const float old = __builtin_amdgcn_exp2f(m - now), w = __builtin_amdgcn_exp2f(pm - now);
-      l = l * old + w * piece[D + 1];
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) o[i] = o[i] * old + w * piece[lane + 64 * i];
-      m = now;
-    }
+    const uint32_t start = place.before + unit * place.entries;
+    const uint32_t g0 = start / shares.c, n = (start + place.entries - 1) / shares.c - g0 + 1;
+    const float* base = a.partials + ((size_t)(g0 + (size_t)b * shares.heads + unit) * kCols + h) * kPiece;
+    const size_t stride = (size_t)kCols * kPiece;
+    if (n <= 16) join_pieces<D, 4>(base, stride, n, wave, o, l);
+    else join_pieces<D, 16>(base, stride, n, wave, o, l);
+    l = wave_sum(l);
   }
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) sums[wave][lane + 64 * i] = o[i];
-  if (lane == 0) refs[wave] = m, ls[wave] = l;
   __syncthreads();
-  if (tid < D) {
-    const float top = __builtin_fmaxf(__builtin_fmaxf(refs[0], refs[1]), __builtin_fmaxf(refs[2], refs[3]));
-    float all = 0.f, sum = 0.f;
+  if (wave != 0) return;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float w = __builtin_amdgcn_exp2f(refs[k] - top);
-      all += w * ls[k], sum += w * sums[k][tid];
-    }
-    ((_Float16*)a.out)[(size_t)blockIdx.x * D + tid] = (_Float16)(place.tiles ? sum / all : 0.f);
+  for (int i = 0; i < D / 64; ++i) {
+    const int ch = lane + 64 * i;
+    const float sum = (sums[0][ch] + sums[1][ch]) + (sums[2][ch] + sums[3][ch]);
+    ((_Float16*)a.out)[(size_t)blockIdx.x * D + ch] = (_Float16)(place.tiles ? sum / l : 0.f);
   }
 }
 

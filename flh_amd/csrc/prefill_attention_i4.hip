@@ -55,12 +55,6 @@ struct Layout {
   static constexpr int kBytes = kWaves * kWave;
 };
 
-// what is made of it here is not made in front of the branch that it is needed behind
-__device__ __forceinline__ int opaque(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
 // KW: waves that share 32 rows and take every fourth tile (4), or waves with rows of their own (1)
 template <int D, int KW>
 __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
