@@ -19,6 +19,7 @@ namespace flh {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4, kCols = 16, kStages = 2;
+constexpr uint32_t kHeadTiles = 12;
 
 struct Decode {
   const __half *q, *k_new, *v_new, *cos, *sin;
@@ -40,9 +41,11 @@ struct Place {
   uint32_t b, length, tiles, entries, before;          // a sequence, its slots taken, tiles of a head, entries of a head, those of the sequences before
 };
 
-// How the work is shared.  Usually: the tiles of all heads are one list, a workgroup takes `c` of its entries.  With few tiles to a workgroup, where a
-// share of two heads would cost a second round of every latency: each head is cut into equal parts of at most c tiles, and the parts are the list, of
-// which a workgroup takes one (5 sequences of 778 slots, 32 heads: 13 tiles a head, 4 to a workgroup).  64 sequences in the lanes at a time.
+// How the work is shared.  Usually: the tiles of all heads are one list, each head's with kHeadTiles empty entries in front, for what a further head
+// costs a workgroup (its queries, the first tile's latency, a piece), and a workgroup takes `c` entries of it.  us, 0 / 4 / 8 / 12 / 16 of them: 1 x
+// 60000 slots of 8 heads 23.8 / 21.5 / 19.4 / 19.1 / 19.2, 32 x up to 8000 51.2 / 49.0 / 48.4 / 49.2 / 47.6, 5 x 778 of 32 heads 13.8 / 13.0 / 12.7 /
+// 13.0 / 14.6.  With few tiles to a workgroup each head is cut into equal parts of at most c tiles, and the parts are the list, of which a workgroup
+// takes one (5 x 778: 17.4 -> 13.8).  64 sequences in the lanes at a time.
 struct Shares {
   uint32_t c, total, heads;                            // .., entries of the list, heads of a sequence
   bool parts;
@@ -51,7 +54,8 @@ struct Shares {
   __device__ __forceinline__ void look(const Decode& a, uint32_t b0) {
     const uint32_t b = b0 + (threadIdx.x & 63);
     const long long n = b < a.B ? a.lengths[b] : -1;
-    tiles = entries = tiles_of(a, n);
+    tiles = tiles_of(a, n);
+    entries = tiles ? tiles + kHeadTiles : 0;
     length = (uint32_t)n;
     up = wave_scan(entries * heads);
     first = b0;
@@ -115,10 +119,11 @@ struct Layout {
   static constexpr int kStage = 2 * kTile + 2 * kTileKeys * 4;               // K, V, their scales (a dword each)
   static constexpr int kQPitch = D * 2 + 16;                                 // bytes of a query's halves
   static constexpr int kPiece = D + 2;                                       // floats of a piece and query
+  static constexpr int kWave = kStages * kStage;
   // the waves' stages; the queries' high and low halves; what their scores begin with; the new row's codes and scales
-  static constexpr int kQ = kWaves * kStages * kStage, kBias = kQ + 2 * kCols * kQPitch, kNew = kBias + kCols * 4,
+  static constexpr int kQ = kWaves * kWave, kBias = kQ + 2 * kCols * kQPitch, kNew = kBias + kCols * 4,
                        kBytes = kNew + 2 * kRowBytes + 16;
-  static_assert(kCols * kPiece * 4 <= kStages * kStage, "a wave's result takes the place of its stages");
+  static_assert(kCols * kPiece * 4 <= kWave, "a wave's result takes the place of its stages");
 };
 
 template <int D>
@@ -128,8 +133,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, kb = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned lds0 = (unsigned)(size_t)lds;
-  uint8_t* const mine = lds + wave * (kStages * L::kStage);
-  const unsigned mine0 = lds0 + wave * (kStages * L::kStage);
+  uint8_t* const mine = lds + wave * L::kWave;
+  const unsigned mine0 = lds0 + wave * L::kWave;
   Shares shares(a);
   uint32_t pos = blockIdx.x * shares.c;
   const uint32_t end = min(shares.total, pos + shares.c);
@@ -155,8 +160,13 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
     const Place place = shares.at(a, pos);
     const uint32_t unit = (pos - place.before) / place.entries;                 // of the sequence's heads x blocks
     const uint32_t entry = pos - place.before - unit * place.entries;
-    const uint32_t first = shares.parts ? (uint32_t)((uint64_t)place.tiles * entry / place.entries) : entry;
-    const uint32_t stop = shares.parts ? (uint32_t)((uint64_t)place.tiles * (entry + 1) / place.entries) : min(place.tiles, first + (end - pos));
+    const uint32_t behind = min(place.entries, entry + (end - pos));            // entries of the head that are this workgroup's: entry .. behind
+    const uint32_t first = shares.parts ? (uint32_t)((uint64_t)place.tiles * entry / place.entries) : max(entry, kHeadTiles) - kHeadTiles;
+    const uint32_t stop = shares.parts ? (uint32_t)((uint64_t)place.tiles * (entry + 1) / place.entries) : max(behind, kHeadTiles) - kHeadTiles;
+    if (first == stop) {                               // (its first entries alone)
+      pos += behind - entry;
+      continue;
+    }
     const uint32_t hkv = unit / a.blocks, q0 = (unit % a.blocks) * kCols, cols = min((uint32_t)kCols, a.rep - q0);
     const uint32_t bh = place.b * a.Hkv + hkv, slot = place.length;
     const bool has_new = stop == place.tiles;
@@ -280,19 +290,27 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       ((unsigned short*)vs)[(lane >> 5) * 32 + (lane & 15) * 2 + ((lane >> 4) & 1)] = (unsigned short)v_raw;
       // ---- scores: tile t of sixteen keys as rows, key 16 t + 4 kb + i in element i
       v4f st[4];
+      unsigned w[4][kSteps];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         st[t] = v4f{bias, bias, bias, bias};
-        unsigned w[kSteps];
-        if constexpr (D == 128) *(v4i*)w = *(const v4i*)(kt + k_at(16 * t + col, kb));
-        else *(v2i*)w = *(const v2i*)(kt + k_at(16 * t + col, kb >> 1) + (kb & 1) * 8);
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-          const h8 k = code_halves(w[j]);
-          st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[j], st[t], 0, 0, 0);
-          st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], st[t], 0, 0, 0);
-        }
+        if constexpr (D == 128) *(v4i*)w[t] = *(const v4i*)(kt + k_at(16 * t + col, kb));
+        else *(v2i*)w[t] = *(const v2i*)(kt + k_at(16 * t + col, kb >> 1) + (kb & 1) * 8);
       }
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {               // (four sums side by side: one's next product waits for its last)
+        h8 k[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          k[t] = code_halves(w[t][j]);
+          st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], qh[j], st[t], 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], ql[j], st[t], 0, 0, 0);
+      }
+      v2i cv[D / 16];
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) cv[i] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i*)(vt + v_at(key, i >> 1) + (i & 1) * 8));
       // ---- probabilities, then weights, in pairs (2 u, 2 u + 1) of tiles as the codes' halves come
       h8 p[2];
       float sum, added;
@@ -355,11 +373,12 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       l += sum, weights += added;
       // ---- output: sixteen channels as rows; a lane's sixteen keys 16 t + 4 kb + i in nibble 4 t + i
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_v2i*)(vt + v_at(key, i >> 1) + (i & 1) * 8));
-        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_halves((unsigned)w[0]), p[0], o[i], 0, 0, 0);
-        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_halves((unsigned)w[1]), p[1], o[i], 0, 0, 0);
-      }
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int w8 = cv[i][u];
+          o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_halves((unsigned)w8), p[u], o[i], 0, 0, 0);
+        }
     }
 
     // ---- the waves' results into one piece
@@ -383,10 +402,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       const uint32_t h = i / D, ch = i % D;
       float m = kLowestRef, w[kWaves], sum = 0.f, total = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) m = __builtin_fmaxf(m, ((const float*)(lds + k * (kStages * L::kStage)))[h * L::kPiece + D]);
+      for (int k = 0; k < kWaves; ++k) m = __builtin_fmaxf(m, ((const float*)(lds + k * L::kWave))[h * L::kPiece + D]);
 #pragma unroll
       for (int k = 0; k < kWaves; ++k) {
-        const float* from = (const float*)(lds + k * (kStages * L::kStage)) + h * L::kPiece;
+        const float* from = (const float*)(lds + k * L::kWave) + h * L::kPiece;
         w[k] = first + k < stop ? __builtin_amdgcn_exp2f(from[D] - m) : 0.f;
         total += first + k < stop ? w[k] * from[ch] : 0.f;
         sum += first + k < stop ? w[k] * from[D + 1] : 0.f;
@@ -395,7 +414,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       if (ch == 0) piece[h * L::kPiece + D] = m, piece[h * L::kPiece + D + 1] = sum;
     }
     __syncthreads();
-    pos += shares.parts ? 1 : stop - first;
+    pos += behind - entry;
   }
 }
 
@@ -442,8 +461,9 @@ __global__ __launch_bounds__(256) void decode_i4_join_kernel(Decode a) {
   const uint32_t hkv = hq / a.rep, in_head = hq % a.rep, unit = hkv * a.blocks + in_head / kCols, h = in_head % kCols;
   float l = 0.f, o[D / 64] = {};
   if (place.tiles) {
+    // (from the workgroup with its first tile on)
     const uint32_t start = place.before + unit * place.entries;
-    const uint32_t g0 = start / shares.c, n = (start + place.entries - 1) / shares.c - g0 + 1;
+    const uint32_t g0 = (start + (shares.parts ? 0 : kHeadTiles)) / shares.c, n = (start + place.entries - 1) / shares.c - g0 + 1;
     const float* base = a.partials + ((size_t)(g0 + (size_t)b * shares.heads + unit) * kCols + h) * kPiece;
     const size_t stride = (size_t)kCols * kPiece;
     if (n <= 16) join_pieces<D, 4>(base, stride, n, wave, o, l);
