@@ -233,6 +233,86 @@ class StaticKVCache:
         return kept, left
 
 
+class QuantizedKVCache:
+    """Preallocated keys / values in 4 bits, a quarter of an fp16 cache's memory and of what a decode step reads of it:
+    codes uint8 [batch, kv_heads, max_len, head_dim / 2] and a scale fp16 [batch, kv_heads, max_len] per row, for keys (as they are after the
+    rotary embedding and the Hadamard rotation of their head) and values of every layer.  Heads of 64 or 128 channels.
+
+    Sequences have lengths of their own, `lengths` (device int64 [batch], zeros at first): a step over T tokens takes the slots
+    lengths .. lengths + T - 1 of every sequence, and `advance` moves the lengths behind it.  Attention reads what the cache holds, the step's own
+    tokens included: a prompt may come in one block, in several, or token by token.  A captured step serves every length.  A sequence whose length is negative, or above max_len - T, takes no part in a step."""
+
+    max_positions = None                    # (the rotary table has max_len rows)
+
+    def __init__(self, layers, batch, kv_heads, max_len, head_dim, device):
+        if head_dim not in (64, 128):
+            raise ValueError(f"a cache in 4 bits has heads of 64 or 128 channels, not {head_dim}")
+        self.max_len, self.head_dim = max_len, head_dim
+        codes, scales = (batch, kv_heads, max_len, head_dim // 2), (batch, kv_heads, max_len)
+        self.layers = [(torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(scales, dtype=torch.float16, device=device),
+                        torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(scales, dtype=torch.float16, device=device))
+                       for _ in range(layers)]
+        self.lengths = torch.zeros(batch, dtype=torch.int64, device=device)
+        self._workspaces = {}               # scratch of the attention kernels, by size: captured graphs keep theirs
+
+    class _Layer:
+        """What a decoder layer takes as `kv_cache` in a step (positions None, cos / sin [B, T, d])."""
+
+        def __init__(self, owner, index):
+            self.owner, self.index = owner, index
+
+        def attend(self, q, k, v, cos, sin):
+            """q [B, T, Hq, d], k / v [B, T, Hkv, d] of the new tokens as projected, cos / sin [B, T, d] -> [B, T, Hq * d]"""
+            owner, cache = self.owner, self.owner.layers[self.index]
+            b, t, hq, d = q.shape
+            if t == 1:
+                out = _ops().decode_attention_rope_i4(q.reshape(b, hq, d), k.reshape(b, -1, d), v.reshape(b, -1, d), cos.reshape(b, d),
+                                                      sin.reshape(b, d), owner.lengths, *cache, workspace=owner._workspace(b, t, hq))
+                return out.view(b, 1, hq * d)
+            q = _ops().rope_quantize_kv_cache_(q, k, v, cos, sin, owner.lengths, *cache)
+            return _ops().prefill_attention_i4(q, owner.lengths, *cache, workspace=owner._workspace(b, t, hq))
+
+    def layer(self, index):
+        return QuantizedKVCache._Layer(self, index)
+
+    def next_positions(self):
+        """The position behind each sequence: its next token's."""
+        return self.lengths
+
+    def advance(self, t, counts=None):
+        """Move the lengths of the sequences that took part in a step over `t` tokens, by t or by `counts` (device int64 [batch], at most t: in a
+        batch of padded rows the tokens that count; what the others have left behind the lengths is overwritten by the next step)."""
+        takes_part = (self.lengths >= 0) & (self.lengths <= self.max_len - t)
+        self.lengths.add_(takes_part * (t if counts is None else counts))
+
+    def read(self, index, first, rows):
+        """Slots first[b] .. first[b] + rows - 1 of layer `index` as fp16 (keys, values) [batch, kv_heads, rows, head_dim], as dequantize_kv_cache."""
+        return _ops().dequantize_kv_cache(*self.layers[index], first, rows)
+
+    def to_static(self, q_heads=None, max_positions=None):
+        """The same sequences in a StaticKVCache, in fp16, with lengths of their own (as after its begin_drafts): for steps over drafted tokens,
+        or to be cut."""
+        codes = self.layers[0][0]
+        static = StaticKVCache(len(self.layers), codes.size(0), codes.size(1), self.max_len, self.head_dim, codes.device, q_heads=q_heads,
+                               max_positions=max_positions)
+        static.begin_drafts().copy_(self.lengths)
+        first = torch.zeros_like(self.lengths)
+        for i in range(len(self.layers)):
+            static.keys[i], static.values[i] = self.read(i, first, self.max_len)
+        return static
+
+    def _workspace(self, batch, t, q_heads):
+        from .. import _lib
+        codes, lib = self.layers[0][0], _lib.load()
+        heads, d = codes.size(1), self.head_dim
+        need = int(lib.flh_decode_attention_i4_workspace_bytes(batch, q_heads, heads, d, self.max_len) if t == 1 else
+                   lib.flh_prefill_attention_i4_workspace_bytes(batch, t, q_heads, heads, d, self.max_len))
+        ws = self._workspaces.get(need)
+        if ws is None:
+            ws = self._workspaces[need] = torch.empty(need, dtype=torch.uint8, device=codes.device)
+        return ws
+
+
 def _stock_call(module, cls):
     """Whether calling `module` is `cls.forward` on plain tensors and nothing else, so that a kernel of this library may stand in
     for it: no hooks (the module's or global ones), no forward of its own, no weight of another tensor class, no trace, no
@@ -459,8 +539,8 @@ class W4A4DecoderLayer(torch.nn.Module):
     def attention(self, x, cos, sin, kv_cache=None, positions=None):
         """x [B, T, hidden] fp16 (already the residual stream); cos / sin [T, head_dim] of the T new positions;
         kv_cache: None, a pair (keys, values) [B, kv_heads, past, head_dim] that grows by concatenation, one layer of a
-        StaticKVCache in a step over drafted tokens (`tree_layer`; cos / sin [B, T, head_dim], positions None), or one layer
-        of a StaticKVCache together with `positions` (device int64 [T]: the slots the new tokens take, which must be
+        StaticKVCache in a step over drafted tokens (`tree_layer`; cos / sin [B, T, head_dim], positions None) or of a
+        QuantizedKVCache (the same), or one layer of a StaticKVCache together with `positions` (device int64 [T]: the slots the new tokens take, which must be
         arange(kv_len - T, kv_len) for the cache's kv_len, the number of slots attention reads -- see StaticKVCache).
         Causal over past + T positions."""
         _, y, cache = self._attention(x, None, cos, sin, kv_cache, positions, fold_residual=False)
@@ -478,16 +558,17 @@ class W4A4DecoderLayer(torch.nn.Module):
         else:
             x, s, z, q = self._residual_norm_quant("attn_in", self.input_layernorm, "input_layernorm",
                                                    self.attn_quantizer1, x, add, qkv)
-            tree = isinstance(kv_cache, StaticKVCache._TreeLayer)
-            mode = None if tree else self._qkv_rope_applies(b * t, q, s, cos, kv_cache, positions)
+            attends = isinstance(kv_cache, (StaticKVCache._TreeLayer, QuantizedKVCache._Layer))
+            mode = None if attends else self._qkv_rope_applies(b * t, q, s, cos, kv_cache, positions)
             if mode:
                 return self._attention_after_fused_qkv(x, q, s, z, cos, sin, kv_cache, positions, fold_residual, mode)
             qs, ks, vs = self._project(qkv, q, s, z)
         self._tap("q_proj", qs), self._tap("k_proj", ks), self._tap("v_proj", vs)
         static = isinstance(kv_cache, StaticKVCache._Layer)
         out = None
-        if isinstance(kv_cache, StaticKVCache._TreeLayer):
-            # drafted tokens against a cache with lengths of its own: rotary embedding, cache write and attention in two launches
+        if isinstance(kv_cache, (StaticKVCache._TreeLayer, QuantizedKVCache._Layer)):
+            # drafted tokens against a cache with lengths of its own, or any against one in 4 bits: rotary embedding, cache write and
+            # attention are its own
             out = kv_cache.attend(qs.view(b, t, self.num_heads, self.head_dim), ks.view(b, t, self.num_kv_heads, self.head_dim),
                                   vs.view(b, t, self.num_kv_heads, self.head_dim), cos, sin)
             cache = kv_cache

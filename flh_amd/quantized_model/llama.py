@@ -18,7 +18,7 @@ import torch
 
 from ..nn.normalization import RMSNorm
 from ..nn.quantization import fast_hadamard_transform
-from .decoder_layer import StaticKVCache, W4A4DecoderLayer, _stock_call, rotary_tables
+from .decoder_layer import QuantizedKVCache, StaticKVCache, W4A4DecoderLayer, _stock_call, rotary_tables
 
 
 class LlamaShape:
@@ -234,10 +234,17 @@ class W4A4LlamaModel(torch.nn.Module):
         for layer in self.layers:
             layer.set_six_bit(six_bit)
 
-    def new_cache(self, batch, max_len, max_positions=None):
-        """`max_positions`: of a cache that is cut on the way (StaticKVCache.evict), the positions that its sequences may reach."""
+    def new_cache(self, batch, max_len, max_positions=None, bits=16):
+        """`max_positions`: of a cache that is cut on the way (StaticKVCache.evict), the positions that its sequences may reach.
+        `bits`: 16 (a StaticKVCache) or 4 (a QuantizedKVCache, for append())."""
         s = self.shape
         dev = self.embed_tokens.weight.device
+        if bits == 4:
+            if max_positions is not None:
+                raise ValueError("a cache in 4 bits is not cut: max_positions is of one in 16")
+            return QuantizedKVCache(s.num_layers, batch, s.num_kv_heads, max_len, s.head_dim, dev)
+        if bits != 16:
+            raise ValueError(f"a cache has 16 or 4 bits, not {bits}")
         return StaticKVCache(s.num_layers, batch, s.num_kv_heads, max_len, s.head_dim, dev, q_heads=s.num_heads,
                              max_positions=max_positions)
 
@@ -292,6 +299,8 @@ class W4A4LlamaModel(torch.nn.Module):
         positions == arange(kv_len - T, kv_len) (what cache.advance(T) returns; see StaticKVCache for why nothing else
         is meaningful).  Returns logits [B, T, vocab] fp16 (or the final hidden state)."""
         if cache is not None:
+            if isinstance(cache, QuantizedKVCache):
+                raise ValueError("a cache in 4 bits: append()")
             if cache.lengths is not None:
                 raise ValueError("the sequences of this cache have lengths of their own: tree_step() (a tree of one node for one token)")
             t = input_ids.size(1)
@@ -317,6 +326,8 @@ class W4A4LlamaModel(torch.nn.Module):
         b, t = input_ids.shape
         if t != len(tree):
             raise ValueError(f"{t} tokens for a tree of {len(tree)} nodes")
+        if isinstance(cache, QuantizedKVCache):
+            raise ValueError("a cache in 4 bits takes no drafts (its to_static() does)")
         if cache.lengths is None:
             raise ValueError("cache.begin_drafts() first")
         if input_ids.size(0) != cache.lengths.numel():
@@ -328,6 +339,31 @@ class W4A4LlamaModel(torch.nn.Module):
         pending, lengths = None, cache.step_lengths(t)
         for i, layer in enumerate(self.layers):
             x, pending, _ = layer.forward_deferred(x, pending, cos, sin, cache.tree_layer(i, tree, lengths))
+        x = self._final_norm(x, pending)
+        return x if return_hidden else self._head(x)
+
+    def append(self, input_ids, cache, counts=None, return_hidden=False):
+        """One step on a QuantizedKVCache: input_ids [B, T] int64 behind what the cache holds of each sequence -> logits [B, T, vocab] fp16
+        (or the final hidden state); the lengths move on by T, or by `counts` (device int64 [B]: of padded rows, the tokens that count; the
+        other rows' logits mean nothing).  A sequence that takes no part keeps its length.  Can be captured into a graph after one eager
+        step over as many tokens: it serves every length, and every replay moves the lengths."""
+        b, t = input_ids.shape
+        if not isinstance(cache, QuantizedKVCache):
+            raise ValueError("append() is for a cache in 4 bits (new_cache(..., bits=4))")
+        if b != cache.lengths.numel():
+            raise ValueError(f"{b} sequences for a cache of {cache.lengths.numel()}")
+        if not 0 < t <= cache.max_len:
+            raise ValueError(f"{t} tokens for a cache of {cache.max_len} slots")
+        if counts is not None and (counts.shape != cache.lengths.shape or counts.dtype != torch.int64 or counts.device != cache.lengths.device):
+            raise ValueError("counts must be int64 [B] on the cache's device")
+        # (a sequence that takes no part has no position: any row of the table will do)
+        positions = (cache.next_positions()[:, None] + torch.arange(t, device=cache.lengths.device)).clamp(0, cache.max_len - 1).reshape(-1)
+        x, cos, sin = self._look_up(input_ids, positions, cache)
+        cos, sin = cos.view(b, t, -1), sin.view(b, t, -1)
+        pending = None
+        for i, layer in enumerate(self.layers):
+            x, pending, _ = layer.forward_deferred(x, pending, cos, sin, cache.layer(i))
+        cache.advance(t, counts)
         x = self._final_norm(x, pending)
         return x if return_hidden else self._head(x)
 
