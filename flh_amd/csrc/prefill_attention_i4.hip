@@ -30,16 +30,78 @@ struct Prefill {
   float scale_log2;
 };
 
-// The tiles of a block are split only as far as every workgroup has kSplitTiles: known on the device alone, like the lengths
-constexpr uint32_t kSplitTiles = 8;
-__device__ __forceinline__ uint32_t splits_for(const Prefill& a, uint32_t tiles) {
-  return max(1u, min(a.splits, (tiles + kSplitTiles - 1) / kSplitTiles));
-}
 // tiles with a slot that a query of the block sees (none: the sequence takes no part)
 __device__ __forceinline__ uint32_t tiles_of(const Prefill& a, long long length, uint32_t block) {
   if (length < 0 || length > (long long)a.max_len - (long long)a.T) return 0;
   return ((uint32_t)length + (min((block + 1) * kBlockRows, a.rows) - 1) / a.rep) / kTileKeys + 1;
 }
+
+// How few rows are shared: a block's tiles go in equal parts over several workgroups, as many as its share of the tiles of all gets it of kParts (two
+// workgroups a compute unit, one round) and none of fewer than kPartTiles tiles.  That is known on the device alone, like the lengths: the parts are
+// one list, and a workgroup takes the entry of its index, parts of a block one after the other, so that a long sequence's lie on all dies.  The same
+// number for every sequence took 59 us for 17 tokens each behind 16000 and three times 200 cached ones (4 sequences, 32 / 8 heads of 128), the list
+// 36; equal lengths lose nothing (4 x 16000: 42 us either way), but where the rounding gives more than kParts (576: 46 us), hence the floor.  A die's
+// entries in one range: 42 us for the ragged batch.  64 sequences lie in the lanes at a time.
+constexpr uint32_t kParts = 512, kPartTiles = 8;
+struct Parts {
+  uint32_t total, heads, all;                          // entries of the list, blocks of all heads of a sequence, tiles of all of them
+  uint32_t entries, up, first, before;                 // of the 64 sequences last looked at
+
+  __device__ __forceinline__ uint32_t longest(const Prefill& a, uint32_t b) const { return b < a.B ? tiles_of(a, a.lengths[b], a.blocks - 1) : 0u; }
+  __device__ __forceinline__ void look(const Prefill& a, uint32_t b0, uint32_t tiles) {
+    // (a sequence that takes no part has its zeros to write: one entry a block)
+    entries = b0 + (threadIdx.x & 63) < a.B ? max(1u, min(min(a.splits, (tiles + kPartTiles - 1) / kPartTiles), tiles * kParts / all)) : 0u;
+    up = wave_scan(entries * heads);
+    first = b0;
+  }
+  __device__ __forceinline__ explicit Parts(const Prefill& a) {
+    heads = a.Hkv * a.blocks;
+    uint32_t tiles = 0;
+    all = 0;                                           // (below 2^28: the caches' slots are bounded, and B x heads is at most kParts / 2)
+    for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+      tiles = longest(a, b0 + (threadIdx.x & 63));
+      all += from_lane(wave_scan(tiles), 63);
+    }
+    all = max(1u, all * heads);
+    total = before = 0;
+    if (a.B <= 64) {
+      look(a, 0, tiles);
+      total = from_lane(up, 63);
+      return;
+    }
+    for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+      look(a, b0, longest(a, b0 + (threadIdx.x & 63)));
+      before = total;
+      total += from_lane(up, 63);
+    }
+  }
+  __device__ __forceinline__ static uint32_t from_lane(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+  // sequence b: its parts a block, and the entries in front of it
+  __device__ __forceinline__ void of(const Prefill& a, uint32_t b, uint32_t& parts, uint32_t& start) {
+    if (b - first >= 64) {
+      before = 0;
+      for (uint32_t b0 = 0;; b0 += 64) {
+        look(a, b0, longest(a, b0 + (threadIdx.x & 63)));
+        if (b - b0 < 64) break;
+        before += from_lane(up, 63);
+      }
+    }
+    parts = from_lane(entries, b - first);
+    start = before + from_lane(up, b - first) - parts * heads;
+  }
+  // the sequence that holds entry `pos` (below total)
+  __device__ __forceinline__ uint32_t at(const Prefill& a, uint32_t pos) {
+    if (a.B > 64) {
+      before = 0;
+      for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+        look(a, b0, longest(a, b0 + (threadIdx.x & 63)));
+        if (before + from_lane(up, 63) > pos) break;
+        before += from_lane(up, 63);
+      }
+    }
+    return first + (uint32_t)__builtin_ctzll(__ballot(before + up > pos));
+  }
+};
 
 // floats of a piece: 32 rows of D sums, their references and sums of exponentials
 template <int D>
@@ -65,19 +127,27 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
   uint8_t* const mine = lds + wave * L::kWave;
   const unsigned mine0 = (unsigned)(size_t)mine;
   // every die takes a contiguous range of (sequence, key / value head) pairs; within one the long blocks (late queries) come first
-  const unsigned w = xcd_contiguous(blockIdx.x, gridDim.x);
-  uint32_t split, block, bh;
+  unsigned w = xcd_contiguous(blockIdx.x, gridDim.x);
+  uint32_t split = 0, splits = 1, block, bh;
   if constexpr (KW == 1) {                             // (one workgroup for four blocks, one piece each)
     const uint32_t quads = (a.blocks + 3) / 4;
-    split = 0, bh = w / quads, block = (quads - 1 - w % quads) * 4 + wave;
+    bh = w / quads, block = (quads - 1 - w % quads) * 4 + wave;
     if (block >= a.blocks) return;
+  } else if (a.splits == 1) {
+    block = a.blocks - 1 - w % a.blocks, bh = w / a.blocks;
   } else {
-    split = w % a.splits, block = a.blocks - 1 - w / a.splits % a.blocks, bh = w / a.splits / a.blocks;
+    Parts parts(a);
+    if (blockIdx.x >= parts.total) return;
+    w = blockIdx.x;
+    const uint32_t b = parts.at(a, w);
+    uint32_t start;
+    parts.of(a, b, splits, start);
+    const uint32_t at = w - start, unit = at / splits;
+    split = at % splits, block = unit % a.blocks, bh = b * a.Hkv + unit / a.blocks;
   }
   const uint32_t b = bh / a.Hkv, hkv = bh % a.Hkv;
   const long long len = a.lengths[b];
-  const uint32_t tiles = tiles_of(a, len, block), splits = KW == 1 ? 1 : splits_for(a, tiles);
-  if (split >= splits) return;
+  const uint32_t tiles = tiles_of(a, len, block);
   const uint32_t length = tiles ? (uint32_t)len : 0u;
 
   const uint32_t first_row = block * kBlockRows, live_rows = min((uint32_t)kBlockRows, a.rows - first_row);
@@ -208,8 +278,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
           }
         }
     };
-    // A reference that holds the scores and the values' largest scale back: p vs < 2^11 when it is set, in the first tile and again where a weight
-    // leaves fp16's range, which few tiles' do
+    // A reference that holds the largest weight back, p vs < 2^11 when it is set, in the first tile and again where a weight leaves fp16's range, which
+    // few tiles' do.  Of the keys that the query sees alone: what it does not see may be NaN or as large as it likes.
     for (;;) {
       if (set_reference) {
         float top = -INFINITY;
@@ -217,18 +287,19 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const v4i k4 = *(const v4i*)(ks + 32 * i + 8 * k + 4 * h);
+          for (int u = 0; u < 2; ++u) {
+            const v4i k0 = *(const v4i*)(ks + 32 * i + 16 * u + 4 * h), k1 = *(const v4i*)(ks + 32 * i + 16 * u + 8 + 4 * h);
+            const v4i v2 = *(const v4i*)(vs + 16 * i + 8 * u + 4 * h);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int f = k4[e];
-              const float y = st[i][4 * k + e] * __int_as_float(f);
-              top = __builtin_fmaxf(top, from + 32 * i + 8 * k + e > limit ? -INFINITY : y);
+              const int a0 = k0[e], a1 = k1[e], vv = v2[e], at = from + 32 * i + 16 * u + e;
+              const float y0 = __builtin_fmaf(st[i][8 * u + e], __int_as_float(a0), (float)((vv >> 10) & 31));
+              const float y1 = __builtin_fmaf(st[i][8 * u + 4 + e], __int_as_float(a1), (float)((vv >> 26) & 31));
+              top = __builtin_fmaxf(top, __builtin_fmaxf(at > limit ? -INFINITY : y0, at + 8 > limit ? -INFINITY : y1));
             }
           }
         top = __builtin_fmaxf(top, lane_xor_f<32>(top));
-        const float most = wave_max((float)(min(v_raw & 0x7FFFu, 0x7C00u) >> 10));
-        const float now = __builtin_fmaxf(ref, top + (most - 25.0f));
+        const float now = __builtin_fmaxf(ref, top - 25.0f);
         const float alpha = __builtin_amdgcn_exp2f(ref - now);
         l *= alpha, weights *= alpha;
 #pragma unroll
@@ -314,7 +385,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
       }
     }
     if (splits > 1) {
-      float* piece = a.pieces + (((size_t)bh * a.blocks + block) * a.splits + split) * kPieceFloats<D>;
+      float* piece = a.pieces + (size_t)w * kPieceFloats<D>;
       *(v4f*)(piece + r * D + ch) = v4f{y[0], y[1], y[2], y[3]};
       *(v4f*)(piece + r * D + ch + 4) = v4f{y[4], y[5], y[6], y[7]};
       if (ch == 0) piece[kBlockRows * D + r] = m, piece[kBlockRows * (D + 1) + r] = sum;
@@ -337,11 +408,14 @@ __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
   if (item >= a.B * a.Hkv * a.rows) return;
   const uint32_t bh = item / a.rows, row = item % a.rows, b = bh / a.Hkv, hkv = bh % a.Hkv;
   const uint32_t block = row / kBlockRows, r = row % kBlockRows;
-  const uint32_t splits = splits_for(a, tiles_of(a, a.lengths[b], block));
+  Parts parts(a);
+  uint32_t splits, start;
+  parts.of(a, b, splits, start);
   if (splits == 1) return;                             // (its workgroup has stored the output)
-  const float* base = a.pieces + ((size_t)bh * a.blocks + block) * a.splits * kPieceFloats<D>;
+  const float* base = a.pieces + (size_t)(start + (hkv * a.blocks + block) * splits) * kPieceFloats<D>;
+  const size_t next = kPieceFloats<D>;
   // lane s: piece s
-  const float* at = base + (size_t)min((uint32_t)lane, splits - 1) * kPieceFloats<D> + kBlockRows * D + r;
+  const float* at = base + min((uint32_t)lane, splits - 1) * next + kBlockRows * D + r;
   const bool have = (uint32_t)lane < splits;
   const float pl = have ? at[kBlockRows] : 0.f;
   const float pm = pl == 0.f ? kLowestRef : at[0];     // (nothing of it is seen)
@@ -355,7 +429,7 @@ __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
     const bool seen = __builtin_amdgcn_readlane(__float_as_int(pl), (int)s) != 0;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
-      const float v = base[(size_t)s * kPieceFloats<D> + r * D + lane + 64 * i];
+      const float v = base[s * next + r * D + lane + 64 * i];
       o[i] += seen ? ws * v : 0.f;
     }
   }
@@ -367,15 +441,16 @@ __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
 // Blocks from which every wave has one of its own
 constexpr uint64_t kOwnRows = 4096;
 
-// Workgroups over which a block's tiles are split: as many as fill the chip, two a compute unit
-uint32_t splits_of(uint64_t groups, uint32_t max_len) {
-  const uint64_t tiles = ((uint64_t)max_len + kTileKeys - 1) / kTileKeys;
-  const uint64_t most = (tiles + kSplitTiles - 1) / kSplitTiles;
-  uint64_t s = 512 / groups;
+// Parts that a block can have: none where the blocks fill the chip
+uint32_t splits_of(uint64_t B, uint64_t heads, uint32_t max_len) {
+  const uint64_t tiles = ((uint64_t)max_len + kTileKeys - 1) / kTileKeys, most = (tiles + kPartTiles - 1) / kPartTiles;
+  uint64_t s = 2 * B * heads > kParts ? 1 : kParts / heads;
   if (s > 64) s = 64;
   if (s > most) s = most;
   return s < 1 ? 1 : (uint32_t)s;
 }
+// entries of the list at most: the parts that kParts workgroups take, and a block's last one each
+uint64_t entries_of(uint64_t B, uint64_t heads) { return kParts + B * heads; }
 
 uint64_t blocks_of(uint64_t T, uint64_t rep) { return (T * rep + kBlockRows - 1) / kBlockRows; }
 
@@ -392,9 +467,8 @@ using namespace flh;
 
 extern "C" size_t flh_prefill_attention_i4_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
   if (Hq == 0 || Hkv == 0 || Hq % Hkv || (head_dim != 128 && head_dim != 64) || max_len == 0 || B == 0 || T == 0 || too_large(B, T, Hq, Hkv, max_len)) return 0;
-  const uint64_t groups = (uint64_t)B * Hkv * blocks_of(T, Hq / Hkv);
-  const uint32_t splits = splits_of(groups, max_len);
-  return splits == 1 ? 0 : (size_t)(groups * splits) * kBlockRows * (head_dim + 2) * sizeof(float);
+  const uint64_t heads = (uint64_t)Hkv * blocks_of(T, Hq / Hkv);
+  return splits_of(B, heads, max_len) == 1 ? 0 : (size_t)entries_of(B, heads) * kBlockRows * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* lengths, const uint8_t* k_codes, const flh_half* k_scales,
@@ -426,7 +500,8 @@ extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* length
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.max_len = max_len, a.rows = T * a.rep, a.blocks = (uint32_t)blocks_of(T, a.rep);
   a.scale_log2 = scale * 1.4426950408889634f;
   const uint64_t groups = (uint64_t)B * Hkv * a.blocks;
-  a.splits = splits_of(groups, max_len);
+  a.splits = splits_of(B, (uint64_t)Hkv * a.blocks, max_len);
+  const uint64_t entries = a.splits == 1 ? groups : entries_of(B, (uint64_t)Hkv * a.blocks);
   auto go = [&](auto kern, auto rows, auto join, size_t smem, LdsGrant& grant, LdsGrant& rows_grant) {
     if (groups >= kOwnRows) {
       if (int rc = reserve_lds((const void*)rows, smem, rows_grant, what)) return rc;
@@ -434,7 +509,7 @@ extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* length
       return check_launch(what);
     }
     if (int rc = reserve_lds((const void*)kern, smem, grant, what)) return rc;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(groups * a.splits)), dim3(kThreads), smem, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)entries), dim3(kThreads), smem, (hipStream_t)stream, a);
     if (int rc = check_launch(what)) return rc;
     if (a.splits == 1) return FLH_OK;
     hipLaunchKernelGGL(join, dim3((unsigned)(((uint64_t)B * Hkv * a.rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);

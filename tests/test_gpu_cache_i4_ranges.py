@@ -1,0 +1,112 @@
+"""Attention over caches in 4 bits where the calls take other ways than at small sizes and magnitudes: blocks whose waves have rows of their own, ragged
+batches whose long sequences are shared by many workgroups, scores and values that grow along the cache, and scales out of a query's sight that are
+larger than those in it.  Tolerances are those of the operators' other tests; what each query sees is evaluated by itself where what it does not see
+must not count."""
+import pytest
+import torch
+
+from test_gpu_cache_i4 import attend64, check_decode, check_prefill, close, decode_case, normal, prefill_case, random_cache, unpacked
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["default", "ctypes"])
+def ops(request):
+    if request.param == "ctypes":
+        from flh_amd import _ops
+        return _ops
+    import flh_amd
+    return flh_amd._CUDA
+
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,d,max_len,lengths", [
+    (64, 65, 32, 32, 128, 200, [(i * 31) % 136 - 1 for i in range(64)]),         # three blocks of rows, a fourth wave without; the first takes no part
+    (20, 70, 96, 32, 64, 333, [(i * 71) % 270 - 3 for i in range(20)]),          # three queries per head: blocks that end inside a token
+    (130, 1, 32, 32, 128, 70, [i % 71 for i in range(130)]),                     # a single row in each; one token past the end takes no part
+    (4, 1100, 32, 32, 64, 1200, [0, 63, 100, 101])])
+def test_waves_with_rows_of_their_own(ops, B, T, Hq, Hkv, d, max_len, lengths):
+    assert B * Hkv * -(-T * (Hq // Hkv) // 32) >= 4096
+    gen = torch.Generator().manual_seed(T + B)
+    q, cache = prefill_case(gen, B, T, Hq, Hkv, d, max_len, lengths)
+    check_prefill(ops, q, lengths, cache)
+
+
+def test_waves_with_rows_of_their_own_non_finite(ops):
+    gen = torch.Generator().manual_seed(7)
+    B, T, H, d, n = 70, 33, 32, 64, 50
+    q, cache = prefill_case(gen, B, T, H, H, d, 100, [n] * B)
+    cache[1][3, 5, n + 20] = float("nan")                              # a key that the queries from the twentieth on see, in one head
+    cache[3][9, 0, n + 4] = float("inf")                               # a value
+    q[11, 30, 2, 7] = float("nan")
+    out = ops.prefill_attention_i4(q.cuda(), torch.tensor([n] * B).cuda(), *(t.cuda() for t in cache)).cpu().view(B, T, H, d)
+    finite = torch.isfinite(out).all(-1)
+    want = torch.ones(B, T, H, dtype=torch.bool)
+    want[3, 20:, 5] = want[9, 4:, 0] = want[11, 30, 2] = False
+    held = torch.where(unpacked(cache[2][9, 0, n + 4]) == 0)[0]        # (a code of zero times an infinite scale is NaN as well)
+    assert held.numel() < d and torch.equal(finite, want)
+
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,d,max_len,lengths", [
+    (4, 5, 32, 8, 128, 9000, [8990, 100, 0, 640]),                     # one sequence has most of the tiles
+    (4, 5, 32, 8, 128, 9000, [100, -1, 8990, 9000]),                   # .. and some take no part
+    (3, 40, 12, 4, 64, 5000, [64, 4960, 2000]),                        # several blocks of rows share a sequence's parts
+    (150, 1, 2, 1, 128, 3000, [2999 if i in (0, 63, 64, 149) else (i * 7) % 300 - 2 for i in range(150)]),   # more sequences than lanes
+    (256, 1, 4, 1, 64, 2000, [1999 if i == 200 else i for i in range(256)])])    # the most that are shared
+def test_ragged_parts(ops, B, T, Hq, Hkv, d, max_len, lengths):
+    gen = torch.Generator().manual_seed(T + B)
+    q, cache = prefill_case(gen, B, T, Hq, Hkv, d, max_len, lengths)
+    out = check_prefill(ops, q, lengths, cache)
+    ws = torch.full((64 << 20,), 255, dtype=torch.uint8, device="cuda")
+    assert torch.equal(out, ops.prefill_attention_i4(q.cuda(), torch.tensor(lengths).cuda(), *(t.cuda() for t in cache), workspace=ws))
+
+
+def growing(cache, n, keys, values):
+    """Scales that change by 2^keys and 2^values over the first n slots."""
+    at = torch.arange(n) / max(n - 1, 1)
+    cache[1][:, :, :n] = (0.01 * torch.exp2(keys * at if keys > 0 else -keys * (1 - at))).half()
+    cache[3][:, :, :n] = (2.0 ** -12 * torch.exp2(values * at if values > 0 else -values * (1 - at))).half()
+
+
+@pytest.mark.parametrize("keys,values", [(7, 0), (-7, 0), (0, 26), (0, -26), (6, 24), (6, -24), (-6, 24)])
+@pytest.mark.parametrize("B,T,Hq,Hkv,n", [(1, 9, 8, 2, 900), (2, 70, 8, 4, 400), (70, 33, 32, 32, 300)])
+def test_blocks_of_growing_scales(ops, B, T, Hq, Hkv, n, keys, values):
+    """References that are raised on the way, and ones that the first tile sets above all others."""
+    gen = torch.Generator().manual_seed(n)
+    cache = random_cache(gen, B, Hkv, n + T, 128)
+    growing(cache, n + T, keys, values)
+    q = normal(gen, B, T, Hq, 128, scale=2.0)
+    if B > 8:                                                          # (the others are for the number of rows; evaluated for one)
+        lengths = [-1] * B
+        lengths[5] = n
+    else:
+        lengths = [n - 3 * b for b in range(B)]
+    check_prefill(ops, q, lengths, cache)
+
+
+@pytest.mark.parametrize("keys,values", [(7, 0), (-7, 0), (0, 26), (0, -26), (6, 24), (6, -24), (-6, 24)])
+@pytest.mark.parametrize("B,Hq,Hkv,d,n", [(1, 8, 2, 128, 900), (2, 40, 2, 64, 1400), (70, 8, 4, 128, 200)])
+def test_tokens_of_growing_scales(ops, B, Hq, Hkv, d, n, keys, values):
+    gen = torch.Generator().manual_seed(n)
+    case = decode_case(gen, B, Hq, Hkv, d, n + 1, [n - b for b in range(B)])
+    growing(case[6], n + 1, keys, values)
+    check_decode(ops, case)
+
+
+@pytest.mark.parametrize("big", [60000.0, float("inf"), float("nan")])
+@pytest.mark.parametrize("B,T,Hq,Hkv", [(1, 30, 8, 2), (70, 33, 32, 32)])
+def test_scales_out_of_sight(ops, B, T, Hq, Hkv, big):
+    """Values of 2^-9 in sight, the largest there are behind them in the same tile: every query has the precision of what it sees."""
+    gen = torch.Generator().manual_seed(T)
+    n, d, rep = 64, 128, Hq // Hkv
+    cache = random_cache(gen, B, Hkv, n + T, d)
+    cache[3][:, :, :n + 20] = 2.0 ** -10
+    cache[3][:, :, n + 20:] = big
+    cache[1][:, :, n + 20:] = big if big != big else 60000.0
+    q = normal(gen, B, T, Hq, d)
+    got = ops.prefill_attention_i4(q.cuda(), torch.full((B,), n).cuda(), *(t.cuda() for t in cache)).cpu().view(B, T, Hq, d)
+    for t in (0, 7, 19):
+        for g in range(Hkv):
+            m = n + t + 1
+            x, tol = attend64(q[0, t, g * rep:(g + 1) * rep], unpacked(cache[0][0, g, :m]), cache[1][0, g, :m], unpacked(cache[2][0, g, :m]),
+                              cache[3][0, g, :m], [m] * rep, d ** -0.5)
+            close(got[0, t, g * rep:(g + 1) * rep], x, tol, (t, g))
