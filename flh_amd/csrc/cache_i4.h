@@ -141,10 +141,23 @@ constexpr int kTileKeys = 64;
 // the fp16 value in the low half of a dword (a mixed-precision multiply-add takes it as it is; left to the compiler, which knows what has to lie
 // between a matrix instruction, or an exponential, and the use of its result)
 __device__ __forceinline__ float low_half(unsigned v) { return (float)__builtin_bit_cast(_Float16, (unsigned short)v); }
-__device__ __forceinline__ float times_half(float acc, unsigned scale) { return __builtin_fmaf(acc, low_half(scale), 0.0f); }
 // {fp16(a * x), fp16(b * y)} of fp16 x, y in the low halves
 __device__ __forceinline__ h2 pair_times_halves(float a, unsigned x, float b, unsigned y) {
   return h2{(_Float16)__builtin_fmaf(a, low_half(x), 0.0f), (_Float16)__builtin_fmaf(b, low_half(y), 0.0f)};
+}
+
+// The reference of a softmax whose largest weight, in powers of two, is `top` (a score's plus its value's scale's exponent, 25 for a factor of 2^10):
+// weights stay below 2^12.  A weight's exponent is one multiply-add, score x factor - reference, and so sees the reference's own rounding: it is
+// put more than that below the largest (2^-22 of it, less than 1 for scores below 2^22), and where the weights of a tile leave fp16's range all the
+// same they are bounded: scores of 10^8 and more, where what lies within their rounding weighs the same.
+__device__ __forceinline__ float reference_for(float top) {
+  const float r = top - 25.0f;
+  return r * (r > 0.f ? 1.0f - 0x1p-22f : 1.0f + 0x1p-22f);
+}
+__device__ __forceinline__ float exponent_of(unsigned half) { return (float)((half >> 10) & 31u); }
+__device__ __forceinline__ float bounded(float x, unsigned half) {
+  const float most = 26.0f - exponent_of(half);
+  return x > most ? most : x;                          // (NaN stays)
 }
 
 // Loads that go straight to LDS, lane i's 16 (4) bytes to lds_base + 16 i (4 i); beyond the descriptor's range they bring zeros
@@ -165,6 +178,7 @@ __device__ __forceinline__ int opaque(int v) {
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 typedef __attribute__((address_space(3))) v2i lds_v2i;
+typedef unsigned short __attribute__((may_alias)) packed_u16;   // a half among dwords
 
 }  // namespace
 

@@ -287,7 +287,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       // the scales for all queries at once: keys' as the scores take them, values' in pairs of keys 16 apart, as the weights are packed
       const unsigned k_raw = ks[lane], v_raw = vs[lane];
       ks[lane] = __builtin_bit_cast(unsigned, low_half(k_raw) * factor);
-      ((unsigned short*)vs)[(lane >> 5) * 32 + (lane & 15) * 2 + ((lane >> 4) & 1)] = (unsigned short)v_raw;
+      ((packed_u16*)vs)[(lane >> 5) * 32 + (lane & 15) * 2 + ((lane >> 4) & 1)] = (unsigned short)v_raw;
       // ---- scores: tile t of sixteen keys as rows, key 16 t + 4 kb + i in element i
       v4f st[4];
       unsigned w[4][kSteps];
@@ -314,8 +314,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       // ---- probabilities, then weights, in pairs (2 u, 2 u + 1) of tiles as the codes' halves come
       h8 p[2];
       float sum, added;
-      auto weigh = [&](auto masked_) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked_)::value;
+      auto weigh = [&](auto masked_, auto bounded_) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_)::value, BOUNDED = decltype(bounded_)::value;
         sum = added = 0.f;
         const int left = MASKED ? opaque((int)(slot - tile * kTileKeys) - 4 * kb) : 0;   // the last of the lane's keys there is
 #pragma unroll
@@ -325,8 +325,9 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int a0 = k0[i], a1 = k1[i], vv = v2[i];
-            float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * u][i], __int_as_float(a0), -ref));
-            float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * u + 1][i], __int_as_float(a1), -ref));
+            float p0 = __builtin_fmaf(st[2 * u][i], __int_as_float(a0), -ref), p1 = __builtin_fmaf(st[2 * u + 1][i], __int_as_float(a1), -ref);
+            if constexpr (BOUNDED) p0 = bounded(p0, (unsigned)vv), p1 = bounded(p1, (unsigned)vv >> 16);
+            p0 = __builtin_amdgcn_exp2f(p0), p1 = __builtin_amdgcn_exp2f(p1);
             if constexpr (MASKED) {                    // (scales behind the sequence come as zeros: so do the weights)
               if (32 * u + i > left) p0 = 0.f;
               if (32 * u + 16 + i > left) p1 = 0.f;
@@ -338,35 +339,40 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
           }
         }
       };
-      // A reference that holds the scores and the values' largest scale back: p vs < 2^11 when it is set, in the first tile and again where a
-      // weight leaves fp16's range, which few tiles' do
+      // A reference that holds the largest weight back, p vs < 2^12 when it is set, in the first tile and again where a weight leaves fp16's range,
+      // which few tiles' do
       for (;;) {
         if (set_reference) {
           float top = -INFINITY;
           const int left = opaque((int)(slot - tile * kTileKeys) - 4 * kb);
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const v4i k4 = *(const v4i*)(ks + 16 * t + 4 * kb);
+          for (int u = 0; u < 2; ++u) {
+            const v4i k0 = *(const v4i*)(ks + 32 * u + 4 * kb), k1 = *(const v4i*)(ks + 32 * u + 16 + 4 * kb);
+            const v4i v2 = *(const v4i*)(vs + 16 * u + 4 * kb);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int f = k4[i];
-              const float y = st[t][i] * __int_as_float(f);
-              top = __builtin_fmaxf(top, 16 * t + i > left ? -INFINITY : y);
+              const int a0 = k0[i], a1 = k1[i], vv = v2[i];
+              const float y0 = __builtin_fmaf(st[2 * u][i], __int_as_float(a0), exponent_of((unsigned)vv));
+              const float y1 = __builtin_fmaf(st[2 * u + 1][i], __int_as_float(a1), exponent_of((unsigned)vv >> 16));
+              top = __builtin_fmaxf(top, __builtin_fmaxf(32 * u + i > left ? -INFINITY : y0, 32 * u + 16 + i > left ? -INFINITY : y1));
             }
           }
           top = __builtin_fmaxf(top, lane_xor_f<16>(top));
           top = __builtin_fmaxf(top, lane_xor_f<32>(top));
-          const float most = wave_max((float)(min(v_raw & 0x7FFFu, 0x7C00u) >> 10));
-          const float now = __builtin_fmaxf(ref, top + (most - 25.0f));
+          const float now = __builtin_fmaxf(ref, reference_for(top));
           const float alpha = __builtin_amdgcn_exp2f(ref - now);
           l *= alpha, weights *= alpha;
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
           ref = now;
         }
-        if (last) weigh(std::true_type{});
-        else weigh(std::false_type{});
-        if (set_reference || __builtin_amdgcn_ballot_w64(!(added < INFINITY)) == 0) break;
+        if (last) weigh(std::true_type{}, std::false_type{});
+        else weigh(std::false_type{}, std::false_type{});
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(added < INFINITY)) == 0, 1)) break;
+        if (set_reference) {                              // (scores of 10^8, or NaN)
+          weigh(std::true_type{}, std::true_type{});
+          break;
+        }
         set_reference = true;
       }
       set_reference = false;

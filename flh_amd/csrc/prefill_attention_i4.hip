@@ -117,9 +117,10 @@ struct Layout {
   static constexpr int kBytes = kWaves * kWave;
 };
 
-// KW: waves that share 32 rows and take every fourth tile (4), or waves with rows of their own (1)
+// KW: waves that share 32 rows and take every fourth tile (4), or waves with rows of their own (1).  Heads of 64: three waves a SIMD where they need 168
+// registers (1111 rows behind 600 slots, 16 / 4 heads: 34 us; 38 at the 172 that two leave room for).
 template <int D, int KW>
-__global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(Prefill a) {
   using L = Layout<D>;
   extern __shared__ __align__(1024) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
     // the scales for all queries at once: keys' as the scores take them, values' in pairs of keys 8 apart, as the weights are packed
     const unsigned k_raw = ks[lane], v_raw = vs[lane];
     ks[lane] = __builtin_bit_cast(unsigned, low_half(k_raw) * factor);
-    ((unsigned short*)vs)[2 * (lane >> 4) * 8 + 2 * (lane & 7) + ((lane >> 3) & 1)] = (unsigned short)v_raw;
+    ((packed_u16*)vs)[2 * (lane >> 4) * 8 + 2 * (lane & 7) + ((lane >> 3) & 1)] = (unsigned short)v_raw;
 #pragma unroll
     for (int j = 0; j < kSteps; ++j)
 #pragma unroll
@@ -251,8 +252,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
     // ---- probabilities, then weights, in pairs (r, r + 4) as the codes' halves come: p[i][u] is slots 16 u .. of tile i
     h8 p[2][2];
     float sum, added;
-    auto weigh = [&](auto masked_) __attribute__((always_inline)) {
-      constexpr bool MASKED = decltype(masked_)::value;
+    auto weigh = [&](auto masked_, auto bounded_) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_)::value, BOUNDED = decltype(bounded_)::value;
       sum = added = 0.f;
       const int from = opaque(key0);
 #pragma unroll
@@ -264,8 +265,10 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int a0 = k0[e], a1 = k1[e], vv = v2[e];
-            float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][8 * u + e], __int_as_float(a0), -ref));
-            float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][8 * u + 4 + e], __int_as_float(a1), -ref));
+            float p0 = __builtin_fmaf(st[i][8 * u + e], __int_as_float(a0), -ref);
+            float p1 = __builtin_fmaf(st[i][8 * u + 4 + e], __int_as_float(a1), -ref);
+            if constexpr (BOUNDED) p0 = bounded(p0, (unsigned)vv), p1 = bounded(p1, (unsigned)vv >> 16);
+            p0 = __builtin_amdgcn_exp2f(p0), p1 = __builtin_amdgcn_exp2f(p1);
             h2 w2 = pair_times_halves(p0, (unsigned)vv & 0xFFFFu, p1, (unsigned)vv >> 16);
             if constexpr (MASKED) {                    // (a value that a query does not see may be NaN)
               const int at = from + 32 * i + 16 * u + e;
@@ -278,7 +281,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
           }
         }
     };
-    // A reference that holds the largest weight back, p vs < 2^11 when it is set, in the first tile and again where a weight leaves fp16's range, which
+    // A reference that holds the largest weight back, p vs < 2^12 when it is set, in the first tile and again where a weight leaves fp16's range, which
     // few tiles' do.  Of the keys that the query sees alone: what it does not see may be NaN or as large as it likes.
     for (;;) {
       if (set_reference) {
@@ -293,22 +296,26 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_i4_kernel(Prefill a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int a0 = k0[e], a1 = k1[e], vv = v2[e], at = from + 32 * i + 16 * u + e;
-              const float y0 = __builtin_fmaf(st[i][8 * u + e], __int_as_float(a0), (float)((vv >> 10) & 31));
-              const float y1 = __builtin_fmaf(st[i][8 * u + 4 + e], __int_as_float(a1), (float)((vv >> 26) & 31));
+              const float y0 = __builtin_fmaf(st[i][8 * u + e], __int_as_float(a0), exponent_of((unsigned)vv));
+              const float y1 = __builtin_fmaf(st[i][8 * u + 4 + e], __int_as_float(a1), exponent_of((unsigned)vv >> 16));
               top = __builtin_fmaxf(top, __builtin_fmaxf(at > limit ? -INFINITY : y0, at + 8 > limit ? -INFINITY : y1));
             }
           }
         top = __builtin_fmaxf(top, lane_xor_f<32>(top));
-        const float now = __builtin_fmaxf(ref, top - 25.0f);
+        const float now = __builtin_fmaxf(ref, reference_for(top));
         const float alpha = __builtin_amdgcn_exp2f(ref - now);
         l *= alpha, weights *= alpha;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
         ref = now;
       }
-      if (tile >= whole) weigh(std::true_type{});
-      else weigh(std::false_type{});
-      if (set_reference || __builtin_amdgcn_ballot_w64(!(added < INFINITY)) == 0) break;
+      if (tile >= whole) weigh(std::true_type{}, std::false_type{});
+      else weigh(std::false_type{}, std::false_type{});
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(added < INFINITY)) == 0, 1)) break;
+      if (set_reference) {                              // (scores of 10^8, or NaN)
+        weigh(std::true_type{}, std::true_type{});
+        break;
+      }
       set_reference = true;
     }
     set_reference = false;
@@ -438,8 +445,10 @@ __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
   for (int i = 0; i < D / 64; ++i) dst[lane + 64 * i] = (_Float16)(o[i] / l);
 }
 
-// Blocks from which every wave has one of its own
-constexpr uint64_t kOwnRows = 4096;
+// Blocks from which every wave has one of its own: four waves on one block leave no tail and need a joint end, 34 us against 41 for 1024 tokens of a
+// prompt (32 / 8 heads of 128: 1024 blocks) and 360 against 390 for 1000 behind 16000, but 84 against 77 for 2048 tokens, 152 against 127 for 3000,
+// 240 against 207 for 4096 and 142 against 114 for 64 sequences of 64 tokens behind 1000.
+constexpr uint64_t kOwnRows = 2048;
 
 // Parts that a block can have: none where the blocks fill the chip
 uint32_t splits_of(uint64_t B, uint64_t heads, uint32_t max_len) {

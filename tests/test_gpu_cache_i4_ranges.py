@@ -5,7 +5,7 @@ must not count."""
 import pytest
 import torch
 
-from test_gpu_cache_i4 import attend64, check_decode, check_prefill, close, decode_case, normal, prefill_case, random_cache, unpacked
+from test_gpu_cache_i4 import attend64, check_decode, check_prefill, close, decode_case, hadamard64, normal, prefill_case, random_cache, turned, unpacked
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,46 @@ def test_scales_out_of_sight(ops, B, T, Hq, Hkv, big):
             x, tol = attend64(q[0, t, g * rep:(g + 1) * rep], unpacked(cache[0][0, g, :m]), cache[1][0, g, :m], unpacked(cache[2][0, g, :m]),
                               cache[3][0, g, :m], [m] * rep, d ** -0.5)
             close(got[0, t, g * rep:(g + 1) * rep], x, tol, (t, g))
+
+
+def check_huge(got, q, kc, ks, vc, vs, scale):
+    """One query's output where scores are so large that their rounding decides between keys next to the largest: a mean of values, and the value of the
+    key with the largest score where that one is out of all others' reach."""
+    v = vc.double() * vs.double()[:, None]
+    s = (kc.double() @ q.double()) * ks.double() * scale
+    bound = (4 * q.numel() + 32) * 2.0 ** -24 * scale * ((kc.double().abs() + 8) @ q.double().abs() * ks.double()).max() + 60
+    first, second = torch.topk(s, 2).values
+    assert torch.isfinite(got).all() and (got.double().abs() <= v.abs().max() * 1.01).all()
+    if first - second > 2 * bound:                                     # (every other key's probability is below 2^-60)
+        x = v[s.argmax()]
+        assert ((got.double() - x).abs() <= 4 * 2.0 ** -11 * x.abs() + 40 * 2.0 ** -18 * vs[s.argmax()].double()).all()
+        return 1
+    return 0
+
+
+@pytest.mark.parametrize("qscale,key,scale", [(100.0, 1.0, 1e3), (1e4, 100.0, 1.0), (1e4, 1e4, 1.0), (1e4, 1e4, 1e9)])
+def test_huge_scores(ops, qscale, key, scale):
+    gen = torch.Generator().manual_seed(3)
+    T, Hq, Hkv, d, n = 9, 8, 2, 128, 900
+    cache = random_cache(gen, 1, Hkv, n + T, d)
+    cache[1].mul_(key)
+    q = normal(gen, 1, T, Hq, d, scale=qscale)
+    dev = [t.cuda() for t in cache]
+    got = ops.prefill_attention_i4(q.cuda(), torch.tensor([n]).cuda(), *dev, scale=scale).cpu().view(T, Hq, d)
+    sure = 0
+    for t in range(T):
+        for h in range(Hq):
+            g, m = h // (Hq // Hkv), n + t + 1
+            sure += check_huge(got[t, h], q[0, t, h], unpacked(cache[0][0, g, :m]), cache[1][0, g, :m], unpacked(cache[2][0, g, :m]), cache[3][0, g, :m], scale)
+    assert sure > T * Hq // 2
+    one, zero = torch.ones(1, d).half(), torch.zeros(1, d).half()      # no turn; the queries' rotation is undone in front
+    x = (q[:, 0].double() @ hadamard64(d)).half()
+    kn, vn = normal(gen, 1, Hkv, d), normal(gen, 1, Hkv, d)
+    got = ops.decode_attention_rope_i4(*(t.cuda() for t in (x, kn, vn, one, zero, torch.tensor([n]))), *dev, scale=scale).cpu()
+    cache = [t.cpu() for t in dev]
+    y = turned(x, one, zero, torch.float64)
+    sure = 0
+    for h in range(Hq):
+        g, m = h // (Hq // Hkv), n + 1
+        sure += check_huge(got[0, h], y[0, h], unpacked(cache[0][0, g, :m]), cache[1][0, g, :m], unpacked(cache[2][0, g, :m]), cache[3][0, g, :m], scale)
+    assert sure > Hq // 2
