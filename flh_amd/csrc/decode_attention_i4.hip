@@ -425,19 +425,22 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
 }
 
 // n pieces, 4 K of them at a time: their references and sums one a lane, the weighted codes of every fourth one by this wave, all requested at once
+// (what is behind the last one is its again, and taken with no weight: with a way out of the loop between them the loads came one after another, 7.0
+// us in place of 3.9 for 59 pieces of 32 heads)
 template <int D, int K>
-__device__ __forceinline__ void join_pieces(const float* base, size_t stride, uint32_t n, int wave, float (&o)[D / 64], float& l) {
+__device__ __forceinline__ void join_pieces(const float* base, uint32_t n, int wave, float (&o)[D / 64], float& l) {
+  constexpr size_t kStride = (size_t)kCols * (D + 2);
   const int lane = threadIdx.x & 63;
   float m = kLowestRef;
   for (uint32_t s0 = 0; s0 < n; s0 += 4 * K) {
     const bool have = lane < 4 * K && s0 + lane < n;
-    const float* at = base + (size_t)min(s0 + lane, n - 1) * stride + D;
+    const float* at = base + min(s0 + lane, n - 1) * kStride + D;
     const float pm = at[0], pl = at[1];
     float v[K][D / 64];
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) v[k][i] = base[(size_t)min(s0 + wave + 4 * k, n - 1) * stride + lane + 64 * i];
+      for (int i = 0; i < D / 64; ++i) v[k][i] = base[min(s0 + wave + 4 * k, n - 1) * kStride + lane + 64 * i];
     const float now = __builtin_fmaxf(m, wave_max(have ? pm : kLowestRef)), old = __builtin_amdgcn_exp2f(m - now);
     const float w = have ? __builtin_amdgcn_exp2f(pm - now) : 0.f;
     l = l * old + (have ? w * pl : 0.f);
@@ -445,10 +448,9 @@ __device__ __forceinline__ void join_pieces(const float* base, size_t stride, ui
     for (int i = 0; i < D / 64; ++i) o[i] *= old;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (s0 + wave + 4 * k >= n) break;
       const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), wave + 4 * k));
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) o[i] = __builtin_fmaf(wk, v[k][i], o[i]);
+      for (int i = 0; i < D / 64; ++i) o[i] += s0 + wave + 4 * k < n ? wk * v[k][i] : 0.f;
     }
     m = now;
   }
@@ -457,7 +459,6 @@ __device__ __forceinline__ void join_pieces(const float* base, size_t stride, ui
 // one workgroup of four waves per (sequence, query head): every wave its share of the pieces, then the waves' sums in a fixed order
 template <int D>
 __global__ __launch_bounds__(256) void decode_i4_join_kernel(Decode a) {
-  constexpr int kPiece = D + 2;
   __shared__ float sums[4][D];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -470,10 +471,9 @@ __global__ __launch_bounds__(256) void decode_i4_join_kernel(Decode a) {
     // (from the workgroup with its first tile on)
     const uint32_t start = place.before + unit * place.entries;
     const uint32_t g0 = (start + (shares.parts ? 0 : kHeadTiles)) / shares.c, n = (start + place.entries - 1) / shares.c - g0 + 1;
-    const float* base = a.partials + ((size_t)(g0 + (size_t)b * shares.heads + unit) * kCols + h) * kPiece;
-    const size_t stride = (size_t)kCols * kPiece;
-    if (n <= 16) join_pieces<D, 4>(base, stride, n, wave, o, l);
-    else join_pieces<D, 16>(base, stride, n, wave, o, l);
+    const float* base = a.partials + ((size_t)(g0 + (size_t)b * shares.heads + unit) * kCols + h) * (D + 2);
+    if (n <= 16) join_pieces<D, 4>(base, n, wave, o, l);
+    else join_pieces<D, 16>(base, n, wave, o, l);
     l = wave_sum(l);
   }
 #pragma unroll
