@@ -14,7 +14,8 @@ struct Write {
 };
 
 // D / 16 lanes per head vector; item order: all query heads of a token, then its key heads, then its value heads.  A lane holds both pieces
-// of a rotary pair and reads them before it writes either, so q_out may be q.
+// of a rotary pair and reads them before it writes either, so q_out may be q.  Bound by the bytes: 8192 tokens of 32 / 8 heads of 128 read 105 MB and
+// write 76 (queries and codes), 37.5 us = 4.8 TB/s; 21 tokens: 4 us.
 template <int D>
 __global__ __launch_bounds__(256) void rope_quant_kernel(Write a) {
   constexpr uint32_t kLanes = HeadRow<D>::kLanes;
@@ -62,7 +63,8 @@ struct Read {
   uint32_t items, rows, Hkv, max_len;
 };
 
-// y = fp16(H c s / sqrt(D)) for keys, fp16(c s) for values: sums of codes are whole numbers and their product with the scale has 22 bits
+// y = fp16(H c s / sqrt(D)) for keys, fp16(c s) for values: sums of codes are whole numbers and their product with the scale has 22 bits.  Bound by the
+// bytes: 4 x up to 3000 slots of 8 heads of 128: 28 us, 4.4 TB/s of what it reads and writes; 900 slots: 3.7 us.
 template <int D>
 __global__ __launch_bounds__(256) void dequant_kernel(Read a) {
   constexpr uint32_t kLanes = HeadRow<D>::kLanes;

@@ -12,6 +12,13 @@
 // LDS as packed codes (8 KiB) by direct-to-LDS loads, the next one while it is worked on; values are transposed by the LDS load for 4 bits.
 //
 // Few rows: the tiles of a block are split over several workgroups, whose pieces (reference, sum, weighted codes) a second launch joins.
+//
+// What bounds it: many rows, the work around the products.  A tile of 64 keys and 32 queries is 16 + 16 matrix instructions, and 7 vector instructions for
+// eight codes, twice, and about 5 for a probability: 4096 tokens of a prompt, 32 / 8 heads of 128: 184 us, 746 TFLOP/s of the products below the
+// diagonal, the vector units busy in 71 % of the cycles and the matrix units in 32 %; 4096 behind 16000: 1400 us, 870 TFLOP/s, at the clock that the card
+// then holds.  64 rows to a wave, whose codes are unpacked once for both halves, took 1370 us there and 238 for the prompt (one wave a SIMD, and the
+// diagonal's pairs of a long and a short block leave it alone).  Few rows: the start and the end of a workgroup (4 x 17 tokens behind 8000 .. 16000: 39 us,
+// of which the codes' bytes are 11) and the blocks' last rows (68 rows are three blocks).
 #include "cache_i4.h"
 
 namespace flh {
@@ -41,7 +48,9 @@ __device__ __forceinline__ uint32_t tiles_of(const Prefill& a, long long length,
 // one list, and a workgroup takes the entry of its index, parts of a block one after the other, so that a long sequence's lie on all dies.  The same
 // number for every sequence took 59 us for 17 tokens each behind 16000 and three times 200 cached ones (4 sequences, 32 / 8 heads of 128), the list
 // 36; equal lengths lose nothing (4 x 16000: 42 us either way), but where the rounding gives more than kParts (576: 46 us), hence the floor.  A die's
-// entries in one range: 42 us for the ragged batch.  64 sequences lie in the lanes at a time.
+// entries in one range: 42 us for the ragged batch.  256 of them: 72 in place of 62 us (4 x 17 behind 16000, with the joining launch), 1024: 67.  Parts of
+// 4 tiles at least: 34 in place of 27 us for 4 tokens behind 16000; of 16: the same, but 15 in place of 22 us where a cache of 1000 slots is then not
+// split.  64 sequences lie in the lanes at a time.
 constexpr uint32_t kParts = 512, kPartTiles = 8;
 struct Parts {
   uint32_t total, heads, all;                          // entries of the list, blocks of all heads of a sequence, tiles of all of them
@@ -117,8 +126,8 @@ struct Layout {
   static constexpr int kBytes = kWaves * kWave;
 };
 
-// KW: waves that share 32 rows and take every fourth tile (4), or waves with rows of their own (1).  Heads of 64: three waves a SIMD where they need 168
-// registers (1111 rows behind 600 slots, 16 / 4 heads: 34 us; 38 at the 172 that two leave room for).
+// KW: waves that share 32 rows and take every KW-th tile: all four, two, or one with rows of its own.  Heads of 64: three waves a SIMD where they need
+// 168 registers (1111 rows behind 600 slots, 16 / 16 heads: 34 us; 38 at the 172 that two leave room for).
 template <int D, int KW>
 __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(Prefill a) {
   using L = Layout<D>;
@@ -127,27 +136,27 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint8_t* const mine = lds + wave * L::kWave;
   const unsigned mine0 = (unsigned)(size_t)mine;
-  // every die takes a contiguous range of (sequence, key / value head) pairs; within one the long blocks (late queries) come first
-  unsigned w = xcd_contiguous(blockIdx.x, gridDim.x);
+  // The long blocks (late queries) of all heads come first, whatever their number: the launch ends with short ones.  Where the (sequence, key / value
+  // head) pairs are a multiple of the dies, each stays on one.  (A die's pairs one after the other, the last one's long blocks late: 4 x 2048 tokens of
+  // 16 heads of 64 98 us in place of 78, 8 x 2048 of 32 heads of 128 460 in place of 420; nothing was slower this way.)
+  constexpr uint32_t kBlocks = kWaves / KW;            // of a workgroup
   uint32_t split = 0, splits = 1, block, bh;
-  if constexpr (KW == 1) {                             // (one workgroup for four blocks, one piece each)
-    const uint32_t quads = (a.blocks + 3) / 4;
-    bh = w / quads, block = (quads - 1 - w % quads) * 4 + wave;
-    if (block >= a.blocks) return;
-  } else if (a.splits == 1) {
-    block = a.blocks - 1 - w % a.blocks, bh = w / a.blocks;
+  if (KW < 4 || a.splits == 1) {
+    const uint32_t pairs = a.B * a.Hkv;
+    bh = blockIdx.x % pairs, block = ((a.blocks - 1) / kBlocks - blockIdx.x / pairs) * kBlocks + wave / KW;
   } else {
     Parts parts(a);
     if (blockIdx.x >= parts.total) return;
-    w = blockIdx.x;
-    const uint32_t b = parts.at(a, w);
+    const uint32_t b = parts.at(a, blockIdx.x);
     uint32_t start;
     parts.of(a, b, splits, start);
-    const uint32_t at = w - start, unit = at / splits;
+    const uint32_t at = blockIdx.x - start, unit = at / splits;
     split = at % splits, block = unit % a.blocks, bh = b * a.Hkv + unit / a.blocks;
   }
   const uint32_t b = bh / a.Hkv, hkv = bh % a.Hkv;
   const long long len = a.lengths[b];
+  const bool behind = block >= a.blocks;               // (waves without a block; they wait for the others)
+  if (behind) block = a.blocks - 1;
   const uint32_t tiles = tiles_of(a, len, block);
   const uint32_t length = tiles ? (uint32_t)len : 0u;
 
@@ -157,7 +166,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
   const size_t q_at = (((size_t)b * a.T + t) * a.Hq + head) * D;
   const int limit = (int)(length + t);                                 // the last slot that the lane's query sees
   const uint32_t slots = length + (first_row + live_rows - 1) / a.rep + 1;   // slots that any of them sees
-  const uint32_t tile0 = (uint32_t)((uint64_t)tiles * split / splits), tile1 = (uint32_t)((uint64_t)tiles * (split + 1) / splits);
+  const uint32_t tile0 = (uint32_t)((uint64_t)tiles * split / splits), tile1 = behind ? 0 : (uint32_t)((uint64_t)tiles * (split + 1) / splits);
   const uint32_t whole = (length + first_row / a.rep + 1) / kTileKeys;       // tiles that all of them see whole
 
   const v4i k_rows = buffer_of(a.k_codes + (size_t)bh * a.max_len * L::kRowBytes, slots * L::kRowBytes);
@@ -192,7 +201,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) x[j] = *(const h8*)(a.q + q_at + h * (D / 2) + 8 * j);
   asm volatile("" ::: "memory");
-  uint32_t tile = tile0 + (KW == 1 ? 0 : wave);
+  uint32_t tile = tile0 + wave % KW;
   if (tile < tile1) request(tile, 0);
   if (tile + KW < tile1) request(tile + KW, 1);
   h8 qf[kSteps];
@@ -352,6 +361,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
       *(v4f*)(there + n * L::kPitch + 32 * dt + 8 * k + 4 * h) = y;
     }
   if constexpr (KW == 1) {
+    if (behind) return;
     // its own rows: normalised on the way to the output, in whole rows
     if (h == 0) there[kBlockRows * L::kPitch + n] = tiles ? 1.0f / l : 0.f;   // (a sequence that takes no part: zeros)
     wait_lds();
@@ -369,17 +379,19 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
   }
   if (h == 0) there[kBlockRows * L::kPitch + n] = ref, there[kBlockRows * L::kPitch + kBlockRows + n] = l;
   __syncthreads();
+  if (behind) return;
   // a thread: eight channels of a row at a time
   constexpr int kChunks = D / 8;
-  for (uint32_t i = tid; i < live_rows * kChunks; i += kThreads) {
+  const uint8_t* const first_wave = lds + wave / KW * KW * L::kWave;
+  for (uint32_t i = tid % (KW * 64); i < live_rows * kChunks; i += KW * 64) {
     const uint32_t r = i / kChunks, ch = i % kChunks * 8;
-    float m = kLowestRef, wt[kWaves], sum = 0.f;
+    float m = kLowestRef, wt[KW], sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) m = __builtin_fmaxf(m, ((const float*)(lds + k * L::kWave))[kBlockRows * L::kPitch + r]);
+    for (int k = 0; k < KW; ++k) m = __builtin_fmaxf(m, ((const float*)(first_wave + k * L::kWave))[kBlockRows * L::kPitch + r]);
     float y[8] = {};
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-      const float* from = (const float*)(lds + k * L::kWave);
+    for (int k = 0; k < KW; ++k) {
+      const float* from = (const float*)(first_wave + k * L::kWave);
       const float lk = from[kBlockRows * L::kPitch + kBlockRows + r];
       wt[k] = __builtin_amdgcn_exp2f(from[kBlockRows * L::kPitch + r] - m);
       if (lk == 0.f) continue;                         // (a wave without a tile, or one whose keys the query does not see)
@@ -391,8 +403,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
         for (int k4 = 0; k4 < 4; ++k4) y[e + k4] += wt[k] * v[k4];
       }
     }
-    if (splits > 1) {
-      float* piece = a.pieces + (size_t)w * kPieceFloats<D>;
+    if (KW == 4 && splits > 1) {
+      float* piece = a.pieces + (size_t)blockIdx.x * kPieceFloats<D>;
       *(v4f*)(piece + r * D + ch) = v4f{y[0], y[1], y[2], y[3]};
       *(v4f*)(piece + r * D + ch + 4) = v4f{y[4], y[5], y[6], y[7]};
       if (ch == 0) piece[kBlockRows * D + r] = m, piece[kBlockRows * (D + 1) + r] = sum;
@@ -445,10 +457,14 @@ __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
   for (int i = 0; i < D / 64; ++i) dst[lane + 64 * i] = (_Float16)(o[i] / l);
 }
 
-// Blocks from which every wave has one of its own: four waves on one block leave no tail and need a joint end, 34 us against 41 for 1024 tokens of a
-// prompt (32 / 8 heads of 128: 1024 blocks) and 360 against 390 for 1000 behind 16000, but 84 against 77 for 2048 tokens, 152 against 127 for 3000,
-// 240 against 207 for 4096 and 142 against 114 for 64 sequences of 64 tokens behind 1000.
-constexpr uint64_t kOwnRows = 2048;
+// Waves that share a block: all four where the blocks are few (a short tail, but a joint end for each), two from `pairs` blocks on, one from twice as
+// many.  us, four / two / one: heads of 128, 32 / 8 of them, prompts of 512 tokens (512 blocks) 15 / 19 / 25, 1024 34 / 31 / 40, 2048 85 / 76 / 77, 4096
+// 255 / 232 / 220, 64 x 64 tokens behind 1000 (4096) 161 / 138 / 125; heads of 64, 16 / 16 of them, whose tiles are less work: 2 x 1111 behind 600 (1120)
+// 40 / 41 / 47, 4096 (2048) 87 / 83 / 97, 4 x 2048 (4096) 98 / 85 / 78, 4 x 4096 (8192) 295 / 264 / 248.
+uint32_t waves_of(uint64_t blocks, uint32_t head_dim) {
+  const uint64_t pairs = head_dim == 128 ? 1024 : 2048;
+  return blocks < pairs ? 4 : blocks < 2 * pairs ? 2 : 1;
+}
 
 // Parts that a block can have: none where the blocks fill the chip
 uint32_t splits_of(uint64_t B, uint64_t heads, uint32_t max_len) {
@@ -508,23 +524,25 @@ extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* length
   a.k_scales = (const __half*)k_scales, a.v_scales = (const __half*)v_scales, a.out = (__half*)out, a.pieces = (float*)workspace;
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.max_len = max_len, a.rows = T * a.rep, a.blocks = (uint32_t)blocks_of(T, a.rep);
   a.scale_log2 = scale * 1.4426950408889634f;
-  const uint64_t groups = (uint64_t)B * Hkv * a.blocks;
-  a.splits = splits_of(B, (uint64_t)Hkv * a.blocks, max_len);
-  const uint64_t entries = a.splits == 1 ? groups : entries_of(B, (uint64_t)Hkv * a.blocks);
-  auto go = [&](auto kern, auto rows, auto join, size_t smem, LdsGrant& grant, LdsGrant& rows_grant) {
-    if (groups >= kOwnRows) {
-      if (int rc = reserve_lds((const void*)rows, smem, rows_grant, what)) return rc;
-      hipLaunchKernelGGL(rows, dim3((unsigned)((uint64_t)B * Hkv * ((a.blocks + 3) / 4))), dim3(kThreads), smem, (hipStream_t)stream, a);
-      return check_launch(what);
-    }
+  const uint64_t heads = (uint64_t)Hkv * a.blocks, blocks = B * heads;
+  a.splits = splits_of(B, heads, max_len);
+  const uint32_t shared = waves_of(blocks, head_dim), each = kWaves / shared;   // blocks of a workgroup
+  const uint64_t groups = a.splits > 1 ? entries_of(B, heads) : (uint64_t)B * Hkv * ((a.blocks + each - 1) / each);
+  auto go = [&](auto kern, auto join, size_t smem, LdsGrant& grant) {
     if (int rc = reserve_lds((const void*)kern, smem, grant, what)) return rc;
-    hipLaunchKernelGGL(kern, dim3((unsigned)entries), dim3(kThreads), smem, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(kThreads), smem, (hipStream_t)stream, a);
     if (int rc = check_launch(what)) return rc;
     if (a.splits == 1) return FLH_OK;
     hipLaunchKernelGGL(join, dim3((unsigned)(((uint64_t)B * Hkv * a.rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
     return check_launch(what);
   };
-  static LdsGrant grant128, grant64, rows128, rows64;
-  return head_dim == 128 ? go(prefill_i4_kernel<128, 4>, prefill_i4_kernel<128, 1>, prefill_i4_join_kernel<128>, Layout<128>::kBytes, grant128, rows128)
-                         : go(prefill_i4_kernel<64, 4>, prefill_i4_kernel<64, 1>, prefill_i4_join_kernel<64>, Layout<64>::kBytes, grant64, rows64);
+  static LdsGrant grants[2][3];
+  auto form = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    LdsGrant* g = grants[D == 64];
+    return shared == 4   ? go(prefill_i4_kernel<D, 4>, prefill_i4_join_kernel<D>, Layout<D>::kBytes, g[0])
+           : shared == 2 ? go(prefill_i4_kernel<D, 2>, prefill_i4_join_kernel<D>, Layout<D>::kBytes, g[1])
+                         : go(prefill_i4_kernel<D, 1>, prefill_i4_join_kernel<D>, Layout<D>::kBytes, g[2]);
+  };
+  return head_dim == 128 ? form(std::integral_constant<int, 128>{}) : form(std::integral_constant<int, 64>{});
 }

@@ -31,9 +31,24 @@ def test_waves_with_rows_of_their_own(ops, B, T, Hq, Hkv, d, max_len, lengths):
     check_prefill(ops, q, lengths, cache)
 
 
-def test_waves_with_rows_of_their_own_non_finite(ops):
+@pytest.mark.parametrize("B,T,Hq,Hkv,d,max_len,lengths", [
+    (20, 65, 32, 32, 128, 300, [(i * 31) % 237 - 1 for i in range(20)]),         # three blocks of rows: two waves without; one takes no part
+    (13, 33, 40, 40, 128, 200, [(i * 47) % 169 for i in range(13)]),             # pairs that are no multiple of eight
+    (37, 17, 28, 28, 128, 100, [(i * 13) % 90 - 2 for i in range(37)]),          # one block: a pair of waves without, in every workgroup
+    (33, 10, 160, 32, 64, 150, [(i * 29) % 141 for i in range(33)]),             # five queries per head
+    (10, 65, 96, 32, 64, 333, [(i * 71) % 270 - 3 for i in range(10)])])
+def test_waves_in_pairs(ops, B, T, Hq, Hkv, d, max_len, lengths):
+    blocks = B * Hkv * -(-T * (Hq // Hkv) // 32)
+    assert 1024 * (128 // d) <= blocks < 2048 * (128 // d)
+    gen = torch.Generator().manual_seed(T + B)
+    q, cache = prefill_case(gen, B, T, Hq, Hkv, d, max_len, lengths)
+    check_prefill(ops, q, lengths, cache)
+
+
+@pytest.mark.parametrize("B,H,d", [(70, 32, 64), (70, 32, 128), (35, 32, 64), (17, 32, 128), (20, 6, 128)])
+def test_waves_with_rows_of_their_own_non_finite(ops, B, H, d):
     gen = torch.Generator().manual_seed(7)
-    B, T, H, d, n = 70, 33, 32, 64, 50
+    T, n = 33, 50
     q, cache = prefill_case(gen, B, T, H, H, d, 100, [n] * B)
     cache[1][3, 5, n + 20] = float("nan")                              # a key that the queries from the twentieth on see, in one head
     cache[3][9, 0, n + 4] = float("inf")                               # a value
