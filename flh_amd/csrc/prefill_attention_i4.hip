@@ -19,6 +19,9 @@
 // then holds.  64 rows to a wave, whose codes are unpacked once for both halves, took 1370 us there and 238 for the prompt (one wave a SIMD, and the
 // diagonal's pairs of a long and a short block leave it alone).  Few rows: the start and the end of a workgroup (4 x 17 tokens behind 8000 .. 16000: 39 us,
 // of which the codes' bytes are 11) and the blocks' last rows (68 rows are three blocks).
+#include <algorithm>
+#include <type_traits>
+
 #include "cache_i4.h"
 
 namespace flh {
@@ -474,8 +477,8 @@ uint32_t splits_of(uint64_t B, uint64_t heads, uint32_t max_len) {
   if (s > most) s = most;
   return s < 1 ? 1 : (uint32_t)s;
 }
-// entries of the list at most: the parts that kParts workgroups take, and a block's last one each
-uint64_t entries_of(uint64_t B, uint64_t heads) { return kParts + B * heads; }
+// entries of the list at most: `splits` a block, and in all the parts that kParts workgroups take and one a block
+uint64_t entries_of(uint64_t B, uint64_t heads, uint32_t splits) { return std::min<uint64_t>(B * heads * splits, kParts + B * heads); }
 
 uint64_t blocks_of(uint64_t T, uint64_t rep) { return (T * rep + kBlockRows - 1) / kBlockRows; }
 
@@ -493,7 +496,8 @@ using namespace flh;
 extern "C" size_t flh_prefill_attention_i4_workspace_bytes(uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len) {
   if (Hq == 0 || Hkv == 0 || Hq % Hkv || (head_dim != 128 && head_dim != 64) || max_len == 0 || B == 0 || T == 0 || too_large(B, T, Hq, Hkv, max_len)) return 0;
   const uint64_t heads = (uint64_t)Hkv * blocks_of(T, Hq / Hkv);
-  return splits_of(B, heads, max_len) == 1 ? 0 : (size_t)entries_of(B, heads) * kBlockRows * (head_dim + 2) * sizeof(float);
+  const uint32_t splits = splits_of(B, heads, max_len);
+  return splits == 1 ? 0 : (size_t)entries_of(B, heads, splits) * kBlockRows * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* lengths, const uint8_t* k_codes, const flh_half* k_scales,
@@ -527,7 +531,7 @@ extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* length
   const uint64_t heads = (uint64_t)Hkv * a.blocks, blocks = B * heads;
   a.splits = splits_of(B, heads, max_len);
   const uint32_t shared = waves_of(blocks, head_dim), each = kWaves / shared;   // blocks of a workgroup
-  const uint64_t groups = a.splits > 1 ? entries_of(B, heads) : (uint64_t)B * Hkv * ((a.blocks + each - 1) / each);
+  const uint64_t groups = a.splits > 1 ? entries_of(B, heads, a.splits) : (uint64_t)B * Hkv * ((a.blocks + each - 1) / each);
   auto go = [&](auto kern, auto join, size_t smem, LdsGrant& grant) {
     if (int rc = reserve_lds((const void*)kern, smem, grant, what)) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(kThreads), smem, (hipStream_t)stream, a);
