@@ -373,7 +373,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
         }
         if (last) weigh(std::true_type{}, std::false_type{});
         else weigh(std::false_type{}, std::false_type{});
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(added < INFINITY)) == 0, 1)) break;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(__builtin_fabsf(added) < INFINITY)) == 0, 1)) break;
         if (set_reference) {                              // (scores of 10^8, or NaN)
           weigh(std::true_type{}, std::true_type{});
           break;

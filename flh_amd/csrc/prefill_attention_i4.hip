@@ -323,7 +323,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
       }
       if (tile >= whole) weigh(std::true_type{}, std::false_type{});
       else weigh(std::false_type{}, std::false_type{});
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(added < INFINITY)) == 0, 1)) break;
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(__builtin_fabsf(added) < INFINITY)) == 0, 1)) break;
       if (set_reference) {                              // (scores of 10^8, or NaN)
         weigh(std::true_type{}, std::true_type{});
         break;

@@ -107,6 +107,37 @@ def test_tokens_of_growing_scales(ops, B, Hq, Hkv, d, n, keys, values):
     check_decode(ops, case)
 
 
+class Negated:
+    """The operators on caches whose values' scales have the other sign, and their outputs with the other sign.  Everything the tolerance counts is the
+    same size for either sign (the bits differ: the matrix instruction does not round both sides of zero alike)."""
+
+    def __init__(self, ops):
+        self.ops = ops
+
+    def prefill_attention_i4(self, q, lengths, kc, ks, vc, vs):
+        return -self.ops.prefill_attention_i4(q, lengths, kc, ks, vc, -vs)
+
+    def decode_attention_rope_i4(self, *x):
+        vs = -x[9]
+        out = self.ops.decode_attention_rope_i4(*x[:9], vs)
+        x[9].copy_(vs.abs())                                           # (the new token's scale is positive)
+        return -out
+
+
+@pytest.mark.parametrize("values", [26, -26])
+def test_scales_of_either_sign(ops, values):
+    """Values whose scales are negative, large enough that weights leave fp16's range on the way."""
+    gen = torch.Generator().manual_seed(12)
+    B, T, Hq, Hkv, n, d = 2, 20, 8, 2, 700, 128
+    cache = random_cache(gen, B, Hkv, n + T, d)
+    growing(cache, n + T, 0, values)
+    q, lengths = normal(gen, B, T, Hq, d, scale=2.0), [n, n - 40]
+    check_prefill(Negated(ops), q, lengths, cache)
+    case = decode_case(gen, B, Hq, Hkv, d, n + T, lengths)
+    case[2].zero_()                                                    # (the new token's value would count with the other sign)
+    check_decode(Negated(ops), (*case[:6], cache))
+
+
 @pytest.mark.parametrize("big", [60000.0, float("inf"), float("nan")])
 @pytest.mark.parametrize("B,T,Hq,Hkv", [(1, 30, 8, 2), (70, 33, 32, 32)])
 def test_scales_out_of_sight(ops, B, T, Hq, Hkv, big):
