@@ -52,8 +52,8 @@ __device__ __forceinline__ uint32_t tiles_of(const Prefill& a, long long length,
 // number for every sequence took 59 us for 17 tokens each behind 16000 and three times 200 cached ones (4 sequences, 32 / 8 heads of 128), the list
 // 36; equal lengths lose nothing (4 x 16000: 42 us either way), but where the rounding gives more than kParts (576: 46 us), hence the floor.  A die's
 // entries in one range: 42 us for the ragged batch.  256 of them: 72 in place of 62 us (4 x 17 behind 16000, with the joining launch), 1024: 67.  Parts of
-// 4 tiles at least: 34 in place of 27 us for 4 tokens behind 16000; of 16: the same, but 15 in place of 22 us where a cache of 1000 slots is then not
-// split.  64 sequences lie in the lanes at a time.
+// 4 tiles at least: 34 in place of 27 us for 4 tokens behind 16000; 5 behind 4000 take 21.5 us with parts of 8, 23.5 of 16, 29 of 32 tiles (of which the
+// host's two launches are about 20 by themselves).  64 sequences lie in the lanes at a time.
 constexpr uint32_t kParts = 512, kPartTiles = 8;
 struct Parts {
   uint32_t total, heads, all;                          // entries of the list, blocks of all heads of a sequence, tiles of all of them

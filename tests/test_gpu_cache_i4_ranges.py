@@ -75,6 +75,24 @@ def test_ragged_parts(ops, B, T, Hq, Hkv, d, max_len, lengths):
     assert torch.equal(out, ops.prefill_attention_i4(q.cuda(), torch.tensor(lengths).cuda(), *(t.cuda() for t in cache), workspace=ws))
 
 
+def test_parts_on_two_streams(ops):
+    """Calls whose parts are joined by a second launch, on two streams at once, each with its default workspace."""
+    gen = torch.Generator().manual_seed(4)
+    cases = [prefill_case(gen, 3, 9, 32, 8, 128, 3000, lengths) for lengths in ([2990, 100, 1500], [700, 2991, 0])]
+    dev = [(q.cuda(), torch.tensor(n).cuda(), *(t.cuda() for t in cache)) for (q, cache), n in zip(cases, ([2990, 100, 1500], [700, 2991, 0]))]
+    alone = [ops.prefill_attention_i4(*d) for d in dev]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in dev]
+    outs = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(ops.prefill_attention_i4(*dev[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
 def growing(cache, n, keys, values):
     """Scales that change by 2^keys and 2^values over the first n slots."""
     at = torch.arange(n) / max(n - 1, 1)
