@@ -2,9 +2,9 @@
 // t sits in slot lengths[b] + t and sees the slots up to its own.  Queries as the cache's writer leaves them (rotated like the keys), token-major
 // [B, T, Hq, D]; output [B, T, Hq * D].
 //
-// The rows of a key / value head are its T x rep queries, token by token: a workgroup has 32 of them, so that heads that share keys share the
-// work of bringing them, and its four waves take every fourth tile of 64 keys each, by themselves, without a barrier.  Both products run on
-// v_mfma_f32_32x32x16_f16 in transposed form (a lane owns one query):
+// The rows of a key / value head are its T x rep queries, token by token, in blocks of 32, so that heads that share keys share the work of bringing
+// them.  The tiles of 64 keys that a block sees are taken by four, two or one of a workgroup's waves in turn (waves_of), each by itself, without a
+// barrier.  Both products run on v_mfma_f32_32x32x16_f16 in transposed form (a lane owns one query):
 //
 //   S^T[key, query] = sum_d ck[key, d] Q[query, d]      O^T[d, query] += sum_key cv[key, d] (p vs)[query, key]
 //

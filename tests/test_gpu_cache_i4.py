@@ -2,8 +2,8 @@
 bit for bit against the same float32 expression on the CPU, attention against float64 over what the cache holds.
 
 Tolerances count roundings (half a step of fp16 is 2^-11 of a value, of float32 2^-24).  Attention: the result and every probability times its
-value's scale are rounded to fp16: 2^-11 of |out| and of sum p |v|; a weight below the smallest normal fp16 is off by 2^-25, where the largest is between
-2^15 and 2^15 / 64 for value scales within a factor of 64 of each other (odd keys' weights are held as sixteenths): 2^-30 of the largest |v| per key.  A
+value's scale are rounded to fp16: 2^-11 of |out| and of sum p |v|; a weight below the smallest normal fp16 is off by 2^-25, where the
+largest is 2^10 or more when its reference is set: 2^-35 of the largest p vs, times codes of up to 8, counted as 2^-30 of the largest |v| per key.  A
 score is a float32 sum of d products (twice, high and low halves of the query) of the query with codes + 8, less eight times the query's sum: (4 d + 32)
 half steps of scale * sum |q| (|code| + 8) ks, which a probability takes twice (numerator and sum).  The sums of p vs (code + 8), and of p vs 8, which
 is taken off: codes enter the matrix instructions as subnormals of 2^-20, whose products are lined up by the exponent of the smallest normal number, 2^-14, and
