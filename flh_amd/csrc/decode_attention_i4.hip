@@ -123,12 +123,14 @@ struct Layout {
   static constexpr int kLoads = kTile / 1024;                                // direct-to-LDS loads for them
   static constexpr int kStage = 2 * kTile + 2 * kTileKeys * 4;               // K, V, their scales (a dword each)
   static constexpr int kQPitch = D * 2 + 16;                                 // bytes of a query's halves
-  static constexpr int kPiece = D + 2;                                       // floats of a piece and query
+  static constexpr int kPiece = D + 2;                                       // floats of a piece and query, as the joining launch reads them
+  static constexpr int kPitch = D + 4;                                       // .. and in LDS, where four at a time lie on 16 bytes
   static constexpr int kWave = kStages * kStage;
   // the waves' stages; the queries' high and low halves; what their scores begin with; the new row's codes and scales
   static constexpr int kQ = kWaves * kWave, kBias = kQ + 2 * kCols * kQPitch, kNew = kBias + kCols * 4,
                        kBytes = kNew + 2 * kRowBytes + 16;
-  static_assert(kCols * kPiece * 4 <= kWave, "a wave's result takes the place of its stages");
+  static_assert(kCols * kPitch * 4 <= kWave, "a wave's result takes the place of its stages");
+  static_assert(kPitch * 4 % 16 == 0 && kWave % 16 == 0, "rows are stored four floats at a time");
 };
 
 template <int D>
@@ -404,19 +406,19 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       v4f y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[i][e], kFromSubnormal, -8.0f * weights);
-      *(v4f*)(there + col * L::kPiece + 16 * i + 4 * kb) = y;
+      *(v4f*)(there + col * L::kPitch + 16 * i + 4 * kb) = y;
     }
-    if (kb == 0) there[col * L::kPiece + D] = ref, there[col * L::kPiece + D + 1] = l;
+    if (kb == 0) there[col * L::kPitch + D] = ref, there[col * L::kPitch + D + 1] = l;
     __syncthreads();
     float* const piece = a.partials + ((size_t)(blockIdx.x + (size_t)place.b * shares.heads + unit) * kCols) * L::kPiece;
     for (uint32_t i = tid; i < cols * D; i += kThreads) {
       const uint32_t h = i / D, ch = i % D;
       float m = kLowestRef, w[kWaves], sum = 0.f, total = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) m = __builtin_fmaxf(m, ((const float*)(lds + k * L::kWave))[h * L::kPiece + D]);
+      for (int k = 0; k < kWaves; ++k) m = __builtin_fmaxf(m, ((const float*)(lds + k * L::kWave))[h * L::kPitch + D]);
 #pragma unroll
       for (int k = 0; k < kWaves; ++k) {
-        const float* from = (const float*)(lds + k * L::kWave) + h * L::kPiece;
+        const float* from = (const float*)(lds + k * L::kWave) + h * L::kPitch;
         w[k] = first + k < stop ? __builtin_amdgcn_exp2f(from[D] - m) : 0.f;
         total += first + k < stop ? w[k] * from[ch] : 0.f;
         sum += first + k < stop ? w[k] * from[D + 1] : 0.f;
