@@ -268,7 +268,16 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
     v4f o[D / 16];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    // eight times the weights, off the sums (of all keys: a query's are in four lanes)
+    auto take_off = [&]() __attribute__((always_inline)) {
+      float eight = weights + lane_xor_f<16>(weights);
+      eight = -8.0f / kFromSubnormal * (eight + lane_xor_f<32>(eight));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[i] += eight;
+      weights = 0.f;
+    };
     bool set_reference = true;
+    int taken = 0;
     for (int stage = 0; tile < stop; tile += kWaves, stage ^= 1) {
       if (tile + kWaves < stop) {
         wait_lds();                                    // (what was read of the stage before)
@@ -392,20 +401,20 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
           const int w8 = cv[i][u];
           o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(code_halves((unsigned)w8), p[u], o[i], 0, 0, 0);
         }
+      if (++taken == kTakeOff) take_off(), taken = 0;
     }
 
     // ---- the waves' results into one piece
     l += lane_xor_f<16>(l);
     l += lane_xor_f<32>(l);
-    weights += lane_xor_f<16>(weights);
-    weights += lane_xor_f<32>(weights);
+    take_off();
     wait_lds();
     float* const there = (float*)mine;                 // (its own stages: everything asked for has come)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       v4f y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[i][e], kFromSubnormal, -8.0f * weights);
+      for (int e = 0; e < 4; ++e) y[e] = o[i][e] * kFromSubnormal;
       *(v4f*)(there + col * L::kPitch + 16 * i + 4 * kb) = y;
     }
     if (kb == 0) there[col * L::kPitch + D] = ref, there[col * L::kPitch + D + 1] = l;

@@ -227,7 +227,15 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
   const int g = lane >> 4, gi = lane & 15;
   const int key = 8 * (gi >> 2) + 4 * (g >> 1) + (gi & 3);             // the row that the lane addresses in a transpose load
 
+  // eight times the weights, off the sums (of all keys: a query's are in two lanes)
+  auto take_off = [&]() __attribute__((always_inline)) {
+    const float eight = -8.0f / kFromSubnormal * (weights + lane_xor_f<32>(weights));
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] += eight;
+    weights = 0.f;
+  };
   bool set_reference = true;
+  int taken = 0;
   for (int stage = 0; tile < tile1; tile += KW, stage ^= 1) {
     if (tile + KW < tile1) wait_vmcnt<2 * L::kLoads + 2>();
     else wait_vmcnt<0>();
@@ -342,6 +350,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
           const int w8 = cv[i][dt][u];
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(code_halves((unsigned)w8), p[i][u], o[dt], 0, 0, 0);
         }
+    if (++taken == kTakeOff) take_off(), taken = 0;
     if (tile + 2 * KW < tile1) {
       wait_lds();                                      // (what was read of this stage)
       request(tile + 2 * KW, stage);
@@ -350,17 +359,16 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
 
   // ---- the waves' results together
   l += lane_xor_f<32>(l);
-  weights += lane_xor_f<32>(weights);
+  take_off();
   wait_lds();
   float* const there = (float*)mine;                   // (its own stages: everything asked for has come)
-  const float eight = -8.0f * weights;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       v4f y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[dt][4 * k + e], kFromSubnormal, eight);
+      for (int e = 0; e < 4; ++e) y[e] = o[dt][4 * k + e] * kFromSubnormal;
       *(v4f*)(there + n * L::kPitch + 32 * dt + 8 * k + 4 * h) = y;
     }
   if constexpr (KW == 1) {
