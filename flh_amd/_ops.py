@@ -885,7 +885,8 @@ def rope_quantize_kv_cache_(q, k, v, cos, sin, lengths, k_codes, k_scales, v_cod
     [B, T, d] fp16 the rotary rows of the tokens' positions, lengths [B] int64 the slots taken.  Keys are turned by the rotary embedding and
     the orthonormal Hadamard matrix of their head, keys and values quantised row by row (scale fp16(max / 7), codes -8 .. 7) and written to
     the slots lengths[b] .. lengths[b] + T - 1 of k_codes / v_codes [B, Hkv, max_len, d / 2] uint8 and k_scales / v_scales [B, Hkv, max_len]
-    fp16.  -> the queries turned alike, [B, T, Hq, d] (q stays as it was).  A sequence whose length is negative or above max_len - T takes
+    fp16.  -> the queries turned alike, [B, T, Hq, d] (q stays as it was; a channel beyond 65504, which takes a head whose 2-norm is, is
+    infinite).  A sequence whose length is negative or above max_len - T takes
     no part: its cache stays as it was.  d in {64, 128}."""
     _check(q.dim() == 4 and k.dim() == 4, "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected")
     B, T, Hq, d = q.shape

@@ -126,8 +126,8 @@ struct Layout {
   static constexpr int kPiece = D + 2;                                       // floats of a piece and query, as the joining launch reads them
   static constexpr int kPitch = D + 4;                                       // .. and in LDS, where four at a time lie on 16 bytes
   static constexpr int kWave = kStages * kStage;
-  // the waves' stages; the queries' high and low halves; what their scores begin with; the new row's codes and scales
-  static constexpr int kQ = kWaves * kWave, kBias = kQ + 2 * kCols * kQPitch, kNew = kBias + kCols * 4,
+  // the waves' stages; the queries' high and low halves; what their scores begin with, and are multiplied by; the new row's codes and scales
+  static constexpr int kQ = kWaves * kWave, kBias = kQ + 2 * kCols * kQPitch, kUp = kBias + kCols * 4, kNew = kUp + kCols * 4,
                        kBytes = kNew + 2 * kRowBytes + 16;
   static_assert(kCols * kPitch * 4 <= kWave, "a wave's result takes the place of its stages");
   static_assert(kPitch * 4 % 16 == 0 && kWave % 16 == 0, "rows are stored four floats at a time");
@@ -219,8 +219,15 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       row.scale(HeadRow<D>::norm());
     }
     if (r < kCols) {
-      // a query as two fp16 values
-      float sum = 0.f;
+      // a query as two fp16 values, by a power of two below what it is where the rotation has taken it out of their range (sums of D channels
+      // over sqrt(D)): its scores are multiplied by that
+      float sum = 0.f, up = 1.f;
+      const unsigned most = row.top();
+      if (most > 0x477FE000u && most < 0x7F800000u) {  // (65504; and finite)
+        const int e = (int)(most >> 23) - (127 + 14);
+        up = __int_as_float((127 + e) << 23);
+        row.scale(__int_as_float((127 - e) << 23));
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         h8 high, low;
@@ -237,7 +244,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       sum += dpp_f<kDppQuadXor1>(sum);
       sum += dpp_f<kDppQuadXor2>(sum);
       if constexpr (kLanes == 8) sum += dpp_f<kDppRowHalfMirror>(sum);
-      if (chunk == 0) ((float*)(lds + L::kBias))[r] = -8.0f / kFromSubnormal * sum;
+      if (chunk == 0) ((float*)(lds + L::kBias))[r] = -8.0f / kFromSubnormal * sum, ((float*)(lds + L::kUp))[r] = up;
     } else if (is_new) {
       const RowCodes codes = quantise(row);
       uint8_t* there = lds + L::kNew + (is_v ? L::kRowBytes : 0);
@@ -262,6 +269,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
       ql[j] = *(const h8*)(lds + L::kQ + (kCols + col) * L::kQPitch + (kb * kSteps + j) * 16);
     }
     const float bias = ((const float*)(lds + L::kBias))[col], factor = kFromSubnormal * a.scale_log2;
+    const bool any_up = __builtin_amdgcn_ballot_w64(((const float*)(lds + L::kUp))[col] != 1.f) != 0;
     const int key = 16 * (col >> 2) + 4 * kb + (col & 3);   // the row that the lane addresses in a transpose load
 
     float ref = kLowestRef, l = 0.f, weights = 0.f;    // .. and the sum of the weights as the second product takes them
@@ -323,6 +331,11 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i4_kernel(Decode a) {
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], ql[j], st[t], 0, 0, 0);
+      }
+      if (__builtin_expect(any_up, 0)) {
+        const float up = ((const float*)(lds + L::kUp))[col];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) st[t] *= up;
       }
       v2i cv[D / 16];
 #pragma unroll

@@ -517,7 +517,8 @@ int flh_evict_kv_cache(int layers, flh_half* const* k_caches, flh_half* const* v
  * scale is not, is held as scale NaN with codes of zero.
  *
  * T new tokens per sequence: token t of sequence b takes slot lengths[b] + t.  q [B, T, Hq, d], k, v [B, T, Hkv, d] fp16 as projected; cos, sin
- * [B, T, d];  q_out [B, T, Hq, d] = fp16(y) of the queries (may be q itself).  A sequence whose length is negative or above max_len - T takes no
+ * [B, T, d];  q_out [B, T, Hq, d] = fp16(y) of the queries (may be q itself): a channel of y is at most the 2-norm of its head, and one above 65504
+ * is infinite in q_out, which spoils that query's attention (the decode step below holds y in more bits).  A sequence whose length is negative or above max_len - T takes no
  * part: nothing is written to its cache. */
 int flh_rope_quant_kv_cache_i4(const flh_half* q, const flh_half* k, const flh_half* v, const flh_half* cos, const flh_half* sin,
                                const int64_t* lengths, flh_half* q_out, uint8_t* k_codes, flh_half* k_scales, uint8_t* v_codes,
@@ -532,7 +533,7 @@ int flh_dequant_kv_cache_i4(const uint8_t* k_codes, const flh_half* k_scales, co
 
 /* A decode step on it: q [B, Hq, d], k_new, v_new [B, Hkv, d] as projected, cos, sin [B, d]; the new token's key and value go to slot
  * lengths[b] (the bytes of flh_rope_quant_kv_cache_i4), and out [B, Hq, d] is attention over the slots 0 .. lengths[b], the new one as it
- * is held among them.  Hq a multiple of Hkv.  A sequence whose length is negative or above max_len - 1: zeros, its cache untouched.  Softmax
+ * is held among them; every finite query will do, also where y is beyond fp16.  Hq a multiple of Hkv.  A sequence whose length is negative or above max_len - 1: zeros, its cache untouched.  Softmax
  * statistics and sums in float32, probabilities (times their value's scale) rounded to fp16 for the second product.  workspace: 16-byte
  * aligned, contents irrelevant; launches that share one must not overlap. */
 size_t flh_decode_attention_i4_workspace_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len);
