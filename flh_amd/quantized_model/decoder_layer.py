@@ -253,7 +253,7 @@ class QuantizedKVCache:
                         torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(scales, dtype=torch.float16, device=device))
                        for _ in range(layers)]
         self.lengths = torch.zeros(batch, dtype=torch.int64, device=device)
-        self._workspaces = {}               # scratch of the attention kernels, by size: captured graphs keep theirs
+        self._workspaces = {}               # scratch of the attention kernels, by query heads: enough for a step of any length, made with the first one
 
     class _Layer:
         """What a decoder layer takes as `kv_cache` in a step (positions None, cos / sin [B, T, d])."""
@@ -267,10 +267,10 @@ class QuantizedKVCache:
             b, t, hq, d = q.shape
             if t == 1:
                 out = _ops().decode_attention_rope_i4(q.reshape(b, hq, d), k.reshape(b, -1, d), v.reshape(b, -1, d), cos.reshape(b, d),
-                                                      sin.reshape(b, d), owner.lengths, *cache, workspace=owner._workspace(b, t, hq))
+                                                      sin.reshape(b, d), owner.lengths, *cache, workspace=owner._workspace(hq))
                 return out.view(b, 1, hq * d)
             q = _ops().rope_quantize_kv_cache_(q, k, v, cos, sin, owner.lengths, *cache)
-            return _ops().prefill_attention_i4(q, owner.lengths, *cache, workspace=owner._workspace(b, t, hq))
+            return _ops().prefill_attention_i4(q, owner.lengths, *cache, workspace=owner._workspace(hq))
 
     def layer(self, index):
         return QuantizedKVCache._Layer(self, index)
@@ -301,15 +301,20 @@ class QuantizedKVCache:
             static.keys[i], static.values[i] = self.read(i, first, self.max_len)
         return static
 
-    def _workspace(self, batch, t, q_heads):
-        from .. import _lib
-        codes, lib = self.layers[0][0], _lib.load()
-        heads, d = codes.size(1), self.head_dim
-        need = int(lib.flh_decode_attention_i4_workspace_bytes(batch, q_heads, heads, d, self.max_len) if t == 1 else
-                   lib.flh_prefill_attention_i4_workspace_bytes(batch, t, q_heads, heads, d, self.max_len))
-        ws = self._workspaces.get(need)
+    def _workspace(self, q_heads):
+        ws = self._workspaces.get(q_heads)
         if ws is None:
-            ws = self._workspaces[need] = torch.empty(need, dtype=torch.uint8, device=codes.device)
+            from .. import _lib
+            codes, lib = self.layers[0][0], _lib.load()
+            if codes.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the cache has no workspace yet: one eager step before the capture makes it")
+            batch, heads, d = codes.size(0), codes.size(1), self.head_dim
+            rep = max(1, q_heads // heads)
+            # of single tokens, and of blocks of every number of 32 rows (a head's blocks are shared while there are 256 of them at most)
+            most = max(int(lib.flh_prefill_attention_i4_workspace_bytes(batch, -(-(32 * rows + 1) // rep), q_heads, heads, d, self.max_len))
+                       for rows in range(256 // max(1, batch * heads) + 1))
+            most = max(most, int(lib.flh_decode_attention_i4_workspace_bytes(batch, q_heads, heads, d, self.max_len)))
+            ws = self._workspaces[q_heads] = torch.empty(most, dtype=torch.uint8, device=codes.device)
         return ws
 
 
