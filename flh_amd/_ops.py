@@ -859,6 +859,15 @@ def prefill_attention_weights(q, k_cache, v_cache, past, weights, scale=None, wo
     return out
 
 
+def _check_counts(counts, batch, device):
+    """-> the address of a padded batch's counts (none: all tokens count)"""
+    if counts is None:
+        return None
+    _check(counts.is_cuda and counts.dtype == torch.int64 and counts.is_contiguous() and tuple(counts.shape) == (batch,)
+           and counts.device == device, "counts must be a contiguous int64 CUDA tensor [B]")
+    return counts.data_ptr()
+
+
 def _check_halves(device, *tensors):
     for t_ in tensors:
         _check(t_.is_cuda and t_.dtype == torch.float16 and t_.is_contiguous() and t_.device == device,
@@ -880,14 +889,15 @@ def _check_cache_i4(device, batch, d, k_codes, k_scales, v_codes, v_scales):
     return k_codes.size(1), k_codes.size(2)
 
 
-def rope_quantize_kv_cache_(q, k, v, cos, sin, lengths, k_codes, k_scales, v_codes, v_scales):
+def rope_quantize_kv_cache_(q, k, v, cos, sin, lengths, k_codes, k_scales, v_codes, v_scales, counts=None):
     """A block of T new tokens per sequence into a cache held in 4 bits: q [B, T, Hq, d], k / v [B, T, Hkv, d] fp16 as projected, cos / sin
     [B, T, d] fp16 the rotary rows of the tokens' positions, lengths [B] int64 the slots taken.  Keys are turned by the rotary embedding and
     the orthonormal Hadamard matrix of their head, keys and values quantised row by row (scale fp16(max / 7), codes -8 .. 7) and written to
     the slots lengths[b] .. lengths[b] + T - 1 of k_codes / v_codes [B, Hkv, max_len, d / 2] uint8 and k_scales / v_scales [B, Hkv, max_len]
     fp16.  -> the queries turned alike, [B, T, Hq, d] (q stays as it was; a channel beyond 65504, which takes a head whose 2-norm is, is
-    infinite).  A sequence whose length is negative or above max_len - T takes
-    no part: its cache stays as it was.  d in {64, 128}."""
+    infinite).  A sequence whose length is negative or above max_len - T takes no part: its cache stays as it was.  d in {64, 128}.
+    `counts` (int64 [B] on the device): of a padded batch, how many of each sequence's T tokens are its own; the others are not written, and a
+    sequence takes part where its own fit (0 <= counts[b] <= T, 0 <= lengths[b] <= max_len - counts[b])."""
     _check(q.dim() == 4 and k.dim() == 4, "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected")
     B, T, Hq, d = q.shape
     _check_halves(q.device, q, k, v, cos, sin)
@@ -895,11 +905,12 @@ def rope_quantize_kv_cache_(q, k, v, cos, sin, lengths, k_codes, k_scales, v_cod
     _check(k.shape == (B, T, Hkv, d) and v.shape == k.shape, "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected")
     _check(cos.shape == (B, T, d) and sin.shape == (B, T, d), "cos / sin must be [B, T, d]")
     _check_lengths(lengths, B, q.device)
+    own = _check_counts(counts, B, q.device)
     _check(Hq > 0 and max(q.shape) < 2 ** 31, "q must have heads, and less than 2^31 of anything")
     out = torch.empty_like(q)
     if B and T:
-        _run("flh_rope_quant_kv_cache_i4", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-             lengths.data_ptr(), out.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), B, T, Hq,
+        _run("flh_rope_quant_kv_cache_i4_counts", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+             lengths.data_ptr(), own, out.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), B, T, Hq,
              Hkv, d, max_len, _stream(q))
     return out
 
@@ -945,11 +956,12 @@ def decode_attention_rope_i4(q, k_new, v_new, cos, sin, lengths, k_codes, k_scal
     return out
 
 
-def prefill_attention_i4(q, lengths, k_codes, k_scales, v_codes, v_scales, scale=None, workspace=None):
+def prefill_attention_i4(q, lengths, k_codes, k_scales, v_codes, v_scales, scale=None, workspace=None, counts=None):
     """Causal attention of a block of T new tokens per sequence over a cache held in 4 bits that rope_quantize_kv_cache_ has written them
     to: q [B, T, Hq, d] fp16 (its result), lengths [B] int64 the slots taken in front of the block; query t sees the slots
     0 .. lengths[b] + t -> [B, T, Hq * d] fp16.  Hq a multiple of Hkv, d in {64, 128}.  A sequence whose length is negative or above
-    max_len - T: zeros.  `workspace` as in decode_attention (calls with many rows take none)."""
+    max_len - T: zeros.  `workspace` as in decode_attention (calls with many rows take none).  `counts` as in rope_quantize_kv_cache_: zeros
+    behind a sequence's own tokens."""
     _check(q.dim() == 4, "q [B, T, Hq, d] expected")
     B, T, Hq, d = q.shape
     _check_halves(q.device, q)
@@ -957,12 +969,13 @@ def prefill_attention_i4(q, lengths, k_codes, k_scales, v_codes, v_scales, scale
     _check_lengths(lengths, B, q.device)
     _check(Hq > 0 and Hq % Hkv == 0, "Hq must be a multiple of Hkv")
     _check(max(q.shape) < 2 ** 31, "q: problem too large")
+    own = _check_counts(counts, B, q.device)
     out = torch.empty((B, T, Hq * d), dtype=torch.float16, device=q.device)
     if B == 0 or T == 0:
         return out
     need = int(_lib.load().flh_prefill_attention_i4_workspace_bytes(B, T, Hq, Hkv, d, max_len))
     with contextlib.nullcontext() if need == 0 else _attention_workspace(q, need, workspace) as ws:
-        _run("flh_prefill_attention_i4", q.device, q.data_ptr(), lengths.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(),
+        _run("flh_prefill_attention_i4_counts", q.device, q.data_ptr(), lengths.data_ptr(), own, k_codes.data_ptr(), k_scales.data_ptr(),
              v_codes.data_ptr(), v_scales.data_ptr(), out.data_ptr(), B, T, Hq, Hkv, d, max_len,
              float(scale if scale is not None else d ** -0.5), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
              _stream(q))

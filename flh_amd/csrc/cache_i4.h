@@ -173,6 +173,13 @@ __device__ __forceinline__ void halves_to_lds(const v4i& d, unsigned voff, unsig
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ushort %1, %2, 0 offen lds" ::"s"(lds_base), "v"(voff), "s"(d) : "memory", "m0");
 }
 
+// Tokens of a block of T that sequence b takes, all or counts[b] of them, in the slots from its length on: none where they do not fit the cache, or
+// the length or the count is out of range
+__device__ __forceinline__ uint32_t tokens_of(const long long* counts, uint32_t b, uint32_t T, long long length, uint32_t max_len) {
+  const long long n = counts ? counts[b] : (long long)T;
+  return n < 0 || n > (long long)T || length < 0 || length > (long long)max_len - n ? 0u : (uint32_t)n;
+}
+
 // what is made of it here is not made in front of the branch that it is needed behind
 __device__ __forceinline__ int opaque(int v) {
   asm volatile("" : "+v"(v));

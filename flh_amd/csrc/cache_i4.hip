@@ -6,7 +6,7 @@ namespace {
 
 struct Write {
   const __half *q, *k, *v, *cos, *sin;
-  const long long* lengths;
+  const long long *lengths, *counts;                   // (counts: of padded rows; null where all T tokens count)
   __half* q_out;
   uint8_t *k_codes, *v_codes;
   __half *k_scales, *v_scales;
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void rope_quant_kernel(Write a) {
   }
   const RowCodes r = quantise(row);
   const long long first = a.lengths[b];
-  if (first < 0 || first > (long long)a.max_len - a.T) return;
+  if (t >= tokens_of(a.counts, b, a.T, first, a.max_len)) return;
   const size_t at = ((size_t)b * a.Hkv + head) * a.max_len + (size_t)first + t;
   uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + at * (D / 2);
   *(unsigned*)(codes + chunk * 4) = r.lo;
@@ -111,6 +111,14 @@ extern "C" int flh_rope_quant_kv_cache_i4(const flh_half* q, const flh_half* k, 
                                           const int64_t* lengths, flh_half* q_out, uint8_t* k_codes, flh_half* k_scales, uint8_t* v_codes,
                                           flh_half* v_scales, uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim,
                                           uint32_t max_len, void* stream) {
+  return flh_rope_quant_kv_cache_i4_counts(q, k, v, cos, sin, lengths, nullptr, q_out, k_codes, k_scales, v_codes, v_scales, B, T, Hq, Hkv, head_dim,
+                                           max_len, stream);
+}
+
+extern "C" int flh_rope_quant_kv_cache_i4_counts(const flh_half* q, const flh_half* k, const flh_half* v, const flh_half* cos, const flh_half* sin,
+                                                 const int64_t* lengths, const int64_t* counts, flh_half* q_out, uint8_t* k_codes,
+                                                 flh_half* k_scales, uint8_t* v_codes, flh_half* v_scales, uint32_t B, uint32_t T, uint32_t Hq,
+                                                 uint32_t Hkv, uint32_t head_dim, uint32_t max_len, void* stream) {
   const char* what = "rope_quant_kv_cache";
   if (!q || !k || !v || !cos || !sin || !lengths || !q_out || !k_codes || !k_scales || !v_codes || !v_scales)
     return fail(FLH_EINVAL, "%s: null pointer", what);
@@ -125,7 +133,8 @@ extern "C" int flh_rope_quant_kv_cache_i4(const flh_half* q, const flh_half* k, 
   if (slots > 1ull << 40) return fail(FLH_EINVAL, "%s: problem too large", what);
   const struct { const void* at; uint64_t bytes; } out[5] = {{k_codes, slots * (head_dim / 2)}, {k_scales, slots * 2}, {v_codes, slots * (head_dim / 2)},
                                                              {v_scales, slots * 2}, {q_out, queries}},
-      in[6] = {{k, rows}, {v, rows}, {cos, tokens * head_dim * 2}, {sin, tokens * head_dim * 2}, {lengths, (uint64_t)B * 8}, {q, queries}};
+      in[7] = {{k, rows}, {v, rows}, {cos, tokens * head_dim * 2}, {sin, tokens * head_dim * 2}, {lengths, (uint64_t)B * 8}, {q, queries},
+               {counts, counts ? (uint64_t)B * 8 : 0}};
   for (int i = 0; i < 5; ++i) {
     for (int j = 0; j < i; ++j)
       if (overlap(out[i].at, out[i].bytes, out[j].at, out[j].bytes)) return fail(FLH_EINVAL, "%s: two outputs share memory", what);
@@ -133,8 +142,8 @@ extern "C" int flh_rope_quant_kv_cache_i4(const flh_half* q, const flh_half* k, 
       if (overlap(out[i].at, out[i].bytes, x.at, x.bytes) && !(i == 4 && out[i].at == x.at && x.at == (const void*)q))
         return fail(FLH_EINVAL, "%s: an output shares memory with an input", what);
   }
-  Write a = {(const __half*)q, (const __half*)k, (const __half*)v, (const __half*)cos, (const __half*)sin, (const long long*)lengths, (__half*)q_out,
-             k_codes, v_codes, (__half*)k_scales, (__half*)v_scales, (uint32_t)(tokens * heads), T, Hq, Hkv, max_len};
+  Write a = {(const __half*)q, (const __half*)k, (const __half*)v, (const __half*)cos, (const __half*)sin, (const long long*)lengths, (const long long*)counts,
+             (__half*)q_out, k_codes, v_codes, (__half*)k_scales, (__half*)v_scales, (uint32_t)(tokens * heads), T, Hq, Hkv, max_len};
   const unsigned groups = (unsigned)((tokens * heads * (head_dim / 16) + 255) / 256);
   if (head_dim == 128) hipLaunchKernelGGL(rope_quant_kernel<128>, dim3(groups), dim3(256), 0, (hipStream_t)stream, a);
   else hipLaunchKernelGGL(rope_quant_kernel<64>, dim3(groups), dim3(256), 0, (hipStream_t)stream, a);

@@ -31,7 +31,7 @@ constexpr int kThreads = 256, kWaves = 4, kBlockRows = 32, kStages = 2;
 
 struct Prefill {
   const __half* q;
-  const long long* lengths;
+  const long long *lengths, *counts;                                        // (counts: of padded rows; null where all T tokens count)
   const uint8_t *k_codes, *v_codes;
   const __half *k_scales, *v_scales;
   __half* out;
@@ -40,10 +40,10 @@ struct Prefill {
   float scale_log2;
 };
 
-// tiles with a slot that a query of the block sees (none: the sequence takes no part)
-__device__ __forceinline__ uint32_t tiles_of(const Prefill& a, long long length, uint32_t block) {
-  if (length < 0 || length > (long long)a.max_len - (long long)a.T) return 0;
-  return ((uint32_t)length + (min((block + 1) * kBlockRows, a.rows) - 1) / a.rep) / kTileKeys + 1;
+// tiles with a slot that a query of the block sees, of a sequence of which `count` tokens count (none: it takes no part, or none of them is in the block)
+__device__ __forceinline__ uint32_t tiles_of(const Prefill& a, long long length, uint32_t count, uint32_t block) {
+  if (block * kBlockRows / a.rep >= count) return 0;
+  return ((uint32_t)length + min((min((block + 1) * kBlockRows, a.rows) - 1) / a.rep, count - 1)) / kTileKeys + 1;
 }
 
 // How few rows are shared: a block's tiles go in equal parts over several workgroups, as many as its share of the tiles of all gets it of kParts (two
@@ -59,7 +59,12 @@ struct Parts {
   uint32_t total, heads, all;                          // entries of the list, blocks of all heads of a sequence, tiles of all of them
   uint32_t entries, up, first, before;                 // of the 64 sequences last looked at
 
-  __device__ __forceinline__ uint32_t longest(const Prefill& a, uint32_t b) const { return b < a.B ? tiles_of(a, a.lengths[b], a.blocks - 1) : 0u; }
+  __device__ __forceinline__ uint32_t longest(const Prefill& a, uint32_t b) const {
+    if (b >= a.B) return 0;
+    const long long length = a.lengths[b];
+    const uint32_t count = tokens_of(a.counts, b, a.T, length, a.max_len);
+    return count ? ((uint32_t)length + count - 1) / kTileKeys + 1 : 0;
+  }
   __device__ __forceinline__ void look(const Prefill& a, uint32_t b0, uint32_t tiles) {
     // (a sequence that takes no part has its zeros to write: one entry a block)
     entries = b0 + (threadIdx.x & 63) < a.B ? max(1u, min(min(a.splits, (tiles + kPartTiles - 1) / kPartTiles), tiles * kParts / all)) : 0u;
@@ -160,15 +165,16 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
   const long long len = a.lengths[b];
   const bool behind = block >= a.blocks;               // (waves without a block; they wait for the others)
   if (behind) block = a.blocks - 1;
-  const uint32_t tiles = tiles_of(a, len, block);
+  const uint32_t count = tokens_of(a.counts, b, a.T, len, a.max_len), tiles = tiles_of(a, len, count, block);
   const uint32_t length = tiles ? (uint32_t)len : 0u;
 
   const uint32_t first_row = block * kBlockRows, live_rows = min((uint32_t)kBlockRows, a.rows - first_row);
   const uint32_t row = first_row + min((uint32_t)n, live_rows - 1);    // (rows past the end repeat the last one; never stored)
   const uint32_t t = row / a.rep, head = hkv * a.rep + row % a.rep;
   const size_t q_at = (((size_t)b * a.T + t) * a.Hq + head) * D;
-  const int limit = (int)(length + t);                                 // the last slot that the lane's query sees
-  const uint32_t slots = length + (first_row + live_rows - 1) / a.rep + 1;   // slots that any of them sees
+  // the last slot that the lane's query sees (rows behind those that count see what the last of these does, and are stored as zeros)
+  const int limit = (int)(length + min(t, count - 1));
+  const uint32_t slots = length + min((first_row + live_rows - 1) / a.rep, count - 1) + 1;   // slots that any of them sees
   const uint32_t tile0 = (uint32_t)((uint64_t)tiles * split / splits), tile1 = behind ? 0 : (uint32_t)((uint64_t)tiles * (split + 1) / splits);
   const uint32_t whole = (length + first_row / a.rep + 1) / kTileKeys;       // tiles that all of them see whole
 
@@ -381,9 +387,11 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
     for (uint32_t i = lane; i < live_rows * kChunks; i += 64) {
       const uint32_t r = i / kChunks, ch = i % kChunks * 8, at = first_row + r;
       const float inv = there[kBlockRows * L::kPitch + r];
+      const bool counts = at / a.rep < count;
       h8 z;
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = (_Float16)(there[r * L::kPitch + ch + e] * inv);
+      if (!counts) z = h8{};
       *(h8*)(a.out + (((size_t)b * a.T + at / a.rep) * a.Hq + hkv * a.rep + at % a.rep) * D + ch) = z;
     }
     return;
@@ -421,10 +429,12 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prefill_i4_kernel(P
       if (ch == 0) piece[kBlockRows * D + r] = m, piece[kBlockRows * (D + 1) + r] = sum;
     } else {
       const float inv = tiles ? 1.0f / sum : 0.f;      // (a sequence that takes no part: zeros)
+      const uint32_t at = first_row + r;
+      const bool counts = at / a.rep < count;
       h8 z;
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = (_Float16)(y[e] * inv);
-      const uint32_t at = first_row + r;
+      if (!counts) z = h8{};
       *(h8*)(a.out + (((size_t)b * a.T + at / a.rep) * a.Hq + hkv * a.rep + at % a.rep) * D + ch) = z;
     }
   }
@@ -438,6 +448,7 @@ __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
   if (item >= a.B * a.Hkv * a.rows) return;
   const uint32_t bh = item / a.rows, row = item % a.rows, b = bh / a.Hkv, hkv = bh % a.Hkv;
   const uint32_t block = row / kBlockRows, r = row % kBlockRows;
+  const bool counts = row / a.rep < tokens_of(a.counts, b, a.T, a.lengths[b], a.max_len);
   Parts parts(a);
   uint32_t splits, start;
   parts.of(a, b, splits, start);
@@ -465,7 +476,7 @@ __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
   }
   _Float16* dst = (_Float16*)(a.out + (((size_t)b * a.T + row / a.rep) * a.Hq + hkv * a.rep + row % a.rep) * D);
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) dst[lane + 64 * i] = (_Float16)(o[i] / l);
+  for (int i = 0; i < D / 64; ++i) dst[lane + 64 * i] = (_Float16)(counts ? o[i] / l : 0.f);
 }
 
 // Waves that share a block: all four where the blocks are few (a short tail, but a joint end for each), two from `pairs` blocks on, one from twice as
@@ -512,6 +523,14 @@ extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* length
                                         const uint8_t* v_codes, const flh_half* v_scales, flh_half* out, uint32_t B, uint32_t T, uint32_t Hq,
                                         uint32_t Hkv, uint32_t head_dim, uint32_t max_len, float scale, void* workspace,
                                         size_t workspace_bytes, void* stream) {
+  return flh_prefill_attention_i4_counts(q, lengths, nullptr, k_codes, k_scales, v_codes, v_scales, out, B, T, Hq, Hkv, head_dim, max_len, scale,
+                                         workspace, workspace_bytes, stream);
+}
+
+extern "C" int flh_prefill_attention_i4_counts(const flh_half* q, const int64_t* lengths, const int64_t* counts, const uint8_t* k_codes,
+                                               const flh_half* k_scales, const uint8_t* v_codes, const flh_half* v_scales, flh_half* out, uint32_t B,
+                                               uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len, float scale,
+                                               void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "prefill_attention (4-bit cache)";
   if (!q || !lengths || !k_codes || !k_scales || !v_codes || !v_scales || !out) return fail(FLH_EINVAL, "%s: null pointer", what);
   if (misaligned16(q, k_codes, v_codes, out)) return fail(FLH_EINVAL, "%s: tensors must be 16-byte aligned", what);
@@ -525,14 +544,15 @@ extern "C" int flh_prefill_attention_i4(const flh_half* q, const int64_t* length
   const size_t need = flh_prefill_attention_i4_workspace_bytes(B, T, Hq, Hkv, head_dim, max_len);
   if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
     return fail(FLH_EINVAL, "%s: a 16-byte aligned workspace of %zu bytes is required", what, need);
-  const struct { const void* at; uint64_t bytes; } in[6] = {{k_codes, slots * (head_dim / 2)}, {k_scales, slots * 2}, {v_codes, slots * (head_dim / 2)},
-                                                            {v_scales, slots * 2}, {lengths, (uint64_t)B * 8}, {q, queries}};
+  const struct { const void* at; uint64_t bytes; } in[7] = {{k_codes, slots * (head_dim / 2)}, {k_scales, slots * 2}, {v_codes, slots * (head_dim / 2)},
+                                                            {v_scales, slots * 2}, {lengths, (uint64_t)B * 8}, {q, queries},
+                                                            {counts, counts ? (uint64_t)B * 8 : 0}};
   for (const auto& x : in)
     if (overlap(out, queries, x.at, x.bytes) || overlap(workspace, need, x.at, x.bytes))
       return fail(FLH_EINVAL, "%s: an output shares memory with an input", what);
   if (overlap(out, queries, workspace, need)) return fail(FLH_EINVAL, "%s: the output shares memory with the workspace", what);
   Prefill a = {};
-  a.q = (const __half*)q, a.lengths = (const long long*)lengths, a.k_codes = k_codes, a.v_codes = v_codes;
+  a.q = (const __half*)q, a.lengths = (const long long*)lengths, a.counts = (const long long*)counts, a.k_codes = k_codes, a.v_codes = v_codes;
   a.k_scales = (const __half*)k_scales, a.v_scales = (const __half*)v_scales, a.out = (__half*)out, a.pieces = (float*)workspace;
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.max_len = max_len, a.rows = T * a.rep, a.blocks = (uint32_t)blocks_of(T, a.rep);
   a.scale_log2 = scale * 1.4426950408889634f;

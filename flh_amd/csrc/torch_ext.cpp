@@ -278,6 +278,14 @@ void check_halves(const c10::Device& device, std::initializer_list<const Tensor*
                 "tensors must be contiguous float16 CUDA tensors on one device");
 }
 
+const int64_t* check_counts(const c10::optional<Tensor>& counts, int64_t batch, const c10::Device& device) {
+  if (!counts.has_value()) return nullptr;
+  TORCH_CHECK(counts->is_cuda() && counts->scalar_type() == torch::kInt64 && counts->is_contiguous() && counts->dim() == 1 &&
+                  counts->size(0) == batch && counts->device() == device,
+              "counts must be a contiguous int64 CUDA tensor [B]");
+  return counts->data_ptr<int64_t>();
+}
+
 int64_t largest(const Tensor& t) {
   int64_t m = 0;
   for (int64_t n : t.sizes()) m = std::max(m, n);
@@ -305,7 +313,7 @@ struct CacheI4 {   // a layer's cache and its sizes
 };
 
 Tensor rope_quantize_kv_cache_(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos, const Tensor& sin, const Tensor& lengths,
-                               Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales) {
+                               Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, const c10::optional<Tensor>& counts) {
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4, "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected");
   const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), d = q.size(3);
   check_halves(q.device(), {&q, &k, &v, &cos, &sin});
@@ -314,12 +322,13 @@ Tensor rope_quantize_kv_cache_(const Tensor& q, const Tensor& k, const Tensor& v
   TORCH_CHECK(k.sizes() == at::IntArrayRef(rows) && v.sizes() == k.sizes(), "q [B, T, Hq, d] and k, v [B, T, Hkv, d] expected");
   TORCH_CHECK(cos.sizes() == at::IntArrayRef(rotary) && sin.sizes() == cos.sizes(), "cos / sin must be [B, T, d]");
   check_lengths(lengths, B, q.device());
+  const int64_t* own = check_counts(counts, B, q.device());
   TORCH_CHECK(Hq > 0 && largest(q) < (1ll << 31), "q must have heads, and less than 2^31 of anything");
   Tensor out = torch::empty_like(q);
   if (B == 0 || T == 0) return out;
   Launch l(q);
-  ok(flh_rope_quant_kv_cache_i4(h(q), h(k), h(v), h(cos), h(sin), lengths.data_ptr<int64_t>(), hm(out), c.k_codes, c.k_scales, c.v_codes,
-                                c.v_scales, B, T, Hq, c.Hkv, d, c.max_len, stream_of(q)));
+  ok(flh_rope_quant_kv_cache_i4_counts(h(q), h(k), h(v), h(cos), h(sin), lengths.data_ptr<int64_t>(), own, hm(out), c.k_codes, c.k_scales,
+                                       c.v_codes, c.v_scales, B, T, Hq, c.Hkv, d, c.max_len, stream_of(q)));
   return out;
 }
 
@@ -360,7 +369,8 @@ Tensor decode_attention_rope_i4(const Tensor& q, const Tensor& k_new, const Tens
 }
 
 Tensor prefill_attention_i4(const Tensor& q, const Tensor& lengths, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes,
-                            const Tensor& v_scales, const c10::optional<double>& scale, const c10::optional<Tensor>& workspace) {
+                            const Tensor& v_scales, const c10::optional<double>& scale, const c10::optional<Tensor>& workspace,
+                            const c10::optional<Tensor>& counts) {
   TORCH_CHECK(q.dim() == 4, "q [B, T, Hq, d] expected");
   const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), d = q.size(3);
   check_halves(q.device(), {&q});
@@ -368,14 +378,16 @@ Tensor prefill_attention_i4(const Tensor& q, const Tensor& lengths, const Tensor
   check_lengths(lengths, B, q.device());
   TORCH_CHECK(Hq > 0 && Hq % c.Hkv == 0, "Hq must be a multiple of Hkv");
   TORCH_CHECK(largest(q) < (1ll << 31), "q: problem too large");
+  const int64_t* own = check_counts(counts, B, q.device());
   Tensor out = torch::empty({B, T, Hq * d}, q.options());
   if (B == 0 || T == 0) return out;
   Launch l(q);
   const size_t need = flh_prefill_attention_i4_workspace_bytes(B, T, Hq, c.Hkv, d, c.max_len);
   Tensor ws;
   if (need) ws = attention_workspace(q, workspace, need);
-  ok(flh_prefill_attention_i4(h(q), lengths.data_ptr<int64_t>(), c.k_codes, c.k_scales, c.v_codes, c.v_scales, hm(out), B, T, Hq, c.Hkv, d,
-                              c.max_len, scale_of(scale, d), need ? ws.data_ptr() : nullptr, need ? ws.numel() : 0, stream_of(q)));
+  ok(flh_prefill_attention_i4_counts(h(q), lengths.data_ptr<int64_t>(), own, c.k_codes, c.k_scales, c.v_codes, c.v_scales, hm(out), B, T, Hq,
+                                     c.Hkv, d, c.max_len, scale_of(scale, d), need ? ws.data_ptr() : nullptr, need ? ws.numel() : 0,
+                                     stream_of(q)));
   return out;
 }
 
@@ -1323,14 +1335,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prefill_attention_weights", &prefill_attention_weights, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("past"),
         py::arg("weights"), py::arg("scale") = py::none(), py::arg("workspace") = py::none());
   m.def("rope_quantize_kv_cache_", &rope_quantize_kv_cache_, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cos"), py::arg("sin"),
-        py::arg("lengths"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"));
+        py::arg("lengths"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("counts") = py::none());
   m.def("dequantize_kv_cache", &dequantize_kv_cache, py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"),
         py::arg("first"), py::arg("rows"));
   m.def("decode_attention_rope_i4", &decode_attention_rope_i4, py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("cos"), py::arg("sin"),
         py::arg("lengths"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("scale") = py::none(),
         py::arg("workspace") = py::none());
   m.def("prefill_attention_i4", &prefill_attention_i4, py::arg("q"), py::arg("lengths"), py::arg("k_codes"), py::arg("k_scales"),
-        py::arg("v_codes"), py::arg("v_scales"), py::arg("scale") = py::none(), py::arg("workspace") = py::none());
+        py::arg("v_codes"), py::arg("v_scales"), py::arg("scale") = py::none(), py::arg("workspace") = py::none(), py::arg("counts") = py::none());
   m.def("tree_commit_", &tree_commit_);
   m.def("evict_kv_cache_", &evict_kv_cache_);
   m.def("rotate_quantize_gemm_i4", &rotate_quantize_gemm_i4, py::arg("x"), py::arg("B"), py::arg("B_scale"));

@@ -240,7 +240,9 @@ class QuantizedKVCache:
 
     Sequences have lengths of their own, `lengths` (device int64 [batch], zeros at first): a step over T tokens takes the slots
     lengths .. lengths + T - 1 of every sequence, and `advance` moves the lengths behind it.  Attention reads what the cache holds, the step's own
-    tokens included: a prompt may come in one block, in several, or token by token.  A captured step serves every length.  A sequence whose length is negative, or above max_len - T, takes no part in a step."""
+    tokens included: a prompt may come in one block, in several, or token by token.  A captured step serves every length.  A sequence whose length is
+    negative, or above max_len - T, takes no part in a step.  In a batch of padded rows `counts` (device int64 [batch], 0 .. T) says how many of
+    each sequence's tokens are its own: the others are not written, and a sequence takes part where its own fit (length up to max_len - counts)."""
 
     max_positions = None                    # (the rotary table has max_len rows)
 
@@ -258,22 +260,28 @@ class QuantizedKVCache:
     class _Layer:
         """What a decoder layer takes as `kv_cache` in a step (positions None, cos / sin [B, T, d])."""
 
-        def __init__(self, owner, index):
-            self.owner, self.index = owner, index
+        def __init__(self, owner, index, counts, lengths):
+            self.owner, self.index, self.counts, self.lengths = owner, index, counts, lengths
 
         def attend(self, q, k, v, cos, sin):
             """q [B, T, Hq, d], k / v [B, T, Hkv, d] of the new tokens as projected, cos / sin [B, T, d] -> [B, T, Hq * d]"""
             owner, cache = self.owner, self.owner.layers[self.index]
             b, t, hq, d = q.shape
             if t == 1:
+                lengths = owner.step_lengths(t, self.counts) if self.lengths is None else self.lengths
                 out = _ops().decode_attention_rope_i4(q.reshape(b, hq, d), k.reshape(b, -1, d), v.reshape(b, -1, d), cos.reshape(b, d),
-                                                      sin.reshape(b, d), owner.lengths, *cache, workspace=owner._workspace(hq))
+                                                      sin.reshape(b, d), lengths, *cache, workspace=owner._workspace(hq))
                 return out.view(b, 1, hq * d)
-            q = _ops().rope_quantize_kv_cache_(q, k, v, cos, sin, owner.lengths, *cache)
-            return _ops().prefill_attention_i4(q, owner.lengths, *cache, workspace=owner._workspace(hq))
+            q = _ops().rope_quantize_kv_cache_(q, k, v, cos, sin, owner.lengths, *cache, counts=self.counts)
+            return _ops().prefill_attention_i4(q, owner.lengths, *cache, workspace=owner._workspace(hq), counts=self.counts)
 
-    def layer(self, index):
-        return QuantizedKVCache._Layer(self, index)
+    def layer(self, index, counts=None, lengths=None):
+        """What a decoder layer takes as `kv_cache` in a step; `lengths`: step_lengths(T, counts), if the caller has it for all layers."""
+        return QuantizedKVCache._Layer(self, index, counts, lengths)
+
+    def step_lengths(self, t, counts=None):
+        """`lengths` in a step over t tokens: of single tokens, -1 where the sequence's is padding (the kernel has no counts)."""
+        return self.lengths if counts is None or t > 1 else torch.where(counts == 1, self.lengths, -1)
 
     def next_positions(self):
         """The position behind each sequence: its next token's."""
@@ -281,9 +289,13 @@ class QuantizedKVCache:
 
     def advance(self, t, counts=None):
         """Move the lengths of the sequences that took part in a step over `t` tokens, by t or by `counts` (device int64 [batch], at most t: in a
-        batch of padded rows the tokens that count; what the others have left behind the lengths is overwritten by the next step)."""
-        takes_part = (self.lengths >= 0) & (self.lengths <= self.max_len - t)
-        self.lengths.add_(takes_part * (t if counts is None else counts))
+        batch of padded rows the tokens that count)."""
+        if counts is None:
+            takes_part = (self.lengths >= 0) & (self.lengths <= self.max_len - t)
+            self.lengths.add_(takes_part * t)
+        else:
+            takes_part = (self.lengths >= 0) & (self.lengths <= self.max_len - counts) & (counts >= 0) & (counts <= t)
+            self.lengths.add_(takes_part * counts)
 
     def read(self, index, first, rows):
         """Slots first[b] .. first[b] + rows - 1 of layer `index` as fp16 (keys, values) [batch, kv_heads, rows, head_dim], as dequantize_kv_cache."""

@@ -344,8 +344,9 @@ class W4A4LlamaModel(torch.nn.Module):
 
     def append(self, input_ids, cache, counts=None, return_hidden=False):
         """One step on a QuantizedKVCache: input_ids [B, T] int64 behind what the cache holds of each sequence -> logits [B, T, vocab] fp16
-        (or the final hidden state); the lengths move on by T, or by `counts` (device int64 [B]: of padded rows, the tokens that count; the
-        other rows' logits mean nothing).  A sequence that takes no part keeps its length.  Can be captured into a graph after one eager
+        (or the final hidden state); the lengths move on by T, or by `counts` (device int64 [B]: of padded rows, the tokens that count, 0 .. T;
+        the other rows' logits mean nothing).  A sequence whose tokens (those that count) do not fit the cache, or whose length is negative,
+        takes no part: it keeps its length, and its logits mean nothing.  Can be captured into a graph after one eager
         step over as many tokens: it serves every length, and every replay moves the lengths."""
         b, t = input_ids.shape
         if not isinstance(cache, QuantizedKVCache):
@@ -356,13 +357,14 @@ class W4A4LlamaModel(torch.nn.Module):
             raise ValueError(f"{t} tokens for a cache of {cache.max_len} slots")
         if counts is not None and (counts.shape != cache.lengths.shape or counts.dtype != torch.int64 or counts.device != cache.lengths.device):
             raise ValueError("counts must be int64 [B] on the cache's device")
+        counts = None if counts is None else counts.contiguous()
         # (a sequence that takes no part has no position: any row of the table will do)
         positions = (cache.next_positions()[:, None] + torch.arange(t, device=cache.lengths.device)).clamp(0, cache.max_len - 1).reshape(-1)
         x, cos, sin = self._look_up(input_ids, positions, cache)
         cos, sin = cos.view(b, t, -1), sin.view(b, t, -1)
-        pending = None
+        pending, lengths = None, cache.step_lengths(t, counts)
         for i, layer in enumerate(self.layers):
-            x, pending, _ = layer.forward_deferred(x, pending, cos, sin, cache.layer(i))
+            x, pending, _ = layer.forward_deferred(x, pending, cos, sin, cache.layer(i, counts, lengths))
         cache.advance(t, counts)
         x = self._final_norm(x, pending)
         return x if return_hidden else self._head(x)

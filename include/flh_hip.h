@@ -524,6 +524,12 @@ int flh_rope_quant_kv_cache_i4(const flh_half* q, const flh_half* k, const flh_h
                                const int64_t* lengths, flh_half* q_out, uint8_t* k_codes, flh_half* k_scales, uint8_t* v_codes,
                                flh_half* v_scales, uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len,
                                void* stream);
+/* The same of a padded batch: counts [B] int64 on the device, the first counts[b] of a sequence's T tokens are its own and the others are not
+ * written (their q_out is).  A sequence takes part where 0 <= counts[b] <= T, lengths[b] >= 0 and lengths[b] + counts[b] <= max_len.  NULL: all T. */
+int flh_rope_quant_kv_cache_i4_counts(const flh_half* q, const flh_half* k, const flh_half* v, const flh_half* cos, const flh_half* sin,
+                                      const int64_t* lengths, const int64_t* counts, flh_half* q_out, uint8_t* k_codes, flh_half* k_scales,
+                                      uint8_t* v_codes, flh_half* v_scales, uint32_t B, uint32_t T, uint32_t Hq, uint32_t Hkv,
+                                      uint32_t head_dim, uint32_t max_len, void* stream);
 
 /* Rows of such a cache back as fp16: keys, values [B, Hkv, rows, d] = slots first[b] .. first[b] + rows - 1 (first [B] int64 on the
  * device), keys with the Hadamard rotation undone.  A slot outside the cache gives zeros. */
@@ -551,6 +557,12 @@ int flh_prefill_attention_i4(const flh_half* q, const int64_t* lengths, const ui
                              const uint8_t* v_codes, const flh_half* v_scales, flh_half* out, uint32_t B, uint32_t T, uint32_t Hq,
                              uint32_t Hkv, uint32_t head_dim, uint32_t max_len, float scale, void* workspace, size_t workspace_bytes,
                              void* stream);
+/* The same of a padded batch (counts as in flh_rope_quant_kv_cache_i4_counts): the rows behind a sequence's own tokens are zeros.  The workspace is
+ * that of T tokens. */
+int flh_prefill_attention_i4_counts(const flh_half* q, const int64_t* lengths, const int64_t* counts, const uint8_t* k_codes,
+                                    const flh_half* k_scales, const uint8_t* v_codes, const flh_half* v_scales, flh_half* out, uint32_t B,
+                                    uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t head_dim, uint32_t max_len, float scale, void* workspace,
+                                    size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,10 +18,10 @@ class Recorder:
     def __init__(self):
         self.given = []
 
-    def rope_quantize_kv_cache_(self, q, *_):
+    def rope_quantize_kv_cache_(self, q, *_, counts):
         return q
 
-    def prefill_attention_i4(self, q, *_, workspace):
+    def prefill_attention_i4(self, q, *_, workspace, counts):
         self.given.append(workspace)
         return q.flatten(2)
 
