@@ -136,9 +136,9 @@ __device__ __forceinline__ constexpr int code_element(int e) { return 2 * (e & 3
 
 constexpr float kFromSubnormal = 1048576.0f;           // 2^20
 // What the 8 adds to an output's sums grows with the number of keys, a sum of signed codes with its root: every so many of its tiles a wave takes it
-// off its accumulators, so that their rounding does not grow with the length (keys of nearly one weight, heads of
-// 128, one wave: 16000 off by 3.6e-4 of the result, 60000 by 6.6e-4, 250000 by 2.4e-3 when it was taken off at the end alone; 3.0e-4 at any of them now,
-// what the weights' and the result's own roundings come to.  No time that could be measured.)
+// off its accumulators, so that their rounding does not grow with the length (keys of nearly one weight, heads of 128, one wave: 16000 off by 3.6e-4
+// of the result, 60000 by 6.6e-4, 250000 by 2.4e-3 when it was taken off at the end alone; 3.0e-4 at any of them now, what the weights' and the result's
+// own roundings come to, for 1 % of a prompt's time: 4096 tokens 195 -> 197 us).
 constexpr int kTakeOff = 16;
 constexpr float kLowestRef = -1e30f;                   // reference of a query that has seen nothing: finite, far below every score
 constexpr int kTileKeys = 64;

@@ -16,7 +16,8 @@
 //
 // What bounds it: long caches, the bytes (32 sequences of up to 8000 slots, 32 / 8 heads of 128: 206 MB, 42 us at a large copy's 4.9 TB/s; 48 us + 4.8 of
 // the joining launch); one long cache, the way of a workgroup before and after its tiles as well (60000 slots: 63 MB, 12.9 us; 19 + 3.9: the list 0.8, the
-// queries 2.3, the waves' results together 1.6 us); short ones, that way and the two launches (300 slots: 8.5 + 3.5 us).  Requesting two tiles ahead was
+// queries 2.3, the waves' results together 1.6 us); short ones, that way and the two launches (300 slots: 8.5 + 3.5 us).  Heads of 64: 14 + 3.9, 28 + 4.0 and
+// 8.0 + 3.1 us for the same slots and numbers of heads, 9.3 + 3.1 for 5 x 777 of 32 / 32.  Requesting two tiles ahead was
 // slower (the other workgroup of the compute unit hides the latency), and queries brought by direct-to-LDS loads gave nothing.
 #include "cache_i4.h"
 
@@ -49,8 +50,9 @@ struct Place {
 // How the work is shared.  Usually: the tiles of all heads are one list, each head's with kHeadTiles empty entries in front, for what a further head
 // costs a workgroup (its queries, the first tile's latency, a piece), and a workgroup takes `c` entries of it.  us, 0 / 4 / 8 / 12 / 16 of them: 1 x
 // 60000 slots of 8 heads 23.8 / 21.5 / 19.4 / 19.1 / 19.2, 32 x up to 8000 51.2 / 49.0 / 48.4 / 49.2 / 47.6, 5 x 778 of 32 heads 13.8 / 13.0 / 12.7 /
-// 13.0 / 14.6.  With few tiles to a workgroup each head is cut into equal parts of at most c tiles, and the parts are the list, of which a workgroup
-// takes one (5 x 778: 17.4 -> 13.8).  64 sequences in the lanes at a time.
+// 13.0 / 14.6; heads of 64: 1 x 60000 of 8 17.0 / 16.7 / 13.7 / 13.9 / 13.4, 32 x up to 8000 28.5 / 28.7 / 27.9 / 27.9 / 26.8, 16 x up to 3000 of 16
+// 18.7 / 18.9 / 17.8 / 18.0 / 17.3, 5 x 777 of 32 9.0 / 9.3 / 9.1 / 9.4 / 10.6.  With few tiles to a workgroup each head is cut into equal parts of at most c
+// tiles, and the parts are the list, of which a workgroup takes one (5 x 778: 17.4 -> 13.8).  64 sequences in the lanes at a time.
 struct Shares {
   uint32_t c, total, heads;                            // .., entries of the list, heads of a sequence
   bool parts;

@@ -14,11 +14,13 @@
 // Few rows: the tiles of a block are split over several workgroups, whose pieces (reference, sum, weighted codes) a second launch joins.
 //
 // What bounds it: many rows, the work around the products.  A tile of 64 keys and 32 queries is 16 + 16 matrix instructions, and 7 vector instructions for
-// eight codes, twice, and about 5 for a probability: 4096 tokens of a prompt, 32 / 8 heads of 128: 184 us, 746 TFLOP/s of the products below the
-// diagonal, the vector units busy in 71 % of the cycles and the matrix units in 32 %; 4096 behind 16000: 1400 us, 870 TFLOP/s, at the clock that the card
-// then holds.  64 rows to a wave, whose codes are unpacked once for both halves, took 1370 us there and 238 for the prompt (one wave a SIMD, and the
-// diagonal's pairs of a long and a short block leave it alone).  Few rows: the start and the end of a workgroup (4 x 17 tokens behind 8000 .. 16000: 39 us,
-// of which the codes' bytes are 11) and the blocks' last rows (68 rows are three blocks).
+// eight codes, twice, and about 5 for a probability: 4096 tokens of a prompt, 32 / 8 heads of 128: 193 us (passes among others; traced, one by one, 200
+// to 217), 712 TFLOP/s of the products below the diagonal, the vector units busy in 71 % of the cycles and the matrix units in 32 %; 4096 behind 16000: 1400
+// us, 870 TFLOP/s, at the clock that the card then holds.  The unpacking is each wave's own, about 900 of a tile's 2000 vector clocks: this library's
+// kernel over an fp16 cache, which has none, takes 50 us for a prompt of 2048 tokens with its write, this one 76.  64 rows to a wave, whose codes are unpacked
+// once for both halves, took 1370 us there and 238 for the prompt (one wave a SIMD, and the diagonal's pairs of a long and a short block leave it alone).
+// Few rows: the start and the end of a workgroup (4 x 17 tokens behind 8000 .. 16000: 41 us, of which the codes' bytes are 11) and the blocks' last
+// rows (68 rows are three blocks).
 #include <algorithm>
 #include <type_traits>
 
@@ -480,15 +482,19 @@ __global__ __launch_bounds__(256) void prefill_i4_join_kernel(Prefill a) {
 }
 
 // Waves that share a block: all four where the blocks are few (a short tail, but a joint end for each), two from `pairs` blocks on, one from twice as
-// many.  us, four / two / one: heads of 128, 32 / 8 of them, prompts of 512 tokens (512 blocks) 15 / 19 / 25, 1024 34 / 31 / 40, 2048 85 / 76 / 77, 4096
-// 255 / 232 / 220, 64 x 64 tokens behind 1000 (4096) 161 / 138 / 125; heads of 64, 16 / 16 of them, whose tiles are less work: 2 x 1111 behind 600 (1120)
-// 40 / 41 / 47, 4096 (2048) 87 / 83 / 97, 4 x 2048 (4096) 98 / 85 / 78, 4 x 4096 (8192) 295 / 264 / 248.
+// many.  us, four / two / one (traced, random codes): heads of 128, 32 / 8 of them, prompts of 512 tokens (512 blocks) 13.1 / 13.9 / 18.6, 1024 26.7 / 23.7 / 31.7,
+// 2048 69 / 61 / 66, 4096 223 / 206 / 191, 2048 behind 2048 (2048) 153 / 144 / 148, 64 x 64 tokens behind 1000 (4096) 141 / 117 / 105; heads of 64, 16 / 16 of
+// them, whose tiles are less work: 2 x 1111 behind 600 (1120) 28.8 / 30.5 / 37.7, 4096 (2048) 68 / 66 / 86, 4 x 2048 (4096) 81 / 69 / 66, 4 x 4096 (8192)
+// 255 / 247 / 220.
 uint32_t waves_of(uint64_t blocks, uint32_t head_dim) {
   const uint64_t pairs = head_dim == 128 ? 1024 : 2048;
   return blocks < pairs ? 4 : blocks < 2 * pairs ? 2 : 1;
 }
 
-// Parts that a block can have: none where the blocks fill the chip
+// Parts that a block can have: one from half a round of workgroups on, whatever the lengths.  That is right for lengths that are alike and not for a batch
+// with a single long one: 2 tokens each, 32 / 8 heads of 128, 32 sequences (256 blocks) and 33: 8000 slots each 61 and 86 us, 500 each 9 and 11, down from
+// 16000 80 and 102, but 60000 and the others 200 42 and 338 (the long one's eight blocks are eight workgroups' then).  64 at most, which the joining launch has
+// a lane each for: a sequence with four key / value heads of one block fills half the workgroups.
 uint32_t splits_of(uint64_t B, uint64_t heads, uint32_t max_len) {
   const uint64_t tiles = ((uint64_t)max_len + kTileKeys - 1) / kTileKeys, most = (tiles + kPartTiles - 1) / kPartTiles;
   uint64_t s = 2 * B * heads > kParts ? 1 : kParts / heads;
