@@ -520,6 +520,9 @@ __global__ __launch_bounds__(256) void decode_i4_join_kernel(Decode a) {
 }
 
 constexpr uint32_t kGroups = 512;                      // two workgroups on each compute unit
+// Sequences of a pair of launches: each workgroup looks through the list of them, and one list for all takes time that grows with their square (8 heads
+// of 64, 41 slots: 2048 sequences 479 us, 16384 22.8 ms, a million would take a minute and a half; 335 us and 2.8 ms in pairs of launches for 1024 each)
+constexpr uint32_t kSequences = 1024;
 
 uint32_t blocks_of(uint32_t rep) { return (rep + kCols - 1) / kCols; }
 
@@ -566,24 +569,33 @@ extern "C" int flh_decode_attention_rope_i4(const flh_half* q, const flh_half* k
     for (int j = 0; j < i; ++j)
       if (overlap(held[i].at, held[i].bytes, held[j].at, held[j].bytes)) return fail(FLH_EINVAL, "%s: outputs, caches or workspace share memory", what);
     // (the joining launch alone writes `out`, behind everything that reads the queries, keys and values; it reads the lengths itself)
+    // (of large batches, in its own pair of launches: the queries' own place will do)
     for (int j = 0; j < 6; ++j)
-      if (overlap(held[i].at, held[i].bytes, in[j].at, in[j].bytes) && (i < 5 || j == 4))
+      if (overlap(held[i].at, held[i].bytes, in[j].at, in[j].bytes) && (i < 5 || j == 4 || (B > kSequences && !(j == 5 && out == q))))
         return fail(FLH_EINVAL, "%s: an output shares memory with an input", what);
   }
   Decode a = {};
-  a.q = (const __half*)q, a.k_new = (const __half*)k_new, a.v_new = (const __half*)v_new, a.cos = (const __half*)cos, a.sin = (const __half*)sin;
-  a.lengths = (const long long*)lengths, a.k_codes = k_codes, a.v_codes = v_codes, a.k_scales = (__half*)k_scales, a.v_scales = (__half*)v_scales;
-  a.out = (__half*)out, a.partials = (float*)workspace;
-  a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.blocks = blocks_of(a.rep), a.max_len = max_len;
+  a.partials = (float*)workspace;
+  a.Hq = Hq, a.Hkv = Hkv, a.rep = Hq / Hkv, a.blocks = blocks_of(a.rep), a.max_len = max_len;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const uint64_t most = (uint64_t)B * Hkv * a.blocks * ((max_len - 1) / kTileKeys + 1);
-  a.groups = (uint32_t)(most < kGroups ? most : kGroups);
   auto go = [&](auto kern, auto join, size_t smem, LdsGrant& grant) {
     if (int rc = reserve_lds((const void*)kern, smem, grant, what)) return rc;
-    hipLaunchKernelGGL(kern, dim3(a.groups), dim3(kThreads), smem, (hipStream_t)stream, a);
-    if (int rc = check_launch(what)) return rc;
-    hipLaunchKernelGGL(join, dim3(B * Hq), dim3(256), 0, (hipStream_t)stream, a);
-    return check_launch(what);
+    for (uint32_t done = 0; done < B; done += a.B) {   // (launches of a stream run in order: the pieces are joined before the next ones are written)
+      const size_t q_at = (size_t)done * Hq * head_dim, new_at = (size_t)done * Hkv * head_dim, row = (size_t)done * Hkv * max_len;
+      a.B = B - done < kSequences ? B - done : kSequences;
+      a.q = (const __half*)q + q_at, a.k_new = (const __half*)k_new + new_at, a.v_new = (const __half*)v_new + new_at;
+      a.cos = (const __half*)cos + (size_t)done * head_dim, a.sin = (const __half*)sin + (size_t)done * head_dim;
+      a.lengths = (const long long*)lengths + done, a.out = (__half*)out + q_at;
+      a.k_codes = k_codes + row * (head_dim / 2), a.v_codes = v_codes + row * (head_dim / 2);
+      a.k_scales = (__half*)k_scales + row, a.v_scales = (__half*)v_scales + row;
+      const uint64_t most = (uint64_t)a.B * Hkv * a.blocks * ((max_len - 1) / kTileKeys + 1);
+      a.groups = (uint32_t)(most < kGroups ? most : kGroups);
+      hipLaunchKernelGGL(kern, dim3(a.groups), dim3(kThreads), smem, (hipStream_t)stream, a);
+      if (int rc = check_launch(what)) return rc;
+      hipLaunchKernelGGL(join, dim3(a.B * Hq), dim3(256), 0, (hipStream_t)stream, a);
+      if (int rc = check_launch(what)) return rc;
+    }
+    return FLH_OK;
   };
   static LdsGrant grant128, grant64;
   return head_dim == 128 ? go(decode_i4_kernel<128>, decode_i4_join_kernel<128>, Layout<128>::kBytes, grant128)

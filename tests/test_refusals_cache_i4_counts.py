@@ -34,3 +34,20 @@ def test_outputs_do_not_lie_on_the_counts(name, count, outputs, sizes):
         p = A[:count]
         p[at] = p[o] + 8
         assert getattr(lib, name)(*p, *sizes) == -1 and b"shares memory" in lib.flh_last_error(), lib.flh_last_error()
+
+
+@pytest.mark.parametrize("B,refused", [(1024, False), (1025, True)])
+def test_outputs_of_large_batches_are_their_own(B, refused):
+    """More than 1024 sequences go in several pairs of launches: an output of the first must not lie on what the next one reads."""
+    lib = _lib.load()
+    place = [(i + 2) << 40 for i in range(12)]
+
+    def call(out, workspace_bytes):
+        p = place[:11]
+        p[10] = out
+        return lib.flh_decode_attention_rope_i4(*p, B, 8, 2, 128, 64, 0.1, place[11], workspace_bytes, None)
+
+    for out in (place[0] + 16, place[1], place[2] + 64, place[3], place[4]):
+        if refused:
+            assert call(out, 1 << 40) == -1 and b"shares memory" in lib.flh_last_error(), lib.flh_last_error()
+        assert call(out, 64) == -1 and b"workspace" in lib.flh_last_error()       # (never launched here)
